@@ -16,6 +16,7 @@ using namespace psb;
 
 void bind_host(py::module_& m);    // host runtime (defined in bindings_host.cpp)
 void bind_dense(py::module_& m);   // dense / GEMM kernels (defined in bindings_dense.cu)
+void bind_block(py::module_& m);   // decoder-block operators (defined in bindings_block.cu)
 
 namespace {
 template <class T>
@@ -246,4 +247,5 @@ PYBIND11_MODULE(_C, m) {
 
     bind_host(m);
     bind_dense(m);
+    bind_block(m);
 }

@@ -1,0 +1,47 @@
+// Activation checkpoints in 8 bits: 32 neighbours of a row share one power of two, each value is a whole number of
+// -127..127 steps. With m the largest magnitude of a block,
+//     e    = the smallest exponent (1..249) at which m / 2^(e-127) rounds to at most 127,
+//     q_i  = round-to-nearest-even(x_i / 2^(e-127)),          x_i is rebuilt as q_i * 2^(e-127).
+// The error of a value is at most half a step, a step is between m / 127.5 and m / 63.7. A step is a power of two, so that
+// scaling never rounds: q * 2^(e-127) has at most 7 significant bits and is exact in bf16, which is what lets the weight
+// gradient feed rebuilt values to the bf16 tensor cores without a second rounding. A block that holds an infinity or NaN is
+// stored as e = 255 with q = 0 (0 * 2^128 = NaN): a training step that has gone wrong shows it in its gradients.
+// (Blocks of 32 with a shared power of two are the layout of the published microscaling formats; the rule for e, which uses
+// the whole range of q, and the mark for blocks that are not finite are this file's.)
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace psb {
+
+namespace {
+
+constexpr int kAct8Block = 32;
+
+// The exponent byte for a block whose largest magnitude has these bits (compared as integers, NaN is above infinity is
+// above every number, so a maximum over the bits carries both). Adding 2^16 carries into the exponent exactly when the
+// mantissa is at least 127.5 / 64.
+__device__ __forceinline__ uint32_t act8_exponent(uint32_t amax_bits) {
+    if (amax_bits >= 0x7F800000u) return 255u;
+    const int e = (int)((amax_bits + 0x10000u) >> 23) - 6;
+    return (uint32_t)(e < 1 ? 1 : e);
+}
+// 2^(127-e), and 0 for e = 255
+__device__ __forceinline__ float act8_inverse_step(uint32_t e) { return e == 255u ? 0.f : __uint_as_float((254u - e) << 23); }
+// 2^(e-127), and infinity for e = 255
+__device__ __forceinline__ float act8_step(uint32_t e) { return __uint_as_float(e << 23); }
+// (the conversion takes NaN = infinity * 0 to 0)
+__device__ __forceinline__ int act8_quantise(float x, float inverse_step) { return __float2int_rn(x * inverse_step); }
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ uint32_t pack_s8x4(int a, int b, int c, int d) {
+    return __byte_perm(__byte_perm((uint32_t)a, (uint32_t)b, 0x0040), __byte_perm((uint32_t)c, (uint32_t)d, 0x0040), 0x5410);
+}
+// byte i of a word as a signed number
+__device__ __forceinline__ float s8_at(uint32_t w, int i) { return (float)(int)(int8_t)(w >> (8 * i)); }
+
+}  // namespace
+
+}  // namespace psb

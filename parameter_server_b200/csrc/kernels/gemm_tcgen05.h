@@ -66,6 +66,7 @@ int gemm_chain_scratch_words();
 // Upper bound on the CTAs (= SMs) of the following launches; 0 = all SMs. A GEMM CTA fills its SM, so a smaller grid
 // leaves whole SMs to kernels of another stream that run at the same time (the sparse push beside the dense backward).
 void gemm_set_cta_limit(int ctas);
+int gemm_cta_limit();
 // CTA pairs (two CTAs of a cluster per 256-row tile) on or off for the following launches. A pair needs two free SMs
 // of one TPC at the same moment; launches that share the GPU with another kernel run better without.
 void gemm_set_pair(int on);

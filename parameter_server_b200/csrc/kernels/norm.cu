@@ -1,0 +1,838 @@
+// Layer norm forward and backward, 8-bit checkpoints of rows, and column sums with a fixed order: the memory-bound
+// operators of a decoder block (the consumer of dense tables; the reference is a storage service and has no model code).
+//
+//   forward   mean = sum(x) / d,  rstd = 1 / sqrt(sum((x - mean)^2) / d + eps),  y = xhat * weight + bias
+//   backward  p = dy * weight:  dx = rstd * (p - sum(p) / d - xhat * sum(p * xhat) / d)  (+ the residual branch's gradient)
+//             dweight = sum_rows dy * xhat,  dbias = sum_rows dy
+//
+// All of it is bound by HBM: a row is read once, kept in registers between the statistics and the output (the squared
+// distances are taken from the mean, not as a difference of sums), and written once. Sums and statistics are fp32.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "act8.cuh"
+#include "norm.h"
+
+namespace psb {
+
+namespace {
+
+constexpr int kMaxTeam = 512;        // threads that share one row
+constexpr int kBwdThreads = 512;
+constexpr int kBwdElems = 16;        // columns per thread of the backward kernel: two fp32 sums each stay in registers
+constexpr int kSms = 148;
+
+// VEC consecutive values of a row as fp32: one 16-byte access, or one element (VEC 1: rows of any alignment).
+template <typename T, int VEC>
+struct Io;
+template <>
+struct Io<__nv_bfloat16, 8> {
+    using Raw = uint4;
+    static __device__ __forceinline__ Raw load(const __nv_bfloat16* p) { return *(const uint4*)p; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float* f) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) {
+        uint4 r;
+        __nv_bfloat162* h = (__nv_bfloat162*)&r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        *(uint4*)p = r;
+    }
+    static __device__ __forceinline__ Raw zero() { return make_uint4(0, 0, 0, 0); }
+};
+template <>
+struct Io<float, 4> {
+    using Raw = float4;
+    static __device__ __forceinline__ Raw load(const float* p) { return *(const float4*)p; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float* f) { f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w; }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *(float4*)p = make_float4(f[0], f[1], f[2], f[3]); }
+    static __device__ __forceinline__ Raw zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+};
+template <>
+struct Io<__nv_bfloat16, 1> {
+    using Raw = __nv_bfloat16;
+    static __device__ __forceinline__ Raw load(const __nv_bfloat16* p) { return *p; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float* f) { f[0] = __bfloat162float(r); }
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) { *p = __float2bfloat16_rn(f[0]); }
+    static __device__ __forceinline__ Raw zero() { return __float2bfloat16_rn(0.f); }
+};
+template <>
+struct Io<float, 1> {
+    using Raw = float;
+    static __device__ __forceinline__ Raw load(const float* p) { return *p; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float* f) { f[0] = r; }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *p = f[0]; }
+    static __device__ __forceinline__ Raw zero() { return 0.f; }
+};
+
+// VEC consecutive whole numbers of a checkpoint row
+template <int VEC>
+struct Q8;
+template <>
+struct Q8<8> {
+    using Raw = uint2;
+    static __device__ __forceinline__ Raw load(const int8_t* p) { return *(const uint2*)p; }
+    static __device__ __forceinline__ Raw zero() { return make_uint2(0, 0); }
+    static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[i] = s8_at(r.x, i) * step;
+            f[4 + i] = s8_at(r.y, i) * step;
+        }
+    }
+    static __device__ __forceinline__ void store(int8_t* p, const int* q) {
+        *(uint2*)p = make_uint2(pack_s8x4(q[0], q[1], q[2], q[3]), pack_s8x4(q[4], q[5], q[6], q[7]));
+    }
+};
+template <>
+struct Q8<4> {
+    using Raw = uint32_t;
+    static __device__ __forceinline__ Raw load(const int8_t* p) { return *(const uint32_t*)p; }
+    static __device__ __forceinline__ Raw zero() { return 0u; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = s8_at(r, i) * step;
+    }
+    static __device__ __forceinline__ void store(int8_t* p, const int* q) { *(uint32_t*)p = pack_s8x4(q[0], q[1], q[2], q[3]); }
+};
+template <>
+struct Q8<1> {
+    using Raw = int8_t;
+    static __device__ __forceinline__ Raw load(const int8_t* p) { return *p; }
+    static __device__ __forceinline__ Raw zero() { return 0; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) { f[0] = (float)r * step; }
+    static __device__ __forceinline__ void store(int8_t* p, const int* q) { *p = (int8_t)q[0]; }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+// largest bits among the lanes that share a block of 32 columns (32 / VEC neighbours; all lanes of the warp call)
+template <int VEC>
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+#pragma unroll
+    for (int o = kAct8Block / VEC / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+// Quantises the VEC values of this thread (col = first column; all lanes of the warp call, `valid` false past the row).
+template <int VEC>
+__device__ __forceinline__ void keep8(const float* f, bool valid, int8_t* qrow, uint8_t* erow, int col) {
+    uint32_t m = 0;
+    if (valid) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(f[j]));
+    }
+    const uint32_t e = act8_exponent(block_max<VEC>(m));
+    if (!valid) return;
+    const float inv = act8_inverse_step(e);
+    int q[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) q[j] = act8_quantise(f[j], inv);
+    Q8<VEC>::store(qrow + col, q);
+    if (col % kAct8Block == 0) erow[col / kAct8Block] = (uint8_t)e;
+}
+
+// ---- forward ---------------------------------------------------------------------------------------------------------
+// `tpr` threads (a power of two, 32..512) hold one row in registers, NV vectors each: thread t has the columns
+// (i * tpr + t) * VEC. A warp per row needs no barrier and is taken while its 64 values a lane fit (d <= 2048 in bf16);
+// with few rows a row is spread over as many threads as have a vector each, since then the latency of one row is the time.
+template <typename T, int VEC, int NV, bool OUT8>
+__global__ void __launch_bounds__(kMaxTeam)
+layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, T* __restrict__ y,
+                      int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
+                      int64_t lde, int64_t rows, int d, float eps, int tpr) {
+    __shared__ float red[2][kMaxTeam / 32];
+    const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
+    const int64_t row = (int64_t)blockIdx.x * teams + team;
+    const bool live = row < rows;
+    const T* xr = x + (live ? row : 0) * ldx;
+    typename Io<T, VEC>::Raw raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int col = (i * tpr + t) * VEC;
+        raw[i] = live && col < d ? Io<T, VEC>::load(xr + col) : Io<T, VEC>::zero();
+    }
+    float v[NV * VEC];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        Io<T, VEC>::unpack(raw[i], v + i * VEC);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += v[i * VEC + j];
+    }
+    const int warps = tpr / 32, w0 = team * warps;
+    auto team_sum = [&](float part, int k) -> float {
+        part = warp_sum(part);
+        if (warps == 1) return part;
+        if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = part;
+        __syncthreads();
+        float all = 0.f;
+        for (int w = 0; w < warps; ++w) all += red[k][w0 + w];
+        return all;
+    };
+    const float mean = team_sum(s, 0) / (float)d;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const bool in = (i * tpr + t) * VEC < d;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            v[i * VEC + j] -= mean;
+            if (in) s += v[i * VEC + j] * v[i * VEC + j];
+        }
+    }
+    const float rstd = rsqrtf(team_sum(s, 1) / (float)d + eps);
+    if (live && t == 0) {
+        if (mean_out != nullptr) mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int col = (i * tpr + t) * VEC;
+        const bool in = live && col < d;
+        float* f = v + i * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] *= rstd;
+        if constexpr (OUT8) keep8<VEC>(f, in, q + (live ? row : 0) * ldq, e + (live ? row : 0) * lde, col);
+        if (!in) continue;
+        if (weight != nullptr) {
+            float g[VEC];
+            Io<T, VEC>::unpack(Io<T, VEC>::load(weight + col), g);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] *= g[j];
+        }
+        if (bias != nullptr) {
+            float b[VEC];
+            Io<T, VEC>::unpack(Io<T, VEC>::load(bias + col), b);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] += b[j];
+        }
+        Io<T, VEC>::store(y + row * ldy + col, f);
+    }
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float all = 0.f;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) all += red[w];
+    return all;
+}
+
+// Rows longer than registers hold: a CTA per row, the row is read again (from L2) for each statistic.
+template <typename T, bool OUT8>
+__global__ void __launch_bounds__(512)
+layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias,
+                           T* __restrict__ y, int64_t ldy, float* mean_out, float* rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
+                           int64_t lde, int d, float eps) {
+    __shared__ float red[16];
+    const int64_t row = blockIdx.x;
+    const T* xr = x + row * ldx;
+    float s = 0.f, f;
+    for (int c = threadIdx.x; c < d; c += blockDim.x) { Io<T, 1>::unpack(xr[c], &f); s += f; }
+    const float mean = block_sum(s, red) / (float)d;
+    s = 0.f;
+    for (int c = threadIdx.x; c < d; c += blockDim.x) { Io<T, 1>::unpack(xr[c], &f); s += (f - mean) * (f - mean); }
+    const float rstd = rsqrtf(block_sum(s, red) / (float)d + eps);
+    if (threadIdx.x == 0) {
+        if (mean_out != nullptr) mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+    for (int c0 = 0; c0 < d; c0 += blockDim.x) {
+        const int c = c0 + threadIdx.x;
+        float h = 0.f, g = 1.f, b = 0.f;
+        if (c < d) {
+            Io<T, 1>::unpack(xr[c], &f);
+            h = (f - mean) * rstd;
+            if (weight != nullptr) Io<T, 1>::unpack(weight[c], &g);
+            if (bias != nullptr) Io<T, 1>::unpack(bias[c], &b);
+            const float o = h * g + b;
+            Io<T, 1>::store(y + row * ldy + c, &o);
+        }
+        if constexpr (OUT8) keep8<1>(&h, c < d, q + row * ldq, e + row * lde, c);
+    }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------
+// Persistent CTAs (one per SM) of blockDim / tpr teams; a team walks rows R at a time and thread t keeps the sums of its 16
+// columns' dweight and dbias in registers over all of them, so that the weight's gradient costs no second pass over dy and
+// x. The two row sums cross the team's warps through shared memory with one barrier for R rows. At the end the teams' sums
+// are added in team order and leave as one partial row per CTA, which column_reduce_kernel adds in CTA order: the result
+// does not depend on timing. (More CTAs per SM would write and read more partial rows: 2 * d floats each.)
+template <typename T, int VEC, bool SRC8>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
+                      int64_t ldq, const uint8_t* __restrict__ e, int64_t lde, const T* __restrict__ weight,
+                      const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const T* __restrict__ join, int64_t ldjoin,
+                      T* __restrict__ dx, int64_t lddx, float* __restrict__ partial, int64_t rows, int d, int tpr) {
+    constexpr int NV = kBwdElems / VEC;
+    constexpr int R = 1;   // rows in flight per team (registers: raw dy, x and join of R rows)
+    using IO = Io<T, VEC>;
+    extern __shared__ float comb[];             // [2][d], for the teams' sums at the end
+    __shared__ float red[2][kBwdThreads / 32][2 * R];
+    const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
+    const int warps = tpr / 32, w0 = team * warps, lane = threadIdx.x & 31;
+    float dg[kBwdElems], db[kBwdElems];
+    typename IO::Raw graw[NV];
+#pragma unroll
+    for (int i = 0; i < kBwdElems; ++i) dg[i] = db[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int col = (i * tpr + t) * VEC;
+        graw[i] = weight != nullptr && col < d ? IO::load(weight + col) : IO::zero();
+    }
+    const bool has_w = weight != nullptr;
+    const float inv_d = 1.f / (float)d;
+    int buf = 0;
+    for (int64_t r0 = ((int64_t)blockIdx.x * teams + team) * R; r0 < rows; r0 += (int64_t)gridDim.x * teams * R, buf ^= 1) {
+        typename IO::Raw ry[R][NV], rx[R][NV], rj[R][NV];
+        typename Q8<VEC>::Raw rq[R][NV];
+        uint32_t re[R][NV];
+        float mean[R], rstd[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = r0 + r;
+            const bool live = row < rows;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int col = (i * tpr + t) * VEC;
+                const bool in = live && col < d;
+                ry[r][i] = in ? IO::load(dy + row * lddy + col) : IO::zero();
+                if constexpr (SRC8) {
+                    rq[r][i] = in ? Q8<VEC>::load(q + row * ldq + col) : Q8<VEC>::zero();
+                    re[r][i] = in ? e[row * lde + col / kAct8Block] : 0u;
+                } else {
+                    rx[r][i] = in ? IO::load(x + row * ldx + col) : IO::zero();
+                }
+                if (join != nullptr) rj[r][i] = in ? IO::load(join + row * ldjoin + col) : IO::zero();
+            }
+            rstd[r] = live ? rstd_in[row] : 0.f;
+            mean[r] = !SRC8 && live ? mean_in[row] : 0.f;
+        }
+        // this thread's part of vector i of row r: gradient, and normalised value (0 past the row's end: rstd * (0 - mean) is not)
+        auto values = [&](int r, int i, float* fy, float* fh) {
+            IO::unpack(ry[r][i], fy);
+            if constexpr (SRC8) {
+                Q8<VEC>::unpack(rq[r][i], act8_step(re[r][i]), fh);
+            } else {
+                IO::unpack(rx[r][i], fh);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) fh[j] = (fh[j] - mean[r]) * rstd[r];
+            }
+        };
+        float sums[2 * R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float fy[VEC], fh[VEC], g[VEC];
+                values(r, i, fy, fh);
+                IO::unpack(graw[i], g);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const int c = i * VEC + j;
+                    const float p = has_w ? fy[j] * g[j] : fy[j];
+                    dg[c] += fy[j] * fh[j];
+                    db[c] += fy[j];
+                    s1 += p;
+                    s2 += p * fh[j];
+                }
+            }
+            sums[2 * r] = warp_sum(s1);
+            sums[2 * r + 1] = warp_sum(s2);
+        }
+        if (warps > 1) {
+            if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < 2 * R; ++k) red[buf][threadIdx.x >> 5][k] = sums[k];
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(tpr) : "memory");
+#pragma unroll
+            for (int k = 0; k < 2 * R; ++k) sums[k] = 0.f;
+            for (int w = 0; w < warps; ++w) {
+#pragma unroll
+                for (int k = 0; k < 2 * R; ++k) sums[k] += red[buf][w0 + w][k];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = r0 + r;
+            if (row >= rows) break;
+            const float a1 = sums[2 * r] * inv_d, a2 = sums[2 * r + 1] * inv_d;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int col = (i * tpr + t) * VEC;
+                if (col >= d) continue;
+                float fy[VEC], fh[VEC], g[VEC], o[VEC];
+                values(r, i, fy, fh);
+                IO::unpack(graw[i], g);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o[j] = rstd[r] * ((has_w ? fy[j] * g[j] : fy[j]) - a1 - fh[j] * a2);
+                if (join != nullptr) {
+                    float fj[VEC];
+                    IO::unpack(rj[r][i], fj);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) o[j] += fj[j];
+                }
+                IO::store(dx + row * lddx + col, o);
+            }
+        }
+    }
+    if (partial == nullptr) return;
+    float* out = partial + (int64_t)blockIdx.x * 2 * d;
+    for (int k = 0; k < teams; ++k) {
+        if (team == k) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const int col = (i * tpr + t) * VEC + j, c = i * VEC + j;
+                    if (col >= d) continue;
+                    float* cg = teams > 1 ? comb : out;
+                    float g1 = dg[c], b1 = db[c];
+                    if (k > 0) { g1 += cg[col]; b1 += cg[d + col]; }
+                    cg[col] = g1;
+                    cg[d + col] = b1;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (teams > 1)
+        for (int c = threadIdx.x; c < 2 * d; c += blockDim.x) out[c] = comb[c];
+}
+
+// Rows longer than 8192 columns: dx with a CTA per row that reads it twice, and the weight's gradient by columns.
+template <typename T, bool SRC8>
+__device__ __forceinline__ float xhat_at(const T* x, int64_t ldx, const int8_t* q, int64_t ldq, const uint8_t* e, int64_t lde, int64_t row,
+                                         int c, float mean, float rstd) {
+    if constexpr (SRC8) return (float)q[row * ldq + c] * act8_step(e[row * lde + c / kAct8Block]);
+    float f;
+    Io<T, 1>::unpack(x[row * ldx + c], &f);
+    return (f - mean) * rstd;
+}
+template <typename T, bool SRC8>
+__global__ void __launch_bounds__(512)
+layer_norm_bwd_long_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* q, int64_t ldq,
+                           const uint8_t* e, int64_t lde, const T* __restrict__ weight, const float* mean_in, const float* rstd_in,
+                           const T* join, int64_t ldjoin, T* __restrict__ dx, int64_t lddx, int d) {
+    __shared__ float red[16];
+    const int64_t row = blockIdx.x;
+    const float rstd = rstd_in[row], mean = SRC8 ? 0.f : mean_in[row];
+    auto p_at = [&](int c) {
+        float f, g = 1.f;
+        Io<T, 1>::unpack(dy[row * lddy + c], &f);
+        if (weight != nullptr) Io<T, 1>::unpack(weight[c], &g);
+        return f * g;
+    };
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < d; c += blockDim.x) {
+        const float p = p_at(c);
+        s1 += p;
+        s2 += p * xhat_at<T, SRC8>(x, ldx, q, ldq, e, lde, row, c, mean, rstd);
+    }
+    s1 = block_sum(s1, red) / (float)d;
+    s2 = block_sum(s2, red) / (float)d;
+    for (int c = threadIdx.x; c < d; c += blockDim.x) {
+        float o = rstd * (p_at(c) - s1 - xhat_at<T, SRC8>(x, ldx, q, ldq, e, lde, row, c, mean, rstd) * s2), j = 0.f;
+        if (join != nullptr) Io<T, 1>::unpack(join[row * ldjoin + c], &j);
+        o += j;
+        Io<T, 1>::store(dx + row * lddx + c, &o);
+    }
+}
+template <typename T, bool SRC8>
+__global__ void __launch_bounds__(256)
+layer_norm_dw_long_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* q, int64_t ldq,
+                          const uint8_t* e, int64_t lde, const float* mean_in, const float* rstd_in, float* partial, int64_t rows, int d) {
+    const int c = blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= d) return;
+    const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r1 = min(rows, (int64_t)(blockIdx.y + 1) * per);
+    float g = 0.f, b = 0.f, f;
+    for (int64_t row = (int64_t)blockIdx.y * per; row < r1; ++row) {
+        Io<T, 1>::unpack(dy[row * lddy + c], &f);
+        g += f * xhat_at<T, SRC8>(x, ldx, q, ldq, e, lde, row, c, SRC8 ? 0.f : mean_in[row], rstd_in[row]);
+        b += f;
+    }
+    partial[(int64_t)blockIdx.y * 2 * d + c] = g;
+    partial[(int64_t)blockIdx.y * 2 * d + d + c] = b;
+}
+
+// out[c] (+)= sum over the partial rows, eight interleaved sums per column that are then added in a fixed order. Column c
+// of the partials goes to out0[c], or to out1[c - split] from `split` on; either may be null.
+__global__ void __launch_bounds__(256)
+column_reduce_kernel(const float* __restrict__ partial, int n, int64_t width, int64_t split, float* out0, float* out1, int accumulate) {
+    __shared__ float part[8][33];
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched ahead of the end of the kernel that writes the partials
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+    float s = 0.f;
+    if (c < width) {
+#pragma unroll 8
+        for (int r = ty; r < n; r += 8) s += partial[(int64_t)r * width + c];
+    }
+    part[ty][tx] = s;
+    __syncthreads();
+    if (ty != 0 || c >= width) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += part[k][tx];
+    float* o = c < split ? (out0 != nullptr ? out0 + c : nullptr) : (out1 != nullptr ? out1 + (c - split) : nullptr);
+    if (o != nullptr) *o = accumulate ? *o + s : s;
+}
+
+// ---- column sums -----------------------------------------------------------------------------------------------------
+// A CTA sums a slab of rows for 128 columns (16 lanes of 8, or 4 bytes wide where rows are not aligned): four rows requested
+// before the first is added, then one partial row per slab.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+column_sum_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, float* __restrict__ partial) {
+    constexpr int TX = 128 / VEC, TY = 256 / TX > 0 ? 256 / TX : 1;
+    __shared__ float part[TY][128 + 4];
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    const int64_t col = (int64_t)blockIdx.x * 128 + tx * VEC;
+    const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r1 = min(rows, (int64_t)(blockIdx.y + 1) * per);
+    float s[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+    if (col < cols) {
+        const T* p = x + col;
+        int64_t r = (int64_t)blockIdx.y * per + ty;
+        for (; r + 3 * TY < r1; r += 4 * TY) {
+            typename Io<T, VEC>::Raw raw[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) raw[k] = Io<T, VEC>::load(p + (r + k * TY) * ldx);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float f[VEC];
+                Io<T, VEC>::unpack(raw[k], f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s[j] += f[j];
+            }
+        }
+        for (; r < r1; r += TY) {
+            float f[VEC];
+            Io<T, VEC>::unpack(Io<T, VEC>::load(p + r * ldx), f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s[j] += f[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) part[ty][tx * VEC + j] = s[j];
+    __syncthreads();
+    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && c < cols) {
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < TY; ++k) a += part[k][threadIdx.x];
+        partial[(int64_t)blockIdx.y * cols + c] = a;
+    }
+}
+
+// ---- 8-bit checkpoints of rows ---------------------------------------------------------------------------------------
+// A warp takes U vectors of a row per lane, all requested before the first is used.
+template <typename T, int VEC, int U>
+__global__ void __launch_bounds__(256)
+act8_pack_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ e, int64_t lde, int64_t rows,
+                 int64_t cols, int64_t per_row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t row = task / per_row, c0 = (task - row * per_row) * (32 * VEC * U) + lane * VEC;
+    if (row >= rows) return;   // a whole warp
+    typename Io<T, VEC>::Raw raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t col = c0 + i * 32 * VEC;
+        raw[i] = col < cols ? Io<T, VEC>::load(x + row * ldx + col) : Io<T, VEC>::zero();
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t col = c0 + i * 32 * VEC;
+        float f[VEC];
+        Io<T, VEC>::unpack(raw[i], f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(f[j]));
+        const uint32_t ex = act8_exponent(block_max<VEC>(m));
+        if (col >= cols) continue;
+        const float inv = act8_inverse_step(ex);
+        int n[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) n[j] = act8_quantise(f[j], inv);
+        Q8<VEC>::store(q + row * ldq + col, n);
+        if (col % kAct8Block == 0) e[row * lde + col / kAct8Block] = (uint8_t)ex;
+    }
+}
+template <typename T, int VEC, int U>
+__global__ void __launch_bounds__(256)
+act8_unpack_kernel(const int8_t* __restrict__ q, int64_t ldq, const uint8_t* __restrict__ e, int64_t lde, T* __restrict__ x, int64_t ldx,
+                   int64_t rows, int64_t cols, int64_t per_row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t row = task / per_row, c0 = (task - row * per_row) * (32 * VEC * U) + lane * VEC;
+    if (row >= rows) return;
+    typename Q8<VEC>::Raw raw[U];
+    uint32_t ex[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t col = c0 + i * 32 * VEC;
+        raw[i] = col < cols ? Q8<VEC>::load(q + row * ldq + col) : Q8<VEC>::zero();
+        ex[i] = col < cols ? e[row * lde + col / kAct8Block] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t col = c0 + i * 32 * VEC;
+        if (col >= cols) continue;
+        float f[VEC];
+        Q8<VEC>::unpack(raw[i], act8_step(ex[i]), f);
+        Io<T, VEC>::store(x + row * ldx + col, f);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+int pow2_at_least(int64_t v, int lo, int hi) {
+    int p = lo;
+    while (p < v && p < hi) p <<= 1;
+    return p;
+}
+template <typename T>
+constexpr int vec_of() { return 16 / (int)sizeof(T); }
+// Whether 16-byte accesses fit: every row of every tensor starts on a 16-byte boundary and holds whole vectors.
+template <typename T>
+bool aligned(int64_t d, std::initializer_list<std::pair<const void*, int64_t>> rows) {
+    if (d % vec_of<T>()) return false;
+    for (const auto& r : rows)
+        if (r.first != nullptr && (((uintptr_t)r.first % 16) || (r.second % vec_of<T>()))) return false;
+    return true;
+}
+bool kept_ok(const Act8View& k) { return ((uintptr_t)k.q % 16) == 0 && (k.ldq % 16) == 0; }
+
+template <typename T, int VEC, int NV>
+int launch_fwd(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep,
+               int64_t rows, int d, float eps, int tpr, cudaStream_t s) {
+    // two rows' worth of warps per CTA at least, four warps: small CTAs so that a wave's end leaves no SM waiting long
+    const int threads = std::max(tpr, 128);
+    const int64_t grid = (rows + threads / tpr - 1) / (threads / tpr);
+    if (grid > 0x7FFFFFFF) return -2;
+    if (keep.q != nullptr)
+        layer_norm_fwd_kernel<T, VEC, NV, true><<<(unsigned)grid, threads, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, (int8_t*)keep.q, keep.ldq,
+                                                                                  (uint8_t*)keep.e, keep.lde, rows, d, eps, tpr);
+    else
+        layer_norm_fwd_kernel<T, VEC, NV, false><<<(unsigned)grid, threads, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, nullptr, 0, nullptr, 0,
+                                                                                   rows, d, eps, tpr);
+    return (int)cudaGetLastError();
+}
+
+template <typename T, int VEC>
+int fwd_vec(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep, int64_t rows,
+            int d, float eps, cudaStream_t s) {
+    constexpr int NV = VEC == 1 ? 16 : 8;
+    const int64_t vecs = (d + VEC - 1) / VEC;
+    // fewer rows than SMs x 4: one vector per thread if 512 threads have the row
+    if (rows <= 4 * kSms && vecs <= kMaxTeam)
+        return launch_fwd<T, VEC, 1>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, pow2_at_least(vecs, 32, kMaxTeam), s);
+    if (vecs <= 64) return launch_fwd<T, VEC, 2>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, 32, s);
+    if (vecs <= (int64_t)kMaxTeam * NV)
+        return launch_fwd<T, VEC, NV>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, pow2_at_least((vecs + NV - 1) / NV, 32, kMaxTeam), s);
+    if (rows > 0x7FFFFFFF) return -2;
+    if (keep.q != nullptr)
+        layer_norm_fwd_long_kernel<T, true><<<(unsigned)rows, 512, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, (int8_t*)keep.q, keep.ldq,
+                                                                          (uint8_t*)keep.e, keep.lde, d, eps);
+    else
+        layer_norm_fwd_long_kernel<T, false><<<(unsigned)rows, 512, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, nullptr, 0, nullptr, 0, d, eps);
+    return (int)cudaGetLastError();
+}
+
+template <typename T>
+int fwd_typed(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep, int64_t rows,
+              int64_t d, float eps, cudaStream_t s) {
+    constexpr int V = vec_of<T>();
+    if (aligned<T>(d, {{x, ldx}, {y, ldy}, {w, 0}, {b, 0}}) && (keep.q == nullptr || kept_ok(keep)))
+        return fwd_vec<T, V>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, (int)d, eps, s);
+    return fwd_vec<T, 1>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, (int)d, eps, s);
+}
+
+struct BwdPlan {
+    bool fits;     // the row fits one team's registers
+    int tpr, threads, grid;
+};
+BwdPlan bwd_plan(int64_t rows, int64_t d) {
+    BwdPlan p;
+    p.fits = d <= (int64_t)kBwdThreads * kBwdElems;
+    p.tpr = pow2_at_least((d + kBwdElems - 1) / kBwdElems, 32, kBwdThreads);
+    // few rows: one team per CTA until every SM has one
+    const int teams = (int)std::max<int64_t>(1, std::min<int64_t>(kBwdThreads / p.tpr, (rows + 2 * kSms - 1) / (2 * kSms)));
+    p.threads = p.tpr * pow2_at_least(teams, 1, kBwdThreads / p.tpr);
+    const int64_t need = (rows + p.threads / p.tpr - 1) / (p.threads / p.tpr);
+    p.grid = p.fits ? (int)std::max<int64_t>(1, std::min<int64_t>(kSms, need))
+                    : (int)std::max<int64_t>(1, std::min<int64_t>(64, (rows + 63) / 64));
+    return p;
+}
+
+int reduce_partials(const float* partial, int n, int64_t width, int64_t split, float* out0, float* out1, int accumulate, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((width + 31) / 32));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute a[1];
+    a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = a;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, column_reduce_kernel, partial, n, width, split, out0, out1, accumulate);
+}
+
+template <typename T, int VEC, bool SRC8>
+int launch_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View& k, const T* w, const float* mean, const float* rstd,
+               const T* join, int64_t ldjoin, T* dx, int64_t lddx, float* partial, int64_t rows, int d, const BwdPlan& p, cudaStream_t s) {
+    const size_t smem = p.threads > p.tpr ? (size_t)2 * d * sizeof(float) : 0;   // at most 32 KB: several teams means d <= 4096
+    layer_norm_bwd_kernel<T, VEC, SRC8><<<p.grid, p.threads, smem, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, w,
+                                                                        mean, rstd, join, ldjoin, dx, lddx, partial, rows, d, p.tpr);
+    return (int)cudaGetLastError();
+}
+
+template <typename T, bool SRC8>
+int bwd_typed(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View& k, const T* w, const float* mean, const float* rstd,
+              const T* join, int64_t ldjoin, T* dx, int64_t lddx, float* dweight, float* dbias, int accumulate, float* partial, int64_t rows,
+              int64_t d, cudaStream_t s) {
+    const BwdPlan p = bwd_plan(rows, d);
+    const bool want = dweight != nullptr || dbias != nullptr;
+    float* part = want ? partial : nullptr;
+    int rc;
+    if (p.fits) {
+        const bool vec = aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}) && (!SRC8 || kept_ok(k));
+        rc = vec ? launch_bwd<T, vec_of<T>(), SRC8>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s)
+                 : launch_bwd<T, 1, SRC8>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s);
+    } else {
+        if (rows > 0x7FFFFFFF) return -2;
+        layer_norm_bwd_long_kernel<T, SRC8><<<(unsigned)rows, 512, 0, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde,
+                                                                          w, mean, rstd, join, ldjoin, dx, lddx, (int)d);
+        rc = (int)cudaGetLastError();
+        if (rc == 0 && want) {
+            layer_norm_dw_long_kernel<T, SRC8><<<dim3((unsigned)((d + 255) / 256), p.grid), 256, 0, s>>>(
+                dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, mean, rstd, part, rows, (int)d);
+            rc = (int)cudaGetLastError();
+        }
+    }
+    if (rc != 0 || !want) return rc;
+    return reduce_partials(part, p.grid, 2 * d, d, dweight, dbias, accumulate, s);
+}
+
+int column_slabs(int64_t rows, int64_t cols) {
+    const int64_t gx = (cols + 127) / 128;
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 63) / 64, (kSms * 8 + gx - 1) / gx));
+}
+
+constexpr int64_t kMaxCols = 1 << 30;   // column indices are 32-bit
+
+}  // namespace
+
+int layer_norm_fwd(int dtype, const void* x, int64_t ldx, const void* weight, const void* bias, void* y, int64_t ldy, float* mean,
+                   float* rstd, const Act8View& keep, int64_t rows, int64_t d, float eps, void* stream) {
+    if (rows <= 0 || d <= 0) return 0;
+    if (d > kMaxCols) return -2;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == 0)
+        return fwd_typed<__nv_bfloat16>((const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)weight, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y,
+                                        ldy, mean, rstd, keep, rows, d, eps, s);
+    if (dtype == 1)
+        return fwd_typed<float>((const float*)x, ldx, (const float*)weight, (const float*)bias, (float*)y, ldy, mean, rstd, keep, rows, d, eps, s);
+    return -2;
+}
+
+int64_t layer_norm_bwd_scratch(int64_t rows, int64_t d) { return (int64_t)bwd_plan(rows, d).grid * 2 * d; }
+
+int layer_norm_bwd(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const Act8View& kept, const void* weight,
+                   const float* mean, const float* rstd, const void* join, int64_t ldjoin, void* dx, int64_t lddx, float* dweight,
+                   float* dbias, int accumulate, float* partial, int64_t rows, int64_t d, void* stream) {
+    cudaStream_t s = (cudaStream_t)stream;
+    if (d <= 0) return 0;
+    if (d > kMaxCols) return -2;
+    if (rows <= 0) {   // sums over no rows
+        cudaError_t rc = cudaSuccess;
+        if (!accumulate && dweight != nullptr) rc = cudaMemsetAsync(dweight, 0, (size_t)d * 4, s);
+        if (rc == cudaSuccess && !accumulate && dbias != nullptr) rc = cudaMemsetAsync(dbias, 0, (size_t)d * 4, s);
+        return (int)rc;
+    }
+#define PSB_BWD(T, SRC8)                                                                                                              \
+    bwd_typed<T, SRC8>((const T*)dy, lddy, (const T*)x, ldx, kept, (const T*)weight, mean, rstd, (const T*)join, ldjoin, (T*)dx, lddx, dweight, \
+                       dbias, accumulate, partial, rows, d, s)
+    if (dtype == 0) return kept.q != nullptr ? PSB_BWD(__nv_bfloat16, true) : PSB_BWD(__nv_bfloat16, false);
+    if (dtype == 1) return kept.q != nullptr ? PSB_BWD(float, true) : PSB_BWD(float, false);
+#undef PSB_BWD
+    return -2;
+}
+
+namespace {
+template <typename T, int VEC, int U, bool PACK>
+int launch_act8(void* x, int64_t ldx, const Act8View& k, int64_t rows, int64_t cols, cudaStream_t s) {
+    const int64_t per_row = (cols + 32 * VEC * U - 1) / (32 * VEC * U);
+    const int64_t grid = (rows * per_row + 7) / 8;
+    if (grid > 0x7FFFFFFF) return -2;
+    if (PACK)
+        act8_pack_kernel<T, VEC, U><<<(unsigned)grid, 256, 0, s>>>((const T*)x, ldx, (int8_t*)k.q, k.ldq, (uint8_t*)k.e, k.lde, rows, cols, per_row);
+    else
+        act8_unpack_kernel<T, VEC, U><<<(unsigned)grid, 256, 0, s>>>((const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, (T*)x, ldx, rows, cols,
+                                                                    per_row);
+    return (int)cudaGetLastError();
+}
+template <typename T, bool PACK>
+int act8_typed(void* x, int64_t ldx, const Act8View& k, int64_t rows, int64_t cols, cudaStream_t s) {
+    constexpr int V = vec_of<T>();
+    if (aligned<T>(cols, {{x, ldx}}) && kept_ok(k))
+        return cols > 32 * V ? launch_act8<T, V, 4, PACK>(x, ldx, k, rows, cols, s) : launch_act8<T, V, 1, PACK>(x, ldx, k, rows, cols, s);
+    return launch_act8<T, 1, 4, PACK>(x, ldx, k, rows, cols, s);
+}
+}  // namespace
+
+int act8_pack(int dtype, const void* x, int64_t ldx, const Act8View& out, int64_t rows, int64_t cols, void* stream) {
+    if (rows <= 0 || cols <= 0) return 0;
+    if (dtype == 0) return act8_typed<__nv_bfloat16, true>((void*)x, ldx, out, rows, cols, (cudaStream_t)stream);
+    if (dtype == 1) return act8_typed<float, true>((void*)x, ldx, out, rows, cols, (cudaStream_t)stream);
+    return -2;
+}
+int act8_unpack(int dtype, const Act8View& in, void* x, int64_t ldx, int64_t rows, int64_t cols, void* stream) {
+    if (rows <= 0 || cols <= 0) return 0;
+    if (dtype == 0) return act8_typed<__nv_bfloat16, false>(x, ldx, in, rows, cols, (cudaStream_t)stream);
+    if (dtype == 1) return act8_typed<float, false>(x, ldx, in, rows, cols, (cudaStream_t)stream);
+    return -2;
+}
+
+int64_t column_sum_scratch(int64_t rows, int64_t cols) { return (int64_t)column_slabs(rows, cols) * cols; }
+
+namespace {
+template <typename T>
+int column_sum_typed(const T* x, int64_t ldx, int64_t rows, int64_t cols, float* out, int accumulate, float* partial, cudaStream_t s) {
+    const int slabs = column_slabs(rows, cols);
+    const int64_t gx = (cols + 127) / 128;
+    if (gx > 0x7FFFFFFF) return -2;
+    dim3 grid((unsigned)gx, (unsigned)slabs);
+    if (aligned<T>(cols, {{x, ldx}})) column_sum_kernel<T, vec_of<T>()><<<grid, 256, 0, s>>>(x, ldx, rows, cols, partial);
+    else column_sum_kernel<T, 1><<<grid, 256, 0, s>>>(x, ldx, rows, cols, partial);
+    const int rc = (int)cudaGetLastError();
+    return rc != 0 ? rc : reduce_partials(partial, slabs, cols, cols, out, nullptr, accumulate, s);
+}
+}  // namespace
+
+int column_sum(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, float* out, int accumulate, float* partial, void* stream) {
+    cudaStream_t s = (cudaStream_t)stream;
+    if (cols <= 0) return 0;
+    if (rows <= 0) return accumulate ? 0 : (int)cudaMemsetAsync(out, 0, (size_t)cols * 4, s);
+    if (dtype == 0) return column_sum_typed<__nv_bfloat16>((const __nv_bfloat16*)x, ldx, rows, cols, out, accumulate, partial, s);
+    if (dtype == 1) return column_sum_typed<float>((const float*)x, ldx, rows, cols, out, accumulate, partial, s);
+    return -2;
+}
+
+}  // namespace psb
