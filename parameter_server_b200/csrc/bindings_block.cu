@@ -1,6 +1,7 @@
 // Bindings of the decoder-block operators: layer norm, fused linear layers, 8-bit activation checkpoints.
 #include <pybind11/pybind11.h>
 
+#include "kernels/linear_fused.h"
 #include "kernels/norm.h"
 
 namespace py = pybind11;
@@ -35,4 +36,39 @@ void bind_block(py::module_& m) {
         return column_sum(dtype, (const void*)x, ldx, rows, cols, (float*)out, accumulate ? 1 : 0, (float*)partial, (void*)s);
     });
     m.def("column_sum_scratch", &column_sum_scratch);
+    m.def("linear_fused", [](bool dgrad, int act, int M, int N, int K, uintptr_t a, int64_t lda, uintptr_t w, int64_t ldw, uintptr_t bias,
+                             bool bias_f32, uintptr_t residual, int64_t ldres, uintptr_t out, int64_t ldo, uintptr_t out2, int64_t ldo2,
+                             uintptr_t pre, int64_t ldpre, uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde, uintptr_t workspace,
+                             uintptr_t err_flag, double wait_limit_s, uintptr_t s) {
+        LinearArgs x;
+        x.dgrad = dgrad ? 1 : 0;
+        x.act = act;
+        x.M = M;
+        x.N = N;
+        x.K = K;
+        x.a = (const void*)a;
+        x.lda = lda;
+        x.w = (const void*)w;
+        x.ldw = ldw;
+        x.bias = (const void*)bias;
+        x.bias_f32 = bias_f32 ? 1 : 0;
+        x.residual = (const void*)residual;
+        x.ldres = ldres;
+        x.out = (void*)out;
+        x.ldo = ldo;
+        x.out2 = (void*)out2;
+        x.ldo2 = ldo2;
+        x.pre = (void*)pre;
+        x.ldpre = ldpre;
+        x.q = (void*)q;
+        x.ldq = ldq;
+        x.e = (void*)e;
+        x.lde = lde;
+        x.workspace = (void*)workspace;
+        x.err_flag = (unsigned*)err_flag;
+        x.wait_limit_s = wait_limit_s;
+        return linear_fused(x, (void*)s);
+    });
+    m.def("linear_workspace_bytes", &linear_workspace_bytes);
+    m.def("linear_workspace_zeros", &linear_workspace_zeros);
 }

@@ -1,0 +1,627 @@
+// Linear layers of a decoder block on the 5th-generation tensor cores, with their neighbours in the epilogue:
+//
+//   forward   h = x w^T + b,   y = act(h) + residual,   h kept for the backward pass in bf16 or in 8 bits
+//   dgrad     dh = (dy w) * act'(h),   and act(h) again, for the weight gradient of the layer that dy belongs to
+//
+// bf16 operands, fp32 accumulation in TMEM; everything in the epilogue is fp32 and rounded once per output. Fusing the
+// neighbours saves their passes over M x N values through HBM; the product itself is bound by the tensor cores and by the
+// operand feed from L2 (see the tile shape below).
+//
+// One persistent launch of CTA pairs (cta_group::2), one pair per two SMs. A pair works on a 256 x BN tile: each CTA loads
+// its 128 rows of A and half of the B tile per k-step of 64 (32 KB for 512 cycles of MMA, which is what an SM's port to L2
+// delivers; a single-CTA tile would need half as much again), the leader issues the MMAs for both, and each CTA drains its
+// own 128 rows. Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-9 epilogue (a warp has one 32-lane quarter of TMEM
+// and half of the tile's columns). The accumulator is double-buffered in TMEM, so the epilogue of a tile runs beside the
+// MMAs of the next. Tiles are dealt out as tile_walk.cuh says. Every wait is bounded; on a time-out the CTA records where,
+// frees its TMEM and returns.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "act8.cuh"
+#include "gemm_tcgen05.h"
+#include "linear_fused.h"
+#include "tcgen05.cuh"
+#include "tile_walk.cuh"
+
+namespace psb {
+
+namespace {
+
+constexpr int kLinEpilogueWarps = 8;
+constexpr int kLinThreads = 32 * (2 + kLinEpilogueWarps);
+
+template <int BN>
+struct LinSmem {
+    static constexpr int kABytes = BM * BK * 2;
+    static constexpr int kBBytes = BN / 2 * BK * 2;          // a CTA of a pair holds half of the B tile
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kTileBytes = kStages * kStageBytes;
+    static constexpr int kBarBytes = 256;
+    static constexpr int kBiasBytes = 2 * BN * 4;            // double-buffered with the accumulator
+    static constexpr int kOutBytes = kLinEpilogueWarps * 2048;   // a warp's [32 rows][64 bytes] on the way out
+    static constexpr int kTotal = kTileBytes + kBarBytes + kBiasBytes + kOutBytes + 1024;   // + alignment slack
+};
+
+struct LinParams {
+    CUtensorMap map_a, map_b;
+    TileGrid grid;
+    int M, N;
+    int b_blocked;                    // MN-major B comes in with one 3-D load per stage
+    const __nv_bfloat16* bias;
+    const float* bias32;
+    const __nv_bfloat16* res;
+    int64_t ldres;
+    __nv_bfloat16* out;
+    int64_t ldo;
+    __nv_bfloat16* out2;
+    int64_t ldo2;
+    __nv_bfloat16* pre;
+    int64_t ldpre;
+    int8_t* q;
+    int64_t ldq;
+    uint8_t* e;
+    int64_t lde;
+    int aux_vec, pre_vec, out_vec, out2_vec;   // rows of residual (forward) / pre / out / out2 are 16-byte aligned
+    float* partial;                   // shared tiles: [pair][2 places][cta][warp][BN / 64 pieces][8][32 lanes][4]
+    unsigned* arrived;                // [shared tile][cta][warp]
+    unsigned* err_flag;
+    unsigned long long limit_ns;
+};
+
+// ---- activations -----------------------------------------------------------------------------------------------------
+// gelu_tanh(h) = h / 2 * (1 + tanh(u)) = h * s(2u) with s(z) = 1 / (1 + exp(-z)) and u = sqrt(2/pi) (h + 0.044715 h^3): no
+// cancellation in the tails, two special-function operations per value.
+constexpr float kGeluC = 1.5957691216057308f;             // 2 sqrt(2 / pi)
+constexpr float kGeluC3 = 1.5957691216057308f * 0.044715f;
+
+__device__ __forceinline__ float sigmoidf_fast(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float h) {
+    if constexpr (ACT == kActRelu) return h > 0.f ? h : (h != h ? h : 0.f);
+    if constexpr (ACT == kActGelu) return 0.5f * h * (1.f + erff(h * 0.70710678118654752f));
+    if constexpr (ACT == kActGeluTanh) return __fdividef(h, 1.f + __expf(-h * (kGeluC + kGeluC3 * h * h)));
+    if constexpr (ACT == kActSilu) return __fdividef(h, 1.f + __expf(-h));
+    return h;
+}
+// act(h) and act'(h). The slope of the saturating tails is taken at |h| <= 20, where it has long reached 0 or 1: the
+// products below would meet infinity * 0 further out.
+template <int ACT>
+__device__ __forceinline__ float act_slope(float h, float* value) {
+    if constexpr (ACT == kActRelu) {
+        *value = act_of<kActRelu>(h);
+        return h > 0.f ? 1.f : (h != h ? h : 0.f);
+    }
+    if constexpr (ACT == kActGelu) {
+        const float cdf = 0.5f * (1.f + erff(h * 0.70710678118654752f));
+        *value = h * cdf;
+        const float c = fminf(fmaxf(h, -20.f), 20.f);
+        return cdf + c * 0.3989422804014327f * __expf(-0.5f * c * c);
+    }
+    if constexpr (ACT == kActGeluTanh || ACT == kActSilu) {
+        const float c = fminf(fmaxf(h, -20.f), 20.f);
+        const float h2 = c * c;
+        const float z = ACT == kActSilu ? c : c * (kGeluC + kGeluC3 * h2);
+        const float dz = ACT == kActSilu ? 1.f : kGeluC + 3.f * kGeluC3 * h2;
+        const float s = sigmoidf_fast(z);
+        *value = h * s;
+        return (s + c * dz * s * (1.f - s)) + (h - h);   // NaN and infinity stay what they are
+    }
+    *value = h;
+    return 1.f;
+}
+
+// ---- epilogue: memory side -------------------------------------------------------------------------------------------
+// 32 values of a bf16 row (64 bytes) that may be unaligned or cut off by the tensor's edge: out of line, rarely taken.
+__device__ __noinline__ void load32_slow(const __nv_bfloat16* p, int n, uint32_t* w) {
+    for (int j = 0; j < 16; ++j) {
+        uint32_t lo = 2 * j < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j]) : 0u;
+        uint32_t hi = 2 * j + 1 < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j + 1]) : 0u;
+        w[j] = lo | (hi << 16);
+    }
+}
+__device__ __forceinline__ void load32(const __nv_bfloat16* p, int n, bool vec, uint4* raw) {
+    if (vec && n >= 32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw[j] = ld_nc_v4(p + 8 * j);
+    } else {
+        uint32_t w[16];
+        load32_slow(p, n, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    }
+}
+__device__ __forceinline__ float bf16_at(const uint4* raw, int j) {   // j is a constant after unrolling
+    const uint4 v = raw[j / 8];
+    const uint32_t w = (j / 2) % 4 == 0 ? v.x : (j / 2) % 4 == 1 ? v.y : (j / 2) % 4 == 2 ? v.z : v.w;
+    return __uint_as_float((j & 1) ? (w & 0xFFFF0000u) : (w << 16));
+}
+// A warp's [32 rows][32 columns] of bf16 results, one row per lane, through the warp's 2 KB of shared memory so that every
+// store instruction writes 8 whole 64-byte row segments instead of 16 bytes in each of 32 rows. The 16-byte blocks of a row
+// are XOR-swizzled by (row / 2) % 4: neither side has bank conflicts.
+__device__ __forceinline__ void store_piece(uint8_t* stage, int lane, const float* f, __nv_bfloat16* out, int64_t ldo, int row0, int col0, int M,
+                                            int N, bool vec) {
+    uint4 raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        __nv_bfloat162* h = (__nv_bfloat162*)&raw[j];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) h[t] = __floats2bfloat162_rn(f[8 * j + 2 * t], f[8 * j + 2 * t + 1]);
+    }
+    __syncwarp();   // the reads of the piece before are done
+    uint8_t* mine = stage + lane * 64;
+    const int sw = (lane >> 1) & 3;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *(uint4*)(mine + ((j ^ sw) << 4)) = raw[j];
+    __syncwarp();
+    const int cb = lane & 3, col = col0 + cb * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        const uint4 d = *(const uint4*)(stage + r * 64 + ((cb ^ ((r >> 1) & 3)) << 4));
+        if (row0 + r < M) {
+            __nv_bfloat16* op = out + (int64_t)(row0 + r) * ldo + col;
+            if (vec && col + 8 <= N) {
+                *(uint4*)op = d;
+            } else {
+                const __nv_bfloat16* h = (const __nv_bfloat16*)&d;
+                for (int t = 0; t < 8; ++t)
+                    if (col + t < N) op[t] = h[t];
+            }
+        }
+    }
+}
+// 32 values of this lane's row into the 8-bit checkpoint; returns the exponent. (Columns past N carry zeros here, and the
+// padding of a row takes them.)
+__device__ __forceinline__ uint32_t keep_row32(const float* f, int8_t* qp, int n, bool live) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m = max(m, abs_bits(f[j]));
+    const uint32_t e = act8_exponent(m);
+    const float inv = act8_inverse_step(e);
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        w[j] = pack_s8x4(act8_quantise(f[4 * j], inv), act8_quantise(f[4 * j + 1], inv), act8_quantise(f[4 * j + 2], inv),
+                         act8_quantise(f[4 * j + 3], inv));
+    if (live) {
+        *(uint4*)qp = make_uint4(w[0], w[1], w[2], w[3]);
+        if (n > 16) *(uint4*)(qp + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    return e;
+}
+
+// ---- the kernel ------------------------------------------------------------------------------------------------------
+template <bool DGRAD, int ACT, int BN>
+__global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __grid_constant__ LinParams p) {
+    using L = LinSmem<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full_bar = (uint64_t*)(smem + L::kTileBytes);
+    uint64_t* empty_bar = full_bar + L::kStages;
+    uint64_t* tfull_bar = empty_bar + L::kStages;   // [2] accumulator complete
+    uint64_t* tempty_bar = tfull_bar + 2;           // [2] accumulator drained
+    uint32_t* tmem_slot = (uint32_t*)(tempty_bar + 2);
+    float* bias_smem = (float*)(smem + L::kTileBytes + L::kBarBytes);
+    uint8_t* stage_out = smem + L::kTileBytes + L::kBarBytes + L::kBiasBytes;
+
+    const int cr = (int)cluster_ctarank();
+    const bool leader = cr == 0;
+    const int pair = (int)blockIdx.x / 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned long long limit_ns = p.limit_ns;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull_bar[b], 1);
+            mbar_init(&tempty_bar[b], 2 * kLinEpilogueWarps);   // the epilogue warps of both CTAs
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * BN))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();   // the peer's barriers must exist before anything is signalled on them
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
+
+    if (warp == 0) {
+        // ---- TMA producer ----
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_b) : "memory");
+            TileWalk walk(p.grid, pair);
+            Tile t;
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && walk.next(p.grid, t)) {
+                const int m0 = t.m * 2 * BM + cr * BM, n0 = t.n * BN + cr * (BN / 2);
+                for (int k = 0; k < t.nk; ++k, ++it) {
+                    const int s = it % L::kStages;
+                    if (!mbar_wait(&empty_bar[s], ((it / L::kStages) & 1u) ^ 1u, limit_ns)) {
+                        atomicCAS(p.err_flag, 0u, 21u);
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sa = smem + s * L::kStageBytes;
+                    uint8_t* sb = sa + L::kABytes;
+                    const int k0 = (t.k0 + k) * BK;
+                    if (leader) mbar_expect_tx(&full_bar[s], 2u * (uint32_t)L::kStageBytes);   // both CTAs' bytes
+                    const uint32_t fb = mapa_cluster(smem_u32(&full_bar[s]), 0);
+                    tma_load_2d_pair(sa, &p.map_a, fb, k0, m0);   // [128 rows][64 k]
+                    if constexpr (!DGRAD) {
+                        tma_load_2d_pair(sb, &p.map_b, fb, k0, n0);   // [BN / 2 rows][64 k]
+                    } else if (p.b_blocked) {
+                        tma_load_3d_pair(sb, &p.map_b, fb, 0, k0, n0 / 64);   // [BN / 128 blocks][64 k][64 n]
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < BN / 128; ++j) tma_load_2d_pair(sb + j * 64 * 128, &p.map_b, fb, n0 + 64 * j, k0);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer ----
+        if (lane == 0 && leader) {
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                                   ((uint32_t)((2 * BM) >> 4) << 24);
+            TileWalk walk(p.grid, pair);
+            Tile t;
+            uint32_t it = 0, tc = 0;
+            bool ok = true;
+            while (ok && walk.next(p.grid, t)) {
+                const uint32_t buf = tc & 1u;
+                if (!mbar_wait(&tempty_bar[buf], ((tc >> 1) & 1u) ^ 1u, limit_ns)) {
+                    atomicCAS(p.err_flag, 0u, 24u);
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t tmem_d = tmem_base + buf * (uint32_t)BN;
+                for (int k = 0; k < t.nk; ++k, ++it) {
+                    const int s = it % L::kStages;
+                    // consumers wait longer than producers, so that the wait that reports is the one at the root
+                    if (!mbar_wait(&full_bar[s], (it / L::kStages) & 1u, limit_ns * 2)) {
+                        atomicCAS(p.err_flag, 0u, 22u);
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t sa = smem_u32(smem + s * L::kStageBytes);
+                    const uint32_t sb = sa + L::kABytes;
+#pragma unroll
+                    for (int u = 0; u < BK / UMMA_K; ++u) {
+                        // K-major: 8-row groups 1024 B apart, 16 k are 32 B inside the swizzle span; MN-major: 64-column
+                        // blocks 8192 B apart, 16 k-rows are 2048 B
+                        const uint64_t da = make_desc(sa + u * 32, 16, 1024);
+                        const uint64_t db = DGRAD ? make_desc(sb + u * 2048, 8192, 1024) : make_desc(sb + u * 32, 16, 1024);
+                        umma_bf16_pair(tmem_d, da, db, idesc, (k | u) ? 1u : 0u);
+                    }
+                    umma_commit_pair(&empty_bar[s]);   // frees the stage in both CTAs when these MMAs have read it
+                }
+                umma_commit_pair(&tfull_bar[buf]);     // (also on error, so that the epilogue moves on)
+                ++tc;
+            }
+        }
+    } else {
+        // ---- epilogue ----
+        const int ew = warp - 2, quarter = warp & 3, half = ew >> 2, etid = ew * 32 + lane;
+        constexpr int kPieces = BN / 64;   // 32-column pieces of a warp
+        uint8_t* stage = stage_out + ew * 2048;
+        TileWalk walk(p.grid, pair);
+        Tile t;
+        uint32_t tc = 0;
+        while (walk.next(p.grid, t)) {
+            const uint32_t buf = tc & 1u;
+            const int tile_n = t.n * BN, row0 = t.m * 2 * BM + cr * BM + quarter * 32, row = row0 + lane;
+            const int cbase = half * (BN / 2), colw = tile_n + cbase;   // first column of this warp
+            const bool live = row < p.M;
+            float* bs = bias_smem + buf * BN;
+            if constexpr (!DGRAD) {
+                if (etid < BN) {   // (BN = 128: the first four warps)
+                    const int col = tile_n + etid;
+                    float v = 0.f;
+                    if (col < p.N) v = p.bias32 != nullptr ? p.bias32[col] : p.bias != nullptr ? __bfloat162float(p.bias[col]) : 0.f;
+                    bs[etid] = v;
+                }
+            }
+            // What a piece needs from memory (residual, or h) is requested one piece ahead, the first one before the wait
+            // for the accumulator.
+            uint4 aux[4];
+            uint32_t ex = 0;
+            const __nv_bfloat16* aux_row = DGRAD ? p.pre : p.res;
+            const int64_t aux_ld = DGRAD ? p.ldpre : p.ldres;
+            const bool aux_vec = DGRAD ? p.pre_vec != 0 : p.aux_vec != 0;
+            const bool kept8 = DGRAD && p.q != nullptr;
+            auto fetch = [&](int c) {
+                const int col = colw + c * 32;
+                if (!live || col >= p.N) return;
+                if (kept8) {
+                    const int8_t* qp = p.q + (int64_t)row * p.ldq + col;
+                    aux[0] = ld_nc_v4(qp);
+                    if (col + 16 < p.N) aux[1] = ld_nc_v4(qp + 16);
+                } else if (aux_row != nullptr) {
+                    load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, aux_vec, aux);
+                }
+            };
+#pragma unroll
+            for (int j = 0; j < 4; ++j) aux[j] = make_uint4(0, 0, 0, 0);
+            if (t.runs == 1) fetch(0);
+            if (kept8 && live && colw < p.N) {   // one byte per piece; rows of e are padded to 16
+                if constexpr (kPieces == 4) ex = *(const uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32);
+                else ex = *(const uint16_t*)(p.e + (int64_t)row * p.lde + colw / 32);
+            }
+            const bool waited = mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // one barrier of the epilogue warps per tile: publishes the bias, and makes the decision to give up uniform
+            uint32_t all_ok;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\t"
+                "setp.ne.u32 q, %1, 0;\n\t"
+                "bar.red.and.pred p, 1, %2, q;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(all_ok)
+                : "r"(waited ? 1u : 0u), "r"(32 * kLinEpilogueWarps)
+                : "memory");
+            if (!all_ok) {
+                if (!waited && lane == 0) atomicCAS(p.err_flag, 0u, 23u);
+                break;
+            }
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)BN + (uint32_t)cbase;
+            auto release = [&]() {   // this warp has read the accumulator
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
+            };
+            // one 32-column piece with its values in f
+            uint32_t ewrite = 0;
+            auto finish = [&](float* f, int c) {
+                const int col = colw + c * 32;
+                if constexpr (!DGRAD) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 b = *(const float4*)(bs + cbase + c * 32 + j);
+                        f[j] += b.x; f[j + 1] += b.y; f[j + 2] += b.z; f[j + 3] += b.w;
+                    }
+                    if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_vec != 0);
+                    if (p.q != nullptr) ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]);
+                    if (p.res != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] += bf16_at(aux, j);
+                    }
+                    if (c + 1 < kPieces) fetch(c + 1);
+                } else {
+                    float a[32];
+                    const float step = act8_step((ex >> (8 * c)) & 255u);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float h;
+                        if (kept8) {
+                            const uint4 v = aux[j / 16];
+                            const uint32_t w = (j / 4) % 4 == 0 ? v.x : (j / 4) % 4 == 1 ? v.y : (j / 4) % 4 == 2 ? v.z : v.w;
+                            h = s8_at(w, j % 4) * step;
+                        } else {
+                            h = bf16_at(aux, j);
+                        }
+                        f[j] *= act_slope<ACT>(h, &a[j]);
+                    }
+                    if (c + 1 < kPieces) fetch(c + 1);
+                    if (p.out2 != nullptr) store_piece(stage, lane, a, p.out2, p.ldo2, row0, col, p.M, p.N, p.out2_vec != 0);
+                }
+                store_piece(stage, lane, f, p.out, p.ldo, row0, col, p.M, p.N, p.out_vec != 0);
+            };
+            uint32_t v[32];
+            if (t.runs == 1) {
+                if (colw < p.N) tmem_ld32_issue(taddr, v);
+#pragma unroll 1
+                for (int c = 0; c < kPieces; ++c) {
+                    if (colw + c * 32 >= p.N) break;   // warp-uniform
+                    tmem_wait_ld(v);
+                    float f[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                    if (c + 1 < kPieces && colw + c * 32 + 32 < p.N) tmem_ld32_issue(taddr + (uint32_t)(c + 1) * 32u, v);
+                    finish(f, c);
+                }
+                release();
+            } else {
+                // shared tile: this pair's part goes to memory; the last one to arrive adds all parts in run order
+                constexpr int64_t kWarpFloats = kPieces * 1024;
+                auto part_of = [&](int worker, int slot) {
+                    return p.partial + ((((int64_t)worker * 2 + slot) * 2 + cr) * kLinEpilogueWarps + ew) * kWarpFloats + lane * 4;
+                };
+                float* mine = part_of(pair, t.slot);
+#pragma unroll 1
+                for (int c = 0; c < kPieces; ++c) {
+                    if (colw + c * 32 >= p.N) break;
+                    tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
+                    tmem_wait_ld(v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *(uint4*)(mine + c * 1024 + j * 128) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                }
+                release();
+                __threadfence();
+                __syncwarp();
+                unsigned last = 0;
+                unsigned* count = p.arrived + ((int64_t)t.index * 2 + cr) * kLinEpilogueWarps + ew;
+                if (lane == 0) last = atomicAdd(count, 1u) == (unsigned)(t.runs - 1) ? 1u : 0u;
+                if (__shfl_sync(0xFFFFFFFFu, last, 0) != 0u) {
+                    __threadfence();
+                    if (lane == 0) *count = 0u;   // at rest for the next launch
+                    fetch(0);
+#pragma unroll 1
+                    for (int c = 0; c < kPieces; ++c) {
+                        if (colw + c * 32 >= p.N) break;
+                        float f[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] = 0.f;
+#pragma unroll 1
+                        for (int r = 0; r < t.runs; ++r) {
+                            const float* src = part_of(t.first + r, TileWalk::slot_of(p.grid, t, r)) + c * 1024;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float4 x = __ldcg((const float4*)(src + j * 128));
+                                f[4 * j] += x.x; f[4 * j + 1] += x.y; f[4 * j + 2] += x.z; f[4 * j + 3] += x.w;
+                            }
+                        }
+                        finish(f, c);
+                    }
+                } else {
+                    ++tc;
+                    continue;
+                }
+            }
+            if constexpr (!DGRAD) {
+                if (p.q != nullptr && live && colw < p.N) {
+                    if constexpr (kPieces == 4) *(uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32) = ewrite;
+                    else *(uint16_t*)(p.e + (int64_t)row * p.lde + colw / 32) = (uint16_t)ewrite;
+                }
+            }
+            ++tc;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();   // until here the peer may signal this CTA's barriers or read its shared memory
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * BN)) : "memory");
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+constexpr int64_t kArrivedWords = (int64_t)kMaxPairs * 2 * kLinEpilogueWarps;
+constexpr int64_t kPartialFloats = (int64_t)kMaxPairs * 2 * 2 * kLinEpilogueWarps * 4 * 1024;
+
+// How many CTA pairs of this kernel the device holds at once, within gemm_set_cta_limit().
+template <auto kern>
+cudaError_t pairs_of(int threads, int smem, int* pairs) {
+    static int cached[64] = {};   // per kernel and device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    int n = dev >= 0 && dev < 64 ? cached[dev] : 0;
+    if (n == 0) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t q = {};
+        q.gridDim = dim3(2);
+        q.blockDim = dim3(threads);
+        q.dynamicSmemBytes = smem;
+        cudaLaunchAttribute a[1];
+        a[0].id = cudaLaunchAttributeClusterDimension;
+        a[0].val.clusterDim.x = 2;
+        a[0].val.clusterDim.y = 1;
+        a[0].val.clusterDim.z = 1;
+        q.attrs = a;
+        q.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&n, kern, &q);
+        if (e != cudaSuccess) return e;
+        if (n <= 0) return cudaErrorLaunchOutOfResources;
+        if (dev >= 0 && dev < 64) cached[dev] = n;
+    }
+    if (gemm_cta_limit() > 0) n = std::min(n, std::max(1, gemm_cta_limit() / 2));
+    *pairs = std::min(n, kMaxPairs);
+    return cudaSuccess;
+}
+template <typename Kernel, typename Params>
+cudaError_t launch_pairs(Kernel kern, int threads, int smem, int pairs, const Params& p, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * pairs);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute a[1];
+    a[0].id = cudaLaunchAttributeClusterDimension;
+    a[0].val.clusterDim.x = 2;
+    a[0].val.clusterDim.y = 1;
+    a[0].val.clusterDim.z = 1;
+    cfg.attrs = a;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+template <bool DGRAD, int ACT, int BN>
+int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
+    constexpr auto kern = linear_fused_kernel<DGRAD, ACT, BN>;
+    int pairs = 0;
+    cudaError_t e = pairs_of<kern>(kLinThreads, LinSmem<BN>::kTotal, &pairs);
+    if (e != cudaSuccess) return (int)e;
+    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 12);
+    return (int)launch_pairs(kern, kLinThreads, LinSmem<BN>::kTotal, p.grid.pairs, p, s);
+}
+
+template <bool DGRAD, int BN>
+int launch_act(int act, LinParams& p, int k_steps, cudaStream_t s) {
+    switch (act) {
+        case kActNone: return launch_linear<DGRAD, kActNone, BN>(p, k_steps, s);
+        case kActRelu: return launch_linear<DGRAD, kActRelu, BN>(p, k_steps, s);
+        case kActGelu: return launch_linear<DGRAD, kActGelu, BN>(p, k_steps, s);
+        case kActGeluTanh: return launch_linear<DGRAD, kActGeluTanh, BN>(p, k_steps, s);
+        case kActSilu: return launch_linear<DGRAD, kActSilu, BN>(p, k_steps, s);
+    }
+    return -2;
+}
+
+bool rows16(const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && (ld % 8) == 0; }
+
+template <bool DGRAD>
+int linear_typed(const LinearArgs& a, cudaStream_t s) {
+    if (!rows16(a.a, a.lda) || !rows16(a.w, a.ldw)) return -2;
+    if (a.q != nullptr && (((uintptr_t)a.q % 16) || (a.ldq % 16) || ((uintptr_t)a.e % 16) || (a.lde % 16))) return -2;
+    // tiles 128 wide only where 256 would be more than half padding: they need twice the operand bytes per flop
+    const int BN = a.N > 128 ? 256 : 128;
+    LinParams p;
+    p.M = a.M;
+    p.N = a.N;
+    p.b_blocked = DGRAD && a.N % 64 == 0 && a.N >= BN ? 1 : 0;
+    if (!make_map(&p.map_a, a.a, (uint64_t)a.M, (uint64_t)a.K, (uint64_t)a.lda, BM)) return -3;
+    const bool ok = !DGRAD ? make_map(&p.map_b, a.w, (uint64_t)a.N, (uint64_t)a.K, (uint64_t)a.ldw, BN / 2)
+                   : p.b_blocked ? make_map_blocked(&p.map_b, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, BN / 128)
+                                 : make_map(&p.map_b, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, 64);
+    if (!ok) return -3;
+    p.bias = a.bias_f32 ? nullptr : (const __nv_bfloat16*)a.bias;
+    p.bias32 = a.bias_f32 ? (const float*)a.bias : nullptr;
+    p.res = (const __nv_bfloat16*)a.residual;
+    p.ldres = a.ldres;
+    p.out = (__nv_bfloat16*)a.out;
+    p.ldo = a.ldo;
+    p.out2 = (__nv_bfloat16*)a.out2;
+    p.ldo2 = a.ldo2;
+    p.pre = (__nv_bfloat16*)a.pre;
+    p.ldpre = a.ldpre;
+    p.q = (int8_t*)a.q;
+    p.ldq = a.ldq;
+    p.e = (uint8_t*)a.e;
+    p.lde = a.lde;
+    p.aux_vec = rows16(a.residual, a.ldres);
+    p.pre_vec = rows16(a.pre, a.ldpre);
+    p.out_vec = rows16(a.out, a.ldo);
+    p.out2_vec = rows16(a.out2, a.ldo2);
+    p.arrived = (unsigned*)a.workspace;
+    p.partial = (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
+    p.err_flag = a.err_flag;
+    p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
+    const int k_steps = (a.K + BK - 1) / BK;
+    return BN == 256 ? launch_act<DGRAD, 256>(a.act, p, k_steps, s) : launch_act<DGRAD, 128>(a.act, p, k_steps, s);
+}
+
+}  // namespace
+
+int linear_fused_fwd(const LinearArgs& a, cudaStream_t s);
+int linear_fused_dgrad(const LinearArgs& a, cudaStream_t s);
+
+}  // namespace psb

@@ -9,6 +9,9 @@ import torch
 from .._lib import C
 
 _err_flags = {}
+# Scratch of the kernels that meet in global memory (``ops.linear``, ``ops.act8``), per device and stream: two launches may
+# only share it in stream order. Its counters are zero between launches, except after a launch that gave up.
+_workspaces = {}
 
 
 def _err_flag(device) -> torch.Tensor:
@@ -24,11 +27,25 @@ def check_gemm_errors(device=None) -> None:
         v = int(flag.item())
         if v:
             flag.zero_()
+            _workspaces.clear()
             raise RuntimeError(f"tcgen05 GEMM on cuda:{key}: bounded wait ran out (site {v})")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def workspace(device_index: int, stream: int) -> torch.Tensor:
+    """The scratch of one stream. Under graph capture every launch gets its own, zeroed by the graph itself: a replay need not
+    be the first thing that runs on its stream."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = None if capturing else _workspaces.get((device_index, stream))
+    if ws is None:
+        ws = torch.empty(C.linear_workspace_bytes(), dtype=torch.uint8, device=torch.device("cuda", device_index))
+        ws[:C.linear_workspace_zeros()].zero_()
+        if not capturing:
+            _workspaces[(device_index, stream)] = ws
+    return ws
 
 
 def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = False,
