@@ -1,6 +1,7 @@
 // Bindings of the decoder-block operators: layer norm, fused linear layers, 8-bit activation checkpoints.
 #include <pybind11/pybind11.h>
 
+#include "kernels/act8_wgrad.h"
 #include "kernels/linear_fused.h"
 #include "kernels/norm.h"
 
@@ -68,6 +69,27 @@ void bind_block(py::module_& m) {
         x.err_flag = (unsigned*)err_flag;
         x.wait_limit_s = wait_limit_s;
         return linear_fused(x, (void*)s);
+    });
+    m.def("act8_wgrad", [](uintptr_t dy, int64_t lddy, uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde, uintptr_t out, int64_t ldo,
+                           bool accumulate, uintptr_t weight, uintptr_t bias, uintptr_t dy_sum, int64_t tokens, int N, int K,
+                           uintptr_t workspace, uintptr_t err_flag, double wait_limit_s, uintptr_t s) {
+        Act8WgradArgs x;
+        x.dy = (const void*)dy;
+        x.lddy = lddy;
+        x.x = view(q, ldq, e, lde);
+        x.out = (float*)out;
+        x.ldo = ldo;
+        x.accumulate = accumulate ? 1 : 0;
+        x.weight = (const void*)weight;
+        x.bias = (const void*)bias;
+        x.dy_sum = (const float*)dy_sum;
+        x.tokens = tokens;
+        x.N = N;
+        x.K = K;
+        x.workspace = (void*)workspace;
+        x.err_flag = (unsigned*)err_flag;
+        x.wait_limit_s = wait_limit_s;
+        return act8_wgrad(x, (void*)s);
     });
     m.def("linear_workspace_bytes", &linear_workspace_bytes);
     m.def("linear_workspace_zeros", &linear_workspace_zeros);

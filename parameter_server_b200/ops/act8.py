@@ -121,3 +121,43 @@ def act8_unpack(a: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     x = torch.empty((a.rows, a.cols), dtype=dtype, device=a.q.device)
     check(C.act8_unpack(dt, *a.args(), x.data_ptr(), a.cols, a.rows, a.cols, s), "act8_unpack")
     return x
+
+
+def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               dy_sum: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False,
+               wait_limit_s: float = 2.0) -> torch.Tensor:
+    """``dy^T x`` in fp32, ``[N, K]``, for ``dy`` ``[..., N]`` (bf16) and the layer's input ``x`` (rows of ``K``) as an 8-bit checkpoint.
+
+    ``weight`` and ``bias`` (bf16, ``[K]``): the layer's input was a layer norm's output and ``x8`` holds its normalised rows
+    (``norm.layer_norm_act8``), so the operand is ``x * weight + bias``. With ``bias``, ``dy_sum`` is the sum of dy's rows (fp32, ``[N]``:
+    the layer's bias gradient, ``linear.linear_bias_grad``). ``out`` is written, or added to with ``accumulate``."""
+    from .linear import _ld, _matrix, workspace, _err_flag   # (linear imports this module)
+
+    what = "act8_wgrad"
+    s = launch_stream(dy)
+    dy2 = _matrix(dy, f"{what} dy")
+    tokens, n = dy2.shape
+    k = x8.cols
+    if x8.rows != tokens or x8.device != dy.device:
+        raise ValueError(f"{what}: checkpoint of {x8.rows} rows on {x8.device}, dy of {tokens} on {dy.device}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (k,) or t.dtype != torch.bfloat16 or t.device != dy.device or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be {k} contiguous bf16 values on {dy.device}")
+    if bias is not None and dy_sum is None:
+        raise ValueError(f"{what}: bias needs dy_sum, the sum of dy's rows")
+    if dy_sum is not None and (dy_sum.shape != (n,) or dy_sum.dtype != torch.float32 or dy_sum.device != dy.device or not dy_sum.is_contiguous()):
+        raise ValueError(f"{what}: dy_sum must be {n} contiguous fp32 values on {dy.device}")
+    if out is None:
+        if accumulate:
+            raise ValueError(f"{what}: accumulate needs out")
+        out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
+    elif out.shape != (n, k) or out.dtype != torch.float32 or out.device != dy.device or (k > 1 and out.stride(1) != 1):
+        raise ValueError(f"{what}: out must be a {n} x {k} fp32 matrix on {dy.device} with contiguous rows")
+    if tokens == 0:
+        return out if accumulate else out.zero_()
+    if n and k:
+        check(C.act8_wgrad(dy2.data_ptr(), _ld(dy2), *x8.args(), out.data_ptr(), row_stride(out), accumulate,
+                           0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                           0 if dy_sum is None else dy_sum.data_ptr(), tokens, n, k, workspace(dy.get_device(), s).data_ptr(),
+                           _err_flag(dy.device).data_ptr(), wait_limit_s, s), what)
+    return out
