@@ -29,27 +29,29 @@ namespace {
 constexpr int kWgThreads = 512;          // warpgroups: 0 producer / MMA, 1 converters, 2 and 3 epilogue
 constexpr int kWgChain = 8;              // k-steps (of 64 tokens) that are added inside TMEM
 constexpr int kWgBN = 256;
-constexpr int kRegsIssue = 40, kRegsConvert = 56, kRegsEpilogue = 208;   // 40 + 56 + 2 * 208 = 4 * 128, the launch's share
+constexpr int kRegsIssue = 40, kRegsConvert = 88, kRegsEpilogue = 192;   // 40 + 88 + 2 * 192 = 4 * 128, the launch's share
 static_assert(kRegsIssue + kRegsConvert + 2 * kRegsEpilogue == 4 * (65536 / kWgThreads), "setmaxnreg would wait for registers that the launch does not have");
 
+template <bool CONVERT>
 struct WgSmem {
     static constexpr int kABytes = BM * BK * 2;       // dy: 2 blocks of [64 tokens][64 n]
-    static constexpr int kBBytes = 128 * BK * 2;      // converted x: the same of the CTA's 128 columns
+    static constexpr int kBBytes = 128 * BK * 2;      // x in bf16: the same of the CTA's 128 columns
     static constexpr int kRawBytes = BK * 128;        // q: [64 tokens][128]
     static constexpr int kExpBytes = BK * 16;         // e: [64 tokens][16], four of them ours
-    static constexpr int kStageBytes = kABytes + kBBytes + kRawBytes + kExpBytes;
-    static constexpr int kStages = 5;
-    static constexpr int kTileBytes = kStages * kStageBytes;
-    static constexpr int kBarBytes = 256;
+    static constexpr int kRawStage = kRawBytes + kExpBytes;
+    static constexpr int kA = 6, kB = CONVERT ? 4 : 6, kRaw = CONVERT ? 5 : 0;   // stages
+    static constexpr int kBOff = kA * kABytes, kRawOff = kBOff + kB * kBBytes;
+    static constexpr int kTileBytes = kRawOff + kRaw * kRawStage;
+    static constexpr int kBarBytes = 512;
     static constexpr int kOutBytes = kLinEpilogueWarps * 2048;
     static constexpr int kTotal = kTileBytes + kBarBytes + kOutBytes + 1024;
 };
 
 struct WgParams {
-    CUtensorMap map_a, map_q, map_e;
+    CUtensorMap map_a, map_b, map_e;   // b: q, or x in bf16
     TileGrid grid;
     int N, K;             // rows and columns of dw
-    int a_blocked;
+    int a_blocked, b_blocked;
     float* out;
     int64_t ldo;
     int accumulate, out_vec;
@@ -62,28 +64,60 @@ struct WgParams {
     unsigned long long limit_ns;
 };
 
-// Two bytes of `w` (selector 0x4140: bytes 0 and 1, 0x4342: bytes 2 and 3) as bf16 times `step`: 128 + the low seven bits,
-// less 128 or, where the sign bit is set, 256 (it is the lowest exponent bit of the subtrahend); both steps are exact.
-__device__ __forceinline__ uint32_t convert2(uint32_t w, uint32_t selector, __nv_bfloat162 step) {
-    const uint32_t t = __byte_perm(w, 0u, selector);
-    uint32_t m = (t & 0x007F007Fu) | 0x43004300u, c = (t & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 v = __hmul2(__hsub2(*(__nv_bfloat162*)&m, *(__nv_bfloat162*)&c), step);
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Two of the bytes of `w` (unsigned, 128 more than the value; chosen by the selectors) as bf16 times the step: byte b in the
+// second byte of 0x4700bb00 is the float 32768 + b, one packed multiply-add takes off 32896 and scales, both exactly.
+__device__ __forceinline__ uint32_t convert2(uint32_t w, uint32_t s0, uint32_t s1, float step, float off) {
+    float a, b;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(a), "=f"(b)
+        : "r"(__byte_perm(w, 0x47000000u, s0)), "r"(__byte_perm(w, 0x47000000u, s1)), "f"(step), "f"(off));
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&v;
 }
+__device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// eight bytes (two words) as bf16 to 16 bytes of shared memory
+__device__ __forceinline__ void sts_converted(uint32_t addr, uint32_t w0, uint32_t w1, float step, float off) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(convert2(w0, 0x7404, 0x7414, step, off)),
+                 "r"(convert2(w0, 0x7424, 0x7434, step, off)), "r"(convert2(w1, 0x7404, 0x7414, step, off)),
+                 "r"(convert2(w1, 0x7424, 0x7434, step, off))
+                 : "memory");
+}
 
+template <bool CONVERT>
 __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_constant__ WgParams p) {
-    using L = WgSmem;
+    using L = WgSmem<CONVERT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* full_bar = (uint64_t*)(smem + L::kTileBytes);   // leader: dy of both CTAs
-    uint64_t* raw_bar = full_bar + L::kStages;                // this CTA's q and e
-    uint64_t* conv_bar = raw_bar + L::kStages;                // leader: both CTAs' converters
-    uint64_t* empty_bar = conv_bar + L::kStages;
-    uint64_t* tfull_bar = empty_bar + L::kStages;
+    uint64_t* afull_bar = (uint64_t*)(smem + L::kTileBytes);   // leader: dy of both CTAs has landed
+    uint64_t* aempty_bar = afull_bar + L::kA;                  // both: the MMAs have read it
+    uint64_t* rfull_bar = aempty_bar + L::kA;                  // own: q and e have landed
+    uint64_t* rempty_bar = rfull_bar + L::kRaw;                // own: the converters have read them
+    uint64_t* bfull_bar = rempty_bar + L::kRaw;                // leader: x in bf16 is there, in both CTAs
+    uint64_t* bempty_bar = bfull_bar + L::kB;               // both: the MMAs have read it
+    uint64_t* tfull_bar = bempty_bar + L::kB;
     uint64_t* tempty_bar = tfull_bar + 2;
     uint32_t* tmem_slot = (uint32_t*)(tempty_bar + 2);
     uint8_t* stage_out = smem + L::kTileBytes + L::kBarBytes;
-    static_assert((4 * L::kStages + 4) * 8 + 4 <= L::kBarBytes, "barriers");
+    static_assert((2 * (L::kA + L::kRaw + L::kB) + 4) * 8 + 4 <= L::kBarBytes, "barriers");
 
     const int cr = (int)cluster_ctarank();
     const bool leader = cr == 0;
@@ -92,12 +126,9 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
     const unsigned long long limit_ns = p.limit_ns;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < L::kStages; ++s) {
-            mbar_init(&full_bar[s], 1);
-            mbar_init(&raw_bar[s], 1);
-            mbar_init(&conv_bar[s], 8);   // four converter warps of each CTA
-            mbar_init(&empty_bar[s], 1);
-        }
+        for (int s = 0; s < L::kA; ++s) { mbar_init(&afull_bar[s], 1); mbar_init(&aempty_bar[s], 1); }
+        for (int s = 0; s < L::kRaw; ++s) { mbar_init(&rfull_bar[s], 1); mbar_init(&rempty_bar[s], 4); }
+        for (int s = 0; s < L::kB; ++s) { mbar_init(&bfull_bar[s], CONVERT ? 8 : 1); mbar_init(&bempty_bar[s], 1); }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull_bar[b], 1);
             mbar_init(&tempty_bar[b], 2 * kLinEpilogueWarps);
@@ -117,10 +148,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
         if (warp == 0 && lane == 0) {
-            // ---- TMA producer ----
+            // ---- TMA producer of dy (and of x, where it is bf16) ----
             asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_a) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_q) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_e) : "memory");
             TileWalk walk(p.grid, pair);
             Tile t;
             uint32_t it = 0;
@@ -128,36 +157,70 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
             while (ok && walk.next(p.grid, t)) {
                 const int m0 = t.m * 2 * BM + cr * BM, n0 = t.n * kWgBN + cr * 128;
                 for (int k = 0; k < t.nk; ++k, ++it) {
-                    const int s = it % L::kStages;
-                    if (!mbar_wait(&empty_bar[s], ((it / L::kStages) & 1u) ^ 1u, limit_ns)) {
+                    const int s = it % L::kA;
+                    // (one commit frees the stages of both operands, and they are as many: one wait covers both)
+                    if (!mbar_wait(&aempty_bar[s], ((it / L::kA) & 1u) ^ 1u, limit_ns)) {
                         atomicCAS(p.err_flag, 0u, 31u);
                         ok = false;
                         break;
                     }
-                    uint8_t* sa = smem + s * L::kStageBytes;
-                    uint8_t* sq = sa + L::kABytes + L::kBBytes;
+                    uint8_t* sa = smem + s * L::kABytes;
                     const int t0 = (t.k0 + k) * BK;   // first token
-                    mbar_expect_tx(&raw_bar[s], (uint32_t)(L::kRawBytes + L::kExpBytes));
-                    tma_load_2d(sq, &p.map_q, &raw_bar[s], n0, t0);
-                    tma_load_2d(sq + L::kRawBytes, &p.map_e, &raw_bar[s], (n0 / kAct8Block) & ~15, t0);   // x is a multiple of 16 bytes
-                    if (leader) mbar_expect_tx(&full_bar[s], 2u * (uint32_t)L::kABytes);
-                    const uint32_t fb = mapa_cluster(smem_u32(&full_bar[s]), 0);
+                    if (leader) mbar_expect_tx(&afull_bar[s], 2u * (uint32_t)(CONVERT ? L::kABytes : L::kABytes + L::kBBytes));
+                    const uint32_t fb = mapa_cluster(smem_u32(&afull_bar[s]), 0);
                     if (p.a_blocked) {
                         tma_load_3d_pair(sa, &p.map_a, fb, 0, t0, m0 / 64);
                     } else {
                         tma_load_2d_pair(sa, &p.map_a, fb, m0, t0);
                         tma_load_2d_pair(sa + 64 * 128, &p.map_a, fb, m0 + 64, t0);
                     }
+                    if constexpr (!CONVERT) {
+                        uint8_t* sb = smem + L::kBOff + s * L::kBBytes;
+                        if (p.b_blocked) {
+                            tma_load_3d_pair(sb, &p.map_b, fb, 0, t0, n0 / 64);
+                        } else {
+                            tma_load_2d_pair(sb, &p.map_b, fb, n0, t0);
+                            tma_load_2d_pair(sb + 64 * 128, &p.map_b, fb, n0 + 64, t0);
+                        }
+                    }
+                }
+            }
+        } else if (CONVERT && warp == 2 && lane == 0) {
+            // ---- TMA producer of the checkpoint ----
+            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_b) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_e) : "memory");
+            TileWalk walk(p.grid, pair);
+            Tile t;
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && walk.next(p.grid, t)) {
+                const int n0 = t.n * kWgBN + cr * 128;
+                for (int k = 0; k < t.nk; ++k, ++it) {
+                    const int s = it % L::kRaw;
+                    if (!mbar_wait(&rempty_bar[s], ((it / L::kRaw) & 1u) ^ 1u, limit_ns)) {
+                        atomicCAS(p.err_flag, 0u, 36u);
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sq = smem + L::kRawOff + s * L::kRawStage;
+                    const int t0 = (t.k0 + k) * BK;
+                    mbar_expect_tx(&rfull_bar[s], (uint32_t)L::kRawStage);
+                    tma_load_2d(sq, &p.map_b, &rfull_bar[s], n0, t0);
+                    tma_load_2d(sq + L::kRawBytes, &p.map_e, &rfull_bar[s], (n0 / kAct8Block) & ~15, t0);   // x is a multiple of 16 bytes
                 }
             }
         } else if (warp == 1 && lane == 0 && leader) {
             // ---- MMA issuer ----
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kWgBN >> 3) << 17) |
                                    ((uint32_t)((2 * BM) >> 4) << 24);
+            // The issue of an MMA blocks while the tensor core's queue is full, and the queue is short: what this thread does
+            // between two k-steps is time in which it may run dry. So the next k-step's barriers are asked before the current
+            // one's MMAs are issued, and descriptors and ring positions are kept as running values.
+            const uint64_t desc_a = make_desc(smem_u32(smem), 8192, 1024), desc_b = make_desc(smem_u32(smem + L::kBOff), 8192, 1024);
             TileWalk walk(p.grid, pair);
             Tile t;
-            uint32_t it = 0, tc = 0;
-            bool ok = true;
+            uint32_t it = 0, tc = 0, ia = 0, ic = 0, pa = 0, pc = 0;
+            bool ok = true, have = false;
             while (ok && walk.next(p.grid, t)) {
                 for (int k = 0; ok && k < t.nk; ++tc) {
                     const uint32_t buf = tc & 1u;
@@ -169,22 +232,27 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t tmem_d = tmem_base + buf * (uint32_t)kWgBN;
                     const int lim = min(t.nk, k + kWgChain);
-                    for (bool fresh = true; k < lim; ++k, ++it) {
-                        const int s = it % L::kStages;
-                        const uint32_t ph = (it / L::kStages) & 1u;
-                        if (!mbar_wait(&full_bar[s], ph, limit_ns * 2) || !mbar_wait(&conv_bar[s], ph, limit_ns * 2)) {
+                    uint32_t add = 0;
+                    for (; k < lim; ++k, ++it) {
+                        if (!have && (!mbar_wait(&afull_bar[ia], pa, limit_ns * 2) || (CONVERT && !mbar_wait(&bfull_bar[ic], pc, limit_ns * 2)))) {
                             atomicCAS(p.err_flag, 0u, 32u);
                             ok = false;
                             break;
                         }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = smem_u32(smem + s * L::kStageBytes), sb = sa + L::kABytes;
-#pragma unroll
-                        for (int u = 0; u < BK / UMMA_K; ++u) {
-                            umma_bf16_pair(tmem_d, make_desc(sa + u * 2048, 8192, 1024), make_desc(sb + u * 2048, 8192, 1024), idesc, fresh ? 0u : 1u);
-                            fresh = false;
-                        }
-                        umma_commit_pair(&empty_bar[s]);
+                        const uint32_t na = ia + 1 == L::kA ? 0 : ia + 1, nc = ic + 1 == L::kB ? 0 : ic + 1;
+                        const uint32_t npa = na == 0 ? pa ^ 1u : pa, npc = nc == 0 ? pc ^ 1u : pc;
+                        const uint64_t da = desc_a + ia * (uint32_t)(L::kABytes >> 4), db = desc_b + ic * (uint32_t)(L::kBBytes >> 4);
+                        umma_bf16_pair(tmem_d, da, db, idesc, add);
+                        have = mbar_try_wait(&afull_bar[na], npa);
+                        umma_bf16_pair(tmem_d, da + 128, db + 128, idesc, 1u);
+                        if constexpr (CONVERT) have = have && mbar_try_wait(&bfull_bar[nc], npc);
+                        umma_bf16_pair(tmem_d, da + 256, db + 256, idesc, 1u);
+                        umma_bf16_pair(tmem_d, da + 384, db + 384, idesc, 1u);
+                        umma_commit_pair(&aempty_bar[ia]);
+                        if constexpr (CONVERT) umma_commit_pair(&bempty_bar[ic]);
+                        add = 1;
+                        ia = na; ic = nc; pa = npa; pc = npc;
                     }
                     umma_commit_pair(&tfull_bar[buf]);   // (also on error, so that the epilogue moves on)
                 }
@@ -192,46 +260,82 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         }
     } else if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
-        // ---- converters: thread = 16 columns of rows r0, r0 + 16, ... of the 64 x 128 tile ----
-        const int ct = threadIdx.x - 128, g = ct & 7, r0 = ct >> 3;
-        const int chunk = (g & 3) * 2;   // 16-byte chunks of the row's 128-byte span in block g / 4
+        if constexpr (CONVERT) {
+        // ---- converters ----
+        // Eight lanes take 16 columns each of two neighbouring rows: columns 0-63 of the even row and 64-127 of the odd one,
+        // then the other halves. Their loads cover 128 bytes of distinct banks, and so do their stores: the two 16-byte
+        // chunks of a thread land at chunk ^ (row % 8) of the row's swizzled span, even positions for one row, odd for the
+        // other. A thread does this for rows r0 and r0 + 32.
+        const int ct = threadIdx.x - 128, gg = ct & 3, rr = (ct >> 2) & 1, r0 = 2 * (ct >> 3) + rr;
+        const int c0 = ((2 * gg) ^ (r0 & 7)) << 4, c1 = ((2 * gg + 1) ^ (r0 & 7)) << 4;
+        // One k-step ahead: the next k-step's bytes are requested before this one's are converted.
+        // One k-step ahead: the next k-step's bytes are requested before this one's are converted, and the barriers of the step
+        // after are asked before they are needed.
         TileWalk walk(p.grid, pair);
         Tile t;
-        uint32_t it = 0;
-        bool ok = true;
-        while (ok && walk.next(p.grid, t)) {
-            const int eb = (((t.n * kWgBN + cr * 128) / kAct8Block) & 15) + g / 2;
-            for (int k = 0; k < t.nk; ++k, ++it) {
-                const int s = it % L::kStages;
-                if (!mbar_wait(&raw_bar[s], (it / L::kStages) & 1u, limit_ns * 2)) {
-                    atomicCAS(p.err_flag, 0u, 35u);
-                    ok = false;
-                    break;
-                }
-                uint8_t* sb = smem + s * L::kStageBytes + L::kABytes + (g >> 2) * 8192;
-                const uint8_t* sq = smem + s * L::kStageBytes + L::kABytes + L::kBBytes;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = r0 + 16 * i;
-                    const uint4 raw = *(const uint4*)(sq + r * 128 + g * 16);
-                    const uint32_t e = sq[L::kRawBytes + r * 16 + eb];
-                    const uint32_t e2 = (e << 7) | (e << 23);
-                    const __nv_bfloat162 step = *(const __nv_bfloat162*)&e2;
-                    uint4 lo, hi;
-                    lo.x = convert2(raw.x, 0x4140, step); lo.y = convert2(raw.x, 0x4342, step);
-                    lo.z = convert2(raw.y, 0x4140, step); lo.w = convert2(raw.y, 0x4342, step);
-                    hi.x = convert2(raw.z, 0x4140, step); hi.y = convert2(raw.z, 0x4342, step);
-                    hi.z = convert2(raw.w, 0x4140, step); hi.w = convert2(raw.w, 0x4342, step);
-                    uint8_t* row = sb + r * 128;
-                    uint8_t *p0 = row + ((chunk ^ (r & 7)) << 4), *p1 = row + (((chunk + 1) ^ (r & 7)) << 4);
-                    // the eight lanes of a row write eight different chunk positions: block 1 starts with its odd ones
-                    if (g < 4) { *(uint4*)p0 = lo; *(uint4*)p1 = hi; }
-                    else { *(uint4*)p1 = hi; *(uint4*)p0 = lo; }
-                }
-                fence_async_smem();   // the MMAs read through the async proxy
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_cluster(smem_u32(&conv_bar[s]), 0));
+        const uint32_t q0 = smem_u32(smem + L::kRawOff) + r0 * 128 + gg * 16 + rr * 64;          // pass 0: row r0, columns of block rr
+        const uint32_t x0 = smem_u32(smem + L::kRawOff + L::kRawBytes) + r0 * 16 + gg / 2 + rr * 2;
+        const uint32_t d0 = smem_u32(smem + L::kBOff) + r0 * 128 + rr * 8192;
+        const uint32_t bfull0 = mapa_cluster(smem_u32(&bfull_bar[0]), 0);
+        const uint32_t other = rr != 0 ? 0u - 8192u : 8192u;   // from one column block of the converted tile to the other
+        uint32_t ir = 0, pr = 0, ic = 0, pc = 1;
+        uint4 raw[4], nraw[4];
+        uint32_t e[4], ne[4];
+        bool have = false;
+        auto load = [&](uint32_t eb) -> bool {
+            if (!have && !mbar_wait(&rfull_bar[ir], pr, limit_ns * 2)) {
+                atomicCAS(p.err_flag, 0u, 35u);
+                return false;
             }
+            const uint32_t sq = q0 + ir * L::kRawStage, sx = x0 + ir * L::kRawStage + eb;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {   // odd: the other column block of the row (neither eb nor gg / 2 touches that bit)
+                nraw[i] = lds_v4(((i & 1) ? (sq ^ 64u) : sq) + 32 * (i / 2) * 128);
+                ne[i] = lds_u8(((i & 1) ? (sx ^ 2u) : sx) + 32 * (i / 2) * 16);
+            }
+            if (++ir == L::kRaw) { ir = 0; pr ^= 1u; }
+            have = false;
+            return true;
+        };
+        bool more = walk.next(p.grid, t);
+        int left = t.nk;
+        uint32_t eb = ((t.n * kWgBN + cr * 128) / kAct8Block) & 15;
+        if (more) more = load(eb);
+        while (more) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { raw[i] = nraw[i]; e[i] = ne[i]; }
+            const uint32_t ir_now = ir == 0 ? L::kRaw - 1 : ir - 1;
+            const bool room = mbar_try_wait(&bempty_bar[ic], pc);
+            if (--left == 0) {
+                more = walk.next(p.grid, t);
+                left = t.nk;
+                eb = ((t.n * kWgBN + cr * 128) / kAct8Block) & 15;
+            }
+            if (more) more = load(eb);
+            if (!room && !mbar_wait(&bempty_bar[ic], pc, limit_ns * 2)) {
+                atomicCAS(p.err_flag, 0u, 37u);
+                break;
+            }
+            const uint32_t sb = d0 + ic * L::kBBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float step = __uint_as_float(e[i] << 23), off = -32896.f * step;
+                const uint32_t w0 = raw[i].x ^ 0x80808080u, w1 = raw[i].y ^ 0x80808080u, w2 = raw[i].z ^ 0x80808080u, w3 = raw[i].w ^ 0x80808080u;
+                const uint32_t dst = sb + ((i & 1) ? other : 0u) + 32 * (i / 2) * 128;
+                sts_converted(dst + c0, w0, w1, step, off);
+                sts_converted(dst + c1, w2, w3, step, off);
+            }
+            if (more) have = mbar_try_wait(&rfull_bar[ir], pr);
+            fence_async_smem();   // the MMAs read through the async proxy
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_pair(bfull0 + ic * 8);
+                // only now that the values have been used is it certain that they have been read: a load alone may be carried out
+                // behind an arrival that follows it
+                mbar_arrive(&rempty_bar[ir_now]);
+            }
+            if (++ic == L::kB) { ic = 0; pc ^= 1u; }
+        }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
@@ -257,16 +361,15 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)kWgBN + (uint32_t)(half * 128);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
-                    tmem_wait_ld(v);
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t v[16];
+                    tmem_ld16(taddr + (uint32_t)c * 16u, v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(v[j]);
+                    for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(v[j]);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
+                if (lane == 0) mbar_arrive_pair(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
             }
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
@@ -296,7 +399,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                     for (int j = 0; j < 32; ++j) {
                         const float4 x = __ldcg((const float4*)(src + j * 128));
                         acc[4 * j] += x.x; acc[4 * j + 1] += x.y; acc[4 * j + 2] += x.z; acc[4 * j + 3] += x.w;
-                        if (j % 8 == 7) asm volatile("" ::: "memory");   // eight loads in flight: more would not fit the registers
+                        if (j % 4 == 3) asm volatile("" ::: "memory");   // eight loads in flight: more would not fit the registers
                     }
                 }
             }
@@ -367,6 +470,16 @@ bool make_byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t c
                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <bool CONVERT>
+int launch_wgrad(WgParams& p, int64_t tokens, cudaStream_t s) {
+    constexpr auto kern = act8_wgrad_kernel<CONVERT>;
+    int pairs = 0;
+    cudaError_t e = pairs_of<kern>(kWgThreads, WgSmem<CONVERT>::kTotal, &pairs);
+    if (e != cudaSuccess) return (int)e;
+    p.grid = plan_tiles((p.N + 2 * BM - 1) / (2 * BM), (p.K + kWgBN - 1) / kWgBN, (int)((tokens + BK - 1) / BK), pairs, 12);
+    return (int)launch_pairs(kern, kWgThreads, WgSmem<CONVERT>::kTotal, p.grid.pairs, p, s);
+}
+
 }  // namespace
 
 int act8_wgrad(const Act8WgradArgs& a, void* stream) {
@@ -374,15 +487,28 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     if (a.tokens <= 0 || a.tokens > 0x7FFFFFFFll - 64 || a.workspace == nullptr || a.err_flag == nullptr || a.out == nullptr) return -2;
     if (a.bias != nullptr && a.dy_sum == nullptr) return -2;
     if (!rows16(a.dy, a.lddy) || ((uintptr_t)a.x.q % 16) || (a.x.ldq % 16) || ((uintptr_t)a.x.e % 16) || (a.x.lde % 16)) return -2;
+    const uint64_t tokens = (uint64_t)a.tokens, blocks = (uint64_t)(a.K + kAct8Block - 1) / kAct8Block;
+    const bool convert = a.scratch == nullptr;
+    const int64_t ldx = ((int64_t)a.K + 7) / 8 * 8;
+    if (!convert) {
+        const int rc = act8_unpack(0, a.x, a.scratch, ldx, a.tokens, a.K, stream);
+        if (rc != 0) return rc;
+    }
     WgParams p;
     p.N = a.N;
     p.K = a.K;
     p.a_blocked = a.N % 64 == 0 && a.N >= BM ? 1 : 0;
-    const uint64_t tokens = (uint64_t)a.tokens, blocks = (uint64_t)(a.K + kAct8Block - 1) / kAct8Block;
-    const bool ok = (p.a_blocked ? make_map_blocked(&p.map_a, a.dy, tokens, (uint64_t)a.N, (uint64_t)a.lddy, BM / 64)
-                                 : make_map(&p.map_a, a.dy, tokens, (uint64_t)a.N, (uint64_t)a.lddy, 64)) &&
-                    make_byte_map(&p.map_q, a.x.q, tokens, (uint64_t)a.K, (uint64_t)a.x.ldq, 128) &&
-                    make_byte_map(&p.map_e, a.x.e, tokens, blocks, (uint64_t)a.x.lde, 16);
+    p.b_blocked = a.K % 64 == 0 && a.K >= 128 ? 1 : 0;
+    bool ok = p.a_blocked ? make_map_blocked(&p.map_a, a.dy, tokens, (uint64_t)a.N, (uint64_t)a.lddy, BM / 64)
+                          : make_map(&p.map_a, a.dy, tokens, (uint64_t)a.N, (uint64_t)a.lddy, 64);
+    if (convert) {
+        ok = ok && make_byte_map(&p.map_b, a.x.q, tokens, (uint64_t)a.K, (uint64_t)a.x.ldq, 128) &&
+             make_byte_map(&p.map_e, a.x.e, tokens, blocks, (uint64_t)a.x.lde, 16);
+    } else {
+        ok = ok && (p.b_blocked ? make_map_blocked(&p.map_b, a.scratch, tokens, (uint64_t)a.K, (uint64_t)ldx, 2)
+                                : make_map(&p.map_b, a.scratch, tokens, (uint64_t)a.K, (uint64_t)ldx, 64));
+        p.map_e = p.map_b;   // not used
+    }
     if (!ok) return -3;
     p.out = a.out;
     p.ldo = a.ldo;
@@ -395,11 +521,11 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     p.partial = (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
-    int pairs = 0;
-    cudaError_t e = pairs_of<act8_wgrad_kernel>(kWgThreads, WgSmem::kTotal, &pairs);
-    if (e != cudaSuccess) return (int)e;
-    p.grid = plan_tiles((a.N + 2 * BM - 1) / (2 * BM), (a.K + kWgBN - 1) / kWgBN, (int)((a.tokens + BK - 1) / BK), pairs, 12);
-    return (int)launch_pairs(act8_wgrad_kernel, kWgThreads, WgSmem::kTotal, p.grid.pairs, p, (cudaStream_t)stream);
+    return convert ? launch_wgrad<true>(p, a.tokens, (cudaStream_t)stream) : launch_wgrad<false>(p, a.tokens, (cudaStream_t)stream);
+}
+
+int64_t act8_wgrad_scratch(int64_t tokens, int N, int K) {
+    return 0;
 }
 
 }  // namespace psb

@@ -20,6 +20,7 @@ struct Act8WgradArgs {
     const float* dy_sum = nullptr;
     int64_t tokens = 0;
     int N = 0, K = 0;
+    void* scratch = nullptr;         // act8_wgrad_scratch() bytes; null: the checkpoint is converted tile by tile
     void* workspace = nullptr;       // as of linear_fused()
     unsigned* err_flag = nullptr;
     double wait_limit_s = 2.0;
@@ -27,5 +28,7 @@ struct Act8WgradArgs {
 
 // Returns 0, a cudaError_t, -2 (alignment or an argument that is not supported) or -3 (tensor map).
 int act8_wgrad(const Act8WgradArgs& args, void* stream);
+// Bytes of `scratch` for the faster of the two ways for these sizes (0: none).
+int64_t act8_wgrad_scratch(int64_t tokens, int N, int K);
 
 }  // namespace psb

@@ -277,10 +277,18 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
         if (lane == 0 && leader) {
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
                                    ((uint32_t)((2 * BM) >> 4) << 24);
+            // The issue of an MMA blocks while the tensor core's queue is full, and the queue is short: what this thread does
+            // between two k-steps is time in which it may run dry. So the next k-step's barrier is asked while the current one's
+            // MMAs are issued, and descriptors and ring positions are kept as running values.
+            // K-major: 8-row groups 1024 B apart, 16 k are 32 B inside the swizzle span; MN-major: 64-column blocks 8192 B
+            // apart, 16 k-rows are 2048 B. (Descriptors count in 16 bytes.)
+            constexpr uint32_t kNextB = DGRAD ? 2048 >> 4 : 32 >> 4;
+            const uint64_t desc_a = make_desc(smem_u32(smem), 16, 1024);
+            const uint64_t desc_b = DGRAD ? make_desc(smem_u32(smem + L::kABytes), 8192, 1024) : make_desc(smem_u32(smem + L::kABytes), 16, 1024);
             TileWalk walk(p.grid, pair);
             Tile t;
-            uint32_t it = 0, tc = 0;
-            bool ok = true;
+            uint32_t s = 0, ph = 0, tc = 0;
+            bool ok = true, have = false;
             while (ok && walk.next(p.grid, t)) {
                 const uint32_t buf = tc & 1u;
                 if (!mbar_wait(&tempty_bar[buf], ((tc >> 1) & 1u) ^ 1u, limit_ns)) {
@@ -289,26 +297,23 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t tmem_d = tmem_base + buf * (uint32_t)BN;
-                for (int k = 0; k < t.nk; ++k, ++it) {
-                    const int s = it % L::kStages;
+                for (int k = 0; k < t.nk; ++k) {
                     // consumers wait longer than producers, so that the wait that reports is the one at the root
-                    if (!mbar_wait(&full_bar[s], (it / L::kStages) & 1u, limit_ns * 2)) {
+                    if (!have && !mbar_wait(&full_bar[s], ph, limit_ns * 2)) {
                         atomicCAS(p.err_flag, 0u, 22u);
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t sa = smem_u32(smem + s * L::kStageBytes);
-                    const uint32_t sb = sa + L::kABytes;
+                    const uint32_t next = s + 1 == L::kStages ? 0 : s + 1, next_ph = next == 0 ? ph ^ 1u : ph;
+                    const uint64_t da = desc_a + s * (uint32_t)(L::kStageBytes >> 4), db = desc_b + s * (uint32_t)(L::kStageBytes >> 4);
+                    umma_bf16_pair(tmem_d, da, db, idesc, k ? 1u : 0u);
+                    have = mbar_try_wait(&full_bar[next], next_ph);
 #pragma unroll
-                    for (int u = 0; u < BK / UMMA_K; ++u) {
-                        // K-major: 8-row groups 1024 B apart, 16 k are 32 B inside the swizzle span; MN-major: 64-column
-                        // blocks 8192 B apart, 16 k-rows are 2048 B
-                        const uint64_t da = make_desc(sa + u * 32, 16, 1024);
-                        const uint64_t db = DGRAD ? make_desc(sb + u * 2048, 8192, 1024) : make_desc(sb + u * 32, 16, 1024);
-                        umma_bf16_pair(tmem_d, da, db, idesc, (k | u) ? 1u : 0u);
-                    }
+                    for (int u = 1; u < BK / UMMA_K; ++u) umma_bf16_pair(tmem_d, da + u * 2, db + u * kNextB, idesc, 1u);
                     umma_commit_pair(&empty_bar[s]);   // frees the stage in both CTAs when these MMAs have read it
+                    s = next;
+                    ph = next_ph;
                 }
                 umma_commit_pair(&tfull_bar[buf]);     // (also on error, so that the epilogue moves on)
                 ++tc;
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             auto release = [&]() {   // this warp has read the accumulator
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
+                if (lane == 0) mbar_arrive_pair(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
             };
             // one 32-column piece with its values in f
             uint32_t ewrite = 0;

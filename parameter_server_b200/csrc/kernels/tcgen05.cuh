@@ -139,6 +139,13 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same with the default (CTA) scope of release: a release at cluster scope makes the thread wait until everything it has
+// stored, in global memory too, is visible there (about 0.8 us for every k-step of a converter warp). Enough where what the
+// barrier hands over is TMEM (ordered by tcgen05.fence) or shared memory of this CTA that only the tensor core and the TMA
+// unit touch next (ordered by fence.proxy.async).
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // Loads of a pair: the data lands in this CTA, the bytes are counted on the LEADER's barrier (no multicast: every
 // CTA fetches its own tiles).
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int c0, int c1) {
