@@ -71,7 +71,7 @@ void bind_block(py::module_& m) {
         return linear_fused(x, (void*)s);
     });
     m.def("act8_wgrad", [](uintptr_t dy, int64_t lddy, uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde, uintptr_t out, int64_t ldo,
-                           bool accumulate, uintptr_t weight, uintptr_t bias, uintptr_t dy_sum, int64_t tokens, int N, int K,
+                           bool accumulate, uintptr_t weight, uintptr_t bias, uintptr_t dy_sum, int64_t tokens, int N, int K, uintptr_t scratch,
                            uintptr_t workspace, uintptr_t err_flag, double wait_limit_s, uintptr_t s) {
         Act8WgradArgs x;
         x.dy = (const void*)dy;
@@ -84,6 +84,7 @@ void bind_block(py::module_& m) {
         x.bias = (const void*)bias;
         x.dy_sum = (const float*)dy_sum;
         x.tokens = tokens;
+        x.scratch = (void*)scratch;
         x.N = N;
         x.K = K;
         x.workspace = (void*)workspace;
@@ -91,6 +92,7 @@ void bind_block(py::module_& m) {
         x.wait_limit_s = wait_limit_s;
         return act8_wgrad(x, (void*)s);
     });
+    m.def("act8_wgrad_scratch", &act8_wgrad_scratch);
     m.def("linear_workspace_bytes", &linear_workspace_bytes);
     m.def("linear_workspace_zeros", &linear_workspace_zeros);
 }

@@ -34,6 +34,25 @@ __device__ __forceinline__ float act8_inverse_step(uint32_t e) { return e == 255
 __device__ __forceinline__ float act8_step(uint32_t e) { return __uint_as_float(e << 23); }
 // (the conversion takes NaN = infinity * 0 to 0)
 __device__ __forceinline__ int act8_quantise(float x, float inverse_step) { return __float2int_rn(x * inverse_step); }
+// The larger magnitude of a and b, NaN if one of them is
+__device__ __forceinline__ float abs_max(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return m;
+}
+// Four values as bytes: adding 1.5 * 2^23 leaves the rounded number in the low bits (one multiply-add per value where a
+// conversion instruction has a quarter of its rate). Only for finite blocks.
+__device__ __forceinline__ uint32_t act8_quantise4(float a, float b, float c, float d, float inverse_step) {
+    const float magic = 12582912.f;
+    const uint32_t x = __float_as_uint(fmaf(a, inverse_step, magic)), y = __float_as_uint(fmaf(b, inverse_step, magic));
+    const uint32_t z = __float_as_uint(fmaf(c, inverse_step, magic)), w = __float_as_uint(fmaf(d, inverse_step, magic));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+// Byte i of `biased` (four numbers with their sign bits flipped) as a float: byte b in the second byte of 0x4700bb00 is 32768 + b
+template <int I>
+__device__ __forceinline__ float s8_of_biased(uint32_t biased) {
+    return __uint_as_float(__byte_perm(biased, 0x47000000u, 0x7404 | (I << 4))) - 32896.f;
+}
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 __device__ __forceinline__ uint32_t pack_s8x4(int a, int b, int c, int d) {

@@ -10,8 +10,8 @@
 // One persistent launch of CTA pairs (cta_group::2), one pair per two SMs. A pair works on a 256 x BN tile: each CTA loads
 // its 128 rows of A and half of the B tile per k-step of 64 (32 KB for 512 cycles of MMA, which is what an SM's port to L2
 // delivers; a single-CTA tile would need half as much again), the leader issues the MMAs for both, and each CTA drains its
-// own 128 rows. Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-9 epilogue (a warp has one 32-lane quarter of TMEM
-// and half of the tile's columns). The accumulator is double-buffered in TMEM, so the epilogue of a tile runs beside the
+// own 128 rows. Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-3 idle, 4-11 epilogue (a warp has one 32-lane quarter
+// of TMEM and half of the tile's columns; the first warpgroup's registers go to them). The accumulator is double-buffered in TMEM, so the epilogue of a tile runs beside the
 // MMAs of the next. Tiles are dealt out as tile_walk.cuh says. Every wait is bounded; on a time-out the CTA records where,
 // frees its TMEM and returns.
 #pragma once
@@ -32,15 +32,20 @@ namespace psb {
 namespace {
 
 constexpr int kLinEpilogueWarps = 8;
-constexpr int kLinThreads = 32 * (2 + kLinEpilogueWarps);
+constexpr int kLinThreads = 32 * (4 + kLinEpilogueWarps);
+constexpr int kLinRegsIssue = 56, kLinRegsEpilogue = 224;   // 56 + 2 * 224 = 3 * 168, the launch's share
+static_assert(kLinRegsIssue + 2 * kLinRegsEpilogue == 3 * (65536 / kLinThreads / 8 * 8), "setmaxnreg would wait for registers that the launch does not have");
 
 template <int BN>
 struct LinSmem {
     static constexpr int kABytes = BM * BK * 2;
     static constexpr int kBBytes = BN / 2 * BK * 2;          // a CTA of a pair holds half of the B tile
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = BN == 256 ? 6 : 8;
-    static constexpr int kTileBytes = kStages * kStageBytes;
+    // k-steps that share a stage and its barriers: half as much for the MMA issuer to do between two MMAs, which counts where
+    // the epilogue keeps the same schedulers busy (dgrad with an 8-bit h: 397 us with one, 383 us with two)
+    static constexpr int kSub = 2;
+    static constexpr int kStages = BN == 256 ? 3 : 4;
+    static constexpr int kTileBytes = kStages * kSub * kStageBytes;
     static constexpr int kBarBytes = 256;
     static constexpr int kBiasBytes = 2 * BN * 4;            // double-buffered with the accumulator
     static constexpr int kOutBytes = kLinEpilogueWarps * 2048;   // a warp's [32 rows][64 bytes] on the way out
@@ -75,22 +80,32 @@ struct LinParams {
 
 // ---- activations -----------------------------------------------------------------------------------------------------
 // gelu_tanh(h) = h / 2 * (1 + tanh(u)) = h * s(2u) with s(z) = 1 / (1 + exp(-z)) and u = sqrt(2/pi) (h + 0.044715 h^3): no
-// cancellation in the tails, two special-function operations per value.
+// cancellation in the tails, two special-function operations per value. Its slope is s + h s (1 - s) d(2u)/dh.
 constexpr float kGeluC = 1.5957691216057308f;             // 2 sqrt(2 / pi)
 constexpr float kGeluC3 = 1.5957691216057308f * 0.044715f;
+constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float sigmoidf_fast(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_of(float h) {
     if constexpr (ACT == kActRelu) return h > 0.f ? h : (h != h ? h : 0.f);
     if constexpr (ACT == kActGelu) return 0.5f * h * (1.f + erff(h * 0.70710678118654752f));
-    if constexpr (ACT == kActGeluTanh) return __fdividef(h, 1.f + __expf(-h * (kGeluC + kGeluC3 * h * h)));
-    if constexpr (ACT == kActSilu) return __fdividef(h, 1.f + __expf(-h));
+    if constexpr (ACT == kActGeluTanh) return h * reciprocal_fast(1.f + exp2_fast(h * fmaf(-kGeluC3 * kLog2e, h * h, -kGeluC * kLog2e)));
+    if constexpr (ACT == kActSilu) return h * reciprocal_fast(1.f + exp2_fast(h * -kLog2e));
     return h;
 }
-// act(h) and act'(h). The slope of the saturating tails is taken at |h| <= 20, where it has long reached 0 or 1: the
-// products below would meet infinity * 0 further out.
+// act(h) and act'(h). The square in the slope stops at 400 (|h| = 20), where s has long reached 0 or 1: further out the
+// products would meet infinity * 0.
 template <int ACT>
 __device__ __forceinline__ float act_slope(float h, float* value) {
     if constexpr (ACT == kActRelu) {
@@ -100,38 +115,37 @@ __device__ __forceinline__ float act_slope(float h, float* value) {
     if constexpr (ACT == kActGelu) {
         const float cdf = 0.5f * (1.f + erff(h * 0.70710678118654752f));
         *value = h * cdf;
-        const float c = fminf(fmaxf(h, -20.f), 20.f);
-        return cdf + c * 0.3989422804014327f * __expf(-0.5f * c * c);
+        return fmaf(h, 0.3989422804014327f * exp2_fast(fminf(h * h, 400.f) * (-0.5f * kLog2e)), cdf);
     }
-    if constexpr (ACT == kActGeluTanh || ACT == kActSilu) {
-        const float c = fminf(fmaxf(h, -20.f), 20.f);
-        const float h2 = c * c;
-        const float z = ACT == kActSilu ? c : c * (kGeluC + kGeluC3 * h2);
-        const float dz = ACT == kActSilu ? 1.f : kGeluC + 3.f * kGeluC3 * h2;
-        const float s = sigmoidf_fast(z);
+    if constexpr (ACT == kActGeluTanh) {
+        const float w = fminf(h * h, 400.f);
+        const float s = reciprocal_fast(1.f + exp2_fast(h * fmaf(-kGeluC3 * kLog2e, w, -kGeluC * kLog2e)));
         *value = h * s;
-        return (s + c * dz * s * (1.f - s)) + (h - h);   // NaN and infinity stay what they are
+        return fmaf(*value * (1.f - s), fmaf(3.f * kGeluC3, w, kGeluC), s);
+    }
+    if constexpr (ACT == kActSilu) {
+        const float s = reciprocal_fast(1.f + exp2_fast(h * -kLog2e));
+        *value = h * s;
+        return fmaf(*value, 1.f - s, s);
     }
     *value = h;
     return 1.f;
 }
 
 // ---- epilogue: memory side -------------------------------------------------------------------------------------------
-// 32 values of a bf16 row (64 bytes) that may be unaligned or cut off by the tensor's edge: out of line, rarely taken.
-__device__ __noinline__ void load32_slow(const __nv_bfloat16* p, int n, uint32_t* w) {
-    for (int j = 0; j < 16; ++j) {
-        uint32_t lo = 2 * j < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j]) : 0u;
-        uint32_t hi = 2 * j + 1 < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j + 1]) : 0u;
-        w[j] = lo | (hi << 16);
-    }
-}
+// 32 values of a bf16 row (64 bytes): four wide loads, or one by one where the row is unaligned or cut off by the tensor's edge
 __device__ __forceinline__ void load32(const __nv_bfloat16* p, int n, bool vec, uint4* raw) {
     if (vec && n >= 32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) raw[j] = ld_nc_v4(p + 8 * j);
     } else {
         uint32_t w[16];
-        load32_slow(p, n, w);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint32_t lo = 2 * j < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j]) : 0u;
+            const uint32_t hi = 2 * j + 1 < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j + 1]) : 0u;
+            w[j] = lo | (hi << 16);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) raw[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     }
@@ -179,16 +193,14 @@ __device__ __forceinline__ void store_piece(uint8_t* stage, int lane, const floa
 // 32 values of this lane's row into the 8-bit checkpoint; returns the exponent. (Columns past N carry zeros here, and the
 // padding of a row takes them.)
 __device__ __forceinline__ uint32_t keep_row32(const float* f, int8_t* qp, int n, bool live) {
-    uint32_t m = 0;
+    float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) m = max(m, abs_bits(f[j]));
-    const uint32_t e = act8_exponent(m);
+    for (int j = 0; j < 32; ++j) m = abs_max(m, f[j]);
+    const uint32_t e = act8_exponent(__float_as_uint(m));
     const float inv = act8_inverse_step(e);
     uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        w[j] = pack_s8x4(act8_quantise(f[4 * j], inv), act8_quantise(f[4 * j + 1], inv), act8_quantise(f[4 * j + 2], inv),
-                         act8_quantise(f[4 * j + 3], inv));
+    for (int j = 0; j < 8; ++j) w[j] = e == 255u ? 0u : act8_quantise4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3], inv);
     if (live) {
         *(uint4*)qp = make_uint4(w[0], w[1], w[2], w[3]);
         if (n > 16) *(uint4*)(qp + 16) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -237,91 +249,103 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
 
-    if (warp == 0) {
-        // ---- TMA producer ----
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_a) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_b) : "memory");
-            TileWalk walk(p.grid, pair);
-            Tile t;
-            uint32_t it = 0;
-            bool ok = true;
-            while (ok && walk.next(p.grid, t)) {
-                const int m0 = t.m * 2 * BM + cr * BM, n0 = t.n * BN + cr * (BN / 2);
-                for (int k = 0; k < t.nk; ++k, ++it) {
-                    const int s = it % L::kStages;
-                    if (!mbar_wait(&empty_bar[s], ((it / L::kStages) & 1u) ^ 1u, limit_ns)) {
-                        atomicCAS(p.err_flag, 0u, 21u);
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* sa = smem + s * L::kStageBytes;
-                    uint8_t* sb = sa + L::kABytes;
-                    const int k0 = (t.k0 + k) * BK;
-                    if (leader) mbar_expect_tx(&full_bar[s], 2u * (uint32_t)L::kStageBytes);   // both CTAs' bytes
-                    const uint32_t fb = mapa_cluster(smem_u32(&full_bar[s]), 0);
-                    tma_load_2d_pair(sa, &p.map_a, fb, k0, m0);   // [128 rows][64 k]
-                    if constexpr (!DGRAD) {
-                        tma_load_2d_pair(sb, &p.map_b, fb, k0, n0);   // [BN / 2 rows][64 k]
-                    } else if (p.b_blocked) {
-                        tma_load_3d_pair(sb, &p.map_b, fb, 0, k0, n0 / 64);   // [BN / 128 blocks][64 k][64 n]
-                    } else {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLinRegsIssue));
+        if (warp == 0) {
+            // ---- TMA producer ----
+            if (lane == 0) {
+                asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_a) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_b) : "memory");
+                TileWalk walk(p.grid, pair);
+                Tile t;
+                uint32_t it = 0;
+                bool ok = true;
+                while (ok && walk.next(p.grid, t)) {
+                    const int m0 = t.m * 2 * BM + cr * BM, n0 = t.n * BN + cr * (BN / 2);
+                    for (int k = 0; k < t.nk; k += L::kSub, ++it) {
+                        const int s = it % L::kStages;
+                        const int n = min(L::kSub, t.nk - k);
+                        if (!mbar_wait(&empty_bar[s], ((it / L::kStages) & 1u) ^ 1u, limit_ns)) {
+                            atomicCAS(p.err_flag, 0u, 21u);
+                            ok = false;
+                            break;
+                        }
+                        if (leader) mbar_expect_tx(&full_bar[s], 2u * (uint32_t)(L::kStageBytes * n));   // both CTAs' bytes
+                        const uint32_t fb = mapa_cluster(smem_u32(&full_bar[s]), 0);
+                        for (int u = 0; u < n; ++u) {
+                            uint8_t* sa = smem + (s * L::kSub + u) * L::kStageBytes;
+                            uint8_t* sb = sa + L::kABytes;
+                            const int k0 = (t.k0 + k + u) * BK;
+                            tma_load_2d_pair(sa, &p.map_a, fb, k0, m0);   // [128 rows][64 k]
+                            if constexpr (!DGRAD) {
+                                tma_load_2d_pair(sb, &p.map_b, fb, k0, n0);   // [BN / 2 rows][64 k]
+                            } else if (p.b_blocked) {
+                                tma_load_3d_pair(sb, &p.map_b, fb, 0, k0, n0 / 64);   // [BN / 128 blocks][64 k][64 n]
+                            } else {
 #pragma unroll
-                        for (int j = 0; j < BN / 128; ++j) tma_load_2d_pair(sb + j * 64 * 128, &p.map_b, fb, n0 + 64 * j, k0);
+                                for (int j = 0; j < BN / 128; ++j) tma_load_2d_pair(sb + j * 64 * 128, &p.map_b, fb, n0 + 64 * j, k0);
+                            }
+                        }
                     }
                 }
             }
-        }
-    } else if (warp == 1) {
-        // ---- MMA issuer ----
-        if (lane == 0 && leader) {
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
-                                   ((uint32_t)((2 * BM) >> 4) << 24);
-            // The issue of an MMA blocks while the tensor core's queue is full, and the queue is short: what this thread does
-            // between two k-steps is time in which it may run dry. So the next k-step's barrier is asked while the current one's
-            // MMAs are issued, and descriptors and ring positions are kept as running values.
-            // K-major: 8-row groups 1024 B apart, 16 k are 32 B inside the swizzle span; MN-major: 64-column blocks 8192 B
-            // apart, 16 k-rows are 2048 B. (Descriptors count in 16 bytes.)
-            constexpr uint32_t kNextB = DGRAD ? 2048 >> 4 : 32 >> 4;
-            const uint64_t desc_a = make_desc(smem_u32(smem), 16, 1024);
-            const uint64_t desc_b = DGRAD ? make_desc(smem_u32(smem + L::kABytes), 8192, 1024) : make_desc(smem_u32(smem + L::kABytes), 16, 1024);
-            TileWalk walk(p.grid, pair);
-            Tile t;
-            uint32_t s = 0, ph = 0, tc = 0;
-            bool ok = true, have = false;
-            while (ok && walk.next(p.grid, t)) {
-                const uint32_t buf = tc & 1u;
-                if (!mbar_wait(&tempty_bar[buf], ((tc >> 1) & 1u) ^ 1u, limit_ns)) {
-                    atomicCAS(p.err_flag, 0u, 24u);
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t tmem_d = tmem_base + buf * (uint32_t)BN;
-                for (int k = 0; k < t.nk; ++k) {
-                    // consumers wait longer than producers, so that the wait that reports is the one at the root
-                    if (!have && !mbar_wait(&full_bar[s], ph, limit_ns * 2)) {
-                        atomicCAS(p.err_flag, 0u, 22u);
-                        ok = false;
+        } else if (warp == 1) {
+            // ---- MMA issuer ----
+            if (lane == 0 && leader) {
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                                       ((uint32_t)((2 * BM) >> 4) << 24);
+                // The issue of an MMA blocks while the tensor core's queue is full, and the queue is short: what this thread does
+                // between two k-steps is time in which it may run dry. So the next k-step's barrier is asked while the current one's
+                // MMAs are issued, and descriptors and ring positions are kept as running values.
+                // K-major: 8-row groups 1024 B apart, 16 k are 32 B inside the swizzle span; MN-major: 64-column blocks 8192 B
+                // apart, 16 k-rows are 2048 B. (Descriptors count in 16 bytes.)
+                constexpr uint32_t kNextB = DGRAD ? 2048 >> 4 : 32 >> 4;
+                const uint64_t desc_a = make_desc(smem_u32(smem), 16, 1024);
+                const uint64_t desc_b = DGRAD ? make_desc(smem_u32(smem + L::kABytes), 8192, 1024) : make_desc(smem_u32(smem + L::kABytes), 16, 1024);
+                TileWalk walk(p.grid, pair);
+                Tile t;
+                uint32_t s = 0, ph = 0, tc = 0;
+                bool ok = true, have = false;
+                while (ok && walk.next(p.grid, t)) {
+                    const uint32_t buf = tc & 1u;
+                    if (!mbar_wait(&tempty_bar[buf], ((tc >> 1) & 1u) ^ 1u, limit_ns)) {
+                        atomicCAS(p.err_flag, 0u, 24u);
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t next = s + 1 == L::kStages ? 0 : s + 1, next_ph = next == 0 ? ph ^ 1u : ph;
-                    const uint64_t da = desc_a + s * (uint32_t)(L::kStageBytes >> 4), db = desc_b + s * (uint32_t)(L::kStageBytes >> 4);
-                    umma_bf16_pair(tmem_d, da, db, idesc, k ? 1u : 0u);
-                    have = mbar_try_wait(&full_bar[next], next_ph);
+                    const uint32_t tmem_d = tmem_base + buf * (uint32_t)BN;
+                    for (int k = 0; k < t.nk; k += L::kSub) {
+                        // consumers wait longer than producers, so that the wait that reports is the one at the root
+                        if (!have && !mbar_wait(&full_bar[s], ph, limit_ns * 2)) {
+                            atomicCAS(p.err_flag, 0u, 22u);
+                            ok = false;
+                            break;
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t next = s + 1 == L::kStages ? 0 : s + 1, next_ph = next == 0 ? ph ^ 1u : ph;
+                        const uint64_t da = desc_a + s * (uint32_t)(L::kSub * L::kStageBytes >> 4), db = desc_b + s * (uint32_t)(L::kSub * L::kStageBytes >> 4);
+                        umma_bf16_pair(tmem_d, da, db, idesc, k ? 1u : 0u);
 #pragma unroll
-                    for (int u = 1; u < BK / UMMA_K; ++u) umma_bf16_pair(tmem_d, da + u * 2, db + u * kNextB, idesc, 1u);
-                    umma_commit_pair(&empty_bar[s]);   // frees the stage in both CTAs when these MMAs have read it
-                    s = next;
-                    ph = next_ph;
+                        for (int u = 1; u < BK / UMMA_K; ++u) umma_bf16_pair(tmem_d, da + u * 2, db + u * kNextB, idesc, 1u);
+                        have = mbar_try_wait(&full_bar[next], next_ph);
+                        if (k + 1 < t.nk) {
+#pragma unroll
+                            for (int u = 0; u < BK / UMMA_K; ++u)
+                                umma_bf16_pair(tmem_d, da + (L::kStageBytes >> 4) + u * 2, db + (L::kStageBytes >> 4) + u * kNextB, idesc, 1u);
+                        }
+                        umma_commit_pair(&empty_bar[s]);   // frees the stage in both CTAs when these MMAs have read it
+                        s = next;
+                        ph = next_ph;
+                    }
+                    umma_commit_pair(&tfull_bar[buf]);     // (also on error, so that the epilogue moves on)
+                    ++tc;
                 }
-                umma_commit_pair(&tfull_bar[buf]);     // (also on error, so that the epilogue moves on)
-                ++tc;
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLinRegsEpilogue));
         // ---- epilogue ----
-        const int ew = warp - 2, quarter = warp & 3, half = ew >> 2, etid = ew * 32 + lane;
+        const int ew = warp - 4, quarter = warp & 3, half = ew >> 2, etid = ew * 32 + lane;
         constexpr int kPieces = BN / 64;   // 32-column pieces of a warp
         uint8_t* stage = stage_out + ew * 2048;
         TileWalk walk(p.grid, pair);
@@ -341,9 +365,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     bs[etid] = v;
                 }
             }
-            // What a piece needs from memory (residual, or h) is requested one piece ahead, the first one before the wait
-            // for the accumulator.
-            uint4 aux[4];
+            // What a piece needs from memory (residual, or h) is requested before the piece ahead of it is worked on, the first
+            // one before the wait for the accumulator.
+            uint4 aux[4], coming[4];
             uint32_t ex = 0;
             const __nv_bfloat16* aux_row = DGRAD ? p.pre : p.res;
             const int64_t aux_ld = DGRAD ? p.ldpre : p.ldres;
@@ -351,17 +375,17 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             const bool kept8 = DGRAD && p.q != nullptr;
             auto fetch = [&](int c) {
                 const int col = colw + c * 32;
-                if (!live || col >= p.N) return;
+                if (!live || c >= kPieces || col >= p.N) return;
                 if (kept8) {
                     const int8_t* qp = p.q + (int64_t)row * p.ldq + col;
-                    aux[0] = ld_nc_v4(qp);
-                    if (col + 16 < p.N) aux[1] = ld_nc_v4(qp + 16);
+                    coming[0] = ld_nc_v4(qp);
+                    if (col + 16 < p.N) coming[1] = ld_nc_v4(qp + 16);
                 } else if (aux_row != nullptr) {
-                    load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, aux_vec, aux);
+                    load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, aux_vec, coming);
                 }
             };
 #pragma unroll
-            for (int j = 0; j < 4; ++j) aux[j] = make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < 4; ++j) coming[j] = make_uint4(0, 0, 0, 0);
             if (t.runs == 1) fetch(0);
             if (kept8 && live && colw < p.N) {   // one byte per piece; rows of e are padded to 16
                 if constexpr (kPieces == 4) ex = *(const uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32);
@@ -393,6 +417,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             uint32_t ewrite = 0;
             auto finish = [&](float* f, int c) {
                 const int col = colw + c * 32;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) aux[j] = coming[j];
+                fetch(c + 1);
                 if constexpr (!DGRAD) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
@@ -407,27 +434,32 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
 #pragma unroll
                         for (int j = 0; j < 32; ++j) f[j] += bf16_at(aux, j);
                     }
-                    if (c + 1 < kPieces) fetch(c + 1);
                 } else {
                     float a[32];
-                    const float step = act8_step((ex >> (8 * c)) & 255u);
+                    if (kept8) {
+                        const float step = act8_step((ex >> (8 * c)) & 255u);
+                        const uint32_t w[8] = {aux[0].x, aux[0].y, aux[0].z, aux[0].w, aux[1].x, aux[1].y, aux[1].z, aux[1].w};
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float h;
-                        if (kept8) {
-                            const uint4 v = aux[j / 16];
-                            const uint32_t w = (j / 4) % 4 == 0 ? v.x : (j / 4) % 4 == 1 ? v.y : (j / 4) % 4 == 2 ? v.z : v.w;
-                            h = s8_at(w, j % 4) * step;
-                        } else {
-                            h = bf16_at(aux, j);
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t biased = w[j] ^ 0x80808080u;
+                            f[4 * j] *= act_slope<ACT>(s8_of_biased<0>(biased) * step, &a[4 * j]);
+                            f[4 * j + 1] *= act_slope<ACT>(s8_of_biased<1>(biased) * step, &a[4 * j + 1]);
+                            f[4 * j + 2] *= act_slope<ACT>(s8_of_biased<2>(biased) * step, &a[4 * j + 2]);
+                            f[4 * j + 3] *= act_slope<ACT>(s8_of_biased<3>(biased) * step, &a[4 * j + 3]);
                         }
-                        f[j] *= act_slope<ACT>(h, &a[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] *= act_slope<ACT>(bf16_at(aux, j), &a[j]);
                     }
-                    if (c + 1 < kPieces) fetch(c + 1);
                     if (p.out2 != nullptr) store_piece(stage, lane, a, p.out2, p.ldo2, row0, col, p.M, p.N, p.out2_vec != 0);
                 }
                 store_piece(stage, lane, f, p.out, p.ldo, row0, col, p.M, p.N, p.out_vec != 0);
             };
+            if (row0 >= p.M) {   // nothing of this warp's 32 rows exists (few rows, or the last tile's second half)
+                release();
+                ++tc;
+                continue;
+            }
             uint32_t v[32];
             if (t.runs == 1) {
                 if (colw < p.N) tmem_ld32_issue(taddr, v);
@@ -565,7 +597,7 @@ int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
     int pairs = 0;
     cudaError_t e = pairs_of<kern>(kLinThreads, LinSmem<BN>::kTotal, &pairs);
     if (e != cudaSuccess) return (int)e;
-    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 12);
+    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 64);
     return (int)launch_pairs(kern, kLinThreads, LinSmem<BN>::kTotal, p.grid.pairs, p, s);
 }
 

@@ -156,8 +156,10 @@ def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = N
     if tokens == 0:
         return out if accumulate else out.zero_()
     if n and k:
+        need = C.act8_wgrad_scratch(tokens, n, k)
+        scratch = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
         check(C.act8_wgrad(dy2.data_ptr(), _ld(dy2), *x8.args(), out.data_ptr(), row_stride(out), accumulate,
                            0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-                           0 if dy_sum is None else dy_sum.data_ptr(), tokens, n, k, workspace(dy.get_device(), s).data_ptr(),
+                           0 if dy_sum is None else dy_sum.data_ptr(), tokens, n, k, 0 if scratch is None else scratch.data_ptr(), workspace(dy.get_device(), s).data_ptr(),
                            _err_flag(dy.device).data_ptr(), wait_limit_s, s), what)
     return out
