@@ -55,12 +55,6 @@ __device__ __forceinline__ float s8_of_biased(uint32_t biased) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-__device__ __forceinline__ uint32_t pack_s8x4(int a, int b, int c, int d) {
-    return __byte_perm(__byte_perm((uint32_t)a, (uint32_t)b, 0x0040), __byte_perm((uint32_t)c, (uint32_t)d, 0x0040), 0x5410);
-}
-// byte i of a word as a signed number
-__device__ __forceinline__ float s8_at(uint32_t w, int i) { return (float)(int)(int8_t)(w >> (8 * i)); }
-
 }  // namespace
 
 }  // namespace psb

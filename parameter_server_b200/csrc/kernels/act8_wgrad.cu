@@ -476,7 +476,7 @@ int launch_wgrad(WgParams& p, int64_t tokens, cudaStream_t s) {
     int pairs = 0;
     cudaError_t e = pairs_of<kern>(kWgThreads, WgSmem<CONVERT>::kTotal, &pairs);
     if (e != cudaSuccess) return (int)e;
-    p.grid = plan_tiles((p.N + 2 * BM - 1) / (2 * BM), (p.K + kWgBN - 1) / kWgBN, (int)((tokens + BK - 1) / BK), pairs, 48);
+    p.grid = plan_tiles((p.N + 2 * BM - 1) / (2 * BM), (p.K + kWgBN - 1) / kWgBN, (int)((tokens + BK - 1) / BK), pairs, 48, 8);
     return (int)launch_pairs(kern, kWgThreads, WgSmem<CONVERT>::kTotal, p.grid.pairs, p, s);
 }
 

@@ -597,7 +597,11 @@ int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
     int pairs = 0;
     cudaError_t e = pairs_of<kern>(kLinThreads, LinSmem<BN>::kTotal, &pairs);
     if (e != cudaSuccess) return (int)e;
-    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 64);
+    // A weight that L2 holds beside the stream of activations is walked along n (16384 x 2048 x 8192 with a residual, sustained:
+    // 429 us, in groups of 8 rows 441); a larger one in blocks (8192^3: 844 us, along n 923).
+    const int group = (int64_t)p.N * k_steps * BK * 2 <= (48ll << 20) ? 1 : 8;
+    // Joining a cut tile takes 10 to 20 us (its parts are read one after the other, eight 16-byte loads in flight per thread).
+    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 64, group);
     return (int)launch_pairs(kern, kLinThreads, LinSmem<BN>::kTotal, p.grid.pairs, p, s);
 }
 

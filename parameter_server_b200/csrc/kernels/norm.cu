@@ -47,6 +47,7 @@ struct Io<__nv_bfloat16, 8> {
         *(uint4*)p = r;
     }
     static __device__ __forceinline__ Raw zero() { return make_uint4(0, 0, 0, 0); }
+    static __device__ __forceinline__ Raw one() { return make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u); }
 };
 template <>
 struct Io<float, 4> {
@@ -55,6 +56,7 @@ struct Io<float, 4> {
     static __device__ __forceinline__ void unpack(const Raw& r, float* f) { f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w; }
     static __device__ __forceinline__ void store(float* p, const float* f) { *(float4*)p = make_float4(f[0], f[1], f[2], f[3]); }
     static __device__ __forceinline__ Raw zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+    static __device__ __forceinline__ Raw one() { return make_float4(1.f, 1.f, 1.f, 1.f); }
 };
 template <>
 struct Io<__nv_bfloat16, 1> {
@@ -63,6 +65,7 @@ struct Io<__nv_bfloat16, 1> {
     static __device__ __forceinline__ void unpack(const Raw& r, float* f) { f[0] = __bfloat162float(r); }
     static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) { *p = __float2bfloat16_rn(f[0]); }
     static __device__ __forceinline__ Raw zero() { return __float2bfloat16_rn(0.f); }
+    static __device__ __forceinline__ Raw one() { return __float2bfloat16_rn(1.f); }
 };
 template <>
 struct Io<float, 1> {
@@ -71,25 +74,33 @@ struct Io<float, 1> {
     static __device__ __forceinline__ void unpack(const Raw& r, float* f) { f[0] = r; }
     static __device__ __forceinline__ void store(float* p, const float* f) { *p = f[0]; }
     static __device__ __forceinline__ Raw zero() { return 0.f; }
+    static __device__ __forceinline__ Raw one() { return 1.f; }
 };
 
 // VEC consecutive whole numbers of a checkpoint row
 template <int VEC>
 struct Q8;
+__device__ __forceinline__ void unpack_word(uint32_t w, float step, float* f) {
+    const uint32_t biased = w ^ 0x80808080u;
+    f[0] = s8_of_biased<0>(biased) * step;
+    f[1] = s8_of_biased<1>(biased) * step;
+    f[2] = s8_of_biased<2>(biased) * step;
+    f[3] = s8_of_biased<3>(biased) * step;
+}
+__device__ __forceinline__ uint32_t pack_word(const float* f, uint32_t e, float inverse_step) {
+    return e == 255u ? 0u : act8_quantise4(f[0], f[1], f[2], f[3], inverse_step);
+}
 template <>
 struct Q8<8> {
     using Raw = uint2;
     static __device__ __forceinline__ Raw load(const int8_t* p) { return *(const uint2*)p; }
     static __device__ __forceinline__ Raw zero() { return make_uint2(0, 0); }
     static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[i] = s8_at(r.x, i) * step;
-            f[4 + i] = s8_at(r.y, i) * step;
-        }
+        unpack_word(r.x, step, f);
+        unpack_word(r.y, step, f + 4);
     }
-    static __device__ __forceinline__ void store(int8_t* p, const int* q) {
-        *(uint2*)p = make_uint2(pack_s8x4(q[0], q[1], q[2], q[3]), pack_s8x4(q[4], q[5], q[6], q[7]));
+    static __device__ __forceinline__ void store(int8_t* p, const float* f, uint32_t e, float inv) {
+        *(uint2*)p = make_uint2(pack_word(f, e, inv), pack_word(f + 4, e, inv));
     }
 };
 template <>
@@ -97,11 +108,8 @@ struct Q8<4> {
     using Raw = uint32_t;
     static __device__ __forceinline__ Raw load(const int8_t* p) { return *(const uint32_t*)p; }
     static __device__ __forceinline__ Raw zero() { return 0u; }
-    static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = s8_at(r, i) * step;
-    }
-    static __device__ __forceinline__ void store(int8_t* p, const int* q) { *(uint32_t*)p = pack_s8x4(q[0], q[1], q[2], q[3]); }
+    static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) { unpack_word(r, step, f); }
+    static __device__ __forceinline__ void store(int8_t* p, const float* f, uint32_t e, float inv) { *(uint32_t*)p = pack_word(f, e, inv); }
 };
 template <>
 struct Q8<1> {
@@ -109,116 +117,160 @@ struct Q8<1> {
     static __device__ __forceinline__ Raw load(const int8_t* p) { return *p; }
     static __device__ __forceinline__ Raw zero() { return 0; }
     static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) { f[0] = (float)r * step; }
-    static __device__ __forceinline__ void store(int8_t* p, const int* q) { *p = (int8_t)q[0]; }
+    static __device__ __forceinline__ void store(int8_t* p, const float* f, uint32_t, float inv) { *p = (int8_t)act8_quantise(f[0], inv); }
 };
+
+// Copies of a thread's own 4, 8 or 16 bytes from global to shared memory, any number in flight; a group is what was issued since
+// the group before.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+template <typename V>
+__device__ __forceinline__ V from_shared(uint32_t addr) { return *(const V*)__cvta_shared_to_generic(addr); }
+__device__ __forceinline__ void close_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void wait_groups() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return v;
 }
-// largest bits among the lanes that share a block of 32 columns (32 / VEC neighbours; all lanes of the warp call)
+// exponent of the block of 32 columns that 32 / VEC neighbouring lanes share (all lanes of the warp call)
 template <int VEC>
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+__device__ __forceinline__ uint32_t block_exponent(const float* f, bool valid) {
+    float m = 0.f;
+    if (valid) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = abs_max(m, f[j]);
+    }
+    uint32_t v = abs_bits(m);
 #pragma unroll
     for (int o = kAct8Block / VEC / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    return v;
+    return act8_exponent(v);
 }
 
 // Quantises the VEC values of this thread (col = first column; all lanes of the warp call, `valid` false past the row).
 template <int VEC>
 __device__ __forceinline__ void keep8(const float* f, bool valid, int8_t* qrow, uint8_t* erow, int col) {
-    uint32_t m = 0;
-    if (valid) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(f[j]));
-    }
-    const uint32_t e = act8_exponent(block_max<VEC>(m));
+    const uint32_t e = block_exponent<VEC>(f, valid);
     if (!valid) return;
-    const float inv = act8_inverse_step(e);
-    int q[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) q[j] = act8_quantise(f[j], inv);
-    Q8<VEC>::store(qrow + col, q);
+    Q8<VEC>::store(qrow + col, f, e, act8_inverse_step(e));
     if (col % kAct8Block == 0) erow[col / kAct8Block] = (uint8_t)e;
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
 // `tpr` threads (a power of two, 32..512) hold one row in registers, NV vectors each: thread t has the columns
-// (i * tpr + t) * VEC. A warp per row needs no barrier and is taken while its 64 values a lane fit (d <= 2048 in bf16);
-// with few rows a row is spread over as many threads as have a vector each, since then the latency of one row is the time.
+// (i * tpr + t) * VEC, and its part of weight and bias, packed, over all rows. (A warp per row up to d = 2048 needs no barrier,
+// but its 64 values a lane leave no registers for the weight, and 4 warps per scheduler do not hide its loads: 39 us.)
+// With few rows a row is spread over as many threads as have a vector each, since then the latency of one row is the time.
+// CTAs are persistent, and a thread copies its part of the next two rows to shared memory while it works on this one (only
+// the thread itself reads it, so no barrier is involved): with loads straight into registers a row's arithmetic and the next
+// row's latency add up (16384 x 2048: 35 us). Rows that are not 16-byte aligned (VEC 1) are read that way all the same.
+constexpr int kFwdSlots = 3;
 template <typename T, int VEC, int NV, bool OUT8>
 __global__ void __launch_bounds__(kMaxTeam)
 layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, T* __restrict__ y,
                       int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
                       int64_t lde, int64_t rows, int d, float eps, int tpr) {
+    constexpr bool kAsync = VEC > 1;
+    using IO = Io<T, VEC>;
+    extern __shared__ uint4 ring[];   // [kFwdSlots][NV][threads]
     __shared__ float red[2][kMaxTeam / 32];
     const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
-    const int64_t row = (int64_t)blockIdx.x * teams + team;
-    const bool live = row < rows;
-    const T* xr = x + (live ? row : 0) * ldx;
-    typename Io<T, VEC>::Raw raw[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int col = (i * tpr + t) * VEC;
-        raw[i] = live && col < d ? Io<T, VEC>::load(xr + col) : Io<T, VEC>::zero();
-    }
-    float v[NV * VEC];
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        Io<T, VEC>::unpack(raw[i], v + i * VEC);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += v[i * VEC + j];
-    }
     const int warps = tpr / 32, w0 = team * warps;
-    auto team_sum = [&](float part, int k) -> float {
-        part = warp_sum(part);
-        if (warps == 1) return part;
-        if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = part;
-        __syncthreads();
-        float all = 0.f;
-        for (int w = 0; w < warps; ++w) all += red[k][w0 + w];
-        return all;
-    };
-    const float mean = team_sum(s, 0) / (float)d;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const bool in = (i * tpr + t) * VEC < d;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            v[i * VEC + j] -= mean;
-            if (in) s += v[i * VEC + j] * v[i * VEC + j];
-        }
-    }
-    const float rstd = rsqrtf(team_sum(s, 1) / (float)d + eps);
-    if (live && t == 0) {
-        if (mean_out != nullptr) mean_out[row] = mean;
-        rstd_out[row] = rstd;
-    }
+    const int64_t step = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams;
+    typename IO::Raw graw[NV], braw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int col = (i * tpr + t) * VEC;
-        const bool in = live && col < d;
-        float* f = v + i * VEC;
+        graw[i] = weight != nullptr && col < d ? IO::load(weight + col) : IO::one();
+        braw[i] = bias != nullptr && col < d ? IO::load(bias + col) : IO::zero();
+    }
+    // running positions: a row's overhead is shared by 32 values only
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16, vec_stride = blockDim.x * 16, slot_stride = NV * vec_stride;
+    const T* ahead = x + (first + team) * ldx + t * VEC;
+    int64_t ahead_row = first + team;
+    auto request = [&](int slot) {   // the next row that has not been asked for
+        if (ahead_row < rows) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] *= rstd;
-        if constexpr (OUT8) keep8<VEC>(f, in, q + (live ? row : 0) * ldq, e + (live ? row : 0) * lde, col);
-        if (!in) continue;
-        if (weight != nullptr) {
-            float g[VEC];
-            Io<T, VEC>::unpack(Io<T, VEC>::load(weight + col), g);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] *= g[j];
+            for (int i = 0; i < NV; ++i)
+                if ((i * tpr + t) * VEC < d) copy_async<16>(mine + slot * slot_stride + i * vec_stride, ahead + i * tpr * VEC);
         }
-        if (bias != nullptr) {
-            float b[VEC];
-            Io<T, VEC>::unpack(Io<T, VEC>::load(bias + col), b);
+        close_group();   // (an empty group where there is no such row: the count of groups stays the same)
+        ahead += step * ldx;
+        ahead_row += step;
+    };
+    int slot = 0;
+    if constexpr (kAsync) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] += b[j];
+        for (int k = 0; k < kFwdSlots - 1; ++k) request(k);
+    }
+    for (int64_t base = first; base < rows; base += step) {
+        const int64_t row = base + team;
+        const bool live = row < rows;
+        float v[NV * VEC];
+        if constexpr (kAsync) {
+            request(slot == 0 ? kFwdSlots - 1 : slot - 1);
+            wait_groups<kFwdSlots - 1>();
         }
-        Io<T, VEC>::store(y + row * ldy + col, f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * tpr + t) * VEC;
+            typename IO::Raw raw = IO::zero();
+            if (live && col < d) {
+                if constexpr (kAsync) raw = from_shared<typename IO::Raw>(mine + slot * slot_stride + i * vec_stride);
+                else raw = IO::load(x + row * ldx + col);
+            }
+            IO::unpack(raw, v + i * VEC);
+        }
+        slot = slot + 1 == kFwdSlots ? 0 : slot + 1;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) s += v[i];
+        auto team_sum = [&](float part, int k) -> float {
+            part = warp_sum(part);
+            if (warps == 1) return part;
+            if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = part;
+            __syncthreads();
+            float all = 0.f;
+            for (int w = 0; w < warps; ++w) all += red[k][w0 + w];
+            return all;
+        };
+        const float mean = team_sum(s, 0) / (float)d;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool in = (i * tpr + t) * VEC < d;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[i * VEC + j] -= mean;
+                if (in) s += v[i * VEC + j] * v[i * VEC + j];
+            }
+        }
+        const float rstd = rsqrtf(team_sum(s, 1) / (float)d + eps);
+        if (live && t == 0) {
+            if (mean_out != nullptr) mean_out[row] = mean;
+            rstd_out[row] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * tpr + t) * VEC;
+            const bool in = live && col < d;
+            float* f = v + i * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] *= rstd;
+            if constexpr (OUT8) keep8<VEC>(f, in, q + (live ? row : 0) * ldq, e + (live ? row : 0) * lde, col);
+            if (!in) continue;
+            float g[VEC], b[VEC];
+            IO::unpack(graw[i], g);
+            IO::unpack(braw[i], b);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = fmaf(f[j], g[j], b[j]);
+            IO::store(y + row * ldy + col, f);
+        }
     }
 }
 
@@ -267,11 +319,22 @@ layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __rest
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
-// Persistent CTAs (one per SM) of blockDim / tpr teams; a team walks rows R at a time and thread t keeps the sums of its 16
-// columns' dweight and dbias in registers over all of them, so that the weight's gradient costs no second pass over dy and
-// x. The two row sums cross the team's warps through shared memory with one barrier for R rows. At the end the teams' sums
-// are added in team order and leave as one partial row per CTA, which column_reduce_kernel adds in CTA order: the result
-// does not depend on timing. (More CTAs per SM would write and read more partial rows: 2 * d floats each.)
+// Persistent CTAs (one per SM) of blockDim / tpr teams; a team walks rows and thread t keeps the sums of its 16 columns'
+// dweight and dbias in registers over all of them, so that the weight's gradient costs no second pass over dy and x. The
+// next rows are copied to shared memory meanwhile, every thread its own part (see the forward kernel; loads into registers
+// left room for one row in flight and took 67 us for 16384 x 2048 with a residual gradient). The two row sums cross the
+// team's warps through shared memory with one barrier per row. At the end the teams' sums are added in team order and leave
+// as one partial row per CTA, which column_reduce_kernel adds in CTA order: the result does not depend on timing. (More CTAs
+// per SM would write and read more partial rows: 2 * d floats each.)
+template <typename T, int VEC, bool SRC8>
+struct BwdRing {
+    static constexpr int kVecs = kBwdElems / VEC;
+    static constexpr int kSlots = sizeof(T) == 2 ? 3 : 2;
+    // per thread and slot: dy, the residual's gradient, and x or (8 or 4 bytes a vector) q with a word of exponents
+    static constexpr int kRowBytes = SRC8 ? kVecs * (32 + VEC + 4) : kVecs * 48;
+    static constexpr int kBytes = VEC > 1 ? kSlots * kRowBytes * kBwdThreads : 0;
+};
+
 template <typename T, int VEC, bool SRC8>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
@@ -279,10 +342,11 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const T* __restrict__ join, int64_t ldjoin,
                       T* __restrict__ dx, int64_t lddx, float* __restrict__ partial, int64_t rows, int d, int tpr) {
     constexpr int NV = kBwdElems / VEC;
-    constexpr int R = 1;   // rows in flight per team (registers: raw dy, x and join of R rows)
+    constexpr bool kAsync = VEC > 1;
     using IO = Io<T, VEC>;
-    extern __shared__ float comb[];             // [2][d], for the teams' sums at the end
-    __shared__ float red[2][kBwdThreads / 32][2 * R];
+    using Ring = BwdRing<T, VEC, SRC8>;
+    extern __shared__ uint4 ring_raw[];         // the ring; at the end [2][d] sums of the teams
+    __shared__ float red[2][kBwdThreads / 32][2];
     const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
     const int warps = tpr / 32, w0 = team * warps, lane = threadIdx.x & 31;
     float dg[kBwdElems], db[kBwdElems];
@@ -292,108 +356,153 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int col = (i * tpr + t) * VEC;
-        graw[i] = weight != nullptr && col < d ? IO::load(weight + col) : IO::zero();
+        graw[i] = weight != nullptr && col < d ? IO::load(weight + col) : IO::one();
     }
-    const bool has_w = weight != nullptr;
     const float inv_d = 1.f / (float)d;
-    int buf = 0;
-    for (int64_t r0 = ((int64_t)blockIdx.x * teams + team) * R; r0 < rows; r0 += (int64_t)gridDim.x * teams * R, buf ^= 1) {
-        typename IO::Raw ry[R][NV], rx[R][NV], rj[R][NV];
-        typename Q8<VEC>::Raw rq[R][NV];
-        uint32_t re[R][NV];
-        float mean[R], rstd[R];
+    // Running positions: a row's overhead is shared by 16 values only. In a slot the thread's vectors of dy, of the residual's
+    // gradient, and of x (or of q and the exponents' words) follow one another with `n` threads between them.
+    const uint32_t n = blockDim.x, base = (uint32_t)__cvta_generic_to_shared(ring_raw);
+    const uint32_t my16 = base + threadIdx.x * 16;
+    const uint32_t ring2 = base + Ring::kSlots * 2 * NV * n * 16;
+    const uint32_t my_q = ring2 + threadIdx.x * VEC, my_e = ring2 + Ring::kSlots * NV * n * VEC + threadIdx.x * 4;
+    auto at_y = [&](int s, int i) { return my16 + (uint32_t)((s * 2 + 0) * NV + i) * n * 16; };
+    auto at_j = [&](int s, int i) { return my16 + (uint32_t)((s * 2 + 1) * NV + i) * n * 16; };
+    auto at_x = [&](int s, int i) { return my16 + (uint32_t)(Ring::kSlots * 2 * NV + s * NV + i) * n * 16; };
+    auto at_q = [&](int s, int i) { return my_q + (uint32_t)(s * NV + i) * n * VEC; };
+    auto at_e = [&](int s, int i) { return my_e + (uint32_t)(s * NV + i) * n * 4; };
+    const int64_t step = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + team;
+    const int c0 = t * VEC;
+    const T *ahead_y = dy + first * lddy + c0, *ahead_x = SRC8 ? nullptr : x + first * ldx + c0, *ahead_j = join != nullptr ? join + first * ldjoin + c0 : nullptr;
+    const int8_t* ahead_q = SRC8 ? q + first * ldq + c0 : nullptr;
+    const uint8_t* ahead_e = SRC8 ? e + first * lde : nullptr;
+    int64_t ahead_row = first;
+    auto request = [&](int s) {   // the next row that has not been asked for
+        if constexpr (kAsync) {
+            if (ahead_row < rows) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = r0 + r;
-            const bool live = row < rows;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int col = (i * tpr + t) * VEC;
-                const bool in = live && col < d;
-                ry[r][i] = in ? IO::load(dy + row * lddy + col) : IO::zero();
-                if constexpr (SRC8) {
-                    rq[r][i] = in ? Q8<VEC>::load(q + row * ldq + col) : Q8<VEC>::zero();
-                    re[r][i] = in ? e[row * lde + col / kAct8Block] : 0u;
-                } else {
-                    rx[r][i] = in ? IO::load(x + row * ldx + col) : IO::zero();
+                for (int i = 0; i < NV; ++i) {
+                    const int off = i * tpr * VEC;
+                    if (c0 + off >= d) continue;
+                    copy_async<16>(at_y(s, i), ahead_y + off);
+                    if (join != nullptr) copy_async<16>(at_j(s, i), ahead_j + off);
+                    if constexpr (SRC8) {
+                        copy_async<VEC>(at_q(s, i), ahead_q + off);
+                        copy_async<4>(at_e(s, i), ahead_e + (c0 + off) / (4 * kAct8Block) * 4);   // the exponents of 128 columns
+                    } else {
+                        copy_async<16>(at_x(s, i), ahead_x + off);
+                    }
                 }
-                if (join != nullptr) rj[r][i] = in ? IO::load(join + row * ldjoin + col) : IO::zero();
             }
-            rstd[r] = live ? rstd_in[row] : 0.f;
-            mean[r] = !SRC8 && live ? mean_in[row] : 0.f;
-        }
-        // this thread's part of vector i of row r: gradient, and normalised value (0 past the row's end: rstd * (0 - mean) is not)
-        auto values = [&](int r, int i, float* fy, float* fh) {
-            IO::unpack(ry[r][i], fy);
+            close_group();
+            ahead_row += step;
+            ahead_y += step * lddy;
             if constexpr (SRC8) {
-                Q8<VEC>::unpack(rq[r][i], act8_step(re[r][i]), fh);
+                ahead_q += step * ldq;
+                ahead_e += step * lde;
             } else {
-                IO::unpack(rx[r][i], fh);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) fh[j] = (fh[j] - mean[r]) * rstd[r];
+                ahead_x += step * ldx;
             }
-        };
-        float sums[2 * R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float fy[VEC], fh[VEC], g[VEC];
-                values(r, i, fy, fh);
-                IO::unpack(graw[i], g);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int c = i * VEC + j;
-                    const float p = has_w ? fy[j] * g[j] : fy[j];
-                    dg[c] += fy[j] * fh[j];
-                    db[c] += fy[j];
-                    s1 += p;
-                    s2 += p * fh[j];
-                }
-            }
-            sums[2 * r] = warp_sum(s1);
-            sums[2 * r + 1] = warp_sum(s2);
+            if (join != nullptr) ahead_j += step * ldjoin;
         }
+    };
+#pragma unroll
+    for (int k = 0; k < Ring::kSlots - 1; ++k) request(k);
+    T* dx_row = dx + first * lddx + c0;
+    float next_rstd = first < rows ? rstd_in[first] : 0.f, next_mean = !SRC8 && first < rows ? mean_in[first] : 0.f;
+    int buf = 0, slot = 0;
+    for (int64_t row = first; row < rows; row += step, buf ^= 1) {
+        request(slot == 0 ? Ring::kSlots - 1 : slot - 1);
+        const float rstd = next_rstd, mean = next_mean;
+        if (row + step < rows) {
+            next_rstd = rstd_in[row + step];
+            if constexpr (!SRC8) next_mean = mean_in[row + step];
+        }
+        if constexpr (kAsync) wait_groups<Ring::kSlots - 1>();
+        typename IO::Raw ry[NV], rx[NV];
+        typename Q8<VEC>::Raw rq[NV];
+        float rs[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * tpr + t) * VEC;
+            const bool in = col < d;
+            if constexpr (kAsync) ry[i] = in ? from_shared<typename IO::Raw>(at_y(slot, i)) : IO::zero();
+            else ry[i] = in ? IO::load(dy + row * lddy + col) : IO::zero();
+            if constexpr (SRC8) {
+                if constexpr (kAsync) {
+                    rq[i] = in ? from_shared<typename Q8<VEC>::Raw>(at_q(slot, i)) : Q8<VEC>::zero();
+                    rs[i] = in ? act8_step((from_shared<uint32_t>(at_e(slot, i)) >> (8 * ((col / kAct8Block) & 3))) & 255u) : 0.f;
+                } else {
+                    rq[i] = in ? Q8<VEC>::load(q + row * ldq + col) : Q8<VEC>::zero();
+                    rs[i] = in ? act8_step(e[row * lde + col / kAct8Block]) : 0.f;
+                }
+            } else {
+                if constexpr (kAsync) rx[i] = in ? from_shared<typename IO::Raw>(at_x(slot, i)) : IO::zero();
+                else rx[i] = in ? IO::load(x + row * ldx + col) : IO::zero();
+            }
+        }
+        float p[kBwdElems], xh[kBwdElems];   // dy * weight and the normalised values (past the row's end the gradient is 0)
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float fy[VEC], g[VEC], *fh = xh + i * VEC;
+            IO::unpack(ry[i], fy);
+            if constexpr (SRC8) {
+                Q8<VEC>::unpack(rq[i], rs[i], fh);
+            } else {
+                IO::unpack(rx[i], fh);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) fh[j] = (fh[j] - mean) * rstd;
+            }
+            IO::unpack(graw[i], g);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int c = i * VEC + j;
+                p[c] = fy[j] * g[j];
+                dg[c] = fmaf(fy[j], fh[j], dg[c]);
+                db[c] += fy[j];
+                s1 += p[c];
+                s2 = fmaf(p[c], fh[j], s2);
+            }
+        }
+        s1 = warp_sum(s1);
+        s2 = warp_sum(s2);
         if (warps > 1) {
             if (lane == 0) {
-#pragma unroll
-                for (int k = 0; k < 2 * R; ++k) red[buf][threadIdx.x >> 5][k] = sums[k];
+                red[buf][threadIdx.x >> 5][0] = s1;
+                red[buf][threadIdx.x >> 5][1] = s2;
             }
             asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(tpr) : "memory");
-#pragma unroll
-            for (int k = 0; k < 2 * R; ++k) sums[k] = 0.f;
+            s1 = s2 = 0.f;
             for (int w = 0; w < warps; ++w) {
-#pragma unroll
-                for (int k = 0; k < 2 * R; ++k) sums[k] += red[buf][w0 + w][k];
+                s1 += red[buf][w0 + w][0];
+                s2 += red[buf][w0 + w][1];
             }
         }
+        const float a1 = s1 * inv_d, a2 = s2 * inv_d;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = r0 + r;
-            if (row >= rows) break;
-            const float a1 = sums[2 * r] * inv_d, a2 = sums[2 * r + 1] * inv_d;
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * tpr + t) * VEC;
+            if (col >= d) continue;
+            float o[VEC];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int col = (i * tpr + t) * VEC;
-                if (col >= d) continue;
-                float fy[VEC], fh[VEC], g[VEC], o[VEC];
-                values(r, i, fy, fh);
-                IO::unpack(graw[i], g);
+            for (int j = 0; j < VEC; ++j) o[j] = rstd * (p[i * VEC + j] - fmaf(xh[i * VEC + j], a2, a1));
+            if (join != nullptr) {
+                float fj[VEC];
+                if constexpr (kAsync) IO::unpack(from_shared<typename IO::Raw>(at_j(slot, i)), fj);
+                else IO::unpack(IO::load(join + row * ldjoin + col), fj);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o[j] = rstd[r] * ((has_w ? fy[j] * g[j] : fy[j]) - a1 - fh[j] * a2);
-                if (join != nullptr) {
-                    float fj[VEC];
-                    IO::unpack(rj[r][i], fj);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) o[j] += fj[j];
-                }
-                IO::store(dx + row * lddx + col, o);
+                for (int j = 0; j < VEC; ++j) o[j] += fj[j];
             }
+            IO::store(dx_row + i * tpr * VEC, o);
         }
+        dx_row += step * lddx;
+        slot = slot + 1 == Ring::kSlots ? 0 : slot + 1;
     }
     if (partial == nullptr) return;
+    float* comb = (float*)ring_raw;
     float* out = partial + (int64_t)blockIdx.x * 2 * d;
+    if constexpr (kAsync) wait_groups<0>();
+    __syncthreads();   // the ring is free: its space takes the teams' sums
     for (int k = 0; k < teams; ++k) {
         if (team == k) {
 #pragma unroll
@@ -562,16 +671,9 @@ act8_pack_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, i
         const int64_t col = c0 + i * 32 * VEC;
         float f[VEC];
         Io<T, VEC>::unpack(raw[i], f);
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) m = max(m, abs_bits(f[j]));
-        const uint32_t ex = act8_exponent(block_max<VEC>(m));
+        const uint32_t ex = block_exponent<VEC>(f, true);   // (lanes past the row hold zeros)
         if (col >= cols) continue;
-        const float inv = act8_inverse_step(ex);
-        int n[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) n[j] = act8_quantise(f[j], inv);
-        Q8<VEC>::store(q + row * ldq + col, n);
+        Q8<VEC>::store(q + row * ldq + col, f, ex, act8_inverse_step(ex));
         if (col % kAct8Block == 0) e[row * lde + col / kAct8Block] = (uint8_t)ex;
     }
 }
@@ -617,28 +719,68 @@ bool aligned(int64_t d, std::initializer_list<std::pair<const void*, int64_t>> r
         if (r.first != nullptr && (((uintptr_t)r.first % 16) || (r.second % vec_of<T>()))) return false;
     return true;
 }
-bool kept_ok(const Act8View& k) { return ((uintptr_t)k.q % 16) == 0 && (k.ldq % 16) == 0; }
+bool kept_ok(const Act8View& k) { return ((uintptr_t)k.q % 16) == 0 && (k.ldq % 16) == 0 && ((uintptr_t)k.e % 4) == 0 && (k.lde % 4) == 0; }
+
+template <auto kern>
+struct Kernel {
+    static constexpr auto value = kern;
+};
+// CTAs of `threads` (32 << i) and `smem` bytes that an SM holds; also allows the kernel that much shared memory. Asked once per
+// kernel, device and shape: the driver's answer costs more than a small launch.
+template <auto kern>
+cudaError_t ctas_per_sm(int threads, int smem, int* count) {
+    static int known[16][8] = {}, bytes[16][8] = {};
+    int dev = 0;
+    cudaError_t rc = cudaGetDevice(&dev);
+    if (rc != cudaSuccess) return rc;
+    int i = 0;
+    while ((32 << i) < threads && i < 7) ++i;
+    const bool keep = dev >= 0 && dev < 16;
+    if (keep && known[dev][i] != 0 && bytes[dev][i] == smem) {
+        *count = known[dev][i];
+        return cudaSuccess;
+    }
+    if (smem > 40 * 1024) {   // with the static part more than a launch gets by default; the largest shape so far sets it
+        static int allowed[16] = {};
+        if (!keep || allowed[dev] < smem) {
+            rc = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (rc != cudaSuccess) return rc;
+            if (keep) allowed[dev] = smem;
+        }
+    }
+    rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(count, kern, threads, smem);
+    if (rc != cudaSuccess) return rc;
+    if (*count < 1) return cudaErrorLaunchOutOfResources;
+    if (keep) {
+        known[dev][i] = *count;
+        bytes[dev][i] = smem;
+    }
+    return cudaSuccess;
+}
 
 template <typename T, int VEC, int NV>
 int launch_fwd(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep,
                int64_t rows, int d, float eps, int tpr, cudaStream_t s) {
-    // two rows' worth of warps per CTA at least, four warps: small CTAs so that a wave's end leaves no SM waiting long
-    const int threads = std::max(tpr, 128);
-    const int64_t grid = (rows + threads / tpr - 1) / (threads / tpr);
-    if (grid > 0x7FFFFFFF) return -2;
-    if (keep.q != nullptr)
-        layer_norm_fwd_kernel<T, VEC, NV, true><<<(unsigned)grid, threads, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, (int8_t*)keep.q, keep.ldq,
-                                                                                  (uint8_t*)keep.e, keep.lde, rows, d, eps, tpr);
-    else
-        layer_norm_fwd_kernel<T, VEC, NV, false><<<(unsigned)grid, threads, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, nullptr, 0, nullptr, 0,
-                                                                                   rows, d, eps, tpr);
-    return (int)cudaGetLastError();
+    // a CTA per row where a row takes several warps, so that a barrier stops nobody else
+    const int threads = tpr == 32 ? 128 : tpr, teams = threads / tpr;
+    const int64_t need = (rows + teams - 1) / teams;
+    const int smem = VEC > 1 ? kFwdSlots * NV * threads * 16 : 0;
+    auto go = [&](auto instance) -> int {
+        constexpr auto kern = decltype(instance)::value;
+        int per_sm = 0;
+        const cudaError_t rc = ctas_per_sm<kern>(threads, smem, &per_sm);
+        if (rc != cudaSuccess) return (int)rc;
+        const unsigned grid = (unsigned)std::min<int64_t>(need, (int64_t)per_sm * kSms);   // one wave of CTAs at most
+        kern<<<grid, threads, smem, s>>>(x, ldx, w, b, y, ldy, mean, rstd, (int8_t*)keep.q, keep.ldq, (uint8_t*)keep.e, keep.lde, rows, d, eps, tpr);
+        return (int)cudaGetLastError();
+    };
+    return keep.q != nullptr ? go(Kernel<layer_norm_fwd_kernel<T, VEC, NV, true>>{}) : go(Kernel<layer_norm_fwd_kernel<T, VEC, NV, false>>{});
 }
 
 template <typename T, int VEC>
 int fwd_vec(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep, int64_t rows,
             int d, float eps, cudaStream_t s) {
-    constexpr int NV = VEC == 1 ? 16 : 8;
+    constexpr int NV = VEC == 1 ? 16 : VEC == 4 ? 8 : 4;   // 32 values (16 where they are read one by one)
     const int64_t vecs = (d + VEC - 1) / VEC;
     // fewer rows than SMs x 4: one vector per thread if 512 threads have the row
     if (rows <= 4 * kSms && vecs <= kMaxTeam)
@@ -673,7 +815,7 @@ BwdPlan bwd_plan(int64_t rows, int64_t d) {
     p.fits = d <= (int64_t)kBwdThreads * kBwdElems;
     p.tpr = pow2_at_least((d + kBwdElems - 1) / kBwdElems, 32, kBwdThreads);
     // few rows: one team per CTA until every SM has one
-    const int teams = (int)std::max<int64_t>(1, std::min<int64_t>(kBwdThreads / p.tpr, (rows + 2 * kSms - 1) / (2 * kSms)));
+    const int teams = (int)std::max<int64_t>(1, std::min<int64_t>(kBwdThreads / p.tpr, (rows + kSms - 1) / kSms));
     p.threads = p.tpr * pow2_at_least(teams, 1, kBwdThreads / p.tpr);
     const int64_t need = (rows + p.threads / p.tpr - 1) / (p.threads / p.tpr);
     p.grid = p.fits ? (int)std::max<int64_t>(1, std::min<int64_t>(kSms, need))
@@ -697,9 +839,15 @@ int reduce_partials(const float* partial, int n, int64_t width, int64_t split, f
 template <typename T, int VEC, bool SRC8>
 int launch_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View& k, const T* w, const float* mean, const float* rstd,
                const T* join, int64_t ldjoin, T* dx, int64_t lddx, float* partial, int64_t rows, int d, const BwdPlan& p, cudaStream_t s) {
-    const size_t smem = p.threads > p.tpr ? (size_t)2 * d * sizeof(float) : 0;   // at most 32 KB: several teams means d <= 4096
-    layer_norm_bwd_kernel<T, VEC, SRC8><<<p.grid, p.threads, smem, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, w,
-                                                                        mean, rstd, join, ldjoin, dx, lddx, partial, rows, d, p.tpr);
+    using Ring = BwdRing<T, VEC, SRC8>;
+    constexpr auto kern = layer_norm_bwd_kernel<T, VEC, SRC8>;
+    // the ring, or the teams' sums (several teams means d <= 4096)
+    const int smem = std::max(Ring::kBytes / kBwdThreads * p.threads, p.threads > p.tpr ? 2 * d * (int)sizeof(float) : 0);
+    int per_sm = 0;
+    const cudaError_t rc = ctas_per_sm<kern>(p.threads, smem, &per_sm);
+    if (rc != cudaSuccess) return (int)rc;
+    kern<<<p.grid, p.threads, smem, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, w, mean, rstd, join, ldjoin, dx,
+                                         lddx, partial, rows, d, p.tpr);
     return (int)cudaGetLastError();
 }
 

@@ -13,8 +13,6 @@ namespace psb {
 
 namespace {
 
-constexpr int kRasterGroup = 8;   // m-tiles that are walked together: the tiles in flight form a block of about 8 x 9, whose
-                                  // rows of A and columns of B are read from HBM once and from L2 after that
 constexpr int kMaxPairs = 74;     // 148 SMs
 constexpr int kMaxRuns = 8;       // of one shared tile: bounds the partial tiles that its last pair has to add
 
@@ -23,6 +21,8 @@ struct TileGrid {
     int pairs;      // launched
     int shared;     // tiles [0, shared) are cut into runs
     int len;        // k-steps of a run
+    int group;      // m-tiles that are walked together: with 8 the tiles in flight form a block of about 8 x 9, whose rows of A
+                    // and columns of B come from HBM once; with 1 the walk goes along n, for a B that stays in L2 as a whole
 };
 
 struct Tile {
@@ -64,11 +64,11 @@ struct TileWalk {
             t.runs = 1;
             t.run = t.first = t.slot = t.index = 0;
         }
-        const int per_group = kRasterGroup * g.n_tiles;
+        const int per_group = g.group * g.n_tiles;
         const int group = index / per_group, in = index - group * per_group;
-        const int height = min(kRasterGroup, g.m_tiles - group * kRasterGroup);
+        const int height = min(g.group, g.m_tiles - group * g.group);
         t.n = in / height;
-        t.m = group * kRasterGroup + in - t.n * height;
+        t.m = group * g.group + in - t.n * height;
         return true;
     }
     // the slot of run `r` of the tile (its pair's first place, or the second if the pair began in an earlier tile)
@@ -78,9 +78,10 @@ struct TileWalk {
 };
 
 // Cutting pays when it shortens the last wave by more than the partial tiles cost: a tile's way through memory and its
-// joining take about as long as 12 k-steps of 64 (`min_gain`).
-inline TileGrid plan_tiles(int m_tiles, int n_tiles, int k_steps, int max_pairs, int min_gain) {
+// joining take about as long as `min_gain` k-steps.
+inline TileGrid plan_tiles(int m_tiles, int n_tiles, int k_steps, int max_pairs, int min_gain, int group) {
     TileGrid g;
+    g.group = group;
     g.m_tiles = m_tiles;
     g.n_tiles = n_tiles;
     g.k_steps = k_steps;
