@@ -21,18 +21,25 @@ BLOCK = 32
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
+# (``torch.cuda.current_stream()`` builds a Stream object: 3 us, as much as a small launch)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def launch_stream(t: torch.Tensor) -> int:
     """The current stream's handle; refuses a tensor that lives on another device than the current one."""
     if not t.is_cuda:
         raise ValueError(f"expected CUDA tensors, got one on {t.device}")
-    s = torch.cuda.current_stream()
-    if s.device_index != t.get_device():
-        raise ValueError(f"tensor on cuda:{t.get_device()}, but the current device is cuda:{s.device_index}")
-    return s.cuda_stream
+    d = t.get_device()
+    if d != _current_device():
+        raise ValueError(f"tensor on cuda:{d}, but the current device is cuda:{_current_device()}")
+    return _raw_stream(d)
 
 
 def rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
     """``t`` as a matrix of its rows (last dimension); rows may be strided, values of a row may not."""
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t
     if t.dim() == 0:
         raise ValueError(f"{what}: needs at least one dimension")
     if t.dim() != 2:

@@ -24,7 +24,7 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu":
 def _matrix(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A bf16 operand of the tensor cores: rows on 16-byte boundaries. Rows that are not are copied once, into rows padded to
     8 elements (what a bulk-tensor load asks for)."""
-    if t.dtype != torch.bfloat16 or (like is not None and t.device != like.device):
+    if t.dtype != torch.bfloat16 or (like is not None and t.get_device() != like.get_device()):
         raise ValueError(f"{what}: expected bf16" + ("" if like is None else f" on {like.device}") + f", got {t.dtype} on {t.device}")
     t = rows2d(t, what)
     if row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0:
@@ -89,14 +89,14 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     else:
         r2 = None
     if out is None:
-        y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+        y = x2.new_empty((M, N))
     else:
         if out.shape != lead + (N,) or out.dtype != torch.bfloat16 or out.device != x.device:
             raise ValueError(f"{what}: out must be {tuple(lead) + (N,)} bf16 on {x.device}")
         y = out if out.dim() == 2 else out.view(M, N)
         if N > 1 and y.stride(1) != 1:
             raise ValueError(f"{what}: the values of a row of out must be contiguous")
-    pre = torch.empty((M, N), dtype=torch.bfloat16, device=x.device) if save == "bf16" else None
+    pre = x2.new_empty((M, N)) if save == "bf16" else None
     kept = Act8.empty(M, N, x.device) if save == "act8" else None
     if M and N:
         _launch(False, code, M, N, K, x2, w, bias, r2, y, None, pre, kept, wait_limit_s, s, what)
@@ -136,8 +136,8 @@ def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, A
         pre = rows2d(h, what)
     elif code != 0 or recompute:
         raise ValueError(f"{what}: h is needed")
-    dh = torch.empty((M, N), dtype=torch.bfloat16, device=dy.device)
-    a = torch.empty((M, N), dtype=torch.bfloat16, device=dy.device) if recompute else None
+    dh = dy2.new_empty((M, N))
+    a = dy2.new_empty((M, N)) if recompute else None
     if M and N:
         _launch(True, code, M, N, K, dy2, w, None, None, dh, a, pre, kept, wait_limit_s, s, what)
     if dy.dim() != 2:
@@ -160,6 +160,6 @@ def linear_bias_grad(dy: torch.Tensor, out: Optional[torch.Tensor] = None, accum
         out = torch.empty(n, dtype=torch.float32, device=dy.device)
     elif out.dtype != torch.float32 or out.shape != (n,) or out.device != dy.device or not out.is_contiguous():
         raise ValueError(f"linear_bias_grad: out must be {n} contiguous fp32 values on {dy.device}")
-    partial = torch.empty(C.column_sum_scratch(rows, n), dtype=torch.float32, device=dy.device)
+    partial = dy2.new_empty(C.column_sum_scratch(rows, n), dtype=torch.float32)
     check(C.column_sum(dt, dy2.data_ptr(), row_stride(dy2), rows, n, out.data_ptr(), accumulate, partial.data_ptr(), s), "linear_bias_grad")
     return out

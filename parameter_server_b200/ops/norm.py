@@ -17,12 +17,12 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _param(t: Optional[torch.Tensor], d: int, x: torch.Tensor, what: str) -> Optional[torch.Tensor]:
+def _param(t: Optional[torch.Tensor], d: int, x: torch.Tensor, what: str, name: str) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if t.dtype != x.dtype or t.device != x.device or t.shape != (d,):
-        raise ValueError(f"{what}: expected {d} values of {x.dtype} on {x.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    return t if t.stride(0) == 1 or d == 1 else t.contiguous()
+    if t.dtype != x.dtype or t.dim() != 1 or t.numel() != d or t.get_device() != x.get_device():
+        raise ValueError(f"{what}: {name}: expected {d} values of {x.dtype} on {x.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _forward(x, weight, bias, eps, keep8, what):
@@ -32,16 +32,16 @@ def _forward(x, weight, bias, eps, keep8, what):
     s = launch_stream(x)
     x2 = rows2d(x, what)
     rows, d = x2.shape
-    if d == 0 and x.numel() == 0 and x.shape[-1] == 0:
+    if d == 0:
         raise ValueError(f"{what}: rows of no columns have no mean")
-    weight, bias = _param(weight, d, x, f"{what} weight"), _param(bias, d, x, f"{what} bias")
-    y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    weight, bias = _param(weight, d, x, what, "weight"), _param(bias, d, x, what, "bias")
+    y = torch.empty_like(x2) if x2.is_contiguous() else x2.new_empty((rows, d))
+    rstd = x2.new_empty(rows, dtype=torch.float32)
     if keep8:
         kept, mean = Act8.empty(rows, d, x.device), None
         k = kept.args()
     else:
-        kept, mean = None, torch.empty(rows, dtype=torch.float32, device=x.device)
+        kept, mean = None, torch.empty_like(rstd)
         k = (0, 0, 0, 0)
     check(C.layer_norm_fwd(dt, x2.data_ptr(), row_stride(x2), _ptr(weight), _ptr(bias), y.data_ptr(), d, _ptr(mean), rstd.data_ptr(), *k,
                            rows, d, eps, s), what)
@@ -78,7 +78,7 @@ def _backward(dy, x, kept, weight, mean, rstd, residual_grad, weight_grad, bias_
         x = rows2d(x, what)
     elif kept.rows != rows or kept.cols != d or kept.device != dy.device:
         raise ValueError(f"{what}: checkpoint of {kept.rows} x {kept.cols} on {kept.device}, dy of {rows} x {d} on {dy.device}")
-    weight = _param(weight, d, dy, f"{what} weight")
+    weight = _param(weight, d, dy, what, "weight")
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t is not None and (t.dtype != torch.float32 or t.numel() != rows or t.device != dy.device or not t.is_contiguous()):
             raise ValueError(f"{what}: {name} must be {rows} contiguous fp32 values on {dy.device}")
@@ -92,12 +92,12 @@ def _backward(dy, x, kept, weight, mean, rstd, residual_grad, weight_grad, bias_
         if t is None:
             if accumulate:
                 raise ValueError(f"{what}: accumulate needs {name}")
-            t = torch.empty(d, dtype=torch.float32, device=dy.device)
+            t = dy2.new_empty(d, dtype=torch.float32)
         elif t.dtype != torch.float32 or t.shape != (d,) or t.device != dy.device or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be {d} contiguous fp32 values on {dy.device}")
         grads.append(t)
-    dx = torch.empty((rows, d), dtype=dy.dtype, device=dy.device)
-    partial = torch.empty(C.layer_norm_bwd_scratch(rows, d), dtype=torch.float32, device=dy.device)
+    dx = torch.empty_like(dy2) if dy2.is_contiguous() else dy2.new_empty((rows, d))
+    partial = dy2.new_empty(C.layer_norm_bwd_scratch(rows, d), dtype=torch.float32)
     check(C.layer_norm_bwd(dt, dy2.data_ptr(), row_stride(dy2), _ptr(x), 0 if x is None else row_stride(x),
                            *((0, 0, 0, 0) if kept is None else kept.args()), _ptr(weight), _ptr(mean), rstd.data_ptr(), _ptr(join),
                            0 if join is None else row_stride(join), dx.data_ptr(), d, grads[0].data_ptr(), grads[1].data_ptr(), accumulate,
