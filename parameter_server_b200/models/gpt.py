@@ -7,7 +7,10 @@ reduce-scatter + sharded AdamW kernel. Dense pull of the QKV weights = the all-g
 GEMM (``ops.gemm.ag_linear``): each layer's ``W_qkv`` is its own table with ``scatter_peers=False``, so
 after a push only the owner's rows are current and the first consumer gathers the rest over NVLink while
 it already multiplies the local rows. Attention itself is model code, not a parameter-server path: it uses
-``torch.nn.functional.scaled_dot_product_attention``; layer norm and GELU are torch ops.
+``torch.nn.functional.scaled_dot_product_attention``; layer norm and GELU are torch ops, or, with ``GPTConfig(fused=True)``,
+the block operators of this package: ``ops.norm`` for layer norm, ``ops.linear`` for linear layers with bias, GELU and residual
+in their epilogue. ``act_bits=8`` keeps what the backward pass needs of a block in 8 bits (``ops.act8``): the norms' rows, the
+hidden layer before GELU, and the attention's output.
 
 The reference ships no model code (it is a storage service); this is the dense-table consumer.
 """
@@ -25,7 +28,10 @@ import torch.nn.functional as F
 
 from .._lib import C
 from ..ops import gemm as G
+from ..ops.act8 import act8_pack, act8_wgrad
 from ..ops.dense import DenseTable
+from ..ops.linear import linear_act, linear_act_dgrad, linear_bias_grad
+from ..ops.norm import layer_norm, layer_norm_act8, layer_norm_act8_backward, layer_norm_backward
 from ..ops.sparse import _dist_info, _stream
 
 
@@ -39,6 +45,8 @@ class GPTConfig:
     seq_len: int = 2048
     lr: float = 3e-4
     weight_decay: float = 0.1
+    fused: bool = False   # blocks on ops.norm / ops.linear instead of torch ops around the GEMM
+    act_bits: int = 16    # of what a fused block keeps for its backward pass: 16 or 8
 
     def n_params(self) -> int:
         d, f = self.d_model, self.d_ff
@@ -74,8 +82,138 @@ class _PSLinear(torch.autograd.Function):
         return dx.view(ctx.shape), None, None, None, None, None, None
 
 
+class _Norm:
+    """A layer norm of a fused model between its two passes: what it kept, and its gradients' places in the dense table."""
+
+    def __init__(self, model: "GPT", name: str, x: torch.Tensor):
+        self.P, self.G, self.name = model.main.params, model.main.grads, name
+        self.g, self.b = self.P[f"{name}.g"].detach(), self.P[f"{name}.b"].detach()
+        self.bits = model.cfg.act_bits
+        if self.bits == 8:
+            self.y, self.xhat8, self.rstd = layer_norm_act8(x, self.g, self.b)
+        else:
+            self.y, self.mean, self.rstd = layer_norm(x, self.g, self.b)
+            self.x = x
+
+    def backward(self, dy: torch.Tensor, residual_grad: Optional[torch.Tensor] = None) -> torch.Tensor:
+        kw = dict(residual_grad=residual_grad, weight_grad=self.G[f"{self.name}.g"], bias_grad=self.G[f"{self.name}.b"], accumulate=True)
+        if self.bits == 8:
+            return layer_norm_act8_backward(dy, self.xhat8, self.g, self.rstd, **kw)[0]
+        return layer_norm_backward(dy, self.x, self.g, self.mean, self.rstd, **kw)[0]
+
+    def wgrad(self, dy: torch.Tensor, w_grad: torch.Tensor, b_grad: torch.Tensor) -> None:
+        """Gradients of the linear layer that took ``y``."""
+        if self.bits == 8:
+            db = linear_bias_grad(dy)
+            act8_wgrad(dy, self.xhat8, weight=self.g, bias=self.b, dy_sum=db, out=w_grad, accumulate=True)
+            b_grad.add_(db)
+        else:
+            G.gemm(dy, self.y, a_mn=True, b_mn=True, out=w_grad, accumulate=True)
+            linear_bias_grad(dy, out=b_grad, accumulate=True)
+
+    def drop_y(self) -> None:
+        """The linear layer has run; only a 16-bit model needs ``y`` again."""
+        if self.bits == 8:
+            self.y = None
+
+
+class _AttentionHalf(torch.autograd.Function):
+    """x + proj(attention(qkv(norm(x)))) of a fused block. Gradients of its parameters go to the dense tables."""
+
+    @staticmethod
+    def forward(ctx, x, model, i):
+        cfg, P = model.cfg, model.main.params
+        B, T, d = x.shape
+        x2 = x.reshape(-1, d)
+        norm = _Norm(model, f"h{i}.ln1", x2)
+        if model.qkv[i] is not None:
+            qkv = G.ag_linear(norm.y, model.qkv[i], "w", bias=P[f"h{i}.qkv.b"])
+        else:
+            qkv = linear_act(norm.y, P[f"h{i}.qkv.w"], P[f"h{i}.qkv.b"])
+        norm.drop_y()
+        qkv = qkv.requires_grad_(True)
+        with torch.enable_grad():   # attention keeps its own graph, which the backward pass runs
+            q, k, v = qkv.view(B, T, 3, cfg.n_head, d // cfg.n_head).permute(2, 0, 3, 1, 4)
+            a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+            a2 = a.transpose(1, 2).reshape(-1, d)
+        out = linear_act(a2.detach(), P[f"h{i}.proj.w"], P[f"h{i}.proj.b"], residual=x2)
+        ctx.model, ctx.i, ctx.norm, ctx.qkv = model, i, norm, qkv
+        # the graph keeps attention's own output; the copy in rows is kept as it is, or in 8 bits with its graph's end before the copy
+        ctx.attention = a
+        ctx.rows = act8_pack(a2.detach()) if cfg.act_bits == 8 else a2.detach()
+        return out.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        model, i, norm = ctx.model, ctx.i, ctx.norm
+        cfg, P, Gr = model.cfg, model.main.params, model.main.grads
+        B, T, d = dy.shape
+        dy2 = dy.reshape(-1, d)
+        if cfg.act_bits == 8:
+            act8_wgrad(dy2, ctx.rows, out=Gr[f"h{i}.proj.w"], accumulate=True)
+        else:
+            G.gemm(dy2, ctx.rows, a_mn=True, b_mn=True, out=Gr[f"h{i}.proj.w"], accumulate=True)
+        linear_bias_grad(dy2, out=Gr[f"h{i}.proj.b"], accumulate=True)
+        da = G.linear_dgrad(dy2, P[f"h{i}.proj.w"])
+        da = da.view(B, T, cfg.n_head, d // cfg.n_head).transpose(1, 2)
+        (dqkv,) = torch.autograd.grad(ctx.attention, ctx.qkv, da)
+        ctx.attention = ctx.qkv = ctx.rows = None
+        table = model.qkv[i]
+        w, wg = (P[f"h{i}.qkv.w"], Gr[f"h{i}.qkv.w"]) if table is None else (table.params["w"], table.grads["w"])
+        norm.wgrad(dqkv, wg, Gr[f"h{i}.qkv.b"])
+        dx = norm.backward(G.linear_dgrad(dqkv, w), residual_grad=dy2)
+        ctx.norm = None
+        return dx.view(dy.shape), None, None
+
+
+class _MlpHalf(torch.autograd.Function):
+    """x + out(gelu(fc(norm(x)))) of a fused block. The hidden layer is kept before GELU only, and formed again behind it."""
+
+    @staticmethod
+    def forward(ctx, x, model, i):
+        P = model.main.params
+        x2 = x.reshape(-1, x.shape[-1])
+        norm = _Norm(model, f"h{i}.ln2", x2)
+        f, ctx.h = linear_act(norm.y, P[f"h{i}.fc.w"], P[f"h{i}.fc.b"], act="gelu_tanh", save="act8" if model.cfg.act_bits == 8 else "bf16")
+        norm.drop_y()
+        ctx.model, ctx.i, ctx.norm = model, i, norm
+        return linear_act(f, P[f"h{i}.out.w"], P[f"h{i}.out.b"], residual=x2).view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        model, i, norm = ctx.model, ctx.i, ctx.norm
+        P, Gr = model.main.params, model.main.grads
+        dy2 = dy.reshape(-1, dy.shape[-1])
+        dh, f = linear_act_dgrad(dy2, P[f"h{i}.out.w"], ctx.h, act="gelu_tanh", recompute=True)
+        ctx.h = None
+        G.gemm(dy2, f, a_mn=True, b_mn=True, out=Gr[f"h{i}.out.w"], accumulate=True)
+        del f
+        linear_bias_grad(dy2, out=Gr[f"h{i}.out.b"], accumulate=True)
+        norm.wgrad(dh, Gr[f"h{i}.fc.w"], Gr[f"h{i}.fc.b"])
+        dx = norm.backward(G.linear_dgrad(dh, P[f"h{i}.fc.w"]), residual_grad=dy2)
+        ctx.norm = None
+        return dx.view(dy.shape), None, None
+
+
+class _FinalNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, model):
+        ctx.norm = _Norm(model, "lnf", x.reshape(-1, x.shape[-1]))
+        y = ctx.norm.y.view(x.shape)
+        ctx.norm.drop_y()
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = ctx.norm.backward(dy.reshape(-1, dy.shape[-1]))
+        ctx.norm = None
+        return dx.view(dy.shape), None
+
+
 class GPT:
     def __init__(self, cfg: GPTConfig, *, device=None, group=None, seed: int = 0, fuse_qkv_gather: bool = True):
+        if cfg.act_bits not in (8, 16) or (cfg.act_bits == 8 and not cfg.fused):
+            raise ValueError("GPTConfig: act_bits is 16, or 8 with fused=True")
         self.cfg = cfg
         self.group = group
         self.world, self.rank = _dist_info(group)
@@ -114,7 +252,7 @@ class GPT:
         # small parameters go through autograd as leaves that alias the table; their .grad is folded in later
         self._leaves = {}
         for name in shapes:
-            if name in ("wte", "wpe") or ".ln" in name or name.startswith("lnf."):
+            if name in ("wte", "wpe") or (not cfg.fused and (".ln" in name or name.startswith("lnf."))):
                 self._leaves[name] = self.main.params[name].requires_grad_(True)
         self.tables = [self.main] + [t for t in self.qkv if t is not None]
 
@@ -131,6 +269,9 @@ class GPT:
         lv = self._leaves
         x = F.embedding(tokens, lv["wte"]) + lv["wpe"][:T]
         for i in range(cfg.n_layer):
+            if cfg.fused:
+                x = _MlpHalf.apply(_AttentionHalf.apply(x, self, i), self, i)
+                continue
             h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln1.g"], lv[f"h{i}.ln1.b"])
             qkv = self._linear(h, f"h{i}.qkv.w", f"h{i}.qkv.b", self.qkv[i])
             q, k, v = qkv.view(B, T, 3, cfg.n_head, cfg.d_model // cfg.n_head).permute(2, 0, 3, 1, 4)
@@ -140,7 +281,7 @@ class GPT:
             h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln2.g"], lv[f"h{i}.ln2.b"])
             h = F.gelu(self._linear(h, f"h{i}.fc.w", f"h{i}.fc.b"), approximate="tanh")
             x = x + self._linear(h, f"h{i}.out.w", f"h{i}.out.b")
-        x = F.layer_norm(x, (cfg.d_model,), lv["lnf.g"], lv["lnf.b"])
+        x = _FinalNorm.apply(x, self) if cfg.fused else F.layer_norm(x, (cfg.d_model,), lv["lnf.g"], lv["lnf.b"])
         # tied output embedding: the GEMM's weight gradient and the embedding's gradient both land in wte's slot
         logits = _PSLinear.apply(x, self.main.params["wte"], None, self.main.grads["wte"], None, None, None)
         if targets is None:
@@ -197,7 +338,7 @@ def _bench(args) -> None:
     torch.cuda.set_device(local)
     if world > 1:
         dist.init_process_group("nccl", device_id=torch.device("cuda", local))
-    cfg = GPTConfig(n_layer=args.layers)
+    cfg = GPTConfig(n_layer=args.layers, fused=args.fused, act_bits=args.act_bits)
     model = GPT(cfg, fuse_qkv_gather=not args.no_fuse)
     B = args.seqs_per_gpu
     gen = torch.Generator().manual_seed(local)
@@ -229,7 +370,8 @@ def _bench(args) -> None:
         print(json.dumps({"metric": "gpt_tokens_per_sec", "value": tokens / (ms / 1e3), "n_gpus": world, "ms_per_step": ms,
                           "model_tflops_per_gpu": flops / (ms / 1e3) / 1e12 / world, "layers": cfg.n_layer,
                           "params": cfg.n_params(), "global_batch_seqs": B * world, "seq_len": cfg.seq_len,
-                          "qkv_gather_fused": model.lazy_qkv, "loss": float(loss.item())}))
+                          "qkv_gather_fused": model.lazy_qkv, "blocks_fused": cfg.fused, "act_bits": cfg.act_bits,
+                          "peak_gb": torch.cuda.max_memory_allocated() / 1e9, "loss": float(loss.item())}))
     if world > 1:
         dist.destroy_process_group()
 
@@ -242,4 +384,6 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=3)
     ap.add_argument("--warmup", type=int, default=2)
     ap.add_argument("--no-fuse", action="store_true", help="all-gather the QKV weights in the dense push instead of in the GEMM")
+    ap.add_argument("--fused", action="store_true", help="blocks on ops.norm / ops.linear")
+    ap.add_argument("--act-bits", type=int, default=16, choices=(16, 8), help="of what a fused block keeps for its backward pass")
     _bench(ap.parse_args())
