@@ -1,0 +1,372 @@
+// The fused linear layers for few tokens, where the weight's way through the chip and the latency of one tile are the time:
+//
+//   forward   h = x w^T + b, y = act(h) + residual        dgrad   dh = (dy w) * act'(h), a = act(h)
+//
+// The weight takes the tensor core's 128 rows and the tokens its columns (16 to 128 of them), so that few tokens are not padded
+// to a tile. A cluster of S CTAs has the same 128 output features (and the same 128 tokens, where there are more) and cuts the
+// contraction in S parts, S chosen so that all SMs read at once; each CTA keeps its part's sums in TMEM. They meet in
+// distributed shared memory: every CTA lays its sums down in its own, and CTA r reads the r-th share of the tokens from all S,
+// adds them in rank order (the same bits every time) and runs the epilogue for its share, with 32 neighbouring features in the
+// lanes of a warp. At most 108 KB of shared memory: two CTAs fit an SM, without which sixteen clusters of eight do not all fit
+// the GPCs at once (16 tokens, 4096 -> 2048: 17 us, two waves).
+#pragma once
+#include "linear_fused.cuh"
+
+namespace psb {
+
+namespace {
+
+constexpr int kFewThreads = 512;
+constexpr int kFewTokens = 128;    // of a tile
+constexpr int kFewMaxStages = 8;
+constexpr int kFewSmem = 108 * 1024;
+
+struct FewParams {
+    CUtensorMap map_w, map_x;
+    int M, N, k_steps;
+    int n_tiles;
+    int columns;          // tokens of a tile padded to 16, 32, 64 or 128
+    int stages, ring_bytes;
+    const __nv_bfloat16* bias;
+    const float* bias32;
+    const __nv_bfloat16* res;
+    int64_t ldres;
+    __nv_bfloat16* out;
+    int64_t ldo;
+    __nv_bfloat16* out2;
+    int64_t ldo2;
+    __nv_bfloat16* pre;
+    int64_t ldpre;
+    int8_t* q;
+    int64_t ldq;
+    uint8_t* e;
+    int64_t lde;
+    int res_wide, out_wide, out2_wide, pre_wide;   // rows on 8-byte boundaries
+    unsigned* err_flag;
+    unsigned long long limit_ns;
+};
+
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// Four neighbours of a bf16 row, `n` of them there; `wide`: the row's 8-byte blocks are aligned
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, int n, bool wide, float* f) {
+    if (wide && n >= 4) {
+        const uint2 r = *(const uint2*)p;
+        f[0] = __uint_as_float(r.x << 16);
+        f[1] = __uint_as_float(r.x & 0xFFFF0000u);
+        f[2] = __uint_as_float(r.y << 16);
+        f[3] = __uint_as_float(r.y & 0xFFFF0000u);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = j < n ? __bfloat162float(p[j]) : 0.f;
+    }
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, int n, bool wide, const float* f) {
+    if (wide && n >= 4) {
+        uint2 r;
+        __nv_bfloat162* h = (__nv_bfloat162*)&r;
+        h[0] = __floats2bfloat162_rn(f[0], f[1]);
+        h[1] = __floats2bfloat162_rn(f[2], f[3]);
+        *(uint2*)p = r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) p[j] = __float2bfloat16_rn(f[j]);
+    }
+}
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// Four features' sums over the S CTAs, in rank order; all loads are on their way before the first is added (one round trip
+// between SMs takes about 0.2 us).
+template <int S>
+__device__ __forceinline__ void add_parts(uint32_t at, float* v) {
+    float4 part[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) part[s] = ld_cluster_v4(mapa_cluster(at, (uint32_t)s));
+    v[0] = part[0].x; v[1] = part[0].y; v[2] = part[0].z; v[3] = part[0].w;
+#pragma unroll
+    for (int s = 1; s < S; ++s) { v[0] += part[s].x; v[1] += part[s].y; v[2] += part[s].z; v[3] += part[s].w; }
+}
+
+template <bool DGRAD, int ACT>
+__global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid_constant__ FewParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = BM * BK * 2 + p.columns * BK * 2;
+    float* parts = (float*)smem;   // [tokens][128 features]: this CTA's sums, where the stages were
+    uint64_t* full_bar = (uint64_t*)(smem + p.ring_bytes);
+    uint64_t* empty_bar = full_bar + kFewMaxStages;
+    uint64_t* done_bar = empty_bar + kFewMaxStages;
+    uint32_t* tmem_slot = (uint32_t*)(done_bar + 1);
+
+    const int S = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
+    const int tile = (int)blockIdx.x / S, n0 = tile % p.n_tiles * BM, m0 = tile / p.n_tiles * kFewTokens;
+    const int tokens = min(p.M - m0, kFewTokens);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int k_begin = (int)((int64_t)p.k_steps * rank / S), k_end = (int)((int64_t)p.k_steps * (rank + 1) / S), nk = k_end - k_begin;
+    const int share = (p.columns + S - 1) / S;   // tokens that one CTA finishes
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        mbar_init(done_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_x) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(128u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *((volatile uint32_t*)tmem_slot);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- TMA producer ----
+            for (int k = 0; k < nk; ++k) {
+                const int s = k % p.stages;
+                if (k >= p.stages && !mbar_wait(&empty_bar[s], ((k / p.stages) & 1u) ^ 1u, p.limit_ns)) {
+                    atomicCAS(p.err_flag, 0u, 41u);
+                    break;
+                }
+                uint8_t* sa = smem + s * stage_bytes;
+                const int k0 = (k_begin + k) * BK;
+                mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
+                if constexpr (!DGRAD) {
+                    tma_load_2d(sa, &p.map_w, &full_bar[s], k0, n0);   // [128 features][64 k]
+                } else {
+                    tma_load_2d(sa, &p.map_w, &full_bar[s], n0, k0);   // two blocks of [64 k][64 features]
+                    tma_load_2d(sa + 64 * 128, &p.map_w, &full_bar[s], n0 + 64, k0);
+                }
+                tma_load_2d(sa + BM * BK * 2, &p.map_x, &full_bar[s], k0, m0);   // [tokens][64 k]
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---- MMA issuer: D[feature][token] ----
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 15) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            for (int k = 0; k < nk; ++k) {
+                const int s = k % p.stages;
+                if (!mbar_wait(&full_bar[s], (k / p.stages) & 1u, p.limit_ns * 2)) {
+                    atomicCAS(p.err_flag, 0u, 42u);
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + BM * BK * 2;
+#pragma unroll
+                for (int u = 0; u < BK / UMMA_K; ++u) {
+                    const uint64_t da = DGRAD ? make_desc(sa + u * 2048, 8192, 1024) : make_desc(sa + u * 32, 16, 1024);
+                    umma_bf16(tmem, da, make_desc(sb + u * 32, 16, 1024), idesc, (k | u) ? 1u : 0u);
+                }
+                umma_commit(&empty_bar[s]);
+            }
+            umma_commit(done_bar);   // (also on error, so that nobody waits for it)
+        }
+    }
+    __syncwarp();
+    // ---- this CTA's sums to its shared memory: the MMAs have read all stages, and no load is in flight ----
+    const bool ok = mbar_wait(done_bar, 0u, p.limit_ns * 4);
+    if (!ok && lane == 0) atomicCAS(p.err_flag, 0u, 43u);
+    __syncwarp();
+    {
+        // four warps share a quarter of TMEM's lanes (warp % 4) and take its columns in turn
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int quarter = warp & 3;
+        for (int t0 = (warp >> 2) * 16; t0 < tokens; t0 += kFewThreads / 128 * 16) {
+            uint32_t v[16];
+            tmem_ld16_issue(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t0, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) parts[(t0 + j) * BM + quarter * 32 + lane] = __uint_as_float(v[j]);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    cluster_sync_all();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128u) : "memory");
+    }
+    // ---- epilogue of this CTA's tokens: a warp has a token, a lane four neighbouring features ----
+    const int n = n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (!DGRAD) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < have) b[j] = p.bias32 != nullptr ? p.bias32[n + j] : p.bias != nullptr ? __bfloat162float(p.bias[n + j]) : 0.f;
+    }
+    const uint32_t mine = smem_u32(parts) + (uint32_t)lane * 16;
+    const int t_end = min(tokens, (rank + 1) * share);
+    for (int t = rank * share + warp; t < t_end; t += kFewThreads / 32) {
+        const int64_t row = m0 + t;
+        float v[4], aux[4] = {0.f, 0.f, 0.f, 0.f};
+        if (have > 0) {
+            if constexpr (!DGRAD) {
+                if (p.res != nullptr) load4(p.res + row * p.ldres + n, have, p.res_wide != 0, aux);
+            } else {
+                if (p.q != nullptr) {
+                    const uint32_t w = *(const uint32_t*)(p.q + row * p.ldq + n) ^ 0x80808080u;   // (rows are padded to 16 bytes)
+                    const float step = act8_step(p.e[row * p.lde + n / kAct8Block]);
+                    aux[0] = s8_of_biased<0>(w) * step;
+                    aux[1] = s8_of_biased<1>(w) * step;
+                    aux[2] = s8_of_biased<2>(w) * step;
+                    aux[3] = s8_of_biased<3>(w) * step;
+                } else if (p.pre != nullptr) {
+                    load4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, aux);
+                }
+            }
+        }
+        const uint32_t at = mine + (uint32_t)(t * BM) * 4;
+        if (S == 8) add_parts<8>(at, v);
+        else if (S == 4) add_parts<4>(at, v);
+        else if (S == 2) add_parts<2>(at, v);
+        else add_parts<1>(at, v);
+        if constexpr (!DGRAD) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += b[j];   // (0 past the last feature: its weights were read as zeros)
+            if (p.pre != nullptr && have > 0) store4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, v);
+            if (p.q != nullptr) {   // a block is eight lanes
+                uint32_t m = abs_bits(abs_max(abs_max(v[0], v[1]), abs_max(v[2], v[3])));
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+                const uint32_t ex = act8_exponent(m);
+                if (have > 0) {
+                    *(uint32_t*)(p.q + row * p.ldq + n) = ex == 255u ? 0u : act8_quantise4(v[0], v[1], v[2], v[3], act8_inverse_step(ex));
+                    if ((lane & 7) == 0) p.e[row * p.lde + n / kAct8Block] = (uint8_t)ex;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = act_of<ACT>(v[j]) + aux[j];
+            if (have > 0) store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
+        } else {
+            float a[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] *= act_slope<ACT>(aux[j], &a[j]);
+            if (have > 0) {
+                store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
+                if (p.out2 != nullptr) store4(p.out2 + row * p.ldo2 + n, have, p.out2_wide != 0, a);
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();   // until here the others may read this CTA's shared memory
+}
+
+template <bool DGRAD, int ACT>
+int launch_few(const FewParams& p, int cluster, int smem, cudaStream_t s) {
+    constexpr auto kern = linear_few_kernel<DGRAD, ACT>;
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+        if (e != cudaSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.n_tiles * ((p.M + kFewTokens - 1) / kFewTokens) * cluster));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute a[1];
+    a[0].id = cudaLaunchAttributeClusterDimension;
+    a[0].val.clusterDim.x = cluster;
+    a[0].val.clusterDim.y = 1;
+    a[0].val.clusterDim.z = 1;
+    cfg.attrs = a;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+// CTAs that share a tile's contraction: doubled while all of them fit the GPU at once (two to an SM) with two k-steps each
+int few_cluster(int64_t M, int64_t N, int64_t K) {
+    const int64_t tiles = (N + BM - 1) / BM * ((M + kFewTokens - 1) / kFewTokens), k_steps = (K + BK - 1) / BK;
+    const int64_t places = gemm_cta_limit() > 0 ? 2 * gemm_cta_limit() : 4 * kMaxPairs;
+    int cluster = 1;
+    while (cluster < 8 && tiles * cluster * 2 <= places && k_steps >= cluster * 4) cluster *= 2;
+    return cluster;
+}
+
+// Which kernel: up to 128 tokens always this one; above, the one whose longest CTA is done first, counted in k-steps: one of a
+// 128 x 128 tile takes about as long as one of a pair's 256 x 256 tile (the same bytes per SM), and the last tile's epilogue, which
+// nothing hides, as long as 10 of them here (sixteen warps, 128 x 128 values) and 20 there. 1024 x 2048 x 2048, in us: 19 here, 20.
+bool few_tokens(const LinearArgs& a) {
+    if (a.M <= kFewTokens) return true;
+    const int64_t k_steps = (a.K + BK - 1) / BK, pairs = gemm_cta_limit() > 0 ? std::max(1, gemm_cta_limit() / 2) : kMaxPairs;
+    const int64_t small = (int64_t)((a.N + BM - 1) / BM) * ((a.M + kFewTokens - 1) / kFewTokens), large = (int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256);
+    const int cluster = few_cluster(a.M, a.N, a.K);
+    if (small * cluster > 4 * pairs) return false;
+    return (small * cluster + 2 * pairs - 1) / (2 * pairs) * ((k_steps + cluster - 1) / cluster) + 10 < (large + pairs - 1) / pairs * k_steps + 20;
+}
+
+template <bool DGRAD>
+int linear_few(const LinearArgs& a, cudaStream_t s) {
+    FewParams p;
+    p.M = a.M;
+    p.N = a.N;
+    p.k_steps = (a.K + BK - 1) / BK;
+    p.columns = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+    if (!make_map(&p.map_x, a.a, (uint64_t)a.M, (uint64_t)a.K, (uint64_t)a.lda, p.columns)) return -3;
+    if (!(DGRAD ? make_map(&p.map_w, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, 64)
+                : make_map(&p.map_w, a.w, (uint64_t)a.N, (uint64_t)a.K, (uint64_t)a.ldw, BM)))
+        return -3;
+    p.bias = a.bias_f32 ? nullptr : (const __nv_bfloat16*)a.bias;
+    p.bias32 = a.bias_f32 ? (const float*)a.bias : nullptr;
+    p.res = (const __nv_bfloat16*)a.residual;
+    p.ldres = a.ldres;
+    p.out = (__nv_bfloat16*)a.out;
+    p.ldo = a.ldo;
+    p.out2 = (__nv_bfloat16*)a.out2;
+    p.ldo2 = a.ldo2;
+    p.pre = (__nv_bfloat16*)a.pre;
+    p.ldpre = a.ldpre;
+    p.q = (int8_t*)a.q;
+    p.ldq = a.ldq;
+    p.e = (uint8_t*)a.e;
+    p.lde = a.lde;
+    auto wide = [](const void* r, int64_t ld) { return (uintptr_t)r % 8 == 0 && ld % 4 == 0 ? 1 : 0; };
+    p.res_wide = wide(a.residual, a.ldres);
+    p.out_wide = wide(a.out, a.ldo);
+    p.out2_wide = wide(a.out2, a.ldo2);
+    p.pre_wide = wide(a.pre, a.ldpre);
+    p.err_flag = a.err_flag;
+    p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
+    p.n_tiles = (a.N + BM - 1) / BM;
+    const int cluster = few_cluster(a.M, a.N, a.K);
+    const int stage_bytes = (BM + p.columns) * BK * 2, extra = 1024 + 512;
+    p.stages = std::min(std::min(kFewMaxStages, (kFewSmem - extra) / stage_bytes), (p.k_steps + cluster - 1) / cluster);
+    p.ring_bytes = std::max(p.stages * stage_bytes, p.columns * BM * 4);
+    const int smem = p.ring_bytes + extra;
+    switch (a.act) {
+        case kActNone: return launch_few<DGRAD, kActNone>(p, cluster, smem, s);
+        case kActRelu: return launch_few<DGRAD, kActRelu>(p, cluster, smem, s);
+        case kActGelu: return launch_few<DGRAD, kActGelu>(p, cluster, smem, s);
+        case kActGeluTanh: return launch_few<DGRAD, kActGeluTanh>(p, cluster, smem, s);
+        case kActSilu: return launch_few<DGRAD, kActSilu>(p, cluster, smem, s);
+    }
+    return -2;
+}
+
+}  // namespace
+
+}  // namespace psb

@@ -621,8 +621,6 @@ bool rows16(const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && (ld 
 
 template <bool DGRAD>
 int linear_typed(const LinearArgs& a, cudaStream_t s) {
-    if (!rows16(a.a, a.lda) || !rows16(a.w, a.ldw)) return -2;
-    if (a.q != nullptr && (((uintptr_t)a.q % 16) || (a.ldq % 16) || ((uintptr_t)a.e % 16) || (a.lde % 16))) return -2;
     // tiles 128 wide only where 256 would be more than half padding: they need twice the operand bytes per flop
     const int BN = a.N > 128 ? 256 : 128;
     LinParams p;

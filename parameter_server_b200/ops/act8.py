@@ -16,6 +16,7 @@ from typing import Optional
 import torch
 
 from .._lib import C
+from .gemm import _err_flag, workspace
 
 BLOCK = 32
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
@@ -54,12 +55,31 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _matrix(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A bf16 operand of the tensor cores: rows on 16-byte boundaries. Rows that are not are copied once, into rows padded to
+    8 elements (what a bulk-tensor load asks for)."""
+    if t.dtype != torch.bfloat16 or (like is not None and t.get_device() != like.get_device()):
+        raise ValueError(f"{what}: expected bf16" + ("" if like is None else f" on {like.device}") + f", got {t.dtype} on {t.device}")
+    t = rows2d(t, what)
+    if row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    rows, cols = t.shape
+    padded = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)[:, :cols]
+    padded.copy_(t)
+    return padded
+
+
+def _ld(t: torch.Tensor) -> int:
+    # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+
+
 class Act8:
     """A checkpoint of ``rows x cols`` values: ``q`` int8 and ``e`` uint8, one exponent per 32 columns.
 
     Both are matrices with rows on 16-byte boundaries; columns past ``cols`` are padding that nothing reads."""
 
-    __slots__ = ("q", "e", "rows", "cols")
+    __slots__ = ("q", "e", "rows", "cols", "_args")
 
     def __init__(self, q: torch.Tensor, e: torch.Tensor, cols: int):
         if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() != 2 or e.dim() != 2 or q.shape[0] != e.shape[0]:
@@ -72,6 +92,7 @@ class Act8:
                           or q.data_ptr() % 16 or e.data_ptr() % 16):
             raise ValueError("Act8: rows of q and e start on 16-byte boundaries")
         self.q, self.e, self.rows, self.cols = q, e, q.shape[0], cols
+        self._args = (q.data_ptr(), row_stride(q), e.data_ptr(), row_stride(e))
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Act8":
@@ -80,6 +101,7 @@ class Act8:
         self.q = torch.empty((rows, ldq), dtype=torch.int8, device=device)
         self.e = torch.empty((rows, lde), dtype=torch.uint8, device=device)
         self.rows, self.cols = rows, cols
+        self._args = (self.q.data_ptr(), ldq, self.e.data_ptr(), lde)
         return self
 
     @property
@@ -96,7 +118,7 @@ class Act8:
 
     def args(self):
         """(q, ldq, e, lde) as the native entry points take them."""
-        return self.q.data_ptr(), row_stride(self.q), self.e.data_ptr(), row_stride(self.e)
+        return self._args
 
     def __repr__(self) -> str:
         return f"Act8({self.rows} x {self.cols}, {self.device})"
@@ -138,8 +160,6 @@ def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = N
     ``weight`` and ``bias`` (bf16, ``[K]``): the layer's input was a layer norm's output and ``x8`` holds its normalised rows
     (``norm.layer_norm_act8``), so the operand is ``x * weight + bias``. With ``bias``, ``dy_sum`` is the sum of dy's rows (fp32, ``[N]``:
     the layer's bias gradient, ``linear.linear_bias_grad``). ``out`` is written, or added to with ``accumulate``."""
-    from .linear import _ld, _matrix, workspace, _err_flag   # (linear imports this module)
-
     what = "act8_wgrad"
     s = launch_stream(dy)
     dy2 = _matrix(dy, f"{what} dy")

@@ -15,29 +15,10 @@ from typing import Optional, Union
 import torch
 
 from .._lib import C
-from .act8 import _DTYPES, Act8, check, launch_stream, row_stride, rows2d
+from .act8 import _DTYPES, _ld, _matrix, Act8, check, launch_stream, row_stride, rows2d
 from .gemm import _err_flag, workspace
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
-
-
-def _matrix(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """A bf16 operand of the tensor cores: rows on 16-byte boundaries. Rows that are not are copied once, into rows padded to
-    8 elements (what a bulk-tensor load asks for)."""
-    if t.dtype != torch.bfloat16 or (like is not None and t.get_device() != like.get_device()):
-        raise ValueError(f"{what}: expected bf16" + ("" if like is None else f" on {like.device}") + f", got {t.dtype} on {t.device}")
-    t = rows2d(t, what)
-    if row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    rows, cols = t.shape
-    padded = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)[:, :cols]
-    padded.copy_(t)
-    return padded
-
-
-def _ld(t: torch.Tensor) -> int:
-    # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
 
 
 def _act_code(act, what: str) -> int:
