@@ -4,18 +4,21 @@
 //   norm form: the layer's input was xhat * g + b, and xhat is what was kept:
 //   dw[n][k] = g[k] * sum_t dy[t][n] * xhat[t][k] + b[k] * sum_t dy[t][n]
 //
-// The checkpoint is read as it is (a byte and a 32nd per value instead of two) and becomes bf16 on its way to the tensor
-// cores, in shared memory; q * 2^(e-127) is exact in bf16, so the products are those of the values that were kept. Unpacking
-// in a pass of its own would move five bytes per value through HBM. The norm form is applied to the fp32 sums, where it
-// needs no rounding of x.
+// q * 2^(e-127) is exact in bf16, so the products are those of the values that were kept. A layer of few outputs reads the
+// checkpoint as it is (a byte and a 32nd per value) and turns it into bf16 in shared memory, on its way to the tensor cores; one
+// of many outputs, which would do that again for every 256 of them, unpacks it once into scratch (act8_wgrad_scratch). The norm
+// form is applied to the fp32 sums, where it needs no rounding of x.
 //
-// CTA pairs on 256 x 256 tiles of dw as in linear_fused.cuh, both operands MN-major, with two more roles per CTA: four warps
-// convert the pair's half of the checkpoint tile ([64 tokens][128 columns], 8 KB) into the swizzled bf16 tile that the MMA
-// reads (5 integer / packed-bf16 instructions per two values, about a third of the issue slots of the 512 cycles that a
-// k-step's MMAs take), and the eight epilogue warps keep the tile's sums in registers: the tensor core adds to its fp32
-// accumulator with truncation, which loses 1e-9 of the sum per token (2e-5 at 16384, all towards zero), so a chain in TMEM
-// ends after 512 tokens and the chains are added in round-to-nearest by the epilogue warps, one TMEM buffer behind the MMAs.
-// Registers move from the producer and converter warps to them (setmaxnreg).
+// CTA pairs on 256 x 256 tiles of dw as in linear_fused.cuh, both operands MN-major. Where x is converted, four more warps per
+// CTA turn the pair's half of the checkpoint tile ([64 tokens][128 columns], 8 KB) into the swizzled bf16 tile that the MMA reads:
+// per two values two byte permutes, a packed multiply-add and a conversion, 450 of the 750 cycles that a k-step takes; dy, the
+// checkpoint and the bf16 tiles have rings of their own, so that no part waits for another's space.
+// The eight epilogue warps keep the tile's sums in registers: the tensor core adds to its fp32 accumulator with truncation, which
+// loses 1e-9 of the sum per token (2e-5 at 16384, all towards zero), so a chain in TMEM ends after 512 tokens and the chains are
+// added in round-to-nearest by the epilogue warps, one TMEM buffer behind the MMAs (1.5e-7 at 16384 tokens). Registers move
+// from the producer and converter warps to them (setmaxnreg).
+// 16384 tokens, 6144 x 2048: 300 us with a cold L2 (1375 TFLOP/s), 347 back to back at the power limit. Bound by the tensor cores and
+// that limit.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -525,12 +528,11 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
 }
 
 // Converting tile by tile repeats the work for every 256 rows of dw and costs the tensor cores a fifth of their time;
-// unpacking once costs five bytes of traffic per value of x. Measured on 16384 tokens, tile by tile against unpacked, in us:
-// 6144 x 2048: 353, 312; 2048 x 8192: 462, 437; 8192 x 2048: 462, 394; 2048 x 2048 (64 tiles, which bf16 copies of 134 MB do not
-// leave in L2): 142, 171; 1024 x 2048: 87, 91; 512 x 2048: 61, 71.
+// unpacking once costs five bytes of traffic per value of x. Measured on 16384 tokens, tile by tile against unpacked, in us with
+// a cold L2 and back to back: 6144 x 2048: 369, 300 and 416, 347; 2048 x 2048: 135, 120 and 137, 126; 1024 x 2048: 86, 89 and
+// 79, 87; 512 x 2048: 61, 69 and 53, 63. On 1024 tokens 2048 x 2048: 27, 24.
 int64_t act8_wgrad_scratch(int64_t tokens, int N, int K) {
-    const int64_t tiles = ((int64_t)N + 255) / 256 * (((int64_t)K + 255) / 256);
-    return N >= 2048 && tiles >= 128 ? tokens * (((int64_t)K + 7) / 8 * 8) * 2 : 0;
+    return N >= 2048 ? tokens * (((int64_t)K + 7) / 8 * 8) * 2 : 0;
 }
 
 }  // namespace psb

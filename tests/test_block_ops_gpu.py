@@ -461,6 +461,20 @@ def test_act8_wgrad_every_token_lands_where_it_belongs():
     G.check_gemm_errors()
 
 
+def test_act8_wgrad_converted_tiles_are_the_right_ones():
+    """The same for a layer of few outputs, whose checkpoint is converted tile by tile: some tokens' rows of x at a time."""
+    T, N, K = 4096, 1536, 2048
+    x8 = act8.act8_pack(rand(T, K, seed=9))
+    x = act8.act8_unpack(x8, F32)
+    for part in range(4):
+        tokens = torch.randperm(T, generator=torch.Generator().manual_seed(part))[:N].cuda()
+        dy = torch.zeros(T, N, device="cuda").bfloat16()
+        dy[tokens, torch.arange(N, device="cuda")] = 1
+        for _ in range(3):
+            assert torch.equal(act8.act8_wgrad(dy, x8), x[tokens])
+    G.check_gemm_errors()
+
+
 def test_act8_wgrad_strides_not_finite_and_large_values():
     T, N, K = 300, 96, 160
     wide = rand(T, 3 * N)
