@@ -168,16 +168,20 @@ __device__ __forceinline__ void keep8(const float* f, bool valid, int8_t* qrow, 
 // With few rows a row is spread over as many threads as have a vector each, since then the latency of one row is the time.
 // CTAs are persistent, and a thread copies its part of the next two rows to shared memory while it works on this one (only
 // the thread itself reads it, so no barrier is involved): with loads straight into registers a row's arithmetic and the next
-// row's latency add up (16384 x 2048: 35 us). Rows that are not 16-byte aligned (VEC 1) are read that way all the same.
+// row's latency add up (16384 x 2048: 35 us). bf16 rows that are not 16-byte aligned (VEC 1; a copy has 4 bytes at least) are
+// read that way all the same.
 constexpr int kFwdSlots = 3;
+template <typename T, int VEC>
+constexpr bool copies_ahead() { return VEC * sizeof(T) >= 4; }
 template <typename T, int VEC, int NV, bool OUT8>
 __global__ void __launch_bounds__(kMaxTeam)
 layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, T* __restrict__ y,
                       int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
                       int64_t lde, int64_t rows, int d, float eps, int tpr) {
-    constexpr bool kAsync = VEC > 1;
+    constexpr bool kAsync = copies_ahead<T, VEC>();
+    constexpr int kVecBytes = VEC * (int)sizeof(T);
     using IO = Io<T, VEC>;
-    extern __shared__ uint4 ring[];   // [kFwdSlots][NV][threads]
+    extern __shared__ uint4 ring[];   // [kFwdSlots][NV][threads] vectors
     __shared__ float red[2][kMaxTeam / 32];
     const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
     const int warps = tpr / 32, w0 = team * warps;
@@ -190,14 +194,14 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
         braw[i] = bias != nullptr && col < d ? IO::load(bias + col) : IO::zero();
     }
     // running positions: a row's overhead is shared by 32 values only
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16, vec_stride = blockDim.x * 16, slot_stride = NV * vec_stride;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * kVecBytes, vec_stride = blockDim.x * kVecBytes, slot_stride = NV * vec_stride;
     const T* ahead = x + (first + team) * ldx + t * VEC;
     int64_t ahead_row = first + team;
     auto request = [&](int slot) {   // the next row that has not been asked for
         if (ahead_row < rows) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if ((i * tpr + t) * VEC < d) copy_async<16>(mine + slot * slot_stride + i * vec_stride, ahead + i * tpr * VEC);
+                if ((i * tpr + t) * VEC < d) copy_async<kAsync ? kVecBytes : 4>(mine + slot * slot_stride + i * vec_stride, ahead + i * tpr * VEC);
         }
         close_group();   // (an empty group where there is no such row: the count of groups stays the same)
         ahead += step * ldx;
@@ -328,11 +332,12 @@ layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __rest
 // per SM would write and read more partial rows: 2 * d floats each.)
 template <typename T, int VEC, bool SRC8>
 struct BwdRing {
-    static constexpr int kVecs = kBwdElems / VEC;
+    static constexpr int kVecs = kBwdElems / VEC, kVecBytes = VEC * (int)sizeof(T);
+    static constexpr bool kAsync = copies_ahead<T, VEC>() && (VEC >= 4 || !SRC8);   // (a vector of q has VEC bytes)
     static constexpr int kSlots = sizeof(T) == 2 ? 3 : 2;
     // per thread and slot: dy, the residual's gradient, and x or (8 or 4 bytes a vector) q with a word of exponents
-    static constexpr int kRowBytes = SRC8 ? kVecs * (32 + VEC + 4) : kVecs * 48;
-    static constexpr int kBytes = VEC > 1 ? kSlots * kRowBytes * kBwdThreads : 0;
+    static constexpr int kRowBytes = SRC8 ? kVecs * (2 * kVecBytes + VEC + 4) : kVecs * 3 * kVecBytes;
+    static constexpr int kBytes = kAsync ? kSlots * kRowBytes * kBwdThreads : 0;
 };
 
 template <typename T, int VEC, bool SRC8>
@@ -342,9 +347,10 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const T* __restrict__ join, int64_t ldjoin,
                       T* __restrict__ dx, int64_t lddx, float* __restrict__ partial, int64_t rows, int d, int tpr) {
     constexpr int NV = kBwdElems / VEC;
-    constexpr bool kAsync = VEC > 1;
     using IO = Io<T, VEC>;
     using Ring = BwdRing<T, VEC, SRC8>;
+    constexpr bool kAsync = Ring::kAsync;
+    constexpr int kVecBytes = Ring::kVecBytes, kCopy = kAsync ? kVecBytes : 4, kCopyQ = kAsync && SRC8 ? VEC : 4;
     extern __shared__ uint4 ring_raw[];         // the ring; at the end [2][d] sums of the teams
     __shared__ float red[2][kBwdThreads / 32][2];
     const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
@@ -362,12 +368,12 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
     // Running positions: a row's overhead is shared by 16 values only. In a slot the thread's vectors of dy, of the residual's
     // gradient, and of x (or of q and the exponents' words) follow one another with `n` threads between them.
     const uint32_t n = blockDim.x, base = (uint32_t)__cvta_generic_to_shared(ring_raw);
-    const uint32_t my16 = base + threadIdx.x * 16;
-    const uint32_t ring2 = base + Ring::kSlots * 2 * NV * n * 16;
+    const uint32_t my_y = base + threadIdx.x * kVecBytes;
+    const uint32_t ring2 = base + Ring::kSlots * 2 * NV * n * kVecBytes;
     const uint32_t my_q = ring2 + threadIdx.x * VEC, my_e = ring2 + Ring::kSlots * NV * n * VEC + threadIdx.x * 4;
-    auto at_y = [&](int s, int i) { return my16 + (uint32_t)((s * 2 + 0) * NV + i) * n * 16; };
-    auto at_j = [&](int s, int i) { return my16 + (uint32_t)((s * 2 + 1) * NV + i) * n * 16; };
-    auto at_x = [&](int s, int i) { return my16 + (uint32_t)(Ring::kSlots * 2 * NV + s * NV + i) * n * 16; };
+    auto at_y = [&](int s, int i) { return my_y + (uint32_t)((s * 2 + 0) * NV + i) * n * kVecBytes; };
+    auto at_j = [&](int s, int i) { return my_y + (uint32_t)((s * 2 + 1) * NV + i) * n * kVecBytes; };
+    auto at_x = [&](int s, int i) { return my_y + (uint32_t)(Ring::kSlots * 2 * NV + s * NV + i) * n * kVecBytes; };
     auto at_q = [&](int s, int i) { return my_q + (uint32_t)(s * NV + i) * n * VEC; };
     auto at_e = [&](int s, int i) { return my_e + (uint32_t)(s * NV + i) * n * 4; };
     const int64_t step = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + team;
@@ -383,13 +389,13 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                 for (int i = 0; i < NV; ++i) {
                     const int off = i * tpr * VEC;
                     if (c0 + off >= d) continue;
-                    copy_async<16>(at_y(s, i), ahead_y + off);
-                    if (join != nullptr) copy_async<16>(at_j(s, i), ahead_j + off);
+                    copy_async<kCopy>(at_y(s, i), ahead_y + off);
+                    if (join != nullptr) copy_async<kCopy>(at_j(s, i), ahead_j + off);
                     if constexpr (SRC8) {
-                        copy_async<VEC>(at_q(s, i), ahead_q + off);
+                        copy_async<kCopyQ>(at_q(s, i), ahead_q + off);
                         copy_async<4>(at_e(s, i), ahead_e + (c0 + off) / (4 * kAct8Block) * 4);   // the exponents of 128 columns
                     } else {
-                        copy_async<16>(at_x(s, i), ahead_x + off);
+                        copy_async<kCopy>(at_x(s, i), ahead_x + off);
                     }
                 }
             }
@@ -764,7 +770,7 @@ int launch_fwd(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ld
     // a CTA per row where a row takes several warps, so that a barrier stops nobody else
     const int threads = tpr == 32 ? 128 : tpr, teams = threads / tpr;
     const int64_t need = (rows + teams - 1) / teams;
-    const int smem = VEC > 1 ? kFwdSlots * NV * threads * 16 : 0;
+    const int smem = copies_ahead<T, VEC>() ? kFwdSlots * NV * threads * VEC * (int)sizeof(T) : 0;
     auto go = [&](auto instance) -> int {
         constexpr auto kern = decltype(instance)::value;
         int per_sm = 0;
