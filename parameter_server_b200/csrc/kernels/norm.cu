@@ -173,18 +173,21 @@ __device__ __forceinline__ void keep8(const float* f, bool valid, int8_t* qrow, 
 constexpr int kFwdSlots = 3;
 template <typename T, int VEC>
 constexpr bool copies_ahead() { return VEC * sizeof(T) >= 4; }
-template <typename T, int VEC, int NV, bool OUT8>
-__global__ void __launch_bounds__(kMaxTeam)
+// TPR: `tpr` known to the compiler, so that a thread's places in the row and in the ring are constants; 0 = `tpr_arg` (few rows).
+template <typename T, int VEC, int NV, bool OUT8, int TPR>
+__global__ void __launch_bounds__(TPR == 0 ? kMaxTeam : TPR == 32 ? 128 : TPR)
 layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, T* __restrict__ y,
                       int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
-                      int64_t lde, int64_t rows, int d, float eps, int tpr) {
+                      int64_t lde, int64_t rows, int d, float eps, int tpr_arg) {
+    const int tpr = TPR > 0 ? TPR : tpr_arg, threads = TPR == 0 ? (int)blockDim.x : TPR == 32 ? 128 : TPR;
     constexpr bool kAsync = copies_ahead<T, VEC>();
     constexpr int kVecBytes = VEC * (int)sizeof(T);
     using IO = Io<T, VEC>;
     extern __shared__ uint4 ring[];   // [kFwdSlots][NV][threads] vectors
     __shared__ float red[2][kMaxTeam / 32];
-    const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
+    const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = threads / tpr;
     const int warps = tpr / 32, w0 = team * warps;
+    const int nv = t * VEC < d ? min(NV, (d - t * VEC + tpr * VEC - 1) / (tpr * VEC)) : 0;   // this thread's vectors that exist
     const int64_t step = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams;
     typename IO::Raw graw[NV], braw[NV];
 #pragma unroll
@@ -194,14 +197,14 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
         braw[i] = bias != nullptr && col < d ? IO::load(bias + col) : IO::zero();
     }
     // running positions: a row's overhead is shared by 32 values only
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * kVecBytes, vec_stride = blockDim.x * kVecBytes, slot_stride = NV * vec_stride;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * kVecBytes, vec_stride = threads * kVecBytes, slot_stride = NV * vec_stride;
     const T* ahead = x + (first + team) * ldx + t * VEC;
     int64_t ahead_row = first + team;
     auto request = [&](int slot) {   // the next row that has not been asked for
         if (ahead_row < rows) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if ((i * tpr + t) * VEC < d) copy_async<kAsync ? kVecBytes : 4>(mine + slot * slot_stride + i * vec_stride, ahead + i * tpr * VEC);
+                if (i < nv) copy_async<kAsync ? kVecBytes : 4>(mine + slot * slot_stride + i * vec_stride, ahead + i * tpr * VEC);
         }
         close_group();   // (an empty group where there is no such row: the count of groups stays the same)
         ahead += step * ldx;
@@ -224,7 +227,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
         for (int i = 0; i < NV; ++i) {
             const int col = (i * tpr + t) * VEC;
             typename IO::Raw raw = IO::zero();
-            if (live && col < d) {
+            if (live && i < nv) {
                 if constexpr (kAsync) raw = from_shared<typename IO::Raw>(mine + slot * slot_stride + i * vec_stride);
                 else raw = IO::load(x + row * ldx + col);
             }
@@ -247,7 +250,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const bool in = (i * tpr + t) * VEC < d;
+            const bool in = i < nv;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i * VEC + j] -= mean;
@@ -262,7 +265,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int col = (i * tpr + t) * VEC;
-            const bool in = live && col < d;
+            const bool in = live && i < nv;
             float* f = v + i * VEC;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) f[j] *= rstd;
@@ -340,13 +343,16 @@ struct BwdRing {
     static constexpr int kBytes = kAsync ? kSlots * kRowBytes * kBwdThreads : 0;
 };
 
-template <typename T, int VEC, bool SRC8>
+// TPR: threads that share a row, known to the compiler, so that a thread's places in the row and in the ring are constants (with
+// a run-time value an element took twice the instructions); 0 = `tpr_arg` (8-bit rows that are not aligned).
+template <typename T, int VEC, bool SRC8, int TPR>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
                       int64_t ldq, const uint8_t* __restrict__ e, int64_t lde, const T* __restrict__ weight,
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const T* __restrict__ join, int64_t ldjoin,
-                      T* __restrict__ dx, int64_t lddx, float* __restrict__ partial, int64_t rows, int d, int tpr) {
+                      T* __restrict__ dx, int64_t lddx, float* __restrict__ partial, int64_t rows, int d, int tpr_arg) {
     constexpr int NV = kBwdElems / VEC;
+    const int tpr = TPR > 0 ? TPR : tpr_arg;
     using IO = Io<T, VEC>;
     using Ring = BwdRing<T, VEC, SRC8>;
     constexpr bool kAsync = Ring::kAsync;
@@ -367,7 +373,8 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
     const float inv_d = 1.f / (float)d;
     // Running positions: a row's overhead is shared by 16 values only. In a slot the thread's vectors of dy, of the residual's
     // gradient, and of x (or of q and the exponents' words) follow one another with `n` threads between them.
-    const uint32_t n = blockDim.x, base = (uint32_t)__cvta_generic_to_shared(ring_raw);
+    constexpr uint32_t n = kBwdThreads;
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring_raw);
     const uint32_t my_y = base + threadIdx.x * kVecBytes;
     const uint32_t ring2 = base + Ring::kSlots * 2 * NV * n * kVecBytes;
     const uint32_t my_q = ring2 + threadIdx.x * VEC, my_e = ring2 + Ring::kSlots * NV * n * VEC + threadIdx.x * 4;
@@ -378,6 +385,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
     auto at_e = [&](int s, int i) { return my_e + (uint32_t)(s * NV + i) * n * 4; };
     const int64_t step = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + team;
     const int c0 = t * VEC;
+    const int nv = c0 < d ? min(NV, (d - c0 + tpr * VEC - 1) / (tpr * VEC)) : 0;   // this thread's vectors that exist
     const T *ahead_y = dy + first * lddy + c0, *ahead_x = SRC8 ? nullptr : x + first * ldx + c0, *ahead_j = join != nullptr ? join + first * ldjoin + c0 : nullptr;
     const int8_t* ahead_q = SRC8 ? q + first * ldq + c0 : nullptr;
     const uint8_t* ahead_e = SRC8 ? e + first * lde : nullptr;
@@ -388,7 +396,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const int off = i * tpr * VEC;
-                    if (c0 + off >= d) continue;
+                    if (i >= nv) continue;
                     copy_async<kCopy>(at_y(s, i), ahead_y + off);
                     if (join != nullptr) copy_async<kCopy>(at_j(s, i), ahead_j + off);
                     if constexpr (SRC8) {
@@ -430,7 +438,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int col = (i * tpr + t) * VEC;
-            const bool in = col < d;
+            const bool in = i < nv;
             if constexpr (kAsync) ry[i] = in ? from_shared<typename IO::Raw>(at_y(slot, i)) : IO::zero();
             else ry[i] = in ? IO::load(dy + row * lddy + col) : IO::zero();
             if constexpr (SRC8) {
@@ -487,15 +495,14 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
         const float a1 = s1 * inv_d, a2 = s2 * inv_d;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * tpr + t) * VEC;
-            if (col >= d) continue;
+            if (i >= nv) continue;
             float o[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o[j] = rstd * (p[i * VEC + j] - fmaf(xh[i * VEC + j], a2, a1));
             if (join != nullptr) {
                 float fj[VEC];
                 if constexpr (kAsync) IO::unpack(from_shared<typename IO::Raw>(at_j(slot, i)), fj);
-                else IO::unpack(IO::load(join + row * ldjoin + col), fj);
+                else IO::unpack(IO::load(join + row * ldjoin + c0 + i * tpr * VEC), fj);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) o[j] += fj[j];
             }
@@ -764,7 +771,7 @@ cudaError_t ctas_per_sm(int threads, int smem, int* count) {
     return cudaSuccess;
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, int TPR>
 int launch_fwd(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep,
                int64_t rows, int d, float eps, int tpr, cudaStream_t s) {
     // a CTA per row where a row takes several warps, so that a barrier stops nobody else
@@ -780,7 +787,7 @@ int launch_fwd(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ld
         kern<<<grid, threads, smem, s>>>(x, ldx, w, b, y, ldy, mean, rstd, (int8_t*)keep.q, keep.ldq, (uint8_t*)keep.e, keep.lde, rows, d, eps, tpr);
         return (int)cudaGetLastError();
     };
-    return keep.q != nullptr ? go(Kernel<layer_norm_fwd_kernel<T, VEC, NV, true>>{}) : go(Kernel<layer_norm_fwd_kernel<T, VEC, NV, false>>{});
+    return keep.q != nullptr ? go(Kernel<layer_norm_fwd_kernel<T, VEC, NV, true, TPR>>{}) : go(Kernel<layer_norm_fwd_kernel<T, VEC, NV, false, TPR>>{});
 }
 
 template <typename T, int VEC>
@@ -790,10 +797,18 @@ int fwd_vec(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, 
     const int64_t vecs = (d + VEC - 1) / VEC;
     // fewer rows than SMs x 4: one vector per thread if 512 threads have the row
     if (rows <= 4 * kSms && vecs <= kMaxTeam)
-        return launch_fwd<T, VEC, 1>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, pow2_at_least(vecs, 32, kMaxTeam), s);
-    if (vecs <= 64) return launch_fwd<T, VEC, 2>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, 32, s);
-    if (vecs <= (int64_t)kMaxTeam * NV)
-        return launch_fwd<T, VEC, NV>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, pow2_at_least((vecs + NV - 1) / NV, 32, kMaxTeam), s);
+        return launch_fwd<T, VEC, 1, 0>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, pow2_at_least(vecs, 32, kMaxTeam), s);
+    if (vecs <= 64) return launch_fwd<T, VEC, 2, 32>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, 32, s);
+    if (vecs <= (int64_t)kMaxTeam * NV) {
+        const int tpr = pow2_at_least((vecs + NV - 1) / NV, 32, kMaxTeam);
+        switch (tpr) {
+            case 32: return launch_fwd<T, VEC, NV, 32>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, tpr, s);
+            case 64: return launch_fwd<T, VEC, NV, 64>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, tpr, s);
+            case 128: return launch_fwd<T, VEC, NV, 128>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, tpr, s);
+            case 256: return launch_fwd<T, VEC, NV, 256>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, tpr, s);
+            default: return launch_fwd<T, VEC, NV, 512>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, tpr, s);
+        }
+    }
     if (rows > 0x7FFFFFFF) return -2;
     if (keep.q != nullptr)
         layer_norm_fwd_long_kernel<T, true><<<(unsigned)rows, 512, 0, s>>>(x, ldx, w, b, y, ldy, mean, rstd, (int8_t*)keep.q, keep.ldq,
@@ -846,15 +861,28 @@ template <typename T, int VEC, bool SRC8>
 int launch_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View& k, const T* w, const float* mean, const float* rstd,
                const T* join, int64_t ldjoin, T* dx, int64_t lddx, float* partial, int64_t rows, int d, const BwdPlan& p, cudaStream_t s) {
     using Ring = BwdRing<T, VEC, SRC8>;
-    constexpr auto kern = layer_norm_bwd_kernel<T, VEC, SRC8>;
     // the ring, or the teams' sums (several teams means d <= 4096)
-    const int smem = std::max(Ring::kBytes / kBwdThreads * p.threads, p.threads > p.tpr ? 2 * d * (int)sizeof(float) : 0);
-    int per_sm = 0;
-    const cudaError_t rc = ctas_per_sm<kern>(p.threads, smem, &per_sm);
-    if (rc != cudaSuccess) return (int)rc;
-    kern<<<p.grid, p.threads, smem, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, w, mean, rstd, join, ldjoin, dx,
-                                         lddx, partial, rows, d, p.tpr);
-    return (int)cudaGetLastError();
+    const int smem = std::max(Ring::kBytes, p.threads > p.tpr ? 2 * d * (int)sizeof(float) : 0);
+    auto go = [&](auto instance) -> int {
+        constexpr auto kern = decltype(instance)::value;
+        int per_sm = 0;
+        const cudaError_t rc = ctas_per_sm<kern>(p.threads, smem, &per_sm);
+        if (rc != cudaSuccess) return (int)rc;
+        kern<<<p.grid, p.threads, smem, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde, w, mean, rstd, join, ldjoin,
+                                             dx, lddx, partial, rows, d, p.tpr);
+        return (int)cudaGetLastError();
+    };
+    if constexpr (SRC8 && VEC == 1) {
+        return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 0>>{});
+    } else {
+        switch (p.tpr) {
+            case 32: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 32>>{});
+            case 64: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 64>>{});
+            case 128: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 128>>{});
+            case 256: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 256>>{});
+            default: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 512>>{});
+        }
+    }
 }
 
 template <typename T, bool SRC8>
