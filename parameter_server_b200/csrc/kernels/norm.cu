@@ -330,7 +330,7 @@ layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __rest
 // dweight and dbias in registers over all of them, so that the weight's gradient costs no second pass over dy and x. The
 // next rows are copied to shared memory meanwhile, every thread its own part (see the forward kernel; loads into registers
 // left room for one row in flight and took 67 us for 16384 x 2048 with a residual gradient). The two row sums cross the
-// team's warps through shared memory with one barrier per row. At the end the teams' sums are added in team order and leave
+// team's warps through shared memory with one barrier per row. At the end the teams' sums are added in a tree and leave
 // as one partial row per CTA, which column_reduce_kernel adds in CTA order: the result does not depend on timing. (More CTAs
 // per SM would write and read more partial rows: 2 * d floats each.)
 template <typename T, int VEC, bool SRC8>
@@ -357,7 +357,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
     using Ring = BwdRing<T, VEC, SRC8>;
     constexpr bool kAsync = Ring::kAsync;
     constexpr int kVecBytes = Ring::kVecBytes, kCopy = kAsync ? kVecBytes : 4, kCopyQ = kAsync && SRC8 ? VEC : 4;
-    extern __shared__ uint4 ring_raw[];         // the ring; at the end [2][d] sums of the teams
+    extern __shared__ uint4 ring_raw[];         // the ring; at the end sums of the teams
     __shared__ float red[2][kBwdThreads / 32][2];
     const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
     const int warps = tpr / 32, w0 = team * warps, lane = threadIdx.x & 31;
@@ -512,30 +512,46 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
         slot = slot + 1 == Ring::kSlots ? 0 : slot + 1;
     }
     if (partial == nullptr) return;
+    // The teams' sums in a tree (the same one every time): the upper half hands its sums over, [16 + 16 sums][threads], and leaves.
     float* comb = (float*)ring_raw;
-    float* out = partial + (int64_t)blockIdx.x * 2 * d;
     if constexpr (kAsync) wait_groups<0>();
-    __syncthreads();   // the ring is free: its space takes the teams' sums
-    for (int k = 0; k < teams; ++k) {
-        if (team == k) {
+    __syncthreads();   // the ring is free
+    for (int half = teams / 2; half > 0; half /= 2) {
+        float* place = comb + (int64_t)(team - (team >= half ? half : 0)) * 2 * kBwdElems * tpr + t;
+        if (team >= half && team < 2 * half) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
+            for (int c = 0; c < kBwdElems; ++c) {
+                place[c * tpr] = dg[c];
+                place[(kBwdElems + c) * tpr] = db[c];
+            }
+        }
+        __syncthreads();
+        if (team < half) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int col = (i * tpr + t) * VEC + j, c = i * VEC + j;
-                    if (col >= d) continue;
-                    float* cg = teams > 1 ? comb : out;
-                    float g1 = dg[c], b1 = db[c];
-                    if (k > 0) { g1 += cg[col]; b1 += cg[d + col]; }
-                    cg[col] = g1;
-                    cg[d + col] = b1;
-                }
+            for (int c = 0; c < kBwdElems; ++c) {
+                dg[c] += place[c * tpr];
+                db[c] += place[(kBwdElems + c) * tpr];
             }
         }
         __syncthreads();
     }
-    if (teams > 1)
-        for (int c = threadIdx.x; c < 2 * d; c += blockDim.x) out[c] = comb[c];
+    if (team != 0) return;
+    float* out = partial + (int64_t)blockIdx.x * 2 * d + c0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (i >= nv) continue;
+        if constexpr (VEC >= 4) {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 4) {
+                const int c = i * VEC + j;
+                *(float4*)(out + i * tpr * VEC + j) = make_float4(dg[c], dg[c + 1], dg[c + 2], dg[c + 3]);
+                *(float4*)(out + d + i * tpr * VEC + j) = make_float4(db[c], db[c + 1], db[c + 2], db[c + 3]);
+            }
+        } else {
+            out[i * tpr] = dg[i];
+            out[d + i * tpr] = db[i];
+        }
+    }
 }
 
 // Rows longer than 8192 columns: dx with a CTA per row that reads it twice, and the weight's gradient by columns.
@@ -861,8 +877,8 @@ template <typename T, int VEC, bool SRC8>
 int launch_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View& k, const T* w, const float* mean, const float* rstd,
                const T* join, int64_t ldjoin, T* dx, int64_t lddx, float* partial, int64_t rows, int d, const BwdPlan& p, cudaStream_t s) {
     using Ring = BwdRing<T, VEC, SRC8>;
-    // the ring, or the teams' sums (several teams means d <= 4096)
-    const int smem = std::max(Ring::kBytes, p.threads > p.tpr ? 2 * d * (int)sizeof(float) : 0);
+    // the ring, or half the teams' sums
+    const int smem = std::max(Ring::kBytes, p.threads > p.tpr ? p.threads / 2 * 2 * kBwdElems * (int)sizeof(float) : 0);
     auto go = [&](auto instance) -> int {
         constexpr auto kern = decltype(instance)::value;
         int per_sm = 0;
