@@ -154,14 +154,14 @@ class _AttentionHalf(torch.autograd.Function):
         else:
             G.gemm(dy2, ctx.rows, a_mn=True, b_mn=True, out=Gr[f"h{i}.proj.w"], accumulate=True)
         linear_bias_grad(dy2, out=Gr[f"h{i}.proj.b"], accumulate=True)
-        da = G.linear_dgrad(dy2, P[f"h{i}.proj.w"])
+        da = linear_act_dgrad(dy2, P[f"h{i}.proj.w"], None)
         da = da.view(B, T, cfg.n_head, d // cfg.n_head).transpose(1, 2)
         (dqkv,) = torch.autograd.grad(ctx.attention, ctx.qkv, da)
         ctx.attention = ctx.qkv = ctx.rows = None
         table = model.qkv[i]
         w, wg = (P[f"h{i}.qkv.w"], Gr[f"h{i}.qkv.w"]) if table is None else (table.params["w"], table.grads["w"])
         norm.wgrad(dqkv, wg, Gr[f"h{i}.qkv.b"])
-        dx = norm.backward(G.linear_dgrad(dqkv, w), residual_grad=dy2)
+        dx = norm.backward(linear_act_dgrad(dqkv, w, None), residual_grad=dy2)
         ctx.norm = None
         return dx.view(dy.shape), None, None
 
@@ -190,7 +190,7 @@ class _MlpHalf(torch.autograd.Function):
         del f
         linear_bias_grad(dy2, out=Gr[f"h{i}.out.b"], accumulate=True)
         norm.wgrad(dh, Gr[f"h{i}.fc.w"], Gr[f"h{i}.fc.b"])
-        dx = norm.backward(G.linear_dgrad(dh, P[f"h{i}.fc.w"]), residual_grad=dy2)
+        dx = norm.backward(linear_act_dgrad(dh, P[f"h{i}.fc.w"], None), residual_grad=dy2)
         ctx.norm = None
         return dx.view(dy.shape), None, None
 
