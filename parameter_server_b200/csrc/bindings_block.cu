@@ -95,4 +95,5 @@ void bind_block(py::module_& m) {
     m.def("act8_wgrad_scratch", &act8_wgrad_scratch);
     m.def("linear_workspace_bytes", &linear_workspace_bytes);
     m.def("linear_workspace_zeros", &linear_workspace_zeros);
+    m.attr("NEEDS_WORKSPACE") = kNeedsWorkspace;
 }

@@ -87,11 +87,6 @@ __device__ __forceinline__ uint32_t convert2(uint32_t w, uint32_t s0, uint32_t s
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&v;
 }
-__device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -293,7 +288,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
             const uint32_t sq = q0 + ir * L::kRawStage, sx = x0 + ir * L::kRawStage + eb;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {   // odd: the other column block of the row (neither eb nor gg / 2 touches that bit)
-                nraw[i] = lds_v4(((i & 1) ? (sq ^ 64u) : sq) + 32 * (i / 2) * 128);
+                nraw[i] = ld_smem_v4(((i & 1) ? (sq ^ 64u) : sq) + 32 * (i / 2) * 128);
                 ne[i] = lds_u8(((i & 1) ? (sx ^ 2u) : sx) + 32 * (i / 2) * 16);
             }
             if (++ir == L::kRaw) { ir = 0; pr ^= 1u; }
@@ -344,7 +339,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
         // ---- epilogue ----
         const int ew = warp - 8, quarter = warp & 3, half = ew >> 2;
-        uint8_t* stage = stage_out + ew * 2048;
+        const uint32_t stage = smem_u32(stage_out) + (uint32_t)ew * 2048;
         TileWalk walk(p.grid, pair);
         Tile t;
         uint32_t tc = 0;
@@ -426,15 +421,17 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        *(float4*)(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-                            make_float4(acc[c * 16 + 4 * j], acc[c * 16 + 4 * j + 1], acc[c * 16 + 4 * j + 2], acc[c * 16 + 4 * j + 3]);
+                        st_smem_v4(stage + (uint32_t)(lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                                   make_uint4(__float_as_uint(acc[c * 16 + 4 * j]), __float_as_uint(acc[c * 16 + 4 * j + 1]),
+                                              __float_as_uint(acc[c * 16 + 4 * j + 2]), __float_as_uint(acc[c * 16 + 4 * j + 3])));
                     __syncwarp();
                     const int cb = lane & 3, col = colw + c * 16 + cb * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int r = i * 8 + (lane >> 2);
                         if (row0 + r >= p.N) continue;
-                        float4 d = *(const float4*)(stage + r * 64 + ((cb ^ ((r >> 1) & 3)) << 4));
+                        const uint4 w = ld_smem_v4(stage + (uint32_t)(r * 64 + ((cb ^ ((r >> 1) & 3)) << 4)));
+                        float4 d = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
                         float* op = p.out + (int64_t)(row0 + r) * p.ldo + col;
                         if (p.out_vec && col + 4 <= p.K) {
                             if (p.accumulate) {
@@ -474,12 +471,16 @@ bool make_byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t c
 }
 
 template <bool CONVERT>
-int launch_wgrad(WgParams& p, int64_t tokens, cudaStream_t s) {
-    constexpr auto kern = act8_wgrad_kernel<CONVERT>;
+int plan_wgrad(WgParams& p, int64_t tokens) {
     int pairs = 0;
-    cudaError_t e = pairs_of<kern>(kWgThreads, WgSmem<CONVERT>::kTotal, &pairs);
+    cudaError_t e = pairs_of<act8_wgrad_kernel<CONVERT>>(kWgThreads, WgSmem<CONVERT>::kTotal, &pairs);
     if (e != cudaSuccess) return (int)e;
     p.grid = plan_tiles((p.N + 2 * BM - 1) / (2 * BM), (p.K + kWgBN - 1) / kWgBN, (int)((tokens + BK - 1) / BK), pairs, 48, 8);
+    return p.grid.shared > 0 && p.arrived == nullptr ? kNeedsWorkspace : 0;
+}
+template <bool CONVERT>
+int launch_wgrad(const WgParams& p, cudaStream_t s) {
+    constexpr auto kern = act8_wgrad_kernel<CONVERT>;
     return (int)launch_pairs(kern, kWgThreads, WgSmem<CONVERT>::kTotal, p.grid.pairs, p, s);
 }
 
@@ -487,19 +488,20 @@ int launch_wgrad(WgParams& p, int64_t tokens, cudaStream_t s) {
 
 int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     if (a.N <= 0 || a.K <= 0) return 0;
-    if (a.tokens <= 0 || a.tokens > 0x7FFFFFFFll - 64 || a.workspace == nullptr || a.err_flag == nullptr || a.out == nullptr) return -2;
+    if (a.tokens <= 0 || a.tokens > 0x7FFFFFFFll - 64 || a.err_flag == nullptr || a.out == nullptr) return -2;
     if (a.bias != nullptr && a.dy_sum == nullptr) return -2;
     if (!rows16(a.dy, a.lddy) || ((uintptr_t)a.x.q % 16) || (a.x.ldq % 16) || ((uintptr_t)a.x.e % 16) || (a.x.lde % 16)) return -2;
     const uint64_t tokens = (uint64_t)a.tokens, blocks = (uint64_t)(a.K + kAct8Block - 1) / kAct8Block;
     const bool convert = a.scratch == nullptr;
     const int64_t ldx = ((int64_t)a.K + 7) / 8 * 8;
-    if (!convert) {
-        const int rc = act8_unpack(0, a.x, a.scratch, ldx, a.tokens, a.K, stream);
-        if (rc != 0) return rc;
-    }
     WgParams p;
     p.N = a.N;
     p.K = a.K;
+    p.arrived = (unsigned*)a.workspace;
+    p.partial = a.workspace == nullptr ? nullptr : (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
+    int rc = convert ? plan_wgrad<true>(p, a.tokens) : plan_wgrad<false>(p, a.tokens);
+    if (rc == 0 && !convert) rc = act8_unpack(0, a.x, a.scratch, ldx, a.tokens, a.K, stream);
+    if (rc != 0) return rc;
     p.a_blocked = a.N % 64 == 0 && a.N >= BM ? 1 : 0;
     p.b_blocked = a.K % 64 == 0 && a.K >= 128 ? 1 : 0;
     bool ok = p.a_blocked ? make_map_blocked(&p.map_a, a.dy, tokens, (uint64_t)a.N, (uint64_t)a.lddy, BM / 64)
@@ -520,11 +522,9 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     p.weight = (const __nv_bfloat16*)a.weight;
     p.bias = (const __nv_bfloat16*)a.bias;
     p.dy_sum = a.dy_sum;
-    p.arrived = (unsigned*)a.workspace;
-    p.partial = (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
-    return convert ? launch_wgrad<true>(p, a.tokens, (cudaStream_t)stream) : launch_wgrad<false>(p, a.tokens, (cudaStream_t)stream);
+    return convert ? launch_wgrad<true>(p, (cudaStream_t)stream) : launch_wgrad<false>(p, (cudaStream_t)stream);
 }
 
 // Converting tile by tile repeats the work for every 256 rows of dw and costs the tensor cores a fifth of their time;

@@ -18,8 +18,8 @@ namespace {
 
 constexpr int kFewThreads = 512;
 constexpr int kFewTokens = 128;    // of a tile
-constexpr int kFewMaxStages = 8;
-constexpr int kFewSmem = 108 * 1024;
+constexpr int kFewMaxStages = 12;
+constexpr int kFewSmem = 220 * 1024, kFewSmemShared = 108 * 1024;   // one CTA on an SM, two
 
 struct FewParams {
     CUtensorMap map_w, map_x;
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = BM * BK * 2 + p.columns * BK * 2;
-    float* parts = (float*)smem;   // [tokens][128 features]: this CTA's sums, where the stages were
+    const uint32_t parts = smem_u32(smem);   // float [tokens][128 features]: this CTA's sums, where the stages were
     uint64_t* full_bar = (uint64_t*)(smem + p.ring_bytes);
     uint64_t* empty_bar = full_bar + kFewMaxStages;
     uint64_t* done_bar = empty_bar + kFewMaxStages;
@@ -121,6 +121,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int k_begin = (int)((int64_t)p.k_steps * rank / S), k_end = (int)((int64_t)p.k_steps * (rank + 1) / S), nk = k_end - k_begin;
     const int share = (p.columns + S - 1) / S;   // tokens that one CTA finishes
+    auto load = [&](int k, int s) {
+        const int k0 = (k_begin + k) * BK;
+        uint8_t* sa = smem + s * stage_bytes;
+        mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
+        if constexpr (!DGRAD) {
+            tma_load_2d(sa, &p.map_w, &full_bar[s], k0, n0);   // [128 features][64 k]
+        } else {
+            tma_load_2d(sa, &p.map_w, &full_bar[s], n0, k0);   // two blocks of [64 k][64 features]
+            tma_load_2d(sa + 64 * 128, &p.map_w, &full_bar[s], n0 + 64, k0);
+        }
+        tma_load_2d(sa + BM * BK * 2, &p.map_x, &full_bar[s], k0, m0);   // [tokens][64 k]
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
@@ -129,8 +141,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         }
         mbar_init(done_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_w) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&p.map_x) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        wait_predecessor();
+        for (int k = 0; k < min(nk, p.stages); ++k) load(k, k);   // the loads need no TMEM: they start before it is there
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(128u) : "memory");
@@ -140,35 +153,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *((volatile uint32_t*)tmem_slot);
+    wait_predecessor();
+    allow_successor();
 
     if (warp == 0) {
         if (lane == 0) {
             // ---- TMA producer ----
-            for (int k = 0; k < nk; ++k) {
-                const int s = k % p.stages;
-                if (k >= p.stages && !mbar_wait(&empty_bar[s], ((k / p.stages) & 1u) ^ 1u, p.limit_ns)) {
+            uint32_t ph = 0;
+            for (int k = p.stages, s = 0; k < nk; ++k) {
+                if (!mbar_wait(&empty_bar[s], ph, p.limit_ns)) {
                     atomicCAS(p.err_flag, 0u, 41u);
                     break;
                 }
-                uint8_t* sa = smem + s * stage_bytes;
-                const int k0 = (k_begin + k) * BK;
-                mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
-                if constexpr (!DGRAD) {
-                    tma_load_2d(sa, &p.map_w, &full_bar[s], k0, n0);   // [128 features][64 k]
-                } else {
-                    tma_load_2d(sa, &p.map_w, &full_bar[s], n0, k0);   // two blocks of [64 k][64 features]
-                    tma_load_2d(sa + 64 * 128, &p.map_w, &full_bar[s], n0 + 64, k0);
+                load(k, s);
+                if (++s == p.stages) {
+                    s = 0;
+                    ph ^= 1u;
                 }
-                tma_load_2d(sa + BM * BK * 2, &p.map_x, &full_bar[s], k0, m0);   // [tokens][64 k]
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             // ---- MMA issuer: D[feature][token] ----
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 15) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-            for (int k = 0; k < nk; ++k) {
-                const int s = k % p.stages;
-                if (!mbar_wait(&full_bar[s], (k / p.stages) & 1u, p.limit_ns * 2)) {
+            uint32_t ph = 0;
+            for (int k = 0, s = 0; k < nk; ++k) {
+                if (!mbar_wait(&full_bar[s], ph, p.limit_ns * 2)) {
                     atomicCAS(p.err_flag, 0u, 42u);
                     break;
                 }
@@ -180,15 +190,48 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
                     umma_bf16(tmem, da, make_desc(sb + u * 32, 16, 1024), idesc, (k | u) ? 1u : 0u);
                 }
                 umma_commit(&empty_bar[s]);
+                if (++s == p.stages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
             umma_commit(done_bar);   // (also on error, so that nobody waits for it)
         }
     }
     __syncwarp();
+    // what the epilogue needs from memory, on its way meanwhile: a warp has a token, a lane four neighbouring features
+    const int n = n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
+    const int t_end = min(tokens, (rank + 1) * share), t_first = rank * share + warp;
+    float b[4] = {0.f, 0.f, 0.f, 0.f}, aux[4];
+    if constexpr (!DGRAD) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < have) b[j] = p.bias32 != nullptr ? p.bias32[n + j] : p.bias != nullptr ? __bfloat162float(p.bias[n + j]) : 0.f;
+    }
+    auto fetch = [&](int t) {   // residual, or h
+#pragma unroll
+        for (int j = 0; j < 4; ++j) aux[j] = 0.f;
+        if (have <= 0 || t >= t_end) return;
+        const int64_t row = m0 + t;
+        if constexpr (!DGRAD) {
+            if (p.res != nullptr) load4(p.res + row * p.ldres + n, have, p.res_wide != 0, aux);
+        } else if (p.q != nullptr) {
+            const uint32_t w = *(const uint32_t*)(p.q + row * p.ldq + n) ^ 0x80808080u;   // (rows are padded to 16 bytes)
+            const float step = act8_step(p.e[row * p.lde + n / kAct8Block]);
+            aux[0] = s8_of_biased<0>(w) * step;
+            aux[1] = s8_of_biased<1>(w) * step;
+            aux[2] = s8_of_biased<2>(w) * step;
+            aux[3] = s8_of_biased<3>(w) * step;
+        } else if (p.pre != nullptr) {
+            load4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, aux);
+        }
+    };
+    fetch(t_first);
     // ---- this CTA's sums to its shared memory: the MMAs have read all stages, and no load is in flight ----
-    const bool ok = mbar_wait(done_bar, 0u, p.limit_ns * 4);
-    if (!ok && lane == 0) atomicCAS(p.err_flag, 0u, 43u);
-    __syncwarp();
+    // (One warp asks the barrier, the others sleep at the CTA's: with all sixteen asking, a k-step's four MMAs took 735 cycles to issue.)
+    if (warp == 1 && !mbar_wait(done_bar, 0u, p.limit_ns * 4) && lane == 0) atomicCAS(p.err_flag, 0u, 43u);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
     {
         // four warps share a quarter of TMEM's lanes (warp % 4) and take its columns in turn
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -197,7 +240,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             uint32_t v[16];
             tmem_ld16_issue(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t0, v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) parts[(t0 + j) * BM + quarter * 32 + lane] = __uint_as_float(v[j]);
+            for (int j = 0; j < 16; ++j)
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(parts + (uint32_t)((t0 + j) * BM + quarter * 32 + lane) * 4), "r"(v[j]) : "memory");
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
@@ -206,35 +250,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128u) : "memory");
     }
-    // ---- epilogue of this CTA's tokens: a warp has a token, a lane four neighbouring features ----
-    const int n = n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (!DGRAD) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < have) b[j] = p.bias32 != nullptr ? p.bias32[n + j] : p.bias != nullptr ? __bfloat162float(p.bias[n + j]) : 0.f;
-    }
-    const uint32_t mine = smem_u32(parts) + (uint32_t)lane * 16;
-    const int t_end = min(tokens, (rank + 1) * share);
-    for (int t = rank * share + warp; t < t_end; t += kFewThreads / 32) {
+    // ---- epilogue of this CTA's tokens ----
+    const uint32_t mine = parts + (uint32_t)lane * 16;
+    for (int t = t_first; t < t_end; t += kFewThreads / 32) {
         const int64_t row = m0 + t;
-        float v[4], aux[4] = {0.f, 0.f, 0.f, 0.f};
-        if (have > 0) {
-            if constexpr (!DGRAD) {
-                if (p.res != nullptr) load4(p.res + row * p.ldres + n, have, p.res_wide != 0, aux);
-            } else {
-                if (p.q != nullptr) {
-                    const uint32_t w = *(const uint32_t*)(p.q + row * p.ldq + n) ^ 0x80808080u;   // (rows are padded to 16 bytes)
-                    const float step = act8_step(p.e[row * p.lde + n / kAct8Block]);
-                    aux[0] = s8_of_biased<0>(w) * step;
-                    aux[1] = s8_of_biased<1>(w) * step;
-                    aux[2] = s8_of_biased<2>(w) * step;
-                    aux[3] = s8_of_biased<3>(w) * step;
-                } else if (p.pre != nullptr) {
-                    load4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, aux);
-                }
-            }
-        }
+        float v[4];
         const uint32_t at = mine + (uint32_t)(t * BM) * 4;
         if (S == 8) add_parts<8>(at, v);
         else if (S == 4) add_parts<4>(at, v);
@@ -256,11 +276,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = act_of<ACT>(v[j]) + aux[j];
+            fetch(t + kFewThreads / 32);   // (before the stores: another lane's residual is never what this one writes)
             if (have > 0) store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
         } else {
             float a[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] *= act_slope<ACT>(aux[j], &a[j]);
+            fetch(t + kFewThreads / 32);
             if (have > 0) {
                 store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
                 if (p.out2 != nullptr) store4(p.out2 + row * p.ldo2 + n, have, p.out2_wide != 0, a);
@@ -288,13 +310,9 @@ int launch_few(const FewParams& p, int cluster, int smem, cudaStream_t s) {
     cfg.blockDim = dim3(kFewThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute a[1];
-    a[0].id = cudaLaunchAttributeClusterDimension;
-    a[0].val.clusterDim.x = cluster;
-    a[0].val.clusterDim.y = 1;
-    a[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute a[2] = {in_clusters(cluster), start_early()};
     cfg.attrs = a;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
@@ -354,7 +372,9 @@ int linear_few(const LinearArgs& a, cudaStream_t s) {
     p.n_tiles = (a.N + BM - 1) / BM;
     const int cluster = few_cluster(a.M, a.N, a.K);
     const int stage_bytes = (BM + p.columns) * BK * 2, extra = 1024 + 512;
-    p.stages = std::min(std::min(kFewMaxStages, (kFewSmem - extra) / stage_bytes), (p.k_steps + cluster - 1) / cluster);
+    const int64_t ctas = (int64_t)p.n_tiles * ((p.M + kFewTokens - 1) / kFewTokens) * cluster;
+    const int room = ctas <= 2 * kMaxPairs && cluster < 8 ? kFewSmem : kFewSmemShared;
+    p.stages = std::min(std::min(kFewMaxStages, (room - extra) / stage_bytes), (p.k_steps + cluster - 1) / cluster);
     p.ring_bytes = std::max(p.stages * stage_bytes, p.columns * BM * 4);
     const int smem = p.ring_bytes + extra;
     switch (a.act) {

@@ -158,7 +158,7 @@ __device__ __forceinline__ float bf16_at(const uint4* raw, int j) {   // j is a 
 // A warp's [32 rows][32 columns] of bf16 results, one row per lane, through the warp's 2 KB of shared memory so that every
 // store instruction writes 8 whole 64-byte row segments instead of 16 bytes in each of 32 rows. The 16-byte blocks of a row
 // are XOR-swizzled by (row / 2) % 4: neither side has bank conflicts.
-__device__ __forceinline__ void store_piece(uint8_t* stage, int lane, const float* f, __nv_bfloat16* out, int64_t ldo, int row0, int col0, int M,
+__device__ __forceinline__ void store_piece(uint32_t stage, int lane, const float* f, __nv_bfloat16* out, int64_t ldo, int row0, int col0, int M,
                                             int N, bool vec) {
     uint4 raw[4];
 #pragma unroll
@@ -168,25 +168,29 @@ __device__ __forceinline__ void store_piece(uint8_t* stage, int lane, const floa
         for (int t = 0; t < 4; ++t) h[t] = __floats2bfloat162_rn(f[8 * j + 2 * t], f[8 * j + 2 * t + 1]);
     }
     __syncwarp();   // the reads of the piece before are done
-    uint8_t* mine = stage + lane * 64;
+    const uint32_t mine = stage + (uint32_t)lane * 64;
     const int sw = (lane >> 1) & 3;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) *(uint4*)(mine + ((j ^ sw) << 4)) = raw[j];
+    for (int j = 0; j < 4; ++j) st_smem_v4(mine + (uint32_t)((j ^ sw) << 4), raw[j]);
     __syncwarp();
-    const int cb = lane & 3, col = col0 + cb * 8;
+    const int cb = lane & 3, r0 = lane >> 2, col = col0 + cb * 8;
+    uint4 d[4];   // rows r0 + 8 i
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        const uint4 d = *(const uint4*)(stage + r * 64 + ((cb ^ ((r >> 1) & 3)) << 4));
-        if (row0 + r < M) {
-            __nv_bfloat16* op = out + (int64_t)(row0 + r) * ldo + col;
-            if (vec && col + 8 <= N) {
-                *(uint4*)op = d;
-            } else {
-                const __nv_bfloat16* h = (const __nv_bfloat16*)&d;
-                for (int t = 0; t < 8; ++t)
-                    if (col + t < N) op[t] = h[t];
-            }
+    for (int i = 0; i < 4; ++i) d[i] = ld_smem_v4(stage + (uint32_t)(i * 512 + r0 * 64 + ((cb ^ ((r0 >> 1) & 3)) << 4)));
+    __nv_bfloat16* op = out + (int64_t)(row0 + r0) * ldo + col;
+    if (vec && col + 8 <= N) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (row0 + r0 + 8 * i < M) *(uint4*)(op + 8 * i * ldo) = d[i];
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            if (row0 + r0 + 8 * i >= M) break;
+            const uint4 x = i == 0 ? d[0] : i == 1 ? d[1] : i == 2 ? d[2] : d[3];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                if (col + t < N) ((unsigned short*)(op + 8 * i * ldo))[t] = (unsigned short)(w[t / 2] >> (16 * (t & 1)));
         }
     }
 }
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
         // ---- epilogue ----
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2, etid = ew * 32 + lane;
         constexpr int kPieces = BN / 64;   // 32-column pieces of a warp
-        uint8_t* stage = stage_out + ew * 2048;
+        const uint32_t stage = smem_u32(stage_out) + (uint32_t)ew * 2048;
         TileWalk walk(p.grid, pair);
         Tile t;
         uint32_t tc = 0;
@@ -356,13 +360,13 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             const int tile_n = t.n * BN, row0 = t.m * 2 * BM + cr * BM + quarter * 32, row = row0 + lane;
             const int cbase = half * (BN / 2), colw = tile_n + cbase;   // first column of this warp
             const bool live = row < p.M;
-            float* bs = bias_smem + buf * BN;
+            const uint32_t bs = smem_u32(bias_smem) + buf * (uint32_t)(BN * 4);
             if constexpr (!DGRAD) {
                 if (etid < BN) {   // (BN = 128: the first four warps)
                     const int col = tile_n + etid;
                     float v = 0.f;
                     if (col < p.N) v = p.bias32 != nullptr ? p.bias32[col] : p.bias != nullptr ? __bfloat162float(p.bias[col]) : 0.f;
-                    bs[etid] = v;
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(bs + (uint32_t)etid * 4), "f"(v) : "memory");
                 }
             }
             // What a piece needs from memory (residual, or h) is requested before the piece ahead of it is worked on, the first
@@ -391,9 +395,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 if constexpr (kPieces == 4) ex = *(const uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32);
                 else ex = *(const uint16_t*)(p.e + (int64_t)row * p.lde + colw / 32);
             }
-            const bool waited = mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            // one barrier of the epilogue warps per tile: publishes the bias, and makes the decision to give up uniform
+            // One barrier of the epilogue warps per tile: publishes the bias, and makes the decision to give up uniform. One warp
+            // asks for the accumulator, the others sleep at this barrier (asking takes issue slots from the MMAs' thread).
+            const bool waited = ew != 0 || mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             uint32_t all_ok;
             asm volatile(
                 "{\n\t.reg .pred p, q;\n\t"
@@ -407,6 +412,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 if (!waited && lane == 0) atomicCAS(p.err_flag, 0u, 23u);
                 break;
             }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)BN + (uint32_t)cbase;
             auto release = [&]() {   // this warp has read the accumulator
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -423,8 +429,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 if constexpr (!DGRAD) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        const float4 b = *(const float4*)(bs + cbase + c * 32 + j);
-                        f[j] += b.x; f[j + 1] += b.y; f[j + 2] += b.z; f[j + 3] += b.w;
+                        const uint4 b = ld_smem_v4(bs + (uint32_t)(cbase + c * 32 + j) * 4);
+                        f[j] += __uint_as_float(b.x); f[j + 1] += __uint_as_float(b.y);
+                        f[j + 2] += __uint_as_float(b.z); f[j + 3] += __uint_as_float(b.w);
                     }
                     if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_vec != 0);
                     if (p.q != nullptr) ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
@@ -602,6 +609,7 @@ int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
     const int group = (int64_t)p.N * k_steps * BK * 2 <= (48ll << 20) ? 1 : 8;
     // Joining a cut tile takes 10 to 20 us (its parts are read one after the other, eight 16-byte loads in flight per thread).
     p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 64, group);
+    if (p.grid.shared > 0 && p.arrived == nullptr) return kNeedsWorkspace;
     return (int)launch_pairs(kern, kLinThreads, LinSmem<BN>::kTotal, p.grid.pairs, p, s);
 }
 
@@ -651,7 +659,7 @@ int linear_typed(const LinearArgs& a, cudaStream_t s) {
     p.out_vec = rows16(a.out, a.ldo);
     p.out2_vec = rows16(a.out2, a.ldo2);
     p.arrived = (unsigned*)a.workspace;
-    p.partial = (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
+    p.partial = a.workspace == nullptr ? nullptr : (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
     const int k_steps = (a.K + BK - 1) / BK;

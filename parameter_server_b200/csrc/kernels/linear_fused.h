@@ -31,12 +31,15 @@ struct LinearArgs {
     int64_t lde = 0;
     int M = 0, N = 0, K = 0;
     void* workspace = nullptr;       // linear_workspace_bytes() bytes; the first linear_workspace_zeros() are zero before the
-                                     // first call and left zero by every call
+                                     // first call and left zero by every call. Null: tried without (see kNeedsWorkspace)
     unsigned* err_flag = nullptr;    // device word, set non-zero when a bounded wait ran out
     double wait_limit_s = 2.0;
 };
 
-// Returns 0, a cudaError_t, -2 (alignment or an argument that is not supported) or -3 (tensor map).
+// Nothing was launched: tiles are cut along the contraction here and meet in a workspace, which is null.
+constexpr int kNeedsWorkspace = -4;
+
+// Returns 0, a cudaError_t, -2 (alignment or an argument that is not supported), -3 (tensor map) or kNeedsWorkspace.
 int linear_fused(const LinearArgs& args, void* stream);
 int64_t linear_workspace_bytes();
 int64_t linear_workspace_zeros();

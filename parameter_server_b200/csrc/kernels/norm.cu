@@ -257,7 +257,7 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
                 if (in) s += v[i * VEC + j] * v[i * VEC + j];
             }
         }
-        const float rstd = rsqrtf(team_sum(s, 1) / (float)d + eps);
+        const float rstd = __frsqrt_rn(team_sum(s, 1) / (float)d + eps);
         if (live && t == 0) {
             if (mean_out != nullptr) mean_out[row] = mean;
             rstd_out[row] = rstd;
@@ -305,7 +305,7 @@ layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __rest
     const float mean = block_sum(s, red) / (float)d;
     s = 0.f;
     for (int c = threadIdx.x; c < d; c += blockDim.x) { Io<T, 1>::unpack(xr[c], &f); s += (f - mean) * (f - mean); }
-    const float rstd = rsqrtf(block_sum(s, red) / (float)d + eps);
+    const float rstd = __frsqrt_rn(block_sum(s, red) / (float)d + eps);
     if (threadIdx.x == 0) {
         if (mean_out != nullptr) mean_out[row] = mean;
         rstd_out[row] = rstd;

@@ -44,7 +44,9 @@ __device__ __forceinline__ unsigned long long gtimer() {
 }
 // Bounded wait; returns false when the limit ran out.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
-    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)   // (the timer is far from the SM: it is asked only in a wait that drags on)
+        if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long t0 = gtimer();
     unsigned spins = 0;
     while (!mbar_try_wait(bar, parity)) {
@@ -202,6 +204,39 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t* v) {
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Programmatic dependent launch: a kernel that was allowed to start beside its predecessor's tail (`start_early`) touches no global
+// memory before wait_predecessor() has returned. It allows its own successor to start once its TMEM is allocated in every CTA: a
+// successor that got the TMEM first would wait for this kernel, and this kernel for the TMEM.
+__device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void allow_successor() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// 16 bytes of this CTA's shared memory by its 32-bit address. (A pointer that was rounded up as an integer is a generic one to the
+// compiler, and a generic access takes several times as long.)
+__device__ __forceinline__ uint4 ld_smem_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_smem_v4(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// ---- host: launches ----------------------------------------------------------------------------------
+inline cudaLaunchAttribute start_early() {
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+inline cudaLaunchAttribute in_clusters(int size) {
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = size;
+    a.val.clusterDim.y = 1;
+    a.val.clusterDim.z = 1;
+    return a;
 }
 
 // ---- host: tensor maps -------------------------------------------------------------------------------

@@ -96,10 +96,20 @@ class Act8:
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Act8":
-        ldq, lde = -(-cols // 16) * 16, -(-(-(-cols // BLOCK)) // 16) * 16
+        return cls._like(torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device), cols)
+
+    @classmethod
+    def for_rows(cls, x: torch.Tensor, cols: int) -> "Act8":
+        """An empty checkpoint for as many rows as the matrix ``x`` has, where it lives."""
+        return cls._like(x.new_empty((x.shape[0], -(-cols // 16) * 16), dtype=torch.int8), cols)
+
+    @classmethod
+    def _like(cls, q: torch.Tensor, cols: int) -> "Act8":
+        rows, ldq = q.shape
+        lde = -(-cols // 512) * 16   # one byte per 32 columns, padded to 16
         self = cls.__new__(cls)
-        self.q = torch.empty((rows, ldq), dtype=torch.int8, device=device)
-        self.e = torch.empty((rows, lde), dtype=torch.uint8, device=device)
+        self.q = q
+        self.e = q.new_empty((rows, lde), dtype=torch.uint8)
         self.rows, self.cols = rows, cols
         self._args = (self.q.data_ptr(), ldq, self.e.data_ptr(), lde)
         return self
@@ -136,7 +146,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
         raise ValueError(f"act8_pack: bf16 or fp32, not {x.dtype}")
     s = launch_stream(x)
     x = rows2d(x, "act8_pack")
-    out = Act8.empty(x.shape[0], x.shape[1], x.device)
+    out = Act8.for_rows(x, x.shape[1])
     check(C.act8_pack(dt, x.data_ptr(), row_stride(x), *out.args(), out.rows, out.cols, s), "act8_pack")
     return out
 
@@ -147,7 +157,7 @@ def act8_unpack(a: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     if dt is None:
         raise ValueError(f"act8_unpack: bf16 or fp32, not {dtype}")
     s = launch_stream(a.q)
-    x = torch.empty((a.rows, a.cols), dtype=dtype, device=a.q.device)
+    x = a.q.new_empty((a.rows, a.cols), dtype=dtype)
     check(C.act8_unpack(dt, *a.args(), x.data_ptr(), a.cols, a.rows, a.cols, s), "act8_unpack")
     return x
 
@@ -177,7 +187,7 @@ def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = N
     if out is None:
         if accumulate:
             raise ValueError(f"{what}: accumulate needs out")
-        out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
+        out = dy2.new_empty((n, k), dtype=torch.float32)
     elif out.shape != (n, k) or out.dtype != torch.float32 or out.device != dy.device or (k > 1 and out.stride(1) != 1):
         raise ValueError(f"{what}: out must be a {n} x {k} fp32 matrix on {dy.device} with contiguous rows")
     if tokens == 0:
@@ -185,8 +195,13 @@ def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = N
     if n and k:
         need = C.act8_wgrad_scratch(tokens, n, k)
         scratch = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
-        check(C.act8_wgrad(dy2.data_ptr(), _ld(dy2), *x8.args(), out.data_ptr(), row_stride(out), accumulate,
-                           0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-                           0 if dy_sum is None else dy_sum.data_ptr(), tokens, n, k, 0 if scratch is None else scratch.data_ptr(), workspace(dy.get_device(), s).data_ptr(),
-                           _err_flag(dy.device).data_ptr(), wait_limit_s, s), what)
+        head = (dy2.data_ptr(), _ld(dy2), *x8.args(), out.data_ptr(), row_stride(out), accumulate, 0 if weight is None else weight.data_ptr(),
+                0 if bias is None else bias.data_ptr(), 0 if dy_sum is None else dy_sum.data_ptr(), tokens, n, k,
+                0 if scratch is None else scratch.data_ptr())
+        tail = (_err_flag(dy.device).data_ptr(), wait_limit_s, s)
+        rc = C.act8_wgrad(*head, 0, *tail)
+        if rc == C.NEEDS_WORKSPACE:   # only where tiles are cut along the contraction
+            joined = workspace(dy.get_device(), s)
+            rc = C.act8_wgrad(*head, joined.data_ptr(), *tail)
+        check(rc, what)
     return out

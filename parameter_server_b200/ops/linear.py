@@ -28,14 +28,17 @@ def _act_code(act, what: str) -> int:
     return code
 
 
-def _launch(dgrad, act, M, N, K, a, w, bias, residual, out, out2, pre, kept, limit, s, what):
+def _launch(dgrad, act, M, N, K, a, w, bias, residual, out, out2, pre, kept, limit, s, what, scratch=0):
     rc = C.linear_fused(dgrad, act, M, N, K, a.data_ptr(), _ld(a), w.data_ptr(), _ld(w),
                         0 if bias is None else bias.data_ptr(), bias is not None and bias.dtype == torch.float32,
                         0 if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
                         out.data_ptr(), row_stride(out), 0 if out2 is None else out2.data_ptr(), N,
                         0 if pre is None else pre.data_ptr(), 0 if pre is None else row_stride(pre),
                         *((0, 0, 0, 0) if kept is None else kept.args()),
-                        workspace(a.get_device(), s).data_ptr(), _err_flag(a.device).data_ptr(), limit, s)
+                        scratch, _err_flag(a.device).data_ptr(), limit, s)
+    if rc == C.NEEDS_WORKSPACE and scratch == 0:   # only where tiles are cut along the contraction
+        scratch = workspace(a.get_device(), s)
+        return _launch(dgrad, act, M, N, K, a, w, bias, residual, out, out2, pre, kept, limit, s, what, scratch.data_ptr())
     check(rc, what)
 
 
@@ -78,7 +81,7 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
         if N > 1 and y.stride(1) != 1:
             raise ValueError(f"{what}: the values of a row of out must be contiguous")
     pre = x2.new_empty((M, N)) if save == "bf16" else None
-    kept = Act8.empty(M, N, x.device) if save == "act8" else None
+    kept = Act8.for_rows(y, N) if save == "act8" else None
     if M and N:
         _launch(False, code, M, N, K, x2, w, bias, r2, y, None, pre, kept, wait_limit_s, s, what)
     if out is not None:
@@ -138,7 +141,7 @@ def linear_bias_grad(dy: torch.Tensor, out: Optional[torch.Tensor] = None, accum
     if out is None:
         if accumulate:
             raise ValueError("linear_bias_grad: accumulate needs out")
-        out = torch.empty(n, dtype=torch.float32, device=dy.device)
+        out = dy2.new_empty(n, dtype=torch.float32)
     elif out.dtype != torch.float32 or out.shape != (n,) or out.device != dy.device or not out.is_contiguous():
         raise ValueError(f"linear_bias_grad: out must be {n} contiguous fp32 values on {dy.device}")
     partial = dy2.new_empty(C.column_sum_scratch(rows, n), dtype=torch.float32)

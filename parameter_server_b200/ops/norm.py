@@ -38,7 +38,7 @@ def _forward(x, weight, bias, eps, keep8, what):
     y = torch.empty_like(x2) if x2.is_contiguous() else x2.new_empty((rows, d))
     rstd = x2.new_empty(rows, dtype=torch.float32)
     if keep8:
-        kept, mean = Act8.empty(rows, d, x.device), None
+        kept, mean = Act8.for_rows(x2, d), None
         k = kept.args()
     else:
         kept, mean = None, torch.empty_like(rstd)
