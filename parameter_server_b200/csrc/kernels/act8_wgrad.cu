@@ -133,15 +133,22 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    cluster_arrive_all();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * kWgBN))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
+    cluster_wait_all();   // the peer's barriers must exist before anything is signalled on them
+    wait_predecessor();
+    uint32_t tmem_base = 0;
+    if (warp == 1 || warp >= 8) {   // (loads and converters need no TMEM and do not wait for it)
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        meet_named(2, 32 * (1 + kLinEpilogueWarps));
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_base = *((volatile uint32_t*)tmem_slot);
+        allow_successor();
+    }
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
@@ -266,7 +273,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         // other. A thread does this for rows r0 and r0 + 32.
         const int ct = threadIdx.x - 128, gg = ct & 3, rr = (ct >> 2) & 1, r0 = 2 * (ct >> 3) + rr;
         const int c0 = ((2 * gg) ^ (r0 & 7)) << 4, c1 = ((2 * gg + 1) ^ (r0 & 7)) << 4;
-        // One k-step ahead: the next k-step's bytes are requested before this one's are converted.
         // One k-step ahead: the next k-step's bytes are requested before this one's are converted, and the barriers of the step
         // after are asked before they are needed.
         TileWalk walk(p.grid, pair);
@@ -350,12 +356,14 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
             for (int j = 0; j < 128; ++j) acc[j] = 0.f;
             for (int k = 0; k < t.nk; k += kWgChain, ++tc) {
                 const uint32_t buf = tc & 1u;
-                if (!mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4)) {
-                    atomicCAS(p.err_flag, 0u, 33u);
+                // one warp asks for the chain's end, the others sleep (asking takes issue slots from the MMAs' thread)
+                const bool waited = ew != 0 || mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                if (!meet_all(1, 32 * kLinEpilogueWarps, waited)) {
+                    if (!waited && lane == 0) atomicCAS(p.err_flag, 0u, 33u);
                     ok = false;
                     break;
                 }
-                __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)kWgBN + (uint32_t)(half * 128);
 #pragma unroll
@@ -369,7 +377,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 __syncwarp();
                 if (lane == 0) mbar_arrive_pair(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
             }
-            ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             if (t.runs > 1) {
                 constexpr int64_t kWarpFloats = 4 * 1024;

@@ -21,6 +21,9 @@ constexpr int kFewTokens = 128;    // of a tile
 constexpr int kFewMaxStages = 12;
 constexpr int kFewSmem = 220 * 1024, kFewSmemShared = 108 * 1024;   // one CTA on an SM, two
 
+// tokens of a tile padded to what the tensor core takes here
+inline int few_columns(int64_t M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+
 struct FewParams {
     CUtensorMap map_w, map_x;
     int M, N, k_steps;
@@ -176,24 +179,28 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         if (lane == 0) {
             // ---- MMA issuer: D[feature][token] ----
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 15) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-            uint32_t ph = 0;
+            // running descriptors (in 16 bytes), and the next stage's barrier asked between this one's MMAs, as in linear_fused.cuh
+            const uint64_t desc_w = make_desc(smem_u32(smem), DGRAD ? 8192 : 16, 1024), desc_x = make_desc(smem_u32(smem) + BM * BK * 2, 16, 1024);
+            constexpr uint32_t kNextW = DGRAD ? 2048 >> 4 : 32 >> 4, kNextX = 32 >> 4;
+            uint32_t ph = 0, at = 0;
+            bool have = false;
             for (int k = 0, s = 0; k < nk; ++k) {
-                if (!mbar_wait(&full_bar[s], ph, p.limit_ns * 2)) {
+                if (!have && !mbar_wait(&full_bar[s], ph, p.limit_ns * 2)) {
                     atomicCAS(p.err_flag, 0u, 42u);
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + BM * BK * 2;
+                const bool wraps = s + 1 == p.stages;
+                const uint64_t dw = desc_w + at, dx = desc_x + at;
+                umma_bf16(tmem, dw, dx, idesc, k ? 1u : 0u);
 #pragma unroll
-                for (int u = 0; u < BK / UMMA_K; ++u) {
-                    const uint64_t da = DGRAD ? make_desc(sa + u * 2048, 8192, 1024) : make_desc(sa + u * 32, 16, 1024);
-                    umma_bf16(tmem, da, make_desc(sb + u * 32, 16, 1024), idesc, (k | u) ? 1u : 0u);
-                }
+                for (int u = 1; u < BK / UMMA_K; ++u) umma_bf16(tmem, dw + u * kNextW, dx + u * kNextX, idesc, 1u);
+                const int next = wraps ? 0 : s + 1;
+                have = mbar_try_wait(&full_bar[next], wraps ? ph ^ 1u : ph);   // (past the last step: not used)
                 umma_commit(&empty_bar[s]);
-                if (++s == p.stages) {
-                    s = 0;
-                    ph ^= 1u;
-                }
+                at = wraps ? 0u : at + ((uint32_t)stage_bytes >> 4);
+                if (wraps) ph ^= 1u;
+                s = next;
             }
             umma_commit(done_bar);   // (also on error, so that nobody waits for it)
         }
@@ -316,25 +323,43 @@ int launch_few(const FewParams& p, int cluster, int smem, cudaStream_t s) {
     return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// CTAs that share a tile's contraction: doubled while all of them fit the GPU at once (two to an SM) with two k-steps each
-int few_cluster(int64_t M, int64_t N, int64_t K) {
+// How many CTAs share a tile's contraction, and the time of the whole in k-steps of a CTA that has its SM for itself (0.25 us).
+// Fewer k-steps per CTA against the exchange of the sums: a 64th of a step per token for every doubling, and three steps more where
+// two CTAs are on an SM. There a step of 128 tokens also takes half as long again (64 KB for both), one of fewer tokens less, since
+// two CTAs wait for memory side by side. Measured, us (1, 2, 4, 8 CTAs): 16 x 8192 x 2048: 12.1, 9.7, 8.5; 128 x 2048 x 2048: 13.7, 9.2,
+// 7.4, 8.8; 512 x 2048 x 2048: 13.9, 10.1, 11.3; 16 x 8192 x 512: 5.7, 4.7, 5.6.
+struct FewPlan {
+    int cluster;
+    float steps;
+};
+FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t tiles = (N + BM - 1) / BM * ((M + kFewTokens - 1) / kFewTokens), k_steps = (K + BK - 1) / BK;
-    const int64_t places = gemm_cta_limit() > 0 ? 2 * gemm_cta_limit() : 4 * kMaxPairs;
-    int cluster = 1;
-    while (cluster < 8 && tiles * cluster * 2 <= places && k_steps >= cluster * 4) cluster *= 2;
-    return cluster;
+    const int64_t sms = gemm_cta_limit() > 0 ? gemm_cta_limit() : 2 * kMaxPairs;
+    const int columns = few_columns(M);
+    FewPlan best = {1, 0.f};
+    for (int cluster = 1, doublings = 0; cluster <= 8; cluster *= 2, ++doublings) {
+        const int64_t ctas = tiles * cluster;
+        const bool crowded = ctas > sms;
+        if (cluster > 1 && (ctas > 2 * sms || cluster > k_steps)) break;
+        // clusters of eight do not all fit the GPCs with an SM for each CTA: they share, with three stages for 128 tokens
+        if (cluster == 8 && columns > 64 && 2 * ctas > sms) break;
+        const float step = !crowded ? 1.f : columns > 64 ? 1.5f : 0.6f;
+        const float steps = (float)((k_steps + cluster - 1) / cluster) * step * (float)((ctas + 2 * sms - 1) / (2 * sms)) +
+                            (float)doublings * ((float)columns / 64.f + (crowded ? 3.f : 0.f));
+        if (cluster == 1 || steps < best.steps) best = {cluster, steps};
+    }
+    return best;
 }
 
-// Which kernel: up to 128 tokens always this one; above, the one whose longest CTA is done first, counted in k-steps: one of a
-// 128 x 128 tile takes about as long as one of a pair's 256 x 256 tile (the same bytes per SM), and the last tile's epilogue, which
-// nothing hides, as long as 10 of them here (sixteen warps, 128 x 128 values) and 20 there. 1024 x 2048 x 2048, in us: 19 here, 20.
+// Which kernel: up to 128 tokens always this one; above, the one whose longest CTA is done first. A k-step of a pair's tile takes as
+// long as one here; its launch, its prologue and its last tile's epilogue (half the warps for twice the values) cost 16 more.
+// 512 x 8192 x 2048, in us: 20.5 here, 20.3; 1024 x 4096 x 4096: 31.9, 29.0; 1024 x 2048 x 8192: 31.6, 42.9.
 bool few_tokens(const LinearArgs& a) {
     if (a.M <= kFewTokens) return true;
     const int64_t k_steps = (a.K + BK - 1) / BK, pairs = gemm_cta_limit() > 0 ? std::max(1, gemm_cta_limit() / 2) : kMaxPairs;
     const int64_t small = (int64_t)((a.N + BM - 1) / BM) * ((a.M + kFewTokens - 1) / kFewTokens), large = (int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256);
-    const int cluster = few_cluster(a.M, a.N, a.K);
-    if (small * cluster > 4 * pairs) return false;
-    return (small * cluster + 2 * pairs - 1) / (2 * pairs) * ((k_steps + cluster - 1) / cluster) + 10 < (large + pairs - 1) / pairs * k_steps + 20;
+    if (small > 4 * pairs) return false;
+    return few_plan(a.M, a.N, a.K).steps < (float)((large + pairs - 1) / pairs * k_steps) + 16.f;
 }
 
 template <bool DGRAD>
@@ -343,7 +368,7 @@ int linear_few(const LinearArgs& a, cudaStream_t s) {
     p.M = a.M;
     p.N = a.N;
     p.k_steps = (a.K + BK - 1) / BK;
-    p.columns = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+    p.columns = few_columns(a.M);
     if (!make_map(&p.map_x, a.a, (uint64_t)a.M, (uint64_t)a.K, (uint64_t)a.lda, p.columns)) return -3;
     if (!(DGRAD ? make_map(&p.map_w, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, 64)
                 : make_map(&p.map_w, a.w, (uint64_t)a.N, (uint64_t)a.K, (uint64_t)a.ldw, BM)))
@@ -370,10 +395,10 @@ int linear_few(const LinearArgs& a, cudaStream_t s) {
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
     p.n_tiles = (a.N + BM - 1) / BM;
-    const int cluster = few_cluster(a.M, a.N, a.K);
+    const int cluster = few_plan(a.M, a.N, a.K).cluster;
     const int stage_bytes = (BM + p.columns) * BK * 2, extra = 1024 + 512;
     const int64_t ctas = (int64_t)p.n_tiles * ((p.M + kFewTokens - 1) / kFewTokens) * cluster;
-    const int room = ctas <= 2 * kMaxPairs && cluster < 8 ? kFewSmem : kFewSmemShared;
+    const int room = ctas <= 2 * kMaxPairs && cluster < 8 ? kFewSmem : kFewSmemShared;   // (clusters of eight: see few_plan)
     p.stages = std::min(std::min(kFewMaxStages, (room - extra) / stage_bytes), (p.k_steps + cluster - 1) / cluster);
     p.ring_bytes = std::max(p.stages * stage_bytes, p.columns * BM * 4);
     const int smem = p.ring_bytes + extra;

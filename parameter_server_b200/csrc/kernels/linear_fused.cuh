@@ -243,15 +243,22 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    cluster_arrive_all();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * BN))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();   // the peer's barriers must exist before anything is signalled on them
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
+    cluster_wait_all();   // the peer's barriers must exist before anything is signalled on them
+    wait_predecessor();
+    uint32_t tmem_base = 0;
+    if (warp == 1 || warp >= 4) {   // (the loads need no TMEM and do not wait for it)
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        meet_named(2, 32 * (1 + kLinEpilogueWarps));
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_base = *((volatile uint32_t*)tmem_slot);
+        allow_successor();
+    }
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLinRegsIssue));
@@ -399,16 +406,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             // asks for the accumulator, the others sleep at this barrier (asking takes issue slots from the MMAs' thread).
             const bool waited = ew != 0 || mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            uint32_t all_ok;
-            asm volatile(
-                "{\n\t.reg .pred p, q;\n\t"
-                "setp.ne.u32 q, %1, 0;\n\t"
-                "bar.red.and.pred p, 1, %2, q;\n\t"
-                "selp.u32 %0, 1, 0, p;\n\t}"
-                : "=r"(all_ok)
-                : "r"(waited ? 1u : 0u), "r"(32 * kLinEpilogueWarps)
-                : "memory");
-            if (!all_ok) {
+            if (!meet_all(1, 32 * kLinEpilogueWarps, waited)) {
                 if (!waited && lane == 0) atomicCAS(p.err_flag, 0u, 23u);
                 break;
             }
@@ -565,11 +563,7 @@ cudaError_t pairs_of(int threads, int smem, int* pairs) {
         q.gridDim = dim3(2);
         q.blockDim = dim3(threads);
         q.dynamicSmemBytes = smem;
-        cudaLaunchAttribute a[1];
-        a[0].id = cudaLaunchAttributeClusterDimension;
-        a[0].val.clusterDim.x = 2;
-        a[0].val.clusterDim.y = 1;
-        a[0].val.clusterDim.z = 1;
+        cudaLaunchAttribute a[1] = {in_clusters(2)};
         q.attrs = a;
         q.numAttrs = 1;
         e = cudaOccupancyMaxActiveClusters(&n, kern, &q);
@@ -588,13 +582,9 @@ cudaError_t launch_pairs(Kernel kern, int threads, int smem, int pairs, const Pa
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute a[1];
-    a[0].id = cudaLaunchAttributeClusterDimension;
-    a[0].val.clusterDim.x = 2;
-    a[0].val.clusterDim.y = 1;
-    a[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute a[2] = {in_clusters(2), start_early()};
     cfg.attrs = a;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
