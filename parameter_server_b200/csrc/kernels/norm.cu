@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "act8.cuh"
+#include "launch.cuh"
 #include "norm.h"
 
 namespace psb {
@@ -179,6 +180,7 @@ __global__ void __launch_bounds__(TPR == 0 ? kMaxTeam : TPR == 32 ? 128 : TPR)
 layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, T* __restrict__ y,
                       int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
                       int64_t lde, int64_t rows, int d, float eps, int tpr_arg) {
+    allow_successor();
     const int tpr = TPR > 0 ? TPR : tpr_arg, threads = TPR == 0 ? (int)blockDim.x : TPR == 32 ? 128 : TPR;
     constexpr bool kAsync = copies_ahead<T, VEC>();
     constexpr int kVecBytes = VEC * (int)sizeof(T);
@@ -297,6 +299,7 @@ __global__ void __launch_bounds__(512)
 layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias,
                            T* __restrict__ y, int64_t ldy, float* mean_out, float* rstd_out, int8_t* q, int64_t ldq, uint8_t* e,
                            int64_t lde, int d, float eps) {
+    allow_successor();
     __shared__ float red[16];
     const int64_t row = blockIdx.x;
     const T* xr = x + row * ldx;
@@ -351,6 +354,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                       int64_t ldq, const uint8_t* __restrict__ e, int64_t lde, const T* __restrict__ weight,
                       const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const T* __restrict__ join, int64_t ldjoin,
                       T* __restrict__ dx, int64_t lddx, float* __restrict__ partial, int64_t rows, int d, int tpr_arg) {
+    allow_successor();
     constexpr int NV = kBwdElems / VEC;
     const int tpr = TPR > 0 ? TPR : tpr_arg;
     using IO = Io<T, VEC>;
@@ -568,6 +572,7 @@ __global__ void __launch_bounds__(512)
 layer_norm_bwd_long_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* q, int64_t ldq,
                            const uint8_t* e, int64_t lde, const T* __restrict__ weight, const float* mean_in, const float* rstd_in,
                            const T* join, int64_t ldjoin, T* __restrict__ dx, int64_t lddx, int d) {
+    allow_successor();
     __shared__ float red[16];
     const int64_t row = blockIdx.x;
     const float rstd = rstd_in[row], mean = SRC8 ? 0.f : mean_in[row];
@@ -596,6 +601,7 @@ template <typename T, bool SRC8>
 __global__ void __launch_bounds__(256)
 layer_norm_dw_long_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* q, int64_t ldq,
                           const uint8_t* e, int64_t lde, const float* mean_in, const float* rstd_in, float* partial, int64_t rows, int d) {
+    allow_successor();
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     if (c >= d) return;
     const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r1 = min(rows, (int64_t)(blockIdx.y + 1) * per);
@@ -612,9 +618,10 @@ layer_norm_dw_long_kernel(const T* __restrict__ dy, int64_t lddy, const T* __res
 // out[c] (+)= sum over the partial rows, eight interleaved sums per column that are then added in a fixed order. Column c
 // of the partials goes to out0[c], or to out1[c - split] from `split` on; either may be null.
 __global__ void __launch_bounds__(256)
-column_reduce_kernel(const float* __restrict__ partial, int n, int64_t width, int64_t split, float* out0, float* out1, int accumulate) {
+column_reduce_kernel(const float* partial, int n, int64_t width, int64_t split, float* out0, float* out1, int accumulate) {
     __shared__ float part[8][33];
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched ahead of the end of the kernel that writes the partials
+    wait_predecessor();   // launched ahead of the end of the kernel that writes the partials (and not __restrict__: nothing is read before)
+    allow_successor();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + tx;
     float s = 0.f;
@@ -637,6 +644,7 @@ column_reduce_kernel(const float* __restrict__ partial, int n, int64_t width, in
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 column_sum_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols, float* __restrict__ partial) {
+    allow_successor();
     constexpr int TX = 128 / VEC, TY = 256 / TX > 0 ? 256 / TX : 1;
     __shared__ float part[TY][128 + 4];
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
@@ -685,6 +693,7 @@ template <typename T, int VEC, int U>
 __global__ void __launch_bounds__(256)
 act8_pack_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ e, int64_t lde, int64_t rows,
                  int64_t cols, int64_t per_row) {
+    allow_successor();
     const int lane = threadIdx.x & 31;
     const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t row = task / per_row, c0 = (task - row * per_row) * (32 * VEC * U) + lane * VEC;
@@ -710,6 +719,7 @@ template <typename T, int VEC, int U>
 __global__ void __launch_bounds__(256)
 act8_unpack_kernel(const int8_t* __restrict__ q, int64_t ldq, const uint8_t* __restrict__ e, int64_t lde, T* __restrict__ x, int64_t ldx,
                    int64_t rows, int64_t cols, int64_t per_row) {
+    allow_successor();
     const int lane = threadIdx.x & 31;
     const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t row = task / per_row, c0 = (task - row * per_row) * (32 * VEC * U) + lane * VEC;
@@ -865,9 +875,7 @@ int reduce_partials(const float* partial, int n, int64_t width, int64_t split, f
     cfg.gridDim = dim3((unsigned)((width + 31) / 32));
     cfg.blockDim = dim3(256);
     cfg.stream = s;
-    cudaLaunchAttribute a[1];
-    a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    a[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute a[1] = {start_early()};
     cfg.attrs = a;
     cfg.numAttrs = 1;
     return (int)cudaLaunchKernelEx(&cfg, column_reduce_kernel, partial, n, width, split, out0, out1, accumulate);

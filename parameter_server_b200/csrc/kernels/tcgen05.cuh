@@ -8,6 +8,8 @@
 #include <cstdint>
 #include <mutex>
 
+#include "launch.cuh"
+
 namespace psb {
 
 namespace {
@@ -208,12 +210,6 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Programmatic dependent launch: a kernel that was allowed to start beside its predecessor's tail (`start_early`) touches no global
-// memory before wait_predecessor() has returned. It allows its own successor to start once its TMEM is allocated in every CTA: a
-// successor that got the TMEM first would wait for this kernel, and this kernel for the TMEM.
-__device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void allow_successor() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // 16 bytes of this CTA's shared memory by its 32-bit address. (A pointer that was rounded up as an integer is a generic one to the
 // compiler, and a generic access takes several times as long.)
 __device__ __forceinline__ uint4 ld_smem_v4(uint32_t addr) {
@@ -242,22 +238,6 @@ __device__ __forceinline__ bool meet_all(int id, int threads, bool ok) {
         : "r"(ok ? 1u : 0u), "r"(id), "r"(threads)
         : "memory");
     return all != 0;
-}
-
-// ---- host: launches ----------------------------------------------------------------------------------
-inline cudaLaunchAttribute start_early() {
-    cudaLaunchAttribute a = {};
-    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    a.val.programmaticStreamSerializationAllowed = 1;
-    return a;
-}
-inline cudaLaunchAttribute in_clusters(int size) {
-    cudaLaunchAttribute a = {};
-    a.id = cudaLaunchAttributeClusterDimension;
-    a.val.clusterDim.x = size;
-    a.val.clusterDim.y = 1;
-    a.val.clusterDim.z = 1;
-    return a;
 }
 
 // ---- host: tensor maps -------------------------------------------------------------------------------
