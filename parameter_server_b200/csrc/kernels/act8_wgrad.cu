@@ -23,7 +23,7 @@
 #include <cuda_runtime.h>
 
 #include "act8_wgrad.h"
-#include "linear_fused.cuh"
+#include "linear_few.cuh"
 
 namespace psb {
 
@@ -49,6 +49,8 @@ struct WgSmem {
     static constexpr int kOutBytes = kLinEpilogueWarps * 2048;
     static constexpr int kTotal = kTileBytes + kBarBytes + kOutBytes + 1024;
 };
+
+constexpr int kWgUnpackN = 2048;   // from so many outputs on x is unpacked once (see act8_wgrad_scratch)
 
 struct WgParams {
     CUtensorMap map_a, map_b, map_e;   // b: q, or x in bf16
@@ -491,6 +493,47 @@ int launch_wgrad(const WgParams& p, cudaStream_t s) {
     return (int)launch_pairs(kern, kWgThreads, WgSmem<CONVERT>::kTotal, p.grid.pairs, p, s);
 }
 
+// Whether a layer has so few tiles that clusters on 128 x 128 of them are done first, from x in bf16. In k-steps (0.25 us), from
+// sweeps: a pair's step takes 1.2, or 1.7 where it converts, its frame and epilogue 34 or 55 and a join of cut tiles 55; the small
+// kernel's frame 24, with two CTAs on an SM 44, and the pass that unpacks x 10 and its bytes. us, without and with the small
+// kernel: 1000 tokens, 512 x 512: 19.6, 10.1; 8192: 33.9, 20.2; 2048 tokens, 1024 x 1024: 26.5, 14.4; 300, 4096 x 1024: 13.0, 17.6.
+bool wgrad_few(int64_t tokens, int N, int K) {
+    const int64_t k_steps = (tokens + BK - 1) / BK, small = (int64_t)((N + BM - 1) / BM) * ((K + BM - 1) / BM);
+    if (small > 4 * kMaxPairs) return false;
+    const FewPlan plan = few_plan(N, K, tokens, true);
+    if (plan.cluster == 0) return false;
+    const TileGrid g = plan_tiles((N + 2 * BM - 1) / (2 * BM), (K + kWgBN - 1) / kWgBN, (int)k_steps, kMaxPairs, 48, 8);
+    const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles, whole = (tiles - g.shared + g.pairs - 1) / g.pairs;
+    const float unpack = 10.f + (float)tokens * (float)K * 2.4e-6f;
+    const bool converts = N < kWgUnpackN;
+    const float pairs = (float)(whole * k_steps + (g.shared > 0 ? g.len : 0)) * (converts ? 1.7f : 1.2f) + (converts ? 55.f : 34.f + unpack) +
+                        (g.shared > 0 ? 55.f : 0.f);
+    return plan.steps + (small * plan.cluster > 2 * kMaxPairs ? 44.f : 24.f) + unpack < pairs;
+}
+
+int wgrad_on_few(const Act8WgradArgs& a, int64_t ldx, cudaStream_t s) {
+    FewParams p = {};
+    p.M = a.N;
+    p.N = a.K;
+    p.k_steps = (int)((a.tokens + BK - 1) / BK);
+    p.columns = a.N <= 64 ? 64 : 128;
+    p.n_tiles = (a.K + BM - 1) / BM;
+    if (!make_map(&p.map_w, a.scratch, (uint64_t)a.tokens, (uint64_t)a.K, (uint64_t)ldx, 64) ||
+        !make_map(&p.map_x, a.dy, (uint64_t)a.tokens, (uint64_t)a.N, (uint64_t)a.lddy, 64))
+        return -3;
+    p.dw = a.out;
+    p.ldo = a.ldo;
+    p.out_wide = ((uintptr_t)a.out % 16) == 0 && a.ldo % 4 == 0;
+    p.accumulate = a.accumulate;
+    p.gain = (const __nv_bfloat16*)a.weight;
+    p.bias = (const __nv_bfloat16*)a.bias;
+    p.dy_sum = a.bias != nullptr ? a.dy_sum : nullptr;
+    p.err_flag = a.err_flag;
+    p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
+    const int rc = act8_unpack(0, a.x, a.scratch, ldx, a.tokens, a.K, s);
+    return rc != 0 ? rc : launch_few<kFewWgrad, kActNone>(p, few_plan(a.N, a.K, a.tokens, true).cluster, s);
+}
+
 }  // namespace
 
 int act8_wgrad(const Act8WgradArgs& a, void* stream) {
@@ -501,6 +544,7 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     const uint64_t tokens = (uint64_t)a.tokens, blocks = (uint64_t)(a.K + kAct8Block - 1) / kAct8Block;
     const bool convert = a.scratch == nullptr;
     const int64_t ldx = ((int64_t)a.K + 7) / 8 * 8;
+    if (!convert && wgrad_few(a.tokens, a.N, a.K)) return wgrad_on_few(a, ldx, (cudaStream_t)stream);
     WgParams p;
     p.N = a.N;
     p.K = a.K;
@@ -539,7 +583,7 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
 // a cold L2 and back to back: 6144 x 2048: 369, 300 and 416, 347; 2048 x 2048: 135, 120 and 137, 126; 1024 x 2048: 86, 89 and
 // 79, 87; 512 x 2048: 61, 69 and 53, 63. On 1024 tokens 2048 x 2048: 27, 24.
 int64_t act8_wgrad_scratch(int64_t tokens, int N, int K) {
-    return N >= 2048 ? tokens * (((int64_t)K + 7) / 8 * 8) * 2 : 0;
+    return N >= kWgUnpackN || wgrad_few(tokens, N, K) ? tokens * (((int64_t)K + 7) / 8 * 8) * 2 : 0;
 }
 
 }  // namespace psb

@@ -1,14 +1,17 @@
-// The fused linear layers for few tokens, where the weight's way through the chip and the latency of one tile are the time:
+// Products with few tiles, where the operands' way through the chip and the latency of one tile are the time:
 //
-//   forward   h = x w^T + b, y = act(h) + residual        dgrad   dh = (dy w) * act'(h), a = act(h)
+//   forward   h = x w^T + b, y = act(h) + residual        dgrad   dh = (dy w) * act'(h), a = act(h)        (few tokens)
+//   wgrad     dw = dy^T x, or (dy^T x) g + (sum dy) b^T    (few weights, x in bf16)
 //
-// The weight takes the tensor core's 128 rows and the tokens its columns (16 to 128 of them), so that few tokens are not padded
-// to a tile. A cluster of S CTAs has the same 128 output features (and the same 128 tokens, where there are more) and cuts the
-// contraction in S parts, S chosen so that all SMs read at once; each CTA keeps its part's sums in TMEM. They meet in
-// distributed shared memory: every CTA lays its sums down in its own, and CTA r reads the r-th share of the tokens from all S,
+// The features of an output row take the tensor core's 128 rows, its rows (the tokens; outputs of the layer in wgrad) the columns,
+// 16 to 128 of them, so that few tokens are not padded to a tile. A cluster of S CTAs has the same 128 features (and the same
+// 128 rows, where there are more) and cuts the contraction in S parts; each CTA keeps its part's sums in TMEM. They meet in
+// distributed shared memory: every CTA lays its sums down in its own, and CTA r reads the r-th share of the rows from all S,
 // adds them in rank order (the same bits every time) and runs the epilogue for its share, with 32 neighbouring features in the
-// lanes of a warp. At most 108 KB of shared memory: two CTAs fit an SM, without which sixteen clusters of eight do not all fit
-// the GPCs at once (16 tokens, 4096 -> 2048: 17 us, two waves).
+// lanes of a warp. Where more CTAs than SMs are needed, two fit an SM (16 tokens, 4096 -> 2048 in clusters of eight with one
+// CTA to an SM: 17 us, two waves).
+// The tensor core cuts its sums off towards zero, a billionth of them per token (act8_wgrad.cu): wgrad, whose contraction is long,
+// starts a new chain in TMEM after 512 tokens, and the chains are added with rounding.
 #pragma once
 #include "linear_fused.cuh"
 
@@ -20,6 +23,12 @@ constexpr int kFewThreads = 512;
 constexpr int kFewTokens = 128;    // of a tile
 constexpr int kFewMaxStages = 12;
 constexpr int kFewSmem = 220 * 1024, kFewSmemShared = 108 * 1024;   // one CTA on an SM, two
+constexpr int kFewFwd = 0, kFewDgrad = 1, kFewWgrad = 2;
+constexpr int kFewChain = 8;       // k-steps (of 64 tokens) of a wgrad chain
+// CTAs that wait for one another (in a cluster, or a pair) must never share an SM with CTAs that hold the TMEM they still need.
+// So each asks for shared memory in proportion to its TMEM: what fits one SM's shared memory fits its TMEM, whichever streams it is
+// from. (The pair kernels have all the TMEM and 211 KB; 512 columns here take more than a 128-column CTA's share leaves.)
+inline int few_smem_floor(int tmem_columns) { return (tmem_columns == 128 ? 58 : tmem_columns == 256 ? 114 : 172) * 1024; }
 
 // tokens of a tile padded to what the tensor core takes here
 inline int few_columns(int64_t M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
@@ -28,7 +37,8 @@ struct FewParams {
     CUtensorMap map_w, map_x;
     int M, N, k_steps;
     int n_tiles;
-    int columns;          // tokens of a tile padded to 16, 32, 64 or 128
+    int columns;          // rows of a tile padded to 16, 32, 64 or 128
+    int tmem_columns;     // 128; wgrad: a power of two that has every chain's
     int stages, ring_bytes;
     const __nv_bfloat16* bias;
     const float* bias32;
@@ -44,7 +54,11 @@ struct FewParams {
     int64_t ldq;
     uint8_t* e;
     int64_t lde;
-    int res_wide, out_wide, out2_wide, pre_wide;   // rows on 8-byte boundaries
+    int res_wide, out_wide, out2_wide, pre_wide;   // rows on 8-byte boundaries (wgrad's out: 16)
+    float* dw;            // wgrad: out, with the norm's weight (null: 1) and, with a bias, the sums of dy's rows
+    const __nv_bfloat16* gain;
+    const float* dy_sum;
+    int accumulate;
     unsigned* err_flag;
     unsigned long long limit_ns;
 };
@@ -107,8 +121,9 @@ __device__ __forceinline__ void add_parts(uint32_t at, float* v) {
     for (int s = 1; s < S; ++s) { v[0] += part[s].x; v[1] += part[s].y; v[2] += part[s].z; v[3] += part[s].w; }
 }
 
-template <bool DGRAD, int ACT>
+template <int MODE, int ACT>
 __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid_constant__ FewParams p) {
+    constexpr bool DGRAD = MODE == kFewDgrad, WGRAD = MODE == kFewWgrad, W_MN = MODE != kFewFwd;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = BM * BK * 2 + p.columns * BK * 2;
@@ -128,13 +143,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         const int k0 = (k_begin + k) * BK;
         uint8_t* sa = smem + s * stage_bytes;
         mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
-        if constexpr (!DGRAD) {
+        if constexpr (!W_MN) {
             tma_load_2d(sa, &p.map_w, &full_bar[s], k0, n0);   // [128 features][64 k]
         } else {
             tma_load_2d(sa, &p.map_w, &full_bar[s], n0, k0);   // two blocks of [64 k][64 features]
             tma_load_2d(sa + 64 * 128, &p.map_w, &full_bar[s], n0 + 64, k0);
         }
-        tma_load_2d(sa + BM * BK * 2, &p.map_x, &full_bar[s], k0, m0);   // [tokens][64 k]
+        if constexpr (!WGRAD) {
+            tma_load_2d(sa + BM * BK * 2, &p.map_x, &full_bar[s], k0, m0);   // [tokens][64 k]
+        } else {
+            for (int c = 0; c < p.columns; c += 64) tma_load_2d(sa + BM * BK * 2 + c * 128, &p.map_x, &full_bar[s], m0 + c, k0);   // [64 k][64 rows]
+        }
     };
 
     if (threadIdx.x == 0) {
@@ -149,7 +168,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         for (int k = 0; k < min(nk, p.stages); ++k) load(k, k);   // the loads need no TMEM: they start before it is there
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(128u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)p.tmem_columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -178,11 +197,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     } else if (warp == 1) {
         if (lane == 0) {
             // ---- MMA issuer: D[feature][token] ----
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((DGRAD ? 1u : 0u) << 15) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((W_MN ? 1u : 0u) << 15) | ((WGRAD ? 1u : 0u) << 16) | ((uint32_t)(p.columns >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
             // running descriptors (in 16 bytes), and the next stage's barrier asked between this one's MMAs, as in linear_fused.cuh
-            const uint64_t desc_w = make_desc(smem_u32(smem), DGRAD ? 8192 : 16, 1024), desc_x = make_desc(smem_u32(smem) + BM * BK * 2, 16, 1024);
-            constexpr uint32_t kNextW = DGRAD ? 2048 >> 4 : 32 >> 4, kNextX = 32 >> 4;
-            uint32_t ph = 0, at = 0;
+            const uint64_t desc_w = make_desc(smem_u32(smem), W_MN ? 8192 : 16, 1024);
+            const uint64_t desc_x = make_desc(smem_u32(smem) + BM * BK * 2, WGRAD ? 8192 : 16, 1024);
+            constexpr uint32_t kNextW = W_MN ? 2048 >> 4 : 32 >> 4, kNextX = WGRAD ? 2048 >> 4 : 32 >> 4;
+            uint32_t ph = 0, at = 0, tmem_d = tmem;
             bool have = false;
             for (int k = 0, s = 0; k < nk; ++k) {
                 if (!have && !mbar_wait(&full_bar[s], ph, p.limit_ns * 2)) {
@@ -192,9 +212,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const bool wraps = s + 1 == p.stages;
                 const uint64_t dw = desc_w + at, dx = desc_x + at;
-                umma_bf16(tmem, dw, dx, idesc, k ? 1u : 0u);
+                const bool opens = k == 0 || (WGRAD && k % kFewChain == 0);
+                if (WGRAD && opens && k) tmem_d += (uint32_t)p.columns;
+                umma_bf16(tmem_d, dw, dx, idesc, opens ? 0u : 1u);
 #pragma unroll
-                for (int u = 1; u < BK / UMMA_K; ++u) umma_bf16(tmem, dw + u * kNextW, dx + u * kNextX, idesc, 1u);
+                for (int u = 1; u < BK / UMMA_K; ++u) umma_bf16(tmem_d, dw + u * kNextW, dx + u * kNextX, idesc, 1u);
                 const int next = wraps ? 0 : s + 1;
                 have = mbar_try_wait(&full_bar[next], wraps ? ph ^ 1u : ph);   // (past the last step: not used)
                 umma_commit(&empty_bar[s]);
@@ -209,7 +231,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     // what the epilogue needs from memory, on its way meanwhile: a warp has a token, a lane four neighbouring features
     const int n = n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
     const int t_end = min(tokens, (rank + 1) * share), t_first = rank * share + warp;
-    float b[4] = {0.f, 0.f, 0.f, 0.f}, aux[4];
+    float b[4] = {0.f, 0.f, 0.f, 0.f}, gain[4] = {1.f, 1.f, 1.f, 1.f}, aux[4], sum = 0.f;
+    if constexpr (WGRAD) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < have && p.gain != nullptr) gain[j] = __bfloat162float(p.gain[n + j]);
+    }
     if constexpr (!DGRAD) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -220,7 +247,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         for (int j = 0; j < 4; ++j) aux[j] = 0.f;
         if (have <= 0 || t >= t_end) return;
         const int64_t row = m0 + t;
-        if constexpr (!DGRAD) {
+        if constexpr (WGRAD) {
+            if (p.dy_sum != nullptr) sum = p.dy_sum[row];
+            if (!p.accumulate) return;
+            const float* old = p.dw + row * p.ldo + n;
+            if (p.out_wide != 0 && have >= 4) {
+                const float4 o = *(const float4*)old;
+                aux[0] = o.x; aux[1] = o.y; aux[2] = o.z; aux[3] = o.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < have) aux[j] = old[j];
+            }
+        } else if constexpr (!DGRAD) {
             if (p.res != nullptr) load4(p.res + row * p.ldres + n, have, p.res_wide != 0, aux);
         } else if (p.q != nullptr) {
             const uint32_t w = *(const uint32_t*)(p.q + row * p.ldq + n) ^ 0x80808080u;   // (rows are padded to 16 bytes)
@@ -246,6 +285,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         for (int t0 = (warp >> 2) * 16; t0 < tokens; t0 += kFewThreads / 128 * 16) {
             uint32_t v[16];
             tmem_ld16_issue(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t0, v);
+            if constexpr (WGRAD) {
+                for (int c = 1; c * kFewChain < nk; ++c) {
+                    uint32_t w[16];
+                    tmem_ld16_issue(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(c * p.columns + t0), w);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 16; ++j)
                 asm volatile("st.shared.u32 [%0], %1;" ::"r"(parts + (uint32_t)((t0 + j) * BM + quarter * 32 + lane) * 4), "r"(v[j]) : "memory");
@@ -255,7 +302,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     cluster_sync_all();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)p.tmem_columns) : "memory");
     }
     // ---- epilogue of this CTA's tokens ----
     const uint32_t mine = parts + (uint32_t)lane * 16;
@@ -267,7 +314,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         else if (S == 4) add_parts<4>(at, v);
         else if (S == 2) add_parts<2>(at, v);
         else add_parts<1>(at, v);
-        if constexpr (!DGRAD) {
+        if constexpr (WGRAD) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = v[j] * gain[j] + sum * b[j] + aux[j];
+            fetch(t + kFewThreads / 32);
+            float* o = p.dw + row * p.ldo + n;
+            if (p.out_wide != 0 && have >= 4) {
+                *(float4*)o = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < have) o[j] = v[j];
+            }
+        } else if constexpr (!DGRAD) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += b[j];   // (0 past the last feature: its weights were read as zeros)
             if (p.pre != nullptr && have > 0) store4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, v);
@@ -300,9 +359,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     cluster_sync_all();   // until here the others may read this CTA's shared memory
 }
 
-template <bool DGRAD, int ACT>
-int launch_few(const FewParams& p, int cluster, int smem, cudaStream_t s) {
-    constexpr auto kern = linear_few_kernel<DGRAD, ACT>;
+template <int MODE, int ACT>
+int launch_few(FewParams& p, int cluster, cudaStream_t s) {
+    constexpr auto kern = linear_few_kernel<MODE, ACT>;
+    const int64_t ctas = (int64_t)p.n_tiles * ((p.M + kFewTokens - 1) / kFewTokens) * cluster;
+    const int nk = (p.k_steps + cluster - 1) / cluster, chains = MODE == kFewWgrad ? (nk + kFewChain - 1) / kFewChain : 1;
+    p.tmem_columns = 128;
+    while (p.tmem_columns < chains * p.columns) p.tmem_columns *= 2;
+    if (p.tmem_columns > 512) return -2;
+    const int stage_bytes = (BM + p.columns) * BK * 2, extra = 1024 + 512;
+    // (clusters of eight do not get SMs of their own: see few_plan)
+    const int room = p.tmem_columns > 256 || (ctas <= 2 * kMaxPairs && cluster < 8) ? kFewSmem : kFewSmemShared;
+    p.stages = std::min(std::min(kFewMaxStages, (room - extra) / stage_bytes), nk);
+    p.ring_bytes = std::max(p.stages * stage_bytes, p.columns * BM * 4);
+    const int smem = std::max(p.ring_bytes + extra, few_smem_floor(p.tmem_columns));
     static bool ready[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -332,21 +402,26 @@ struct FewPlan {
     int cluster;
     float steps;
 };
-FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
+FewPlan few_plan(int64_t M, int64_t N, int64_t K, bool wgrad = false) {
     const int64_t tiles = (N + BM - 1) / BM * ((M + kFewTokens - 1) / kFewTokens), k_steps = (K + BK - 1) / BK;
     const int64_t sms = gemm_cta_limit() > 0 ? gemm_cta_limit() : 2 * kMaxPairs;
     const int columns = few_columns(M);
-    FewPlan best = {1, 0.f};
+    FewPlan best = {0, 0.f};   // wgrad: cluster 0 where the chains never fit TMEM
     for (int cluster = 1, doublings = 0; cluster <= 8; cluster *= 2, ++doublings) {
         const int64_t ctas = tiles * cluster;
-        const bool crowded = ctas > sms;
-        if (cluster > 1 && (ctas > 2 * sms || cluster > k_steps)) break;
-        // clusters of eight do not all fit the GPCs with an SM for each CTA: they share, with three stages for 128 tokens
-        if (cluster == 8 && columns > 64 && 2 * ctas > sms) break;
+        // (chains past the first take TMEM that a second CTA would need)
+        const int64_t fit = wgrad && k_steps > kFewChain * cluster ? sms : 2 * sms;
+        const bool crowded = ctas > sms && fit > sms;
+        if (cluster > 1 && (ctas > fit || cluster > k_steps)) break;
+        if (wgrad && (k_steps + cluster - 1) / cluster > (int64_t)kFewChain * 512 / BM) continue;
+        // clusters of eight do not all fit the GPCs with an SM for each CTA: they share, with three stages for 128 tokens, or (wgrad with
+        // more chains) come in two waves
+        const bool eights = cluster == 8 && columns > 64 && 2 * ctas > sms;
+        if (eights && fit > sms) break;
         const float step = !crowded ? 1.f : columns > 64 ? 1.5f : 0.6f;
-        const float steps = (float)((k_steps + cluster - 1) / cluster) * step * (float)((ctas + 2 * sms - 1) / (2 * sms)) +
+        const float steps = (float)((k_steps + cluster - 1) / cluster) * step * (float)(eights ? 2 : (ctas + fit - 1) / fit) +
                             (float)doublings * ((float)columns / 64.f + (crowded ? 3.f : 0.f));
-        if (cluster == 1 || steps < best.steps) best = {cluster, steps};
+        if (best.cluster == 0 || steps < best.steps) best = {cluster, steps};
     }
     return best;
 }
@@ -396,18 +471,12 @@ int linear_few(const LinearArgs& a, cudaStream_t s) {
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
     p.n_tiles = (a.N + BM - 1) / BM;
     const int cluster = few_plan(a.M, a.N, a.K).cluster;
-    const int stage_bytes = (BM + p.columns) * BK * 2, extra = 1024 + 512;
-    const int64_t ctas = (int64_t)p.n_tiles * ((p.M + kFewTokens - 1) / kFewTokens) * cluster;
-    const int room = ctas <= 2 * kMaxPairs && cluster < 8 ? kFewSmem : kFewSmemShared;   // (clusters of eight: see few_plan)
-    p.stages = std::min(std::min(kFewMaxStages, (room - extra) / stage_bytes), (p.k_steps + cluster - 1) / cluster);
-    p.ring_bytes = std::max(p.stages * stage_bytes, p.columns * BM * 4);
-    const int smem = p.ring_bytes + extra;
     switch (a.act) {
-        case kActNone: return launch_few<DGRAD, kActNone>(p, cluster, smem, s);
-        case kActRelu: return launch_few<DGRAD, kActRelu>(p, cluster, smem, s);
-        case kActGelu: return launch_few<DGRAD, kActGelu>(p, cluster, smem, s);
-        case kActGeluTanh: return launch_few<DGRAD, kActGeluTanh>(p, cluster, smem, s);
-        case kActSilu: return launch_few<DGRAD, kActSilu>(p, cluster, smem, s);
+        case kActNone: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActNone>(p, cluster, s);
+        case kActRelu: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActRelu>(p, cluster, s);
+        case kActGelu: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActGelu>(p, cluster, s);
+        case kActGeluTanh: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActGeluTanh>(p, cluster, s);
+        case kActSilu: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActSilu>(p, cluster, s);
     }
     return -2;
 }
