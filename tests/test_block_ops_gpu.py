@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from parameter_server_b200._lib import C
 from parameter_server_b200.ops import act8, linear, norm
 from parameter_server_b200.ops import gemm as G
 
@@ -553,4 +554,48 @@ def test_overlapping_launches_keep_their_order():
         one, other = chain(tokens, True), chain(tokens, False)
         assert all(torch.equal(p, q) for p, q in zip(one, other))
         assert all(torch.isfinite(p).all() for p in one)
+    G.check_gemm_errors()
+
+
+# few tiles on clusters with one and several chains, two waves of clusters, tiles cut into runs, unpacked and pairs
+@pytest.mark.parametrize("T,N,K", [(512, 128, 128), (1000, 520, 328), (4100, 65, 200), (16384, 256, 256), (16384, 300, 2048), (16384, 512, 512),
+                                   (2048, 1024, 1024), (300, 4096, 1024), (8192, 2048, 520)])
+def test_act8_wgrad_either_way(T, N, K):
+    """The way that is taken for these sizes, and a checkpoint that is converted tile by tile, with a gradient that is added to."""
+    dy, x8, g, b, base = rand(T, N), act8.act8_pack(rand(T, K, seed=1)), rand(K, seed=2), rand(K, seed=3), rand(N, K, seed=4, dtype=F32)
+    x, s = act8.act8_unpack(x8, F32).double(), linear.linear_bias_grad(dy)
+    size = dy.double().abs().t() @ x.abs()
+    want = base.double() + dy.double().t() @ (x * g.double() + b.double())
+    slack = ((34 * 2.0 ** -23 + (T / 512 + 8) * 2.0 ** -24) * size * g.double().abs()
+             + 2.0 ** -20 * dy.double().abs().sum(0)[:, None] * b.double().abs() + 2.0 ** -22 * (want.abs() + base.double().abs()))
+    got = act8.act8_wgrad(dy, x8, weight=g, bias=b, dy_sum=s, out=base.clone(), accumulate=True)
+    near(got, want, slack)
+    for _ in range(3):
+        assert torch.equal(got, act8.act8_wgrad(dy, x8, weight=g, bias=b, dy_sum=s, out=base.clone(), accumulate=True))
+    if N % 8 == 0:
+        out, stream = base.clone(), torch.cuda.current_stream().cuda_stream
+        assert C.act8_wgrad(dy.data_ptr(), N, *x8.args(), out.data_ptr(), K, True, g.data_ptr(), b.data_ptr(), s.data_ptr(), T, N, K, 0,
+                            G.workspace(0, stream).data_ptr(), G._err_flag(dy.device).data_ptr(), 2.0, stream) == 0
+        near(out, want, slack)
+    G.check_gemm_errors()
+
+
+def test_products_of_two_streams_share_the_gpu():
+    """Small and large products side by side: clusters of one stream, pairs of another, each as alone."""
+    small = [(rand(t, 256, seed=t), rand(384, 256, seed=t + 1)) for t in (1, 16, 100)]
+    large = [(rand(700, 512, seed=t), rand(2304, 512, seed=t + 1)) for t in (1, 2)]
+    alone = [linear.linear_act(x, w, act="silu") for x, w in small + large]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    seen = [[], []]
+    for _ in range(40):
+        for s, cases, out in zip(streams, (small, large), seen):
+            with torch.cuda.stream(s):
+                out += [linear.linear_act(x, w, act="silu") for x, w in cases]
+    torch.cuda.synchronize()
+    for i, out in enumerate(seen[0]):
+        assert torch.equal(out, alone[i % 3])
+    for i, out in enumerate(seen[1]):
+        assert torch.equal(out, alone[3 + i % 2])
     G.check_gemm_errors()
