@@ -7,7 +7,8 @@
 // q * 2^(e-127) is exact in bf16, so the products are those of the values that were kept. A layer of few outputs reads the
 // checkpoint as it is (a byte and a 32nd per value) and turns it into bf16 in shared memory, on its way to the tensor cores; one
 // of many outputs, which would do that again for every 256 of them, unpacks it once into scratch (act8_wgrad_scratch). The norm
-// form is applied to the fp32 sums, where it needs no rounding of x.
+// form is applied to the fp32 sums, where it needs no rounding of x. Layers with few tiles are unpacked as well and go to the
+// clusters of linear_few.cuh (wgrad_few).
 //
 // CTA pairs on 256 x 256 tiles of dw as in linear_fused.cuh, both operands MN-major. Where x is converted, four more warps per
 // CTA turn the pair's half of the checkpoint tile ([64 tokens][128 columns], 8 KB) into the swizzled bf16 tile that the MMA reads:

@@ -7,6 +7,9 @@
 //
 // All of it is bound by HBM: a row is read once, kept in registers between the statistics and the output (the squared
 // distances are taken from the mean, not as a difference of sums), and written once. Sums and statistics are fp32.
+// 16384 x 2048 in bf16, back to back in a graph: forward 24 us (5.6 TB/s), with the 8-bit rows 32 us (5.3), backward 37 us (5.4; 47
+// with a residual gradient, 5.7), from 8-bit rows 42 us (4.0: conversions take their share), column sums 10 us (L2), packing and
+// unpacking 17 us (5.9). A plain copy reaches 6.5 TB/s. 16 rows: 3 us forward, 4.5 backward, most of it the launch.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
