@@ -11,14 +11,15 @@ write a checkpoint beside their output, and the backward passes read it as it is
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from .._lib import C
-from .gemm import _err_flag, workspace
+from .gemm import err_ptr, workspace
 
 BLOCK = 32
+NEEDS_WORKSPACE = C.NEEDS_WORKSPACE
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
@@ -55,31 +56,40 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _matrix(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """A bf16 operand of the tensor cores: rows on 16-byte boundaries. Rows that are not are copied once, into rows padded to
-    8 elements (what a bulk-tensor load asks for)."""
-    if t.dtype != torch.bfloat16 or (like is not None and t.get_device() != like.get_device()):
-        raise ValueError(f"{what}: expected bf16" + ("" if like is None else f" on {like.device}") + f", got {t.dtype} on {t.device}")
+def operand(t: torch.Tensor, what: str, device: int) -> Tuple[torch.Tensor, int, int]:
+    """A bf16 operand of the tensor cores as ``(matrix, address, elements between rows)``: rows on 16-byte boundaries. Rows that are
+    not, or that are all the same one, are copied once, into rows padded to 8 elements (what a bulk-tensor load asks for)."""
+    if t.dtype is not torch.bfloat16 or t.get_device() != device:
+        raise ValueError(f"{what}: expected bf16 on cuda:{device}, got {t.dtype} on {t.device}")
     t = rows2d(t, what)
-    if row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
     rows, cols = t.shape
-    padded = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)[:, :cols]
+    at = t.data_ptr()
+    if at % 16 == 0:
+        ld = t.stride(0)
+        if rows <= 1:
+            return t, at, -(-cols // 8) * 8   # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
+        if ld % 8 == 0 and ld > 0:
+            return t, at, ld
+    padded = t.new_empty((rows, -(-cols // 8) * 8))[:, :cols]
     padded.copy_(t)
-    return padded
+    return padded, padded.data_ptr(), -(-cols // 8) * 8
 
 
-def _ld(t: torch.Tensor) -> int:
-    # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+def vector(t: torch.Tensor, n: int, dtypes, device: int, what: str) -> int:
+    """The address of ``n`` contiguous values of one of ``dtypes`` on the device."""
+    if t.dim() != 1 or t.numel() != n or t.dtype not in dtypes or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be {n} contiguous values ({' or '.join(str(d) for d in dtypes)}) on cuda:{device}, "
+                         f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 class Act8:
     """A checkpoint of ``rows x cols`` values: ``q`` int8 and ``e`` uint8, one exponent per 32 columns.
 
-    Both are matrices with rows on 16-byte boundaries; columns past ``cols`` are padding that nothing reads."""
+    Both are matrices with rows on 16-byte boundaries; columns past ``cols`` are padding that nothing reads. One that an operator
+    makes is a single allocation, of which ``q`` and ``e`` are views that are made when asked for."""
 
-    __slots__ = ("q", "e", "rows", "cols", "_args")
+    __slots__ = ("_q", "_e", "_both", "rows", "cols", "device_index", "_args")
 
     def __init__(self, q: torch.Tensor, e: torch.Tensor, cols: int):
         if q.dtype != torch.int8 or e.dtype != torch.uint8 or q.dim() != 2 or e.dim() != 2 or q.shape[0] != e.shape[0]:
@@ -91,28 +101,38 @@ class Act8:
         if q.numel() and (q.stride(1) != 1 or e.stride(1) != 1 or row_stride(q) % 16 or row_stride(e) % 16
                           or q.data_ptr() % 16 or e.data_ptr() % 16):
             raise ValueError("Act8: rows of q and e start on 16-byte boundaries")
-        self.q, self.e, self.rows, self.cols = q, e, q.shape[0], cols
+        self._q, self._e, self._both, self.rows, self.cols = q, e, None, q.shape[0], cols
+        self.device_index = q.get_device()
         self._args = (q.data_ptr(), row_stride(q), e.data_ptr(), row_stride(e))
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Act8":
-        return cls._like(torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device), cols)
+        return cls.for_rows(torch.empty((rows, 0), dtype=torch.uint8, device=device), cols)
 
     @classmethod
     def for_rows(cls, x: torch.Tensor, cols: int) -> "Act8":
         """An empty checkpoint for as many rows as the matrix ``x`` has, where it lives."""
-        return cls._like(x.new_empty((x.shape[0], -(-cols // 16) * 16), dtype=torch.int8), cols)
-
-    @classmethod
-    def _like(cls, q: torch.Tensor, cols: int) -> "Act8":
-        rows, ldq = q.shape
-        lde = -(-cols // 512) * 16   # one byte per 32 columns, padded to 16
         self = cls.__new__(cls)
-        self.q = q
-        self.e = q.new_empty((rows, lde), dtype=torch.uint8)
-        self.rows, self.cols = rows, cols
-        self._args = (self.q.data_ptr(), ldq, self.e.data_ptr(), lde)
+        rows = x.shape[0]
+        ldq, lde = -(-cols // 16) * 16, -(-cols // 512) * 16   # one byte of e per 32 columns; both padded to 16
+        self._q = self._e = None
+        self._both = both = x.new_empty(rows * (ldq + lde), dtype=torch.uint8)
+        at = both.data_ptr()
+        self.rows, self.cols, self.device_index, self._args = rows, cols, both.get_device(), (at, ldq, at + rows * ldq, lde)
         return self
+
+    @property
+    def q(self) -> torch.Tensor:
+        if self._q is None:
+            ldq = self._args[1]
+            self._q = self._both[:self.rows * ldq].view(torch.int8).view(self.rows, ldq)
+        return self._q
+
+    @property
+    def e(self) -> torch.Tensor:
+        if self._e is None:
+            self._e = self._both[self.rows * self._args[1]:].view(self.rows, self._args[3])
+        return self._e
 
     @property
     def shape(self):
@@ -120,11 +140,11 @@ class Act8:
 
     @property
     def device(self):
-        return self.q.device
+        return (self._q if self._both is None else self._both).device
 
     @property
     def nbytes(self) -> int:
-        return self.q.numel() + self.e.numel()
+        return self._q.numel() + self._e.numel() if self._both is None else self._both.numel()
 
     def args(self):
         """(q, ldq, e, lde) as the native entry points take them."""
@@ -156,8 +176,9 @@ def act8_unpack(a: Act8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     dt = _DTYPES.get(dtype)
     if dt is None:
         raise ValueError(f"act8_unpack: bf16 or fp32, not {dtype}")
-    s = launch_stream(a.q)
-    x = a.q.new_empty((a.rows, a.cols), dtype=dtype)
+    held = a.q if a._both is None else a._both
+    s = launch_stream(held)
+    x = held.new_empty((a.rows, a.cols), dtype=dtype)
     check(C.act8_unpack(dt, *a.args(), x.data_ptr(), a.cols, a.rows, a.cols, s), "act8_unpack")
     return x
 
@@ -171,37 +192,32 @@ def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = N
     (``norm.layer_norm_act8``), so the operand is ``x * weight + bias``. With ``bias``, ``dy_sum`` is the sum of dy's rows (fp32, ``[N]``:
     the layer's bias gradient, ``linear.linear_bias_grad``). ``out`` is written, or added to with ``accumulate``."""
     what = "act8_wgrad"
-    s = launch_stream(dy)
-    dy2 = _matrix(dy, f"{what} dy")
+    s, dev = launch_stream(dy), dy.get_device()
+    dy2, dyp, lddy = operand(dy, "act8_wgrad dy", dev)
     tokens, n = dy2.shape
     k = x8.cols
-    if x8.rows != tokens or x8.device != dy.device:
+    if x8.rows != tokens or x8.device_index != dev:
         raise ValueError(f"{what}: checkpoint of {x8.rows} rows on {x8.device}, dy of {tokens} on {dy.device}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.shape != (k,) or t.dtype != torch.bfloat16 or t.device != dy.device or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be {k} contiguous bf16 values on {dy.device}")
+    wp = 0 if weight is None else vector(weight, k, (torch.bfloat16,), dev, "act8_wgrad: weight")
+    bp = 0 if bias is None else vector(bias, k, (torch.bfloat16,), dev, "act8_wgrad: bias")
     if bias is not None and dy_sum is None:
         raise ValueError(f"{what}: bias needs dy_sum, the sum of dy's rows")
-    if dy_sum is not None and (dy_sum.shape != (n,) or dy_sum.dtype != torch.float32 or dy_sum.device != dy.device or not dy_sum.is_contiguous()):
-        raise ValueError(f"{what}: dy_sum must be {n} contiguous fp32 values on {dy.device}")
+    sp = 0 if dy_sum is None else vector(dy_sum, n, (torch.float32,), dev, "act8_wgrad: dy_sum")
     if out is None:
         if accumulate:
             raise ValueError(f"{what}: accumulate needs out")
         out = dy2.new_empty((n, k), dtype=torch.float32)
-    elif out.shape != (n, k) or out.dtype != torch.float32 or out.device != dy.device or (k > 1 and out.stride(1) != 1):
+    elif out.shape != (n, k) or out.dtype is not torch.float32 or out.get_device() != dev or (k > 1 and out.stride(1) != 1):
         raise ValueError(f"{what}: out must be a {n} x {k} fp32 matrix on {dy.device} with contiguous rows")
     if tokens == 0:
         return out if accumulate else out.zero_()
     if n and k:
         need = C.act8_wgrad_scratch(tokens, n, k)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
-        head = (dy2.data_ptr(), _ld(dy2), *x8.args(), out.data_ptr(), row_stride(out), accumulate, 0 if weight is None else weight.data_ptr(),
-                0 if bias is None else bias.data_ptr(), 0 if dy_sum is None else dy_sum.data_ptr(), tokens, n, k,
-                0 if scratch is None else scratch.data_ptr())
-        tail = (_err_flag(dy.device).data_ptr(), wait_limit_s, s)
-        rc = C.act8_wgrad(*head, 0, *tail)
-        if rc == C.NEEDS_WORKSPACE:   # only where tiles are cut along the contraction
-            joined = workspace(dy.get_device(), s)
-            rc = C.act8_wgrad(*head, joined.data_ptr(), *tail)
+        scratch = dy2.new_empty(need, dtype=torch.uint8) if need else None
+        head = (dyp, lddy, *x8._args, out.data_ptr(), row_stride(out), accumulate, wp, bp, sp, tokens, n, k, 0 if scratch is None else scratch.data_ptr())
+        rc = C.act8_wgrad(*head, 0, err_ptr(dev), wait_limit_s, s)
+        if rc == NEEDS_WORKSPACE:   # only where tiles are cut along the contraction
+            joined = workspace(dev, s)
+            rc = C.act8_wgrad(*head, joined.data_ptr(), err_ptr(dev), wait_limit_s, s)
         check(rc, what)
     return out

@@ -21,6 +21,17 @@ def _err_flag(device) -> torch.Tensor:
     return _err_flags[key]
 
 
+_err_ptrs = {}   # the flags live as long as the process
+
+
+def err_ptr(device_index: int) -> int:
+    """Address of the device's error word (a dictionary look-up where a call's latency counts)."""
+    p = _err_ptrs.get(device_index)
+    if p is None:
+        p = _err_ptrs[device_index] = _err_flag(torch.device("cuda", device_index)).data_ptr()
+    return p
+
+
 def check_gemm_errors(device=None) -> None:
     """Synchronise and raise if a bounded wait inside a GEMM kernel ran out."""
     for key, flag in _err_flags.items():

@@ -15,10 +15,12 @@ from typing import Optional, Union
 import torch
 
 from .._lib import C
-from .act8 import _DTYPES, _ld, _matrix, Act8, check, launch_stream, row_stride, rows2d
-from .gemm import _err_flag, workspace
+from .act8 import _DTYPES, NEEDS_WORKSPACE, Act8, check, launch_stream, operand, row_stride, rows2d, vector
+from .gemm import err_ptr, workspace
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_BIAS_TYPES = (torch.bfloat16, torch.float32)
+_NOT_KEPT = (0, 0, 0, 0)
 
 
 def _act_code(act, what: str) -> int:
@@ -28,17 +30,16 @@ def _act_code(act, what: str) -> int:
     return code
 
 
-def _launch(dgrad, act, M, N, K, a, w, bias, residual, out, out2, pre, kept, limit, s, what, scratch=0):
-    rc = C.linear_fused(dgrad, act, M, N, K, a.data_ptr(), _ld(a), w.data_ptr(), _ld(w),
-                        0 if bias is None else bias.data_ptr(), bias is not None and bias.dtype == torch.float32,
-                        0 if residual is None else residual.data_ptr(), 0 if residual is None else row_stride(residual),
-                        out.data_ptr(), row_stride(out), 0 if out2 is None else out2.data_ptr(), N,
-                        0 if pre is None else pre.data_ptr(), 0 if pre is None else row_stride(pre),
-                        *((0, 0, 0, 0) if kept is None else kept.args()),
-                        scratch, _err_flag(a.device).data_ptr(), limit, s)
-    if rc == C.NEEDS_WORKSPACE and scratch == 0:   # only where tiles are cut along the contraction
-        scratch = workspace(a.get_device(), s)
-        return _launch(dgrad, act, M, N, K, a, w, bias, residual, out, out2, pre, kept, limit, s, what, scratch.data_ptr())
+def _like(t: torch.Tensor, shape, device: int, what: str) -> None:
+    if t.shape != shape or t.dtype is not torch.bfloat16 or t.get_device() != device:
+        raise ValueError(f"{what} must be {tuple(shape)} bf16 on cuda:{device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+
+
+def _run(dev, s, what, head, tail, limit):
+    rc = C.linear_fused(*head, *tail, 0, err_ptr(dev), limit, s)
+    if rc == NEEDS_WORKSPACE:   # only where tiles are cut along the contraction
+        scratch = workspace(dev, s)
+        rc = C.linear_fused(*head, *tail, scratch.data_ptr(), err_ptr(dev), limit, s)
     check(rc, what)
 
 
@@ -54,43 +55,41 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     code = _act_code(act, what)
     if save not in (None, "bf16", "act8"):
         raise ValueError(f"{what}: save is None, 'bf16' or 'act8', not {save!r}")
-    s = launch_stream(x)
-    x2, w = _matrix(x, f"{what} x"), _matrix(w, f"{what} w", x)
+    s, dev = launch_stream(x), x.get_device()
+    x2, xp, ldx = operand(x, "linear_act x", dev)
+    w, wp, ldw = operand(w, "linear_act w", dev)
     M, K = x2.shape
     N = w.shape[0]
     if w.shape[1] != K:
         raise ValueError(f"{what}: x has {K} columns, w has {w.shape[1]}")
     if K == 0:
         raise ValueError(f"{what}: a sum over no columns")
-    if bias is not None and (bias.shape != (N,) or bias.dtype not in (torch.bfloat16, torch.float32) or bias.device != x.device
-                             or not bias.is_contiguous()):
-        raise ValueError(f"{what}: bias must be {N} contiguous bf16 or fp32 values on {x.device}")
-    lead = x.shape[:-1]
+    bp = 0 if bias is None else vector(bias, N, _BIAS_TYPES, dev, "linear_act: bias")
+    shape = None if residual is None and out is None and x.dim() == 2 else x.shape[:-1] + (N,)
+    r2 = None
     if residual is not None:
-        if residual.shape != lead + (N,) or residual.dtype != torch.bfloat16 or residual.device != x.device:
-            raise ValueError(f"{what}: residual must be {tuple(lead) + (N,)} bf16 on {x.device}")
+        _like(residual, shape, dev, "linear_act: residual")
         r2 = rows2d(residual, what)
-    else:
-        r2 = None
     if out is None:
         y = x2.new_empty((M, N))
     else:
-        if out.shape != lead + (N,) or out.dtype != torch.bfloat16 or out.device != x.device:
-            raise ValueError(f"{what}: out must be {tuple(lead) + (N,)} bf16 on {x.device}")
+        _like(out, shape, dev, "linear_act: out")
         y = out if out.dim() == 2 else out.view(M, N)
         if N > 1 and y.stride(1) != 1:
             raise ValueError(f"{what}: the values of a row of out must be contiguous")
-    pre = x2.new_empty((M, N)) if save == "bf16" else None
+    pre = torch.empty_like(y) if save == "bf16" and out is None else x2.new_empty((M, N)) if save == "bf16" else None
     kept = Act8.for_rows(y, N) if save == "act8" else None
     if M and N:
-        _launch(False, code, M, N, K, x2, w, bias, r2, y, None, pre, kept, wait_limit_s, s, what)
+        _run(dev, s, what, (False, code, M, N, K, xp, ldx, wp, ldw, bp, bias is not None and bias.dtype is torch.float32),
+             (0 if r2 is None else r2.data_ptr(), 0 if r2 is None else row_stride(r2), y.data_ptr(), N if out is None else row_stride(y), 0, N,
+              0 if pre is None else pre.data_ptr(), N, *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
     if out is not None:
         y = out
     elif x.dim() != 2:
-        y = y.view(*lead, N)
+        y = y.view(shape)
     if save is None:
         return y
-    return y, (kept if pre is None else pre.view(*lead, N))
+    return y, (kept if pre is None else pre if x.dim() == 2 else pre.view(x.shape[:-1] + (N,)))
 
 
 def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, Act8, None], *, act: Optional[str] = None,
@@ -100,33 +99,35 @@ def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, A
     With ``recompute``: ``(dh, a)``, where ``a`` (bf16) is what the weight gradient of that layer needs."""
     what = "linear_act_dgrad"
     code = _act_code(act, what)
-    s = launch_stream(dy)
-    dy2, w = _matrix(dy, f"{what} dy"), _matrix(w, f"{what} w", dy)
+    s, dev = launch_stream(dy), dy.get_device()
+    dy2, dyp, lddy = operand(dy, "linear_act_dgrad dy", dev)
+    w, wp, ldw = operand(w, "linear_act_dgrad w", dev)
     M, K = dy2.shape
     N = w.shape[1]
     if w.shape[0] != K:
         raise ValueError(f"{what}: dy has {K} columns, w has {w.shape[0]} rows")
     if K == 0:
         raise ValueError(f"{what}: a sum over no columns")
-    lead = dy.shape[:-1]
     pre = kept = None
     if isinstance(h, Act8):
-        if h.rows != M or h.cols != N or h.device != dy.device:
+        if h.rows != M or h.cols != N or h.device_index != dev:
             raise ValueError(f"{what}: checkpoint of {h.rows} x {h.cols} on {h.device}, expected {M} x {N} on {dy.device}")
         kept = h
     elif h is not None:
-        if h.shape != lead + (N,) or h.dtype != torch.bfloat16 or h.device != dy.device:
-            raise ValueError(f"{what}: h must be {tuple(lead) + (N,)} bf16 on {dy.device}")
+        _like(h, dy.shape[:-1] + (N,), dev, "linear_act_dgrad: h")
         pre = rows2d(h, what)
     elif code != 0 or recompute:
         raise ValueError(f"{what}: h is needed")
     dh = dy2.new_empty((M, N))
-    a = dy2.new_empty((M, N)) if recompute else None
+    a = torch.empty_like(dh) if recompute else None
     if M and N:
-        _launch(True, code, M, N, K, dy2, w, None, None, dh, a, pre, kept, wait_limit_s, s, what)
+        _run(dev, s, what, (True, code, M, N, K, dyp, lddy, wp, ldw, 0, False),
+             (0, 0, dh.data_ptr(), N, 0 if a is None else a.data_ptr(), N, 0 if pre is None else pre.data_ptr(), 0 if pre is None else row_stride(pre),
+              *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
     if dy.dim() != 2:
-        dh = dh.view(*lead, N)
-        a = None if a is None else a.view(*lead, N)
+        shape = dy.shape[:-1] + (N,)
+        dh = dh.view(shape)
+        a = None if a is None else a.view(shape)
     return (dh, a) if recompute else dh
 
 

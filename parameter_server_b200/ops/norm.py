@@ -69,22 +69,22 @@ def _backward(dy, x, kept, weight, mean, rstd, residual_grad, weight_grad, bias_
     dt = _DTYPES.get(dy.dtype)
     if dt is None:
         raise ValueError(f"{what}: bf16 or fp32, not {dy.dtype}")
-    s = launch_stream(dy)
+    s, dev = launch_stream(dy), dy.get_device()
     dy2 = rows2d(dy, what)
     rows, d = dy2.shape
     if x is not None:
-        if x.shape != dy.shape or x.dtype != dy.dtype or x.device != dy.device:
+        if x.shape != dy.shape or x.dtype != dy.dtype or x.get_device() != dev:
             raise ValueError(f"{what}: x and dy differ ({tuple(x.shape)} of {x.dtype}, {tuple(dy.shape)} of {dy.dtype})")
         x = rows2d(x, what)
-    elif kept.rows != rows or kept.cols != d or kept.device != dy.device:
+    elif kept.rows != rows or kept.cols != d or kept.device_index != dev:
         raise ValueError(f"{what}: checkpoint of {kept.rows} x {kept.cols} on {kept.device}, dy of {rows} x {d} on {dy.device}")
     weight = _param(weight, d, dy, what, "weight")
     for name, t in (("mean", mean), ("rstd", rstd)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != rows or t.device != dy.device or not t.is_contiguous()):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != rows or t.get_device() != dev or not t.is_contiguous()):
             raise ValueError(f"{what}: {name} must be {rows} contiguous fp32 values on {dy.device}")
     join = None
     if residual_grad is not None:
-        if residual_grad.shape != dy.shape or residual_grad.dtype != dy.dtype or residual_grad.device != dy.device:
+        if residual_grad.shape != dy.shape or residual_grad.dtype != dy.dtype or residual_grad.get_device() != dev:
             raise ValueError(f"{what}: residual_grad must be like dy ({tuple(dy.shape)} of {dy.dtype})")
         join = rows2d(residual_grad, what)
     grads = []
@@ -93,7 +93,7 @@ def _backward(dy, x, kept, weight, mean, rstd, residual_grad, weight_grad, bias_
             if accumulate:
                 raise ValueError(f"{what}: accumulate needs {name}")
             t = dy2.new_empty(d, dtype=torch.float32)
-        elif t.dtype != torch.float32 or t.shape != (d,) or t.device != dy.device or not t.is_contiguous():
+        elif t.dtype != torch.float32 or t.shape != (d,) or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be {d} contiguous fp32 values on {dy.device}")
         grads.append(t)
     dx = torch.empty_like(dy2) if dy2.is_contiguous() else dy2.new_empty((rows, d))

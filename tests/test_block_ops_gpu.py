@@ -599,3 +599,19 @@ def test_products_of_two_streams_share_the_gpu():
     for i, out in enumerate(seen[1]):
         assert torch.equal(out, alone[3 + i % 2])
     G.check_gemm_errors()
+
+
+def test_rows_that_are_all_the_same_one():
+    """Operands expanded from one row: every row at the same address."""
+    one, w, dy = rand(1, 72), rand(40, 72, seed=1), rand(1, 40, seed=2)
+    full = one.expand(5, 72)
+    assert torch.equal(linear.linear_act(full, w), linear.linear_act(full.contiguous(), w))
+    assert torch.equal(linear.linear_act(one, w[:1].expand(40, 72)), linear.linear_act(one, w[:1].expand(40, 72).contiguous()))
+    assert torch.equal(linear.linear_act_dgrad(dy.expand(5, 40), w, None), linear.linear_act_dgrad(dy.expand(5, 40).contiguous(), w, None))
+    x8 = act8.act8_pack(full)
+    assert torch.equal(act8.act8_unpack(x8), act8.act8_unpack(act8.act8_pack(full.contiguous())))
+    assert torch.equal(act8.act8_wgrad(dy.expand(5, 40), x8), act8.act8_wgrad(dy.expand(5, 40).contiguous(), x8))
+    assert torch.equal(linear.linear_bias_grad(dy.expand(5, 40)), linear.linear_bias_grad(dy.expand(5, 40).contiguous()))
+    got, want = (norm.layer_norm(v, one[0], one[0]) for v in (full, full.contiguous()))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    G.check_gemm_errors()
