@@ -137,6 +137,63 @@ __device__ __forceinline__ void close_group() { asm volatile("cp.async.commit_gr
 template <int PENDING>
 __device__ __forceinline__ void wait_groups() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
+// Eight bf16 of a row on any 2-byte boundary ("loose"), beside eight whole numbers of a checkpoint: the aligned words that hold them,
+// five at most, on their way and in shared memory (a stride of five words: no bank conflicts), shifted by half a word where the row
+// starts on one. `m` of the eight exist. 16384 x 1001, one value at a time and so, us: backward from 8-bit rows 90, 39; from x one at a
+// time is faster, since its accesses lie side by side: 29, 42.
+constexpr int kLooseBytes = 20;
+__device__ __forceinline__ uint32_t half_of(const void* p) { return (uint32_t)(uintptr_t)p & 2u; }
+__device__ __forceinline__ void loose_copy(uint32_t dst, const __nv_bfloat16* p, int m) {
+    const uint32_t odd = half_of(p);
+    const char* w = (const char*)p - odd;
+    const int words = ((int)odd + 2 * m + 3) / 4;
+#pragma unroll
+    for (int k = 0; k < 5; ++k)
+        if (k < words) copy_async<4>(dst + 4 * k, w + 4 * k);
+}
+__device__ __forceinline__ uint4 loose_read(uint32_t src, uint32_t odd, int m) {
+    uint32_t w[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = from_shared<uint32_t>(src + 4 * k);
+    const uint32_t shift = odd * 8;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], shift);
+    if (m < 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = 2 * k >= m ? 0u : 2 * k + 1 >= m ? w[k] & 0xFFFFu : w[k];
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 loose_load(const __nv_bfloat16* p, int m) {   // straight from memory: once per kernel
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < m) w[j / 2] |= (uint32_t)((const unsigned short*)p)[j] << (16 * (j & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void loose_store(__nv_bfloat16* p, const float* f, int m) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+        w[k] = *(const uint32_t*)&h;
+    }
+    unsigned short* o = (unsigned short*)p;
+    if (m < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < m) o[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+    } else if (half_of(p) == 0u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *(uint32_t*)(o + 2 * k) = w[k];
+    } else {
+        o[0] = (unsigned short)w[0];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *(uint32_t*)(o + 2 * k + 1) = __funnelshift_r(w[k], w[k + 1], 16);
+        o[7] = (unsigned short)(w[3] >> 16);
+    }
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -151,8 +208,12 @@ __device__ __forceinline__ uint32_t block_exponent(const float* f, bool valid) {
         for (int j = 0; j < VEC; ++j) m = abs_max(m, f[j]);
     }
     uint32_t v = abs_bits(m);
+    if constexpr (VEC == 1) {
+        v = __reduce_max_sync(0xFFFFFFFFu, v);
+    } else {
 #pragma unroll
-    for (int o = kAct8Block / VEC / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+        for (int o = kAct8Block / VEC / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    }
     return act8_exponent(v);
 }
 
@@ -339,10 +400,10 @@ layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ldx, const T* __rest
 // team's warps through shared memory with one barrier per row. At the end the teams' sums are added in a tree and leave
 // as one partial row per CTA, which column_reduce_kernel adds in CTA order: the result does not depend on timing. (More CTAs
 // per SM would write and read more partial rows: 2 * d floats each.)
-template <typename T, int VEC, bool SRC8>
+template <typename T, int VEC, bool SRC8, bool LOOSE>
 struct BwdRing {
-    static constexpr int kVecs = kBwdElems / VEC, kVecBytes = VEC * (int)sizeof(T);
-    static constexpr bool kAsync = copies_ahead<T, VEC>() && (VEC >= 4 || !SRC8);   // (a vector of q has VEC bytes)
+    static constexpr int kVecs = kBwdElems / VEC, kVecBytes = LOOSE ? kLooseBytes : VEC * (int)sizeof(T);
+    static constexpr bool kAsync = LOOSE || copies_ahead<T, VEC>() && (VEC >= 4 || !SRC8);   // (a vector of q has VEC bytes)
     static constexpr int kSlots = sizeof(T) == 2 ? 3 : 2;
     // per thread and slot: dy, the residual's gradient, and x or (8 or 4 bytes a vector) q with a word of exponents
     static constexpr int kRowBytes = SRC8 ? kVecs * (2 * kVecBytes + VEC + 4) : kVecs * 3 * kVecBytes;
@@ -350,8 +411,8 @@ struct BwdRing {
 };
 
 // TPR: threads that share a row, known to the compiler, so that a thread's places in the row and in the ring are constants (with
-// a run-time value an element took twice the instructions); 0 = `tpr_arg` (8-bit rows that are not aligned).
-template <typename T, int VEC, bool SRC8, int TPR>
+// a run-time value an element took twice the instructions); 0 = `tpr_arg` (8-bit rows beside fp32 ones that are not aligned).
+template <typename T, int VEC, bool SRC8, int TPR, bool LOOSE>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
                       int64_t ldq, const uint8_t* __restrict__ e, int64_t lde, const T* __restrict__ weight,
@@ -361,9 +422,9 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
     constexpr int NV = kBwdElems / VEC;
     const int tpr = TPR > 0 ? TPR : tpr_arg;
     using IO = Io<T, VEC>;
-    using Ring = BwdRing<T, VEC, SRC8>;
+    using Ring = BwdRing<T, VEC, SRC8, LOOSE>;
     constexpr bool kAsync = Ring::kAsync;
-    constexpr int kVecBytes = Ring::kVecBytes, kCopy = kAsync ? kVecBytes : 4, kCopyQ = kAsync && SRC8 ? VEC : 4;
+    constexpr int kVecBytes = Ring::kVecBytes, kCopy = kAsync && !LOOSE ? kVecBytes : 4, kCopyQ = kAsync && SRC8 ? VEC : 4;
     extern __shared__ uint4 ring_raw[];         // the ring; at the end sums of the teams
     __shared__ float red[2][kBwdThreads / 32][2];
     const int team = threadIdx.x / tpr, t = threadIdx.x % tpr, teams = blockDim.x / tpr;
@@ -375,7 +436,8 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int col = (i * tpr + t) * VEC;
-        graw[i] = weight != nullptr && col < d ? IO::load(weight + col) : IO::one();
+        if constexpr (LOOSE) graw[i] = weight != nullptr ? loose_load(weight + col, d - col) : IO::one();
+        else graw[i] = weight != nullptr && col < d ? IO::load(weight + col) : IO::one();
     }
     const float inv_d = 1.f / (float)d;
     // Running positions: a row's overhead is shared by 16 values only. In a slot the thread's vectors of dy, of the residual's
@@ -397,6 +459,14 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
     const int8_t* ahead_q = SRC8 ? q + first * ldq + c0 : nullptr;
     const uint8_t* ahead_e = SRC8 ? e + first * lde : nullptr;
     int64_t ahead_row = first;
+    auto copy = [&](uint32_t to, const T* from, int i) {
+        if constexpr (LOOSE) loose_copy(to, from, min(VEC, d - c0 - i * tpr * VEC));
+        else copy_async<kCopy>(to, from);
+    };
+    auto fetched = [&](uint32_t at, const T* row_start, int i) -> typename IO::Raw {
+        if constexpr (LOOSE) return loose_read(at, half_of(row_start), d - c0 - i * tpr * VEC);
+        else return from_shared<typename IO::Raw>(at);
+    };
     auto request = [&](int s) {   // the next row that has not been asked for
         if constexpr (kAsync) {
             if (ahead_row < rows) {
@@ -404,13 +474,13 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                 for (int i = 0; i < NV; ++i) {
                     const int off = i * tpr * VEC;
                     if (i >= nv) continue;
-                    copy_async<kCopy>(at_y(s, i), ahead_y + off);
-                    if (join != nullptr) copy_async<kCopy>(at_j(s, i), ahead_j + off);
+                    copy(at_y(s, i), ahead_y + off, i);
+                    if (join != nullptr) copy(at_j(s, i), ahead_j + off, i);
                     if constexpr (SRC8) {
                         copy_async<kCopyQ>(at_q(s, i), ahead_q + off);
                         copy_async<4>(at_e(s, i), ahead_e + (c0 + off) / (4 * kAct8Block) * 4);   // the exponents of 128 columns
                     } else {
-                        copy_async<kCopy>(at_x(s, i), ahead_x + off);
+                        copy(at_x(s, i), ahead_x + off, i);
                     }
                 }
             }
@@ -442,11 +512,22 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
         typename IO::Raw ry[NV], rx[NV];
         typename Q8<VEC>::Raw rq[NV];
         float rs[NV];
+        // one value at a time: the residual's gradient is requested with the rest of its row, and kept in pairs
+        constexpr bool kPairs = !kAsync && sizeof(T) == 2;
+        uint32_t rj[kPairs ? kBwdElems / 2 : 1];
+        if constexpr (kPairs) {
+            if (join != nullptr) {
+                const unsigned short* j = (const unsigned short*)(join + row * ldjoin + c0);
+#pragma unroll
+                for (int i = 0; i < NV; i += 2)
+                    rj[i / 2] = (i < nv ? (uint32_t)j[i * tpr] : 0u) | (i + 1 < nv ? (uint32_t)j[(i + 1) * tpr] << 16 : 0u);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int col = (i * tpr + t) * VEC;
             const bool in = i < nv;
-            if constexpr (kAsync) ry[i] = in ? from_shared<typename IO::Raw>(at_y(slot, i)) : IO::zero();
+            if constexpr (kAsync) ry[i] = in ? fetched(at_y(slot, i), dy + row * lddy, i) : IO::zero();
             else ry[i] = in ? IO::load(dy + row * lddy + col) : IO::zero();
             if constexpr (SRC8) {
                 if constexpr (kAsync) {
@@ -457,7 +538,7 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                     rs[i] = in ? act8_step(e[row * lde + col / kAct8Block]) : 0.f;
                 }
             } else {
-                if constexpr (kAsync) rx[i] = in ? from_shared<typename IO::Raw>(at_x(slot, i)) : IO::zero();
+                if constexpr (kAsync) rx[i] = in ? fetched(at_x(slot, i), x + row * ldx, i) : IO::zero();
                 else rx[i] = in ? IO::load(x + row * ldx + col) : IO::zero();
             }
         }
@@ -508,12 +589,14 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
             for (int j = 0; j < VEC; ++j) o[j] = rstd * (p[i * VEC + j] - fmaf(xh[i * VEC + j], a2, a1));
             if (join != nullptr) {
                 float fj[VEC];
-                if constexpr (kAsync) IO::unpack(from_shared<typename IO::Raw>(at_j(slot, i)), fj);
+                if constexpr (kAsync) IO::unpack(fetched(at_j(slot, i), join + row * ldjoin, i), fj);
+                else if constexpr (kPairs) fj[0] = __uint_as_float(i & 1 ? rj[i / 2] & 0xFFFF0000u : rj[i / 2] << 16);
                 else IO::unpack(IO::load(join + row * ldjoin + c0 + i * tpr * VEC), fj);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) o[j] += fj[j];
             }
-            IO::store(dx_row + i * tpr * VEC, o);
+            if constexpr (LOOSE) loose_store(dx_row + i * tpr * VEC, o, d - c0 - i * tpr * VEC);
+            else IO::store(dx_row + i * tpr * VEC, o);
         }
         dx_row += step * lddx;
         slot = slot + 1 == Ring::kSlots ? 0 : slot + 1;
@@ -547,7 +630,14 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (i >= nv) continue;
-        if constexpr (VEC >= 4) {
+        if constexpr (LOOSE) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (c0 + i * tpr * VEC + j >= d) continue;
+                out[i * tpr * VEC + j] = dg[i * VEC + j];
+                out[d + i * tpr * VEC + j] = db[i * VEC + j];
+            }
+        } else if constexpr (VEC >= 4) {
 #pragma unroll
             for (int j = 0; j < VEC; j += 4) {
                 const int c = i * VEC + j;
@@ -884,10 +974,10 @@ int reduce_partials(const float* partial, int n, int64_t width, int64_t split, f
     return (int)cudaLaunchKernelEx(&cfg, column_reduce_kernel, partial, n, width, split, out0, out1, accumulate);
 }
 
-template <typename T, int VEC, bool SRC8>
+template <typename T, int VEC, bool SRC8, bool LOOSE = false>
 int launch_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View& k, const T* w, const float* mean, const float* rstd,
                const T* join, int64_t ldjoin, T* dx, int64_t lddx, float* partial, int64_t rows, int d, const BwdPlan& p, cudaStream_t s) {
-    using Ring = BwdRing<T, VEC, SRC8>;
+    using Ring = BwdRing<T, VEC, SRC8, LOOSE>;
     // the ring, or half the teams' sums
     const int smem = std::max(Ring::kBytes, p.threads > p.tpr ? p.threads / 2 * 2 * kBwdElems * (int)sizeof(float) : 0);
     auto go = [&](auto instance) -> int {
@@ -900,14 +990,14 @@ int launch_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8Vie
         return (int)cudaGetLastError();
     };
     if constexpr (SRC8 && VEC == 1) {
-        return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 0>>{});
+        return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 0, LOOSE>>{});
     } else {
         switch (p.tpr) {
-            case 32: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 32>>{});
-            case 64: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 64>>{});
-            case 128: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 128>>{});
-            case 256: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 256>>{});
-            default: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 512>>{});
+            case 32: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 32, LOOSE>>{});
+            case 64: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 64, LOOSE>>{});
+            case 128: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 128, LOOSE>>{});
+            case 256: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 256, LOOSE>>{});
+            default: return go(Kernel<layer_norm_bwd_kernel<T, VEC, SRC8, 512, LOOSE>>{});
         }
     }
 }
@@ -922,8 +1012,10 @@ int bwd_typed(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View
     int rc;
     if (p.fits) {
         const bool vec = aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}) && (!SRC8 || kept_ok(k));
+        constexpr bool kLoose = sizeof(T) == 2 && SRC8;   // unaligned rows otherwise: one value at a time
+        if (kLoose && !kept_ok(k)) return -2;
         rc = vec ? launch_bwd<T, vec_of<T>(), SRC8>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s)
-                 : launch_bwd<T, 1, SRC8>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s);
+                 : launch_bwd<T, kLoose ? 8 : 1, SRC8, kLoose>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s);
     } else {
         if (rows > 0x7FFFFFFF) return -2;
         layer_norm_bwd_long_kernel<T, SRC8><<<(unsigned)rows, 512, 0, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde,
