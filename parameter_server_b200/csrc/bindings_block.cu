@@ -37,6 +37,9 @@ void bind_block(py::module_& m) {
         return column_sum(dtype, (const void*)x, ldx, rows, cols, (float*)out, accumulate ? 1 : 0, (float*)partial, (void*)s);
     });
     m.def("column_sum_scratch", &column_sum_scratch);
+    m.def("pad_rows", [](uintptr_t src, int64_t ld, uintptr_t dst, int64_t ldp, int64_t rows, int64_t cols, uintptr_t s) {
+        return pad_rows((const void*)src, ld, (void*)dst, ldp, rows, cols, (void*)s);
+    });
     m.def("linear_fused", [](bool dgrad, int act, int M, int N, int K, uintptr_t a, int64_t lda, uintptr_t w, int64_t ldw, uintptr_t bias,
                              bool bias_f32, uintptr_t residual, int64_t ldres, uintptr_t out, int64_t ldo, uintptr_t out2, int64_t ldo2,
                              uintptr_t pre, int64_t ldpre, uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde, uintptr_t workspace,

@@ -103,6 +103,26 @@ __device__ __forceinline__ void sts_converted(uint32_t addr, uint32_t w0, uint32
                  : "memory");
 }
 
+// A piece of [32 rows][16 floats] whose rows do not start on 16-byte boundaries: the lanes cover two rows side by side.
+__device__ __noinline__ void put_floats(uint32_t stage, int lane, float* out, int64_t ldo, int rows, int cols, int accumulate) {
+    const int c = lane & 15;
+    if (c >= cols) return;
+    float* o = out + (lane >> 4) * ldo + c;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(in_piece(stage, i * 2 + (lane >> 4), c * 4)) : "memory");
+    if (accumulate) {
+        float old[16];   // all on their way before the first is needed
+#pragma unroll
+        for (int i = 0; i < 16; ++i) old[i] = i * 2 + (lane >> 4) < rows ? o[i * 2 * ldo] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] += old[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (i * 2 + (lane >> 4) < rows) o[i * 2 * ldo] = v[i];
+}
+
 template <bool CONVERT>
 __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_constant__ WgParams p) {
     using L = WgSmem<CONVERT>;
@@ -435,6 +455,11 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                                    make_uint4(__float_as_uint(acc[c * 16 + 4 * j]), __float_as_uint(acc[c * 16 + 4 * j + 1]),
                                               __float_as_uint(acc[c * 16 + 4 * j + 2]), __float_as_uint(acc[c * 16 + 4 * j + 3])));
                     __syncwarp();
+                    if (!p.out_vec) {
+                        put_floats(stage, lane, p.out + (int64_t)row0 * p.ldo + colw + c * 16, p.ldo, min(32, p.N - row0), min(16, p.K - colw - c * 16),
+                                   p.accumulate);
+                        continue;
+                    }
                     const int cb = lane & 3, col = colw + c * 16 + cb * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -443,7 +468,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                         const uint4 w = ld_smem_v4(stage + (uint32_t)(r * 64 + ((cb ^ ((r >> 1) & 3)) << 4)));
                         float4 d = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
                         float* op = p.out + (int64_t)(row0 + r) * p.ldo + col;
-                        if (p.out_vec && col + 4 <= p.K) {
+                        if (col + 4 <= p.K) {
                             if (p.accumulate) {
                                 const float4 o = *(const float4*)op;
                                 d.x += o.x; d.y += o.y; d.z += o.z; d.w += o.w;

@@ -121,6 +121,21 @@ __device__ __forceinline__ void add_parts(uint32_t at, float* v) {
     for (int s = 1; s < S; ++s) { v[0] += part[s].x; v[1] += part[s].y; v[2] += part[s].z; v[3] += part[s].w; }
 }
 
+// The same for four features 32 apart
+__device__ __forceinline__ void add_parts_apart(uint32_t at, int S, float* v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = 0.f;
+    for (int s = 0; s < S; ++s) {
+        const uint32_t from = mapa_cluster(at, (uint32_t)s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float x;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from + 128 * j) : "memory");
+            v[j] = s == 0 ? x : v[j] + x;
+        }
+    }
+}
+
 template <int MODE, int ACT>
 __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid_constant__ FewParams p) {
     constexpr bool DGRAD = MODE == kFewDgrad, WGRAD = MODE == kFewWgrad, W_MN = MODE != kFewFwd;
@@ -229,18 +244,22 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     }
     __syncwarp();
     // what the epilogue needs from memory, on its way meanwhile: a warp has a token, a lane four neighbouring features
-    const int n = n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
+    // (wgrad with rows that are not aligned: four features 32 apart, so that the lanes' single values lie side by side)
+    const bool apart = WGRAD && p.out_wide == 0;
+    const int n = apart ? n0 + lane : n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
+    const int stride = apart ? 32 : 1;                                 // between them
     const int t_end = min(tokens, (rank + 1) * share), t_first = rank * share + warp;
     float b[4] = {0.f, 0.f, 0.f, 0.f}, gain[4] = {1.f, 1.f, 1.f, 1.f}, aux[4], sum = 0.f;
     if constexpr (WGRAD) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < have && p.gain != nullptr) gain[j] = __bfloat162float(p.gain[n + j]);
+            if (j * stride < have && p.gain != nullptr) gain[j] = __bfloat162float(p.gain[n + j * stride]);
     }
     if constexpr (!DGRAD) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < have) b[j] = p.bias32 != nullptr ? p.bias32[n + j] : p.bias != nullptr ? __bfloat162float(p.bias[n + j]) : 0.f;
+            if (j * stride < have)
+                b[j] = p.bias32 != nullptr ? p.bias32[n + j * stride] : p.bias != nullptr ? __bfloat162float(p.bias[n + j * stride]) : 0.f;
     }
     auto fetch = [&](int t) {   // residual, or h
 #pragma unroll
@@ -257,7 +276,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j < have) aux[j] = old[j];
+                    if (j * stride < have) aux[j] = old[j * stride];
             }
         } else if constexpr (!DGRAD) {
             if (p.res != nullptr) load4(p.res + row * p.ldres + n, have, p.res_wide != 0, aux);
@@ -305,12 +324,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)p.tmem_columns) : "memory");
     }
     // ---- epilogue of this CTA's tokens ----
-    const uint32_t mine = parts + (uint32_t)lane * 16;
+    const uint32_t mine = parts + (uint32_t)lane * (apart ? 4 : 16);
     for (int t = t_first; t < t_end; t += kFewThreads / 32) {
         const int64_t row = m0 + t;
         float v[4];
         const uint32_t at = mine + (uint32_t)(t * BM) * 4;
-        if (S == 8) add_parts<8>(at, v);
+        if (WGRAD && apart) add_parts_apart(at, S, v);
+        else if (S == 8) add_parts<8>(at, v);
         else if (S == 4) add_parts<4>(at, v);
         else if (S == 2) add_parts<2>(at, v);
         else add_parts<1>(at, v);
@@ -324,7 +344,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j < have) o[j] = v[j];
+                    if (j * stride < have) o[j * stride] = v[j];
             }
         } else if constexpr (!DGRAD) {
 #pragma unroll

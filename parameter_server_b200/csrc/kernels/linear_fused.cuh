@@ -76,7 +76,7 @@ struct LinParams {
     int64_t ldq;
     uint8_t* e;
     int64_t lde;
-    int aux_vec, pre_vec, out_vec, out2_vec;   // rows of residual (forward) / pre / out / out2 are 16-byte aligned
+    int aux_width, pre_width, out_width, out2_width;   // rows of residual (forward) / pre / out / out2 start on multiples of 16, 8, 4 or 2
     float* partial;                   // shared tiles: [pair][2 places][cta][warp][BN / 64 pieces][8][32 lanes][4]
     unsigned* arrived;                // [shared tile][cta][warp]
     unsigned* err_flag;
@@ -138,9 +138,9 @@ __device__ __forceinline__ float act_slope(float h, float* value) {
 }
 
 // ---- epilogue: memory side -------------------------------------------------------------------------------------------
-// 32 values of a bf16 row (64 bytes): four wide loads, or one by one where the row is unaligned or cut off by the tensor's edge
-__device__ __forceinline__ void load32(const __nv_bfloat16* p, int n, bool vec, uint4* raw) {
-    if (vec && n >= 32) {
+// 32 values of a bf16 row on a 16-byte boundary: four wide loads, or one by one where the tensor's edge cuts it off
+__device__ __forceinline__ void load32(const __nv_bfloat16* p, int n, uint4* raw) {
+    if (n >= 32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) raw[j] = ld_nc_v4(p + 8 * j);
     } else {
@@ -160,11 +160,70 @@ __device__ __forceinline__ float bf16_at(const uint4* raw, int j) {   // j is a 
     const uint32_t w = (j / 2) % 4 == 0 ? v.x : (j / 2) % 4 == 1 ? v.y : (j / 2) % 4 == 2 ? v.z : v.w;
     return __uint_as_float((j & 1) ? (w & 0xFFFF0000u) : (w << 16));
 }
+// Where in the warp's 2 KB the bytes [16 j, 16 j + 16) of row r of a [32 rows][64 bytes] piece lie
+__device__ __forceinline__ uint32_t in_piece(uint32_t stage, int r, int byte) {
+    return stage + (uint32_t)(r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+}
+// The pieces of rows that do not start on 16-byte boundaries, W bytes at a time (8, 4 or 2: what all of them start on): the lanes
+// cover a row side by side, so that an access is a few whole row segments. (One lane's 2 bytes at a time at a stride of 16, as a
+// row's wide blocks lie, took ten times as long: 12837 x 7860 with h kept, 888 us.) Out of line: most calls never come here.
+template <int W, typename V>
+__device__ __forceinline__ void put_narrow_of(uint32_t stage, int lane, char* out, int64_t ld_bytes, int rows, int bytes) {
+    constexpr int kLanes = 64 / W, kRows = 32 / kLanes;
+    const int byte = lane % kLanes * W;
+#pragma unroll 4
+    for (int i = 0; i < 32 / kRows; ++i) {
+        const int r = i * kRows + lane / kLanes;
+        const uint32_t at = in_piece(stage, r, byte);
+        char* o = out + r * ld_bytes + byte;
+        if (r >= rows) continue;
+        if (byte + W <= bytes) {
+            *(V*)o = *(const V*)__cvta_shared_to_generic(at);
+        } else {
+            for (int b = 0; byte + b < bytes; b += 2) *(unsigned short*)(o + b) = *(const unsigned short*)__cvta_shared_to_generic(at + b);
+        }
+    }
+}
+__device__ __noinline__ void put_narrow(uint32_t stage, int lane, void* out, int64_t ld_bytes, int rows, int bytes, int width) {
+    if (width == 8) put_narrow_of<8, uint2>(stage, lane, (char*)out, ld_bytes, rows, bytes);
+    else if (width == 4) put_narrow_of<4, uint32_t>(stage, lane, (char*)out, ld_bytes, rows, bytes);
+    else put_narrow_of<2, unsigned short>(stage, lane, (char*)out, ld_bytes, rows, bytes);
+}
+template <int W, typename V>
+__device__ __forceinline__ void get_narrow_of(uint32_t stage, int lane, const char* src, int64_t ld_bytes, int rows, int bytes) {
+    constexpr int kLanes = 64 / W, kRows = 32 / kLanes, kBatch = 8;
+    const int byte = lane % kLanes * W;
+#pragma unroll 1
+    for (int i = 0; i < 32 / kRows; i += kBatch) {
+        V v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int r = (i + k) * kRows + lane / kLanes;
+            const char* p = src + r * ld_bytes + byte;
+            v[k] = V{};
+            if (r >= rows) continue;
+            if (byte + W <= bytes) {
+                v[k] = *(const V*)p;
+            } else {
+                for (int b = 0; byte + b < bytes; b += 2) ((unsigned short*)&v[k])[b / 2] = *(const unsigned short*)(p + b);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) *(V*)__cvta_shared_to_generic(in_piece(stage, (i + k) * kRows + lane / kLanes, byte)) = v[k];
+    }
+}
+__device__ __noinline__ void get_narrow(uint32_t stage, int lane, const void* src, int64_t ld_bytes, int rows, int bytes, int width) {
+    __syncwarp();   // the reads of the piece before are done
+    if (width == 8) get_narrow_of<8, uint2>(stage, lane, (const char*)src, ld_bytes, rows, bytes);
+    else if (width == 4) get_narrow_of<4, uint32_t>(stage, lane, (const char*)src, ld_bytes, rows, bytes);
+    else get_narrow_of<2, unsigned short>(stage, lane, (const char*)src, ld_bytes, rows, bytes);
+    __syncwarp();
+}
 // A warp's [32 rows][32 columns] of bf16 results, one row per lane, through the warp's 2 KB of shared memory so that every
 // store instruction writes 8 whole 64-byte row segments instead of 16 bytes in each of 32 rows. The 16-byte blocks of a row
 // are XOR-swizzled by (row / 2) % 4: neither side has bank conflicts.
 __device__ __forceinline__ void store_piece(uint32_t stage, int lane, const float* f, __nv_bfloat16* out, int64_t ldo, int row0, int col0, int M,
-                                            int N, bool vec) {
+                                            int N, int width) {
     uint4 raw[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -178,12 +237,16 @@ __device__ __forceinline__ void store_piece(uint32_t stage, int lane, const floa
 #pragma unroll
     for (int j = 0; j < 4; ++j) st_smem_v4(mine + (uint32_t)((j ^ sw) << 4), raw[j]);
     __syncwarp();
+    if (width != 16) {
+        put_narrow(stage, lane, out + (int64_t)row0 * ldo + col0, ldo * 2, min(32, M - row0), 2 * min(32, N - col0), width);
+        return;
+    }
     const int cb = lane & 3, r0 = lane >> 2, col = col0 + cb * 8;
     uint4 d[4];   // rows r0 + 8 i
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[i] = ld_smem_v4(stage + (uint32_t)(i * 512 + r0 * 64 + ((cb ^ ((r0 >> 1) & 3)) << 4)));
     __nv_bfloat16* op = out + (int64_t)(row0 + r0) * ldo + col;
-    if (vec && col + 8 <= N) {
+    if (col + 8 <= N) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (row0 + r0 + 8 * i < M) *(uint4*)(op + 8 * i * ldo) = d[i];
@@ -387,17 +450,24 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             uint32_t ex = 0;
             const __nv_bfloat16* aux_row = DGRAD ? p.pre : p.res;
             const int64_t aux_ld = DGRAD ? p.ldpre : p.ldres;
-            const bool aux_vec = DGRAD ? p.pre_vec != 0 : p.aux_vec != 0;
+            const int aux_width = DGRAD ? p.pre_width : p.aux_width;
             const bool kept8 = DGRAD && p.q != nullptr;
             auto fetch = [&](int c) {
                 const int col = colw + c * 32;
-                if (!live || c >= kPieces || col >= p.N) return;
+                if (c >= kPieces || col >= p.N) return;   // warp-uniform
+                if (!kept8 && aux_row != nullptr && aux_width != 16) {
+                    get_narrow(stage, lane, aux_row + (int64_t)row0 * aux_ld + col, aux_ld * 2, min(32, p.M - row0), 2 * min(32, p.N - col), aux_width);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) coming[j] = ld_smem_v4(in_piece(stage, lane, j * 16));
+                    return;
+                }
+                if (!live) return;
                 if (kept8) {
                     const int8_t* qp = p.q + (int64_t)row * p.ldq + col;
                     coming[0] = ld_nc_v4(qp);
                     if (col + 16 < p.N) coming[1] = ld_nc_v4(qp + 16);
                 } else if (aux_row != nullptr) {
-                    load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, aux_vec, coming);
+                    load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, coming);
                 }
             };
 #pragma unroll
@@ -436,7 +506,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                         f[j] += __uint_as_float(b.x); f[j + 1] += __uint_as_float(b.y);
                         f[j + 2] += __uint_as_float(b.z); f[j + 3] += __uint_as_float(b.w);
                     }
-                    if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_vec != 0);
+                    if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
                     if (p.q != nullptr) ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]);
@@ -461,9 +531,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
 #pragma unroll
                         for (int j = 0; j < 32; ++j) f[j] *= act_slope<ACT>(bf16_at(aux, j), &a[j]);
                     }
-                    if (p.out2 != nullptr) store_piece(stage, lane, a, p.out2, p.ldo2, row0, col, p.M, p.N, p.out2_vec != 0);
+                    if (p.out2 != nullptr) store_piece(stage, lane, a, p.out2, p.ldo2, row0, col, p.M, p.N, p.out2_width);
                 }
-                store_piece(stage, lane, f, p.out, p.ldo, row0, col, p.M, p.N, p.out_vec != 0);
+                store_piece(stage, lane, f, p.out, p.ldo, row0, col, p.M, p.N, p.out_width);
             };
             if (row0 >= p.M) {   // nothing of this warp's 32 rows exists (few rows, or the last tile's second half)
                 release();
@@ -620,6 +690,11 @@ int launch_act(int act, LinParams& p, int k_steps, cudaStream_t s) {
     return -2;
 }
 
+// the largest of 16, 8, 4 and 2 bytes that every row of a bf16 matrix starts on
+int width_of(const void* p, int64_t ld) {
+    const uint64_t both = (uint64_t)(uintptr_t)p | (uint64_t)(ld * 2) | 16u;
+    return (int)(both & (~both + 1));
+}
 bool rows16(const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && (ld % 8) == 0; }
 
 template <bool DGRAD>
@@ -649,10 +724,10 @@ int linear_typed(const LinearArgs& a, cudaStream_t s) {
     p.ldq = a.ldq;
     p.e = (uint8_t*)a.e;
     p.lde = a.lde;
-    p.aux_vec = rows16(a.residual, a.ldres);
-    p.pre_vec = rows16(a.pre, a.ldpre);
-    p.out_vec = rows16(a.out, a.ldo);
-    p.out2_vec = rows16(a.out2, a.ldo2);
+    p.aux_width = width_of(a.residual, a.ldres);
+    p.pre_width = width_of(a.pre, a.ldpre);
+    p.out_width = width_of(a.out, a.ldo);
+    p.out2_width = width_of(a.out2, a.ldo2);
     p.arrived = (unsigned*)a.workspace;
     p.partial = a.workspace == nullptr ? nullptr : (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
     p.err_flag = a.err_flag;

@@ -835,6 +835,35 @@ act8_unpack_kernel(const int8_t* __restrict__ q, int64_t ldq, const uint8_t* __r
     }
 }
 
+// ---- bf16 rows onto 16-byte boundaries, which is what loads by tensor map ask for ------------------------------------------
+// A thread writes one block of 16 bytes: the two aligned blocks of the source row that hold its values (the second is the
+// neighbour's first, and comes from L1), shifted by what the row starts past a boundary. A block that is read holds a value of the row.
+__global__ void __launch_bounds__(256)
+pad_rows_kernel(const __nv_bfloat16* __restrict__ src, int64_t ld, __nv_bfloat16* __restrict__ dst, int64_t ldp, int64_t total, int64_t cols, uint32_t per_row) {
+    allow_successor();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int64_t row = total <= 0xFFFFFFFFll ? (int64_t)((uint32_t)i / per_row) : i / per_row;
+    const int64_t j = i - row * per_row;
+    const uintptr_t start = (uintptr_t)(src + row * ld), past = start & 15, end = start + 2 * cols;
+    const uintptr_t block = start - past + 16 * j;
+    const uint4 a = *(const uint4*)block;
+    uint4 b = make_uint4(0, 0, 0, 0);
+    if (past != 0 && block + 16 < end) b = *(const uint4*)(block + 16);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (past & 8) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+    }
+    if (past & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+    }
+    const uint32_t shift = (uint32_t)(past & 2) * 8;
+    *(uint4*)(dst + row * ldp + 8 * j) = make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
+                                                    __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------
 int pow2_at_least(int64_t v, int lo, int hi) {
     int p = lo;
@@ -1134,6 +1163,15 @@ int column_sum(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols
     if (dtype == 0) return column_sum_typed<__nv_bfloat16>((const __nv_bfloat16*)x, ldx, rows, cols, out, accumulate, partial, s);
     if (dtype == 1) return column_sum_typed<float>((const float*)x, ldx, rows, cols, out, accumulate, partial, s);
     return -2;
+}
+
+int pad_rows(const void* src, int64_t ld, void* dst, int64_t ldp, int64_t rows, int64_t cols, void* stream) {
+    if (rows <= 0 || cols <= 0) return 0;
+    const int64_t per_row = (cols + 7) / 8, total = rows * per_row;
+    if ((uintptr_t)dst % 16 || ldp % 8 || ldp < per_row * 8 || (uintptr_t)src % 2 || per_row > 0x7FFFFFFF || (total + 255) / 256 > 0x7FFFFFFF) return -2;
+    pad_rows_kernel<<<(unsigned)((total + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)src, ld, (__nv_bfloat16*)dst, ldp, total,
+                                                                                     cols, (uint32_t)per_row);
+    return (int)cudaGetLastError();
 }
 
 }  // namespace psb

@@ -32,4 +32,7 @@ int column_sum(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols
                void* stream);
 int64_t column_sum_scratch(int64_t rows, int64_t cols);
 
+// bf16 rows to rows on 16-byte boundaries (dst, ldp a multiple of 8 elements and at least cols rounded up to 8)
+int pad_rows(const void* src, int64_t ld, void* dst, int64_t ldp, int64_t rows, int64_t cols, void* stream);
+
 }  // namespace psb

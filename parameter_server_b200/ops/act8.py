@@ -56,9 +56,10 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def operand(t: torch.Tensor, what: str, device: int) -> Tuple[torch.Tensor, int, int]:
-    """A bf16 operand of the tensor cores as ``(matrix, address, elements between rows)``: rows on 16-byte boundaries. Rows that are
-    not, or that are all the same one, are copied once, into rows padded to 8 elements (what a bulk-tensor load asks for)."""
+def operand(t: torch.Tensor, what: str, device: int):
+    """A bf16 operand of the tensor cores as ``(matrix, address, elements between rows, copy)``: rows on 16-byte boundaries. Rows that
+    are not, or that are all the same one, are copied once, into rows padded to 8 elements (what a bulk-tensor load asks for); the
+    address is the copy's then, which the caller holds until its launch."""
     if t.dtype is not torch.bfloat16 or t.get_device() != device:
         raise ValueError(f"{what}: expected bf16 on cuda:{device}, got {t.dtype} on {t.device}")
     t = rows2d(t, what)
@@ -67,12 +68,23 @@ def operand(t: torch.Tensor, what: str, device: int) -> Tuple[torch.Tensor, int,
     if at % 16 == 0:
         ld = t.stride(0)
         if rows <= 1:
-            return t, at, -(-cols // 8) * 8   # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
+            return t, at, -(-cols // 8) * 8, None   # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
         if ld % 8 == 0 and ld > 0:
-            return t, at, ld
-    padded = t.new_empty((rows, -(-cols // 8) * 8))[:, :cols]
-    padded.copy_(t)
-    return padded, padded.data_ptr(), -(-cols // 8) * 8
+            return t, at, ld, None
+    ld = -(-cols // 8) * 8
+    padded = t.new_empty((rows, ld))
+    to = padded.data_ptr()
+    check(C.pad_rows(at, t.stride(0), to, ld, rows, cols, _raw_stream(device)), what)
+    return t, to, ld, padded
+
+
+def result(like: torch.Tensor, rows: int, cols: int) -> Tuple[torch.Tensor, int]:
+    """An empty bf16 matrix and the elements between its rows: rows start on 16-byte boundaries, so that the tensor cores' next
+    operator takes it as it is (``cols`` that are no multiple of 8 give a view of padded rows)."""
+    if cols % 8 == 0:
+        return like.new_empty((rows, cols)), cols
+    ld = -(-cols // 8) * 8
+    return like.new_empty((rows, ld)).narrow(1, 0, cols), ld
 
 
 def vector(t: torch.Tensor, n: int, dtypes, device: int, what: str) -> int:
@@ -193,7 +205,7 @@ def act8_wgrad(dy: torch.Tensor, x8: Act8, *, weight: Optional[torch.Tensor] = N
     the layer's bias gradient, ``linear.linear_bias_grad``). ``out`` is written, or added to with ``accumulate``."""
     what = "act8_wgrad"
     s, dev = launch_stream(dy), dy.get_device()
-    dy2, dyp, lddy = operand(dy, "act8_wgrad dy", dev)
+    dy2, dyp, lddy, _held = operand(dy, "act8_wgrad dy", dev)
     tokens, n = dy2.shape
     k = x8.cols
     if x8.rows != tokens or x8.device_index != dev:

@@ -15,7 +15,7 @@ from typing import Optional, Union
 import torch
 
 from .._lib import C
-from .act8 import _DTYPES, NEEDS_WORKSPACE, Act8, check, launch_stream, operand, row_stride, rows2d, vector
+from .act8 import _DTYPES, NEEDS_WORKSPACE, Act8, check, launch_stream, operand, result, row_stride, rows2d, vector
 from .gemm import err_ptr, workspace
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -50,14 +50,15 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     ``residual`` ``[..., N]`` (bf16). ``act``: "none", "relu", "gelu", "gelu_tanh" or "silu".
 
     ``save`` = "bf16" or "act8" also returns ``h = x w^T + bias`` as :func:`linear_act_dgrad` takes it: ``(y, h)`` with ``h`` a bf16
-    tensor like ``y``, or an :class:`~.act8.Act8`. ``out`` (bf16, may be ``residual`` itself) receives ``y``."""
+    tensor like ``y``, or an :class:`~.act8.Act8`. ``out`` (bf16, may be ``residual`` itself) receives ``y``. Results whose ``N`` is no
+    multiple of 8 have padded rows (``stride(-2)``), as the next product wants them."""
     what = "linear_act"
     code = _act_code(act, what)
     if save not in (None, "bf16", "act8"):
         raise ValueError(f"{what}: save is None, 'bf16' or 'act8', not {save!r}")
     s, dev = launch_stream(x), x.get_device()
-    x2, xp, ldx = operand(x, "linear_act x", dev)
-    w, wp, ldw = operand(w, "linear_act w", dev)
+    x2, xp, ldx, _held = operand(x, "linear_act x", dev)
+    w, wp, ldw, _held_w = operand(w, "linear_act w", dev)
     M, K = x2.shape
     N = w.shape[0]
     if w.shape[1] != K:
@@ -71,18 +72,19 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
         _like(residual, shape, dev, "linear_act: residual")
         r2 = rows2d(residual, what)
     if out is None:
-        y = x2.new_empty((M, N))
+        y, ldy = result(x2, M, N)
     else:
         _like(out, shape, dev, "linear_act: out")
         y = out if out.dim() == 2 else out.view(M, N)
         if N > 1 and y.stride(1) != 1:
             raise ValueError(f"{what}: the values of a row of out must be contiguous")
-    pre = torch.empty_like(y) if save == "bf16" and out is None else x2.new_empty((M, N)) if save == "bf16" else None
+        ldy = row_stride(y)
+    pre, ldpre = result(x2, M, N) if save == "bf16" else (None, 0)
     kept = Act8.for_rows(y, N) if save == "act8" else None
     if M and N:
         _run(dev, s, what, (False, code, M, N, K, xp, ldx, wp, ldw, bp, bias is not None and bias.dtype is torch.float32),
-             (0 if r2 is None else r2.data_ptr(), 0 if r2 is None else row_stride(r2), y.data_ptr(), N if out is None else row_stride(y), 0, N,
-              0 if pre is None else pre.data_ptr(), N, *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
+             (0 if r2 is None else r2.data_ptr(), 0 if r2 is None else row_stride(r2), y.data_ptr(), ldy, 0, 0,
+              0 if pre is None else pre.data_ptr(), ldpre, *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
     if out is not None:
         y = out
     elif x.dim() != 2:
@@ -100,8 +102,8 @@ def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, A
     what = "linear_act_dgrad"
     code = _act_code(act, what)
     s, dev = launch_stream(dy), dy.get_device()
-    dy2, dyp, lddy = operand(dy, "linear_act_dgrad dy", dev)
-    w, wp, ldw = operand(w, "linear_act_dgrad w", dev)
+    dy2, dyp, lddy, _held = operand(dy, "linear_act_dgrad dy", dev)
+    w, wp, ldw, _held_w = operand(w, "linear_act_dgrad w", dev)
     M, K = dy2.shape
     N = w.shape[1]
     if w.shape[0] != K:
@@ -118,11 +120,11 @@ def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, A
         pre = rows2d(h, what)
     elif code != 0 or recompute:
         raise ValueError(f"{what}: h is needed")
-    dh = dy2.new_empty((M, N))
-    a = torch.empty_like(dh) if recompute else None
+    dh, ld = result(dy2, M, N)
+    a = result(dy2, M, N)[0] if recompute else None
     if M and N:
         _run(dev, s, what, (True, code, M, N, K, dyp, lddy, wp, ldw, 0, False),
-             (0, 0, dh.data_ptr(), N, 0 if a is None else a.data_ptr(), N, 0 if pre is None else pre.data_ptr(), 0 if pre is None else row_stride(pre),
+             (0, 0, dh.data_ptr(), ld, 0 if a is None else a.data_ptr(), ld, 0 if pre is None else pre.data_ptr(), 0 if pre is None else row_stride(pre),
               *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
     if dy.dim() != 2:
         shape = dy.shape[:-1] + (N,)

@@ -7,6 +7,7 @@ import math
 
 import pytest
 import torch
+import torch.nn.functional as F
 
 from parameter_server_b200._lib import C
 from parameter_server_b200.ops import act8, linear, norm
@@ -614,4 +615,41 @@ def test_rows_that_are_all_the_same_one():
     assert torch.equal(linear.linear_bias_grad(dy.expand(5, 40)), linear.linear_bias_grad(dy.expand(5, 40).contiguous()))
     got, want = (norm.layer_norm(v, one[0], one[0]) for v in (full, full.contiguous()))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    G.check_gemm_errors()
+
+
+@pytest.mark.parametrize("M,N,K", [(4200, 1100, 136), (4200, 1098, 72), (4200, 1101, 72), (70, 44, 40), (70, 42, 40), (300, 41, 40)])
+def test_linear_results_and_neighbours_on_any_boundary(M, N, K):
+    """Residual, result, kept value and its gradient in matrices whose rows start on multiples of 8, 4 and 2 bytes: bit for bit what
+    aligned ones give, and nothing written beside them."""
+    x, w, b, res = rand(M, K), rand(N, K, seed=1), rand(N, seed=2), rand(M, N, seed=3)
+    wide = lambda t: F.pad(t, (0, -N % 8))[:, :N]  # noqa: E731
+    y, h = linear.linear_act(x, w, b, act="silu", residual=wide(res), save="bf16")
+    assert y.stride(0) % 8 == 0 and h.stride(0) % 8 == 0
+    room = torch.full((M * N + 16,), 7.0, dtype=BF, device="cuda")
+    out = room[8:8 + M * N].view(M, N)
+    assert torch.equal(linear.linear_act(x, w, b, act="silu", residual=res.contiguous(), out=out), y)
+    assert (room[:8] == 7).all() and (room[8 + M * N:] == 7).all()
+    cols = torch.full((M, N + 3), 7.0, dtype=BF, device="cuda")
+    linear.linear_act(x, w, b, act="silu", residual=res, out=cols[:, 1:N + 1])
+    assert torch.equal(cols[:, 1:N + 1], y) and (cols[:, 0] == 7).all() and (cols[:, N + 1:] == 7).all()
+    near(linear.linear_act(x, w), x.double() @ w.double().t(), sum_slack(x.double(), w.double().t()))
+    dy, w2 = rand(M, K, seed=4), rand(K, N, seed=5)
+    one = linear.linear_act_dgrad(dy, w2, h, act="gelu", recompute=True)
+    other = linear.linear_act_dgrad(dy, F.pad(w2, (0, -N % 8))[:, :N], h.contiguous(), act="gelu", recompute=True)
+    assert all(torch.equal(p, q) for p, q in zip(one, other))
+    G.check_gemm_errors()
+
+
+@pytest.mark.parametrize("T,N,K", [(50, 2100, 1030), (50, 40, 203), (700, 2049, 1029), (20000, 257, 1035)])
+def test_act8_wgrad_results_on_any_boundary(T, N, K):
+    """Rows of the gradient that start on no 16-byte boundary, written and added to: bit for bit the aligned result."""
+    dy, x8 = rand(T, N), act8.act8_pack(rand(T, K, seed=1))
+    wide = torch.zeros(N, -(-K // 4) * 4, device="cuda")
+    want = act8.act8_wgrad(dy, x8, out=wide[:, :K]).clone()
+    room = torch.full((N * K + 8,), 7.0, device="cuda")
+    got = act8.act8_wgrad(dy, x8, out=room[4:4 + N * K].view(N, K))
+    assert torch.equal(got, want) and (room[:4] == 7).all() and (room[4 + N * K:] == 7).all()
+    act8.act8_wgrad(dy, x8, out=wide[:, :K], accumulate=True)
+    assert torch.equal(act8.act8_wgrad(dy, x8, out=got, accumulate=True), wide[:, :K])
     G.check_gemm_errors()
