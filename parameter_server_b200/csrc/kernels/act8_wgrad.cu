@@ -60,7 +60,7 @@ struct WgParams {
     int a_blocked, b_blocked;
     float* out;
     int64_t ldo;
-    int accumulate, out_vec;
+    int accumulate;
     const __nv_bfloat16* weight;
     const __nv_bfloat16* bias;
     const float* dy_sum;
@@ -103,27 +103,8 @@ __device__ __forceinline__ void sts_converted(uint32_t addr, uint32_t w0, uint32
                  : "memory");
 }
 
-// A piece of [32 rows][16 floats] whose rows do not start on 16-byte boundaries: the lanes cover two rows side by side.
-__device__ __noinline__ void put_floats(uint32_t stage, int lane, float* out, int64_t ldo, int rows, int cols, int accumulate) {
-    const int c = lane & 15;
-    if (c >= cols) return;
-    float* o = out + (lane >> 4) * ldo + c;
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(in_piece(stage, i * 2 + (lane >> 4), c * 4)) : "memory");
-    if (accumulate) {
-        float old[16];   // all on their way before the first is needed
-#pragma unroll
-        for (int i = 0; i < 16; ++i) old[i] = i * 2 + (lane >> 4) < rows ? o[i * 2 * ldo] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += old[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i * 2 + (lane >> 4) < rows) o[i * 2 * ldo] = v[i];
-}
-
-template <bool CONVERT>
+// WIDE: rows of dw start on 16-byte boundaries (a kernel of its own: the epilogue is long, and bound by instruction fetch)
+template <bool CONVERT, bool WIDE>
 __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_constant__ WgParams p) {
     using L = WgSmem<CONVERT>;
     extern __shared__ uint8_t smem_raw[];
@@ -374,6 +355,41 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         uint32_t tc = 0;
         bool ok = true;
         while (ok && walk.next(p.grid, t)) {
+            const int row0 = t.m * 2 * BM + cr * BM + quarter * 32, colw = t.n * kWgBN + half * 128;
+            // Chunk c of this lane's part of the gradient that is added to: four blocks of 16 bytes, or, where rows do not start on
+            // 16-byte boundaries, sixteen values, so that the lanes cover two rows side by side. One chunk is always on its way.
+            // (50 tokens, 4096 x 4096: 39 us, loaded when needed, between the stores: 57; 3336 x 2574, on no boundary: 32, 96.)
+            float old[16];
+            auto request_old = [&](int c) {
+                const int col0 = colw + c * 16;
+                if (!p.accumulate || c >= 8 || col0 >= p.K) return;   // warp-uniform
+                if constexpr (WIDE) {
+                    const int col = col0 + (lane & 3) * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = i * 8 + (lane >> 2);
+                        const float* o = p.out + (int64_t)(row0 + r) * p.ldo + col;
+                        if (row0 + r >= p.N) continue;
+                        if (col + 4 <= p.K) {
+                            const float4 x = *(const float4*)o;
+                            old[4 * i] = x.x; old[4 * i + 1] = x.y; old[4 * i + 2] = x.z; old[4 * i + 3] = x.w;
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (col + k < p.K) old[4 * i + k] = o[k];
+                        }
+                    }
+                } else {
+                    const float* o = p.out + (int64_t)(row0 + (lane >> 4)) * p.ldo + col0 + (lane & 15);
+                    const int left = col0 + (lane & 15) < p.K ? p.N - row0 - (lane >> 4) : 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (2 * i < left) old[i] = o[2 * i * p.ldo];
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 16; ++i) old[i] = 0.f;
+            if (t.runs == 1) request_old(0);
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.f;
@@ -418,6 +434,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 if (__shfl_sync(0xFFFFFFFFu, last, 0) == 0u) continue;
                 __threadfence();
                 if (lane == 0) *count = 0u;
+                request_old(0);
 #pragma unroll
                 for (int j = 0; j < 128; ++j) acc[j] = 0.f;
 #pragma unroll 1
@@ -431,7 +448,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                     }
                 }
             }
-            const int row0 = t.m * 2 * BM + cr * BM + quarter * 32, colw = t.n * kWgBN + half * 128;
             const bool affine = p.weight != nullptr || p.bias != nullptr;
             const float sum = p.dy_sum != nullptr && row0 + lane < p.N ? p.dy_sum[row0 + lane] : 0.f;
             // 16 columns at a time through the warp's 2 KB, so that stores (and the loads of a gradient that is added to)
@@ -455,31 +471,41 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                                    make_uint4(__float_as_uint(acc[c * 16 + 4 * j]), __float_as_uint(acc[c * 16 + 4 * j + 1]),
                                               __float_as_uint(acc[c * 16 + 4 * j + 2]), __float_as_uint(acc[c * 16 + 4 * j + 3])));
                     __syncwarp();
-                    if (!p.out_vec) {
-                        put_floats(stage, lane, p.out + (int64_t)row0 * p.ldo + colw + c * 16, p.ldo, min(32, p.N - row0), min(16, p.K - colw - c * 16),
-                                   p.accumulate);
-                        continue;
-                    }
-                    const int cb = lane & 3, col = colw + c * 16 + cb * 4;
+                    float now[16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = i * 8 + (lane >> 2);
-                        if (row0 + r >= p.N) continue;
-                        const uint4 w = ld_smem_v4(stage + (uint32_t)(r * 64 + ((cb ^ ((r >> 1) & 3)) << 4)));
-                        float4 d = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
-                        float* op = p.out + (int64_t)(row0 + r) * p.ldo + col;
-                        if (col + 4 <= p.K) {
-                            if (p.accumulate) {
-                                const float4 o = *(const float4*)op;
-                                d.x += o.x; d.y += o.y; d.z += o.z; d.w += o.w;
+                    for (int i = 0; i < 16; ++i) now[i] = old[i];
+                    request_old(c + 1);
+                    const int col0 = colw + c * 16;
+                    if constexpr (WIDE) {
+                        const int cb = lane & 3, col = col0 + cb * 4;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = i * 8 + (lane >> 2);
+                            if (row0 + r >= p.N) continue;
+                            const uint4 w = ld_smem_v4(in_piece(stage, r, cb * 16));
+                            const float x[4] = {__uint_as_float(w.x) + now[4 * i], __uint_as_float(w.y) + now[4 * i + 1],
+                                                __uint_as_float(w.z) + now[4 * i + 2], __uint_as_float(w.w) + now[4 * i + 3]};
+                            float* op = p.out + (int64_t)(row0 + r) * p.ldo + col;
+                            if (col + 4 <= p.K) {
+                                *(float4*)op = make_float4(x[0], x[1], x[2], x[3]);
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (col + k < p.K) op[k] = x[k];
                             }
-                            *(float4*)op = d;
-                        } else {
-                            const float x[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (col + k < p.K) op[k] = p.accumulate ? op[k] + x[k] : x[k];
                         }
+                    } else {
+                        float* o = p.out + (int64_t)(row0 + (lane >> 4)) * p.ldo + col0 + (lane & 15);
+                        const int left = col0 + (lane & 15) < p.K ? p.N - row0 - (lane >> 4) : 0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float x;
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(in_piece(stage, i * 2 + (lane >> 4), (lane & 15) * 4)) : "memory");
+                            now[i] += x;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (2 * i < left) o[2 * i * p.ldo] = now[i];
                     }
                 }
             }
@@ -505,17 +531,17 @@ bool make_byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t c
                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool CONVERT>
+template <bool CONVERT, bool WIDE>
 int plan_wgrad(WgParams& p, int64_t tokens) {
     int pairs = 0;
-    cudaError_t e = pairs_of<act8_wgrad_kernel<CONVERT>>(kWgThreads, WgSmem<CONVERT>::kTotal, &pairs);
+    cudaError_t e = pairs_of<act8_wgrad_kernel<CONVERT, WIDE>>(kWgThreads, WgSmem<CONVERT>::kTotal, &pairs);
     if (e != cudaSuccess) return (int)e;
     p.grid = plan_tiles((p.N + 2 * BM - 1) / (2 * BM), (p.K + kWgBN - 1) / kWgBN, (int)((tokens + BK - 1) / BK), pairs, 48, 8);
     return p.grid.shared > 0 && p.arrived == nullptr ? kNeedsWorkspace : 0;
 }
-template <bool CONVERT>
+template <bool CONVERT, bool WIDE>
 int launch_wgrad(const WgParams& p, cudaStream_t s) {
-    constexpr auto kern = act8_wgrad_kernel<CONVERT>;
+    constexpr auto kern = act8_wgrad_kernel<CONVERT, WIDE>;
     return (int)launch_pairs(kern, kWgThreads, WgSmem<CONVERT>::kTotal, p.grid.pairs, p, s);
 }
 
@@ -576,7 +602,9 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     p.K = a.K;
     p.arrived = (unsigned*)a.workspace;
     p.partial = a.workspace == nullptr ? nullptr : (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
-    int rc = convert ? plan_wgrad<true>(p, a.tokens) : plan_wgrad<false>(p, a.tokens);
+    const bool wide = ((uintptr_t)a.out % 16) == 0 && a.ldo % 4 == 0;
+    int rc = convert ? (wide ? plan_wgrad<true, true>(p, a.tokens) : plan_wgrad<true, false>(p, a.tokens))
+                     : (wide ? plan_wgrad<false, true>(p, a.tokens) : plan_wgrad<false, false>(p, a.tokens));
     if (rc == 0 && !convert) rc = act8_unpack(0, a.x, a.scratch, ldx, a.tokens, a.K, stream);
     if (rc != 0) return rc;
     p.a_blocked = a.N % 64 == 0 && a.N >= BM ? 1 : 0;
@@ -595,13 +623,14 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
     p.out = a.out;
     p.ldo = a.ldo;
     p.accumulate = a.accumulate;
-    p.out_vec = ((uintptr_t)a.out % 16) == 0 && a.ldo % 4 == 0;
     p.weight = (const __nv_bfloat16*)a.weight;
     p.bias = (const __nv_bfloat16*)a.bias;
     p.dy_sum = a.dy_sum;
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
-    return convert ? launch_wgrad<true>(p, (cudaStream_t)stream) : launch_wgrad<false>(p, (cudaStream_t)stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (convert) return wide ? launch_wgrad<true, true>(p, st) : launch_wgrad<true, false>(p, st);
+    return wide ? launch_wgrad<false, true>(p, st) : launch_wgrad<false, false>(p, st);
 }
 
 // Converting tile by tile repeats the work for every 256 rows of dw and costs the tensor cores a fifth of their time;
