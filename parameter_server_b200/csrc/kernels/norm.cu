@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "act8.cuh"
 #include "launch.cuh"
@@ -28,7 +29,7 @@ constexpr int kBwdThreads = 512;
 constexpr int kBwdElems = 16;        // columns per thread of the backward kernel: two fp32 sums each stay in registers
 constexpr int kSms = 148;
 
-// VEC consecutive values of a row as fp32: one 16-byte access, or one element (VEC 1: rows of any alignment).
+// VEC consecutive values of a row as fp32: one 16-byte access, two bf16 (rows on 4-byte boundaries), or one element.
 template <typename T, int VEC>
 struct Io;
 template <>
@@ -61,6 +62,18 @@ struct Io<float, 4> {
     static __device__ __forceinline__ void store(float* p, const float* f) { *(float4*)p = make_float4(f[0], f[1], f[2], f[3]); }
     static __device__ __forceinline__ Raw zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
     static __device__ __forceinline__ Raw one() { return make_float4(1.f, 1.f, 1.f, 1.f); }
+};
+template <>
+struct Io<__nv_bfloat16, 2> {
+    using Raw = uint32_t;
+    static __device__ __forceinline__ Raw load(const __nv_bfloat16* p) { return *(const uint32_t*)p; }
+    static __device__ __forceinline__ void unpack(const Raw& r, float* f) {
+        f[0] = __uint_as_float(r << 16);
+        f[1] = __uint_as_float(r & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) { *(__nv_bfloat162*)p = __floats2bfloat162_rn(f[0], f[1]); }
+    static __device__ __forceinline__ Raw zero() { return 0u; }
+    static __device__ __forceinline__ Raw one() { return 0x3F803F80u; }
 };
 template <>
 struct Io<__nv_bfloat16, 1> {
@@ -114,6 +127,14 @@ struct Q8<4> {
     static __device__ __forceinline__ Raw zero() { return 0u; }
     static __device__ __forceinline__ void unpack(const Raw& r, float step, float* f) { unpack_word(r, step, f); }
     static __device__ __forceinline__ void store(int8_t* p, const float* f, uint32_t e, float inv) { *(uint32_t*)p = pack_word(f, e, inv); }
+};
+template <>
+struct Q8<2> {
+    using Raw = uint16_t;
+    static __device__ __forceinline__ Raw zero() { return 0; }
+    static __device__ __forceinline__ void store(int8_t* p, const float* f, uint32_t, float inv) {
+        *(uint16_t*)p = (uint16_t)((act8_quantise(f[0], inv) & 255) | (act8_quantise(f[1], inv) & 255) << 8);
+    }
 };
 template <>
 struct Q8<1> {
@@ -233,8 +254,8 @@ __device__ __forceinline__ void keep8(const float* f, bool valid, int8_t* qrow, 
 // With few rows a row is spread over as many threads as have a vector each, since then the latency of one row is the time.
 // CTAs are persistent, and a thread copies its part of the next two rows to shared memory while it works on this one (only
 // the thread itself reads it, so no barrier is involved): with loads straight into registers a row's arithmetic and the next
-// row's latency add up (16384 x 2048: 35 us). bf16 rows that are not 16-byte aligned (VEC 1; a copy has 4 bytes at least) are
-// read that way all the same.
+// row's latency add up (16384 x 2048: 35 us). bf16 rows on 4-byte boundaries go in pairs (10923 x 2086: 29 us, one by one 47); on
+// none (VEC 1; a copy has 4 bytes at least) they are read straight into registers all the same.
 constexpr int kFwdSlots = 3;
 template <typename T, int VEC>
 constexpr bool copies_ahead() { return VEC * sizeof(T) >= 4; }
@@ -645,8 +666,11 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restric
                 *(float4*)(out + d + i * tpr * VEC + j) = make_float4(db[c], db[c + 1], db[c + 2], db[c + 3]);
             }
         } else {
-            out[i * tpr] = dg[i];
-            out[d + i * tpr] = db[i];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                out[i * tpr * VEC + j] = dg[i * VEC + j];
+                out[d + i * tpr * VEC + j] = db[i * VEC + j];
+            }
         }
     }
 }
@@ -872,12 +896,13 @@ int pow2_at_least(int64_t v, int lo, int hi) {
 }
 template <typename T>
 constexpr int vec_of() { return 16 / (int)sizeof(T); }
-// Whether 16-byte accesses fit: every row of every tensor starts on a 16-byte boundary and holds whole vectors.
+// Whether accesses of `bytes` fit: every row of every tensor starts on such a boundary and holds whole vectors.
 template <typename T>
-bool aligned(int64_t d, std::initializer_list<std::pair<const void*, int64_t>> rows) {
-    if (d % vec_of<T>()) return false;
+bool aligned(int64_t d, std::initializer_list<std::pair<const void*, int64_t>> rows, int bytes = 16) {
+    const int vec = bytes / (int)sizeof(T);
+    if (d % vec) return false;
     for (const auto& r : rows)
-        if (r.first != nullptr && (((uintptr_t)r.first % 16) || (r.second % vec_of<T>()))) return false;
+        if (r.first != nullptr && (((uintptr_t)r.first % bytes) || (r.second % vec))) return false;
     return true;
 }
 bool kept_ok(const Act8View& k) { return ((uintptr_t)k.q % 16) == 0 && (k.ldq % 16) == 0 && ((uintptr_t)k.e % 4) == 0 && (k.lde % 4) == 0; }
@@ -941,10 +966,11 @@ int launch_fwd(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ld
 template <typename T, int VEC>
 int fwd_vec(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy, float* mean, float* rstd, const Act8View& keep, int64_t rows,
             int d, float eps, cudaStream_t s) {
-    constexpr int NV = VEC == 1 ? 16 : VEC == 4 ? 8 : 4;   // 32 values (16 where they are read one by one)
+    constexpr int NV = VEC <= 2 ? 16 : VEC == 4 ? 8 : 4;   // 32 values (16 where they are read one by one)
     const int64_t vecs = (d + VEC - 1) / VEC;
-    // fewer rows than SMs x 4: one vector per thread if 512 threads have the row
-    if (rows <= 4 * kSms && vecs <= kMaxTeam)
+    // fewer rows than SMs x 4: one vector per thread if 512 threads have the row (with two values a thread the meeting of sixteen
+    // warps costs more than it saves: 300 x 1002, 5.2 us for 3.2)
+    if (rows <= 4 * kSms && vecs <= (VEC == 2 ? kMaxTeam / 2 : kMaxTeam))
         return launch_fwd<T, VEC, 1, 0>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, pow2_at_least(vecs, 32, kMaxTeam), s);
     if (vecs <= 64) return launch_fwd<T, VEC, 2, 32>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, d, eps, 32, s);
     if (vecs <= (int64_t)kMaxTeam * NV) {
@@ -972,6 +998,10 @@ int fwd_typed(const T* x, int64_t ldx, const T* w, const T* b, T* y, int64_t ldy
     constexpr int V = vec_of<T>();
     if (aligned<T>(d, {{x, ldx}, {y, ldy}, {w, 0}, {b, 0}}) && (keep.q == nullptr || kept_ok(keep)))
         return fwd_vec<T, V>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, (int)d, eps, s);
+    if constexpr (sizeof(T) == 2) {
+        if (aligned<T>(d, {{x, ldx}, {y, ldy}, {w, 0}, {b, 0}}, 4) && (keep.q == nullptr || kept_ok(keep)))
+            return fwd_vec<T, 2>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, (int)d, eps, s);
+    }
     return fwd_vec<T, 1>(x, ldx, w, b, y, ldy, mean, rstd, keep, rows, (int)d, eps, s);
 }
 
@@ -1043,8 +1073,16 @@ int bwd_typed(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View
         const bool vec = aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}) && (!SRC8 || kept_ok(k));
         constexpr bool kLoose = sizeof(T) == 2 && SRC8;   // unaligned rows otherwise: one value at a time
         if (kLoose && !kept_ok(k)) return -2;
-        rc = vec ? launch_bwd<T, vec_of<T>(), SRC8>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s)
-                 : launch_bwd<T, kLoose ? 8 : 1, SRC8, kLoose>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part, rows, (int)d, p, s);
+        const bool two = sizeof(T) == 2 && !SRC8 && aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}, 4);
+        auto go = [&](auto vec_c, auto loose_c) {
+            return launch_bwd<T, decltype(vec_c)::value, SRC8, decltype(loose_c)::value>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part,
+                                                                                        rows, (int)d, p, s);
+        };
+        using No = std::false_type;
+        constexpr int kTwo = sizeof(T) == 2 && !SRC8 ? 2 : 1;
+        rc = vec   ? go(std::integral_constant<int, vec_of<T>()>{}, No{})
+             : two ? go(std::integral_constant<int, kTwo>{}, No{})
+                   : go(std::integral_constant<int, kLoose ? 8 : 1>{}, std::bool_constant<kLoose>{});
     } else {
         if (rows > 0x7FFFFFFF) return -2;
         layer_norm_bwd_long_kernel<T, SRC8><<<(unsigned)rows, 512, 0, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde,
