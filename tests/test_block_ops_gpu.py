@@ -653,3 +653,29 @@ def test_act8_wgrad_results_on_any_boundary(T, N, K):
     act8.act8_wgrad(dy, x8, out=wide[:, :K], accumulate=True)
     assert torch.equal(act8.act8_wgrad(dy, x8, out=got, accumulate=True), wide[:, :K])
     G.check_gemm_errors()
+
+
+@pytest.mark.parametrize("rows,d", [(5, 2), (700, 34), (3000, 534), (700, 2050), (3, 4102), (2, 8190), (3000, 1003)])
+def test_layer_norm_rows_on_few_bytes(rows, d):
+    """Rows that start on multiples of 4 or 2 bytes, in pairs and one by one, with and without 8-bit rows; and the same rows inside
+    wider ones, at an offset: the result does not depend on where they lie, nothing beside it is read into it."""
+    test_layer_norm_forward(rows, d, BF)
+    for join in (False, True):
+        test_layer_norm_backward(rows, d, join, BF)
+    x, dy, g = rand(rows, d) * 3 + 1, rand(rows, d, seed=3), rand(d, seed=1)
+    y, mean, rstd = norm.layer_norm(x, g)
+    want = norm64_grads(dy, norm64(x, g, torch.zeros_like(g))[3], rstd.double(), g, None)
+    for start, room in ((1, 3), (2, 4)):
+        def inside(t):
+            w = torch.full((rows, d + room), math.nan, dtype=BF, device="cuda")
+            w[:, start:start + d] = t
+            return w[:, start:start + d]
+        xs, dys = inside(x), inside(dy)
+        ys, means, rstds = norm.layer_norm(xs, g)
+        # sums in another order: a value that lies on the edge of two bf16 may go the other way
+        assert ((ys.double() - y.double()).abs() <= 2.0 ** -7 * y.double().abs() + 2.0 ** -18).all() and torch.isfinite(means).all()
+        y8, x8, r8 = norm.layer_norm_act8(xs, g)
+        assert torch.equal(y8, ys) and torch.equal(r8, rstds)
+        for dx, dw, db in (norm.layer_norm_backward(dys, xs, g, means, rstds), norm.layer_norm_act8_backward(dys, x8, g, r8)):
+            assert all(torch.isfinite(t).all() for t in (dx, dw, db))
+            near(db, want[2], 2.0 ** -20 * dy.double().abs().sum(0))
