@@ -12,7 +12,7 @@
 //
 // CTA pairs on 256 x 256 tiles of dw as in linear_fused.cuh, both operands MN-major. Where x is converted, four more warps per
 // CTA turn the pair's half of the checkpoint tile ([64 tokens][128 columns], 8 KB) into the swizzled bf16 tile that the MMA reads:
-// per two values two byte permutes, a packed multiply-add and a conversion, 450 of the 750 cycles that a k-step takes; dy, the
+// per two values two byte permutes, a packed sum, a packed product and a conversion, 450 of the 750 cycles that a k-step takes; dy, the
 // checkpoint and the bf16 tiles have rings of their own, so that no part waits for another's space.
 // The eight epilogue warps keep the tile's sums in registers: the tensor core adds to its fp32 accumulator with truncation, which
 // loses 1e-9 of the sum per token (2e-5 at 16384, all towards zero), so a chain in TMEM ends after 512 tokens and the chains are
@@ -80,13 +80,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
         : "memory");
 }
 // Two of the bytes of `w` (unsigned, 128 more than the value; chosen by the selectors) as bf16 times the step: byte b in the
-// second byte of 0x4700bb00 is the float 32768 + b, one packed multiply-add takes off 32896 and scales, both exactly.
-__device__ __forceinline__ uint32_t convert2(uint32_t w, uint32_t s0, uint32_t s1, float step, float off) {
+// second byte of 0x4700bb00 is the float 32768 + b, a packed sum takes off 32896 and a packed product scales, both exactly. (One
+// multiply-add with -32896 steps would do, but that is infinite from a step of 2^113 on, and the format's largest is 2^122.)
+__device__ __forceinline__ uint32_t convert2(uint32_t w, uint32_t s0, uint32_t s1, float step) {
     float a, b;
     asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        "add.rn.f32x2 x, x, z;\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
         : "=f"(a), "=f"(b)
-        : "r"(__byte_perm(w, 0x47000000u, s0)), "r"(__byte_perm(w, 0x47000000u, s1)), "f"(step), "f"(off));
+        : "r"(__byte_perm(w, 0x47000000u, s0)), "r"(__byte_perm(w, 0x47000000u, s1)), "f"(step), "f"(-32896.f));
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&v;
 }
@@ -96,10 +97,10 @@ __device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
     return v;
 }
 // eight bytes (two words) as bf16 to 16 bytes of shared memory
-__device__ __forceinline__ void sts_converted(uint32_t addr, uint32_t w0, uint32_t w1, float step, float off) {
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(convert2(w0, 0x7404, 0x7414, step, off)),
-                 "r"(convert2(w0, 0x7424, 0x7434, step, off)), "r"(convert2(w1, 0x7404, 0x7414, step, off)),
-                 "r"(convert2(w1, 0x7424, 0x7434, step, off))
+__device__ __forceinline__ void sts_converted(uint32_t addr, uint32_t w0, uint32_t w1, float step) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(convert2(w0, 0x7404, 0x7414, step)),
+                 "r"(convert2(w0, 0x7424, 0x7434, step)), "r"(convert2(w1, 0x7404, 0x7414, step)),
+                 "r"(convert2(w1, 0x7424, 0x7434, step))
                  : "memory");
 }
 
@@ -327,11 +328,11 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
             const uint32_t sb = d0 + ic * L::kBBytes;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float step = __uint_as_float(e[i] << 23), off = -32896.f * step;
+                const float step = act8_step(e[i]);
                 const uint32_t w0 = raw[i].x ^ 0x80808080u, w1 = raw[i].y ^ 0x80808080u, w2 = raw[i].z ^ 0x80808080u, w3 = raw[i].w ^ 0x80808080u;
                 const uint32_t dst = sb + ((i & 1) ? other : 0u) + 32 * (i / 2) * 128;
-                sts_converted(dst + c0, w0, w1, step, off);
-                sts_converted(dst + c1, w2, w3, step, off);
+                sts_converted(dst + c0, w0, w1, step);
+                sts_converted(dst + c1, w2, w3, step);
             }
             if (more) have = mbar_try_wait(&rfull_bar[ir], pr);
             fence_async_smem();   // the MMAs read through the async proxy
