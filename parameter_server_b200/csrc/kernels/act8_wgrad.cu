@@ -639,6 +639,7 @@ int act8_wgrad(const Act8WgradArgs& a, void* stream) {
 // a cold L2 and back to back: 6144 x 2048: 369, 300 and 416, 347; 2048 x 2048: 135, 120 and 137, 126; 1024 x 2048: 86, 89 and
 // 79, 87; 512 x 2048: 61, 69 and 53, 63. On 1024 tokens 2048 x 2048: 27, 24.
 int64_t act8_wgrad_scratch(int64_t tokens, int N, int K) {
+    if (tokens <= 0 || N <= 0 || K <= 0) return 0;
     return N >= kWgUnpackN || wgrad_few(tokens, N, K) ? tokens * (((int64_t)K + 7) / 8 * 8) * 2 : 0;
 }
 

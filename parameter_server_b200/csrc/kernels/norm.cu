@@ -1099,6 +1099,7 @@ int bwd_typed(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View
 }
 
 int column_slabs(int64_t rows, int64_t cols) {
+    if (cols <= 0) return 1;
     const int64_t gx = (cols + 127) / 128;
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 63) / 64, (kSms * 8 + gx - 1) / gx));
 }
