@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         meet_named(2, 32 * (1 + kLinEpilogueWarps));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_base = *((volatile uint32_t*)tmem_slot);
+        tmem_base = tmem_address(tmem_slot);
         allow_successor();
     }
 
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                     const int s = it % L::kA;
                     // (one commit frees the stages of both operands, and they are as many: one wait covers both)
                     if (!mbar_wait(&aempty_bar[s], ((it / L::kA) & 1u) ^ 1u, limit_ns)) {
-                        atomicCAS(p.err_flag, 0u, 31u);
+                        give_up_pair(p.err_flag, 31u, tmem_slot);
                         ok = false;
                         break;
                     }
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 for (int k = 0; k < t.nk; ++k, ++it) {
                     const int s = it % L::kRaw;
                     if (!mbar_wait(&rempty_bar[s], ((it / L::kRaw) & 1u) ^ 1u, limit_ns)) {
-                        atomicCAS(p.err_flag, 0u, 36u);
+                        give_up_pair(p.err_flag, 36u, tmem_slot);
                         ok = false;
                         break;
                     }
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 for (int k = 0; ok && k < t.nk; ++tc) {
                     const uint32_t buf = tc & 1u;
                     if (!mbar_wait(&tempty_bar[buf], ((tc >> 1) & 1u) ^ 1u, limit_ns)) {
-                        atomicCAS(p.err_flag, 0u, 34u);
+                        give_up_pair(p.err_flag, 34u, tmem_slot);
                         ok = false;
                         break;
                     }
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                     uint32_t add = 0;
                     for (; k < lim; ++k, ++it) {
                         if (!have && (!mbar_wait(&afull_bar[ia], pa, limit_ns * 2) || (CONVERT && !mbar_wait(&bfull_bar[ic], pc, limit_ns * 2)))) {
-                            atomicCAS(p.err_flag, 0u, 32u);
+                            give_up_pair(p.err_flag, 32u, tmem_slot);
                             ok = false;
                             break;
                         }
@@ -288,12 +288,15 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
         const uint32_t bfull0 = mapa_cluster(smem_u32(&bfull_bar[0]), 0);
         const uint32_t other = rr != 0 ? 0u - 8192u : 8192u;   // from one column block of the converted tile to the other
         uint32_t ir = 0, pr = 0, ic = 0, pc = 1;
+        uint32_t site = 0;   // of the wait that ran out
         uint4 raw[4], nraw[4];
         uint32_t e[4], ne[4];
         bool have = false;
         auto load = [&](uint32_t eb) -> bool {
-            if (!have && !mbar_wait(&rfull_bar[ir], pr, limit_ns * 2)) {
-                atomicCAS(p.err_flag, 0u, 35u);
+            // (The warp's lanes decide together: one that left alone would be missed at the next __syncwarp. Asked once more after a
+            // wait only: with one vote for both, 16384 tokens, 512 x 2048 take 61.1 us, so 59.8, and 58.9 if lanes could part.)
+            if (!__all_sync(0xFFFFFFFFu, have) && !__all_sync(0xFFFFFFFFu, mbar_wait(&rfull_bar[ir], pr, limit_ns * 2))) {
+                site = 35u;
                 return false;
             }
             const uint32_t sq = q0 + ir * L::kRawStage, sx = x0 + ir * L::kRawStage + eb;
@@ -321,8 +324,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 eb = ((t.n * kWgBN + cr * 128) / kAct8Block) & 15;
             }
             if (more) more = load(eb);
-            if (!room && !mbar_wait(&bempty_bar[ic], pc, limit_ns * 2)) {
-                atomicCAS(p.err_flag, 0u, 37u);
+            if (!__all_sync(0xFFFFFFFFu, room) && !__all_sync(0xFFFFFFFFu, mbar_wait(&bempty_bar[ic], pc, limit_ns * 2))) {
+                site = 37u;
                 break;
             }
             const uint32_t sb = d0 + ic * L::kBBytes;
@@ -345,6 +348,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
             }
             if (++ic == L::kB) { ic = 0; pc ^= 1u; }
         }
+        if (site != 0 && lane == 0) give_up_pair(p.err_flag, site, tmem_slot);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
                 const bool waited = ew != 0 || mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 if (!meet_all(1, 32 * kLinEpilogueWarps, waited)) {
-                    if (!waited && lane == 0) atomicCAS(p.err_flag, 0u, 33u);
+                    if (!waited && lane == 0) give_up_pair(p.err_flag, 33u, tmem_slot);
                     ok = false;
                     break;
                 }
@@ -515,6 +519,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) act8_wgrad_kernel(const __grid_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();
     if (warp == 1) {
+        if (gave_up(tmem_slot)) let_copies_land();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * kWgBN)) : "memory");
     }

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *((volatile uint32_t*)tmem_slot);
+    const uint32_t tmem = tmem_address(tmem_slot);
     wait_predecessor();
     allow_successor();
 
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             uint32_t ph = 0;
             for (int k = p.stages, s = 0; k < nk; ++k) {
                 if (!mbar_wait(&empty_bar[s], ph, p.limit_ns)) {
-                    atomicCAS(p.err_flag, 0u, 41u);
+                    give_up(p.err_flag, 41u, tmem_slot);
                     break;
                 }
                 load(k, s);
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             bool have = false;
             for (int k = 0, s = 0; k < nk; ++k) {
                 if (!have && !mbar_wait(&full_bar[s], ph, p.limit_ns * 2)) {
-                    atomicCAS(p.err_flag, 0u, 42u);
+                    give_up(p.err_flag, 42u, tmem_slot);
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     fetch(t_first);
     // ---- this CTA's sums to its shared memory: the MMAs have read all stages, and no load is in flight ----
     // (One warp asks the barrier, the others sleep at the CTA's: with all sixteen asking, a k-step's four MMAs took 735 cycles to issue.)
-    if (warp == 1 && !mbar_wait(done_bar, 0u, p.limit_ns * 4) && lane == 0) atomicCAS(p.err_flag, 0u, 43u);
+    if (warp == 1 && !mbar_wait(done_bar, 0u, p.limit_ns * 4) && lane == 0) give_up(p.err_flag, 43u, tmem_slot);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     {
@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     }
     cluster_sync_all();
     if (warp == 1) {
+        if (gave_up(tmem_slot)) let_copies_land();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)p.tmem_columns) : "memory");
     }

@@ -18,7 +18,7 @@
 // own 128 rows. Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-3 idle, 4-11 epilogue (a warp has one 32-lane quarter
 // of TMEM and half of the tile's columns; the first warpgroup's registers go to them). The accumulator is double-buffered in
 // TMEM, so the epilogue of a tile runs beside the MMAs of the next. Tiles are dealt out as tile_walk.cuh says. Every wait is
-// bounded; on a time-out the CTA records where, frees its TMEM and returns.
+// bounded; on a time-out the CTA records where, lets what it has under way land, frees its TMEM and returns.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         meet_named(2, 32 * (1 + kLinEpilogueWarps));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_base = *((volatile uint32_t*)tmem_slot);
+        tmem_base = tmem_address(tmem_slot);
         allow_successor();
     }
 
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                         const int s = it % L::kStages;
                         const int n = min(L::kSub, t.nk - k);
                         if (!mbar_wait(&empty_bar[s], ((it / L::kStages) & 1u) ^ 1u, limit_ns)) {
-                            atomicCAS(p.err_flag, 0u, 21u);
+                            give_up_pair(p.err_flag, 21u, tmem_slot);
                             ok = false;
                             break;
                         }
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 while (ok && walk.next(p.grid, t)) {
                     const uint32_t buf = tc & 1u;
                     if (!mbar_wait(&tempty_bar[buf], ((tc >> 1) & 1u) ^ 1u, limit_ns)) {
-                        atomicCAS(p.err_flag, 0u, 24u);
+                        give_up_pair(p.err_flag, 24u, tmem_slot);
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     for (int k = 0; k < t.nk; k += L::kSub) {
                         // consumers wait longer than producers, so that the wait that reports is the one at the root
                         if (!have && !mbar_wait(&full_bar[s], ph, limit_ns * 2)) {
-                            atomicCAS(p.err_flag, 0u, 22u);
+                            give_up_pair(p.err_flag, 22u, tmem_slot);
                             ok = false;
                             break;
                         }
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             const bool waited = ew != 0 || mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (!meet_all(1, 32 * kLinEpilogueWarps, waited)) {
-                if (!waited && lane == 0) atomicCAS(p.err_flag, 0u, 23u);
+                if (!waited && lane == 0) give_up_pair(p.err_flag, 23u, tmem_slot);
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -614,6 +614,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();   // until here the peer may signal this CTA's barriers or read its shared memory
     if (warp == 1) {
+        if (gave_up(tmem_slot)) let_copies_land();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * BN)) : "memory");
     }

@@ -57,6 +57,25 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
     return true;
 }
 
+// A wait that ran out, at `site`: the host reads the error word, and the CTA's word with the TMEM address, whose top bit is free, makes
+// it leave with care. (A producer may give up before the address is there, which then takes the bit away; but then the MMAs' thread,
+// which waits for what was never loaded, gives up after it. A word of its own, set to 0 in the prologue, cost the weight gradient
+// of 16384 tokens, 6144 x 2048, 2.5%: 319 -> 328 us.)
+constexpr uint32_t kGaveUp = 0x80000000u;
+__device__ __forceinline__ void give_up(unsigned* err_flag, uint32_t site, uint32_t* tmem_slot) {
+    atomicCAS(err_flag, 0u, site);
+    asm volatile("red.relaxed.cta.shared::cta.or.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kGaveUp) : "memory");
+}
+__device__ __forceinline__ bool gave_up(const uint32_t* tmem_slot) { return (*(const volatile uint32_t*)tmem_slot & kGaveUp) != 0u; }
+__device__ __forceinline__ uint32_t tmem_address(const uint32_t* tmem_slot) { return *(const volatile uint32_t*)tmem_slot & ~kGaveUp; }
+// What a CTA does then, behind its last barrier and before its TMEM and shared memory are anyone else's: loads, MMAs and their
+// arrivals may still be under way, for microseconds, and no barrier tells when the last has landed (a pair counts both CTAs' bytes on
+// one, of which some may never have been asked for). So it stays for 5 ms.
+__device__ __forceinline__ void let_copies_land() {
+    const unsigned long long t0 = gtimer();
+    for (int i = 0; i < (1 << 20) && gtimer() - t0 < 5000000ull; ++i) __nanosleep(1000);
+}
+
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -135,6 +154,12 @@ __device__ __forceinline__ uint32_t mapa_cluster(uint32_t local, uint32_t rank) 
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
     return r;
+}
+// give_up() for a pair: the other CTA's loads and barriers hang on this one's
+__device__ __forceinline__ void give_up_pair(unsigned* err_flag, uint32_t site, uint32_t* tmem_slot) {
+    atomicCAS(err_flag, 0u, site);
+    for (uint32_t r = 0; r < 2; ++r)
+        asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(mapa_cluster(smem_u32(tmem_slot), r)), "r"(kGaveUp) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
