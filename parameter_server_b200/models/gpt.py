@@ -9,8 +9,8 @@ after a push only the owner's rows are current and the first consumer gathers th
 it already multiplies the local rows. Attention itself is model code, not a parameter-server path: it uses
 ``torch.nn.functional.scaled_dot_product_attention``; layer norm and GELU are torch ops, or, with ``GPTConfig(fused=True)``,
 the block operators of this package: ``ops.norm`` for layer norm, ``ops.linear`` for linear layers with bias, GELU and residual
-in their epilogue. ``act_bits=8`` keeps what the backward pass needs of a block in 8 bits (``ops.act8``): the norms' rows, the
-hidden layer before GELU, and the attention's output.
+in their epilogue. ``act_bits=8`` keeps the norms' rows and the hidden layer before GELU in 8 bits for the backward pass
+(``ops.act8``); what attention itself keeps (q, k, v and its output, which the projection's weight gradient reads too) stays in 16.
 
 The reference ships no model code (it is a storage service); this is the dense-table consumer.
 """
@@ -28,7 +28,7 @@ import torch.nn.functional as F
 
 from .._lib import C
 from ..ops import gemm as G
-from ..ops.act8 import act8_pack, act8_wgrad
+from ..ops.act8 import act8_wgrad
 from ..ops.dense import DenseTable
 from ..ops.linear import linear_act, linear_act_dgrad, linear_bias_grad
 from ..ops.norm import layer_norm, layer_norm_act8, layer_norm_act8_backward, layer_norm_backward
@@ -46,7 +46,7 @@ class GPTConfig:
     lr: float = 3e-4
     weight_decay: float = 0.1
     fused: bool = False   # blocks on ops.norm / ops.linear instead of torch ops around the GEMM
-    act_bits: int = 16    # of what a fused block keeps for its backward pass: 16 or 8
+    act_bits: int = 16    # of what a fused block's norms and hidden layer keep for the backward pass: 16 or 8
 
     def n_params(self) -> int:
         d, f = self.d_model, self.d_ff
@@ -137,10 +137,8 @@ class _AttentionHalf(torch.autograd.Function):
             a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
             a2 = a.transpose(1, 2).reshape(-1, d)
         out = linear_act(a2.detach(), P[f"h{i}.proj.w"], P[f"h{i}.proj.b"], residual=x2)
-        ctx.model, ctx.i, ctx.norm, ctx.qkv = model, i, norm, qkv
-        # the graph keeps attention's own output; the copy in rows is kept as it is, or in 8 bits with its graph's end before the copy
-        ctx.attention = a
-        ctx.rows = act8_pack(a2.detach()) if cfg.act_bits == 8 else a2.detach()
+        # attention's graph keeps its output in 16 bits (laid out by rows: a2 is a view of it), so that there is nothing to gain in 8
+        ctx.model, ctx.i, ctx.norm, ctx.qkv, ctx.attention = model, i, norm, qkv, a
         return out.view(x.shape)
 
     @staticmethod
@@ -149,15 +147,13 @@ class _AttentionHalf(torch.autograd.Function):
         cfg, P, Gr = model.cfg, model.main.params, model.main.grads
         B, T, d = dy.shape
         dy2 = dy.reshape(-1, d)
-        if cfg.act_bits == 8:
-            act8_wgrad(dy2, ctx.rows, out=Gr[f"h{i}.proj.w"], accumulate=True)
-        else:
-            G.gemm(dy2, ctx.rows, a_mn=True, b_mn=True, out=Gr[f"h{i}.proj.w"], accumulate=True)
+        a2 = ctx.attention.detach().transpose(1, 2).reshape(-1, d)
+        G.gemm(dy2, a2, a_mn=True, b_mn=True, out=Gr[f"h{i}.proj.w"], accumulate=True)
         linear_bias_grad(dy2, out=Gr[f"h{i}.proj.b"], accumulate=True)
         da = linear_act_dgrad(dy2, P[f"h{i}.proj.w"], None)
         da = da.view(B, T, cfg.n_head, d // cfg.n_head).transpose(1, 2)
         (dqkv,) = torch.autograd.grad(ctx.attention, ctx.qkv, da)
-        ctx.attention = ctx.qkv = ctx.rows = None
+        ctx.attention = ctx.qkv = None
         table = model.qkv[i]
         w, wg = (P[f"h{i}.qkv.w"], Gr[f"h{i}.qkv.w"]) if table is None else (table.params["w"], table.grads["w"])
         norm.wgrad(dqkv, wg, Gr[f"h{i}.qkv.b"])
@@ -385,5 +381,5 @@ if __name__ == "__main__":
     ap.add_argument("--warmup", type=int, default=2)
     ap.add_argument("--no-fuse", action="store_true", help="all-gather the QKV weights in the dense push instead of in the GEMM")
     ap.add_argument("--fused", action="store_true", help="blocks on ops.norm / ops.linear")
-    ap.add_argument("--act-bits", type=int, default=16, choices=(16, 8), help="of what a fused block keeps for its backward pass")
+    ap.add_argument("--act-bits", type=int, default=16, choices=(16, 8), help="of what a fused block's norms and hidden layer keep for the backward pass")
     _bench(ap.parse_args())
