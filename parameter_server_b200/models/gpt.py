@@ -25,10 +25,11 @@ from typing import Dict, List, Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .._lib import C
 from ..ops import gemm as G
-from ..ops.act8 import act8_wgrad
+from ..ops.act8 import Act8, act8_wgrad
 from ..ops.dense import DenseTable
 from ..ops.linear import linear_act, linear_act_dgrad, linear_bias_grad
 from ..ops.norm import layer_norm, layer_norm_act8, layer_norm_act8_backward, layer_norm_backward
@@ -83,83 +84,95 @@ class _PSLinear(torch.autograd.Function):
 
 
 class _Norm:
-    """A layer norm of a fused model between its two passes: what it kept, and its gradients' places in the dense table."""
+    """A layer norm of a fused model: its parameters, their gradients' places in the dense table, and its two passes. What lies between
+    these (``kept``) is autograd's to save."""
 
-    def __init__(self, model: "GPT", name: str, x: torch.Tensor):
-        self.P, self.G, self.name = model.main.params, model.main.grads, name
-        self.g, self.b = self.P[f"{name}.g"].detach(), self.P[f"{name}.b"].detach()
+    def __init__(self, model: "GPT", name: str):
+        P, Gr = model.main.params, model.main.grads
+        self.g, self.b = P[f"{name}.g"].detach(), P[f"{name}.b"].detach()
+        self.g_grad, self.b_grad = Gr[f"{name}.g"], Gr[f"{name}.b"]
         self.bits = model.cfg.act_bits
-        if self.bits == 8:
-            self.y, self.xhat8, self.rstd = layer_norm_act8(x, self.g, self.b)
-        else:
-            self.y, self.mean, self.rstd = layer_norm(x, self.g, self.b)
-            self.x = x
 
-    def backward(self, dy: torch.Tensor, residual_grad: Optional[torch.Tensor] = None) -> torch.Tensor:
-        kw = dict(residual_grad=residual_grad, weight_grad=self.G[f"{self.name}.g"], bias_grad=self.G[f"{self.name}.b"], accumulate=True)
+    def forward(self, x: torch.Tensor):
+        """(y, kept)"""
         if self.bits == 8:
-            return layer_norm_act8_backward(dy, self.xhat8, self.g, self.rstd, **kw)[0]
-        return layer_norm_backward(dy, self.x, self.g, self.mean, self.rstd, **kw)[0]
+            y, xhat8, rstd = layer_norm_act8(x, self.g, self.b)
+            return y, (self.g, self.b, xhat8.q, xhat8.e, rstd)
+        y, mean, rstd = layer_norm(x, self.g, self.b)
+        return y, (self.g, self.b, x, mean, rstd, y)
 
-    def wgrad(self, dy: torch.Tensor, w_grad: torch.Tensor, b_grad: torch.Tensor) -> None:
+    def backward(self, kept, dy: torch.Tensor, residual_grad: Optional[torch.Tensor] = None) -> torch.Tensor:
+        kw = dict(residual_grad=residual_grad, weight_grad=self.g_grad, bias_grad=self.b_grad, accumulate=True)
+        if self.bits == 8:
+            g, _, q, e, rstd = kept
+            return layer_norm_act8_backward(dy, Act8(q, e, g.numel()), g, rstd, **kw)[0]
+        g, _, x, mean, rstd, _ = kept
+        return layer_norm_backward(dy, x, g, mean, rstd, **kw)[0]
+
+    def wgrad(self, kept, dy: torch.Tensor, w_grad: torch.Tensor, b_grad: torch.Tensor) -> None:
         """Gradients of the linear layer that took ``y``."""
         if self.bits == 8:
+            g, b, q, e, _ = kept
             db = linear_bias_grad(dy)
-            act8_wgrad(dy, self.xhat8, weight=self.g, bias=self.b, dy_sum=db, out=w_grad, accumulate=True)
+            act8_wgrad(dy, Act8(q, e, g.numel()), weight=g, bias=b, dy_sum=db, out=w_grad, accumulate=True)
             b_grad.add_(db)
         else:
-            G.gemm(dy, self.y, a_mn=True, b_mn=True, out=w_grad, accumulate=True)
+            G.gemm(dy, kept[-1], a_mn=True, b_mn=True, out=w_grad, accumulate=True)
             linear_bias_grad(dy, out=b_grad, accumulate=True)
 
-    def drop_y(self) -> None:
-        """The linear layer has run; only a 16-bit model needs ``y`` again."""
-        if self.bits == 8:
-            self.y = None
 
-
-class _AttentionHalf(torch.autograd.Function):
-    """x + proj(attention(qkv(norm(x)))) of a fused block. Gradients of its parameters go to the dense tables."""
+class _NormedQkv(torch.autograd.Function):
+    """(qkv(norm(x)), x) of a fused block: x goes on to the residual sum through here, so that its gradient joins the norm's where that is
+    formed. Gradients of the parameters go to the dense tables."""
 
     @staticmethod
     def forward(ctx, x, model, i):
-        cfg, P = model.cfg, model.main.params
-        B, T, d = x.shape
-        x2 = x.reshape(-1, d)
-        norm = _Norm(model, f"h{i}.ln1", x2)
-        if model.qkv[i] is not None:
-            qkv = G.ag_linear(norm.y, model.qkv[i], "w", bias=P[f"h{i}.qkv.b"])
+        P, table = model.main.params, model.qkv[i]
+        ctx.norm = _Norm(model, f"h{i}.ln1")
+        y, kept = ctx.norm.forward(x.reshape(-1, x.shape[-1]))
+        if table is not None:
+            w, ctx.w_grad = table.params["w"], table.grads["w"]
+            qkv = G.ag_linear(y, table, "w", bias=P[f"h{i}.qkv.b"])
         else:
-            qkv = linear_act(norm.y, P[f"h{i}.qkv.w"], P[f"h{i}.qkv.b"])
-        norm.drop_y()
-        qkv = qkv.requires_grad_(True)
-        with torch.enable_grad():   # attention keeps its own graph, which the backward pass runs
-            q, k, v = qkv.view(B, T, 3, cfg.n_head, d // cfg.n_head).permute(2, 0, 3, 1, 4)
-            a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-            a2 = a.transpose(1, 2).reshape(-1, d)
-        out = linear_act(a2.detach(), P[f"h{i}.proj.w"], P[f"h{i}.proj.b"], residual=x2)
-        # attention's graph keeps its output in 16 bits (laid out by rows: a2 is a view of it), so that there is nothing to gain in 8
-        ctx.model, ctx.i, ctx.norm, ctx.qkv, ctx.attention = model, i, norm, qkv, a
-        return out.view(x.shape)
+            w, ctx.w_grad = P[f"h{i}.qkv.w"], model.main.grads[f"h{i}.qkv.w"]
+            qkv = linear_act(y, w, P[f"h{i}.qkv.b"])
+        ctx.b_grad = model.main.grads[f"h{i}.qkv.b"]
+        ctx.save_for_backward(w, *kept)
+        return qkv, x
 
     @staticmethod
+    @once_differentiable
+    def backward(ctx, dqkv, dx):
+        w, *kept = ctx.saved_tensors
+        dqkv = dqkv.contiguous()
+        ctx.norm.wgrad(kept, dqkv, ctx.w_grad, ctx.b_grad)
+        dx2 = ctx.norm.backward(kept, linear_act_dgrad(dqkv, w, None), residual_grad=dx.reshape(-1, dx.shape[-1]))
+        return dx2.view(dx.shape), None, None
+
+
+class _ProjResidual(torch.autograd.Function):
+    """x + proj(a) of a fused block, for attention's output ``a`` ``[B, heads, T, d / heads]``. Attention's own graph keeps ``a`` too (laid
+    out by rows: a matrix of rows is a view of it)."""
+
+    @staticmethod
+    def forward(ctx, a, x, model, i):
+        P, Gr = model.main.params, model.main.grads
+        w = P[f"h{i}.proj.w"]
+        ctx.w_grad, ctx.b_grad = Gr[f"h{i}.proj.w"], Gr[f"h{i}.proj.b"]
+        ctx.save_for_backward(w, a)
+        d = x.shape[-1]
+        return linear_act(a.transpose(1, 2).reshape(-1, d), w, P[f"h{i}.proj.b"], residual=x.reshape(-1, d)).view(x.shape)
+
+    @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        model, i, norm = ctx.model, ctx.i, ctx.norm
-        cfg, P, Gr = model.cfg, model.main.params, model.main.grads
-        B, T, d = dy.shape
-        dy2 = dy.reshape(-1, d)
-        a2 = ctx.attention.detach().transpose(1, 2).reshape(-1, d)
-        G.gemm(dy2, a2, a_mn=True, b_mn=True, out=Gr[f"h{i}.proj.w"], accumulate=True)
-        linear_bias_grad(dy2, out=Gr[f"h{i}.proj.b"], accumulate=True)
-        da = linear_act_dgrad(dy2, P[f"h{i}.proj.w"], None)
-        da = da.view(B, T, cfg.n_head, d // cfg.n_head).transpose(1, 2)
-        (dqkv,) = torch.autograd.grad(ctx.attention, ctx.qkv, da)
-        ctx.attention = ctx.qkv = None
-        table = model.qkv[i]
-        w, wg = (P[f"h{i}.qkv.w"], Gr[f"h{i}.qkv.w"]) if table is None else (table.params["w"], table.grads["w"])
-        norm.wgrad(dqkv, wg, Gr[f"h{i}.qkv.b"])
-        dx = norm.backward(linear_act_dgrad(dqkv, w, None), residual_grad=dy2)
-        ctx.norm = None
-        return dx.view(dy.shape), None, None
+        w, a = ctx.saved_tensors
+        B, heads, T, hd = a.shape
+        dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
+        G.gemm(dy2, a.transpose(1, 2).reshape(-1, heads * hd), a_mn=True, b_mn=True, out=ctx.w_grad, accumulate=True)
+        linear_bias_grad(dy2, out=ctx.b_grad, accumulate=True)
+        da = linear_act_dgrad(dy2, w, None)
+        return da.view(B, T, heads, hd).transpose(1, 2), dy, None, None
 
 
 class _MlpHalf(torch.autograd.Function):
@@ -167,43 +180,44 @@ class _MlpHalf(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, model, i):
-        P = model.main.params
+        P, Gr = model.main.params, model.main.grads
         x2 = x.reshape(-1, x.shape[-1])
-        norm = _Norm(model, f"h{i}.ln2", x2)
-        f, ctx.h = linear_act(norm.y, P[f"h{i}.fc.w"], P[f"h{i}.fc.b"], act="gelu_tanh", save="act8" if model.cfg.act_bits == 8 else "bf16")
-        norm.drop_y()
-        ctx.model, ctx.i, ctx.norm = model, i, norm
-        return linear_act(f, P[f"h{i}.out.w"], P[f"h{i}.out.b"], residual=x2).view(x.shape)
+        ctx.norm = _Norm(model, f"h{i}.ln2")
+        y, kept = ctx.norm.forward(x2)
+        w1, w2 = P[f"h{i}.fc.w"], P[f"h{i}.out.w"]
+        f, h = linear_act(y, w1, P[f"h{i}.fc.b"], act="gelu_tanh", save="act8" if model.cfg.act_bits == 8 else "bf16")
+        ctx.grads = [Gr[f"h{i}.{name}"] for name in ("fc.w", "fc.b", "out.w", "out.b")]
+        ctx.save_for_backward(w1, w2, *((h.q, h.e) if model.cfg.act_bits == 8 else (h, None)), *kept)
+        return linear_act(f, w2, P[f"h{i}.out.b"], residual=x2).view(x.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        model, i, norm = ctx.model, ctx.i, ctx.norm
-        P, Gr = model.main.params, model.main.grads
-        dy2 = dy.reshape(-1, dy.shape[-1])
-        dh, f = linear_act_dgrad(dy2, P[f"h{i}.out.w"], ctx.h, act="gelu_tanh", recompute=True)
-        ctx.h = None
-        G.gemm(dy2, f, a_mn=True, b_mn=True, out=Gr[f"h{i}.out.w"], accumulate=True)
+        w1, w2, h, e, *kept = ctx.saved_tensors
+        w1_grad, b1_grad, w2_grad, b2_grad = ctx.grads
+        dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
+        dh, f = linear_act_dgrad(dy2, w2, h if e is None else Act8(h, e, w1.shape[0]), act="gelu_tanh", recompute=True)
+        del h, e
+        G.gemm(dy2, f, a_mn=True, b_mn=True, out=w2_grad, accumulate=True)
         del f
-        linear_bias_grad(dy2, out=Gr[f"h{i}.out.b"], accumulate=True)
-        norm.wgrad(dh, Gr[f"h{i}.fc.w"], Gr[f"h{i}.fc.b"])
-        dx = norm.backward(linear_act_dgrad(dh, P[f"h{i}.fc.w"], None), residual_grad=dy2)
-        ctx.norm = None
+        linear_bias_grad(dy2, out=b2_grad, accumulate=True)
+        ctx.norm.wgrad(kept, dh, w1_grad, b1_grad)
+        dx = ctx.norm.backward(kept, linear_act_dgrad(dh, w1, None), residual_grad=dy2)
         return dx.view(dy.shape), None, None
 
 
 class _FinalNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, model):
-        ctx.norm = _Norm(model, "lnf", x.reshape(-1, x.shape[-1]))
-        y = ctx.norm.y.view(x.shape)
-        ctx.norm.drop_y()
-        return y
+        ctx.norm = _Norm(model, "lnf")
+        y, kept = ctx.norm.forward(x.reshape(-1, x.shape[-1]))
+        ctx.save_for_backward(*kept)
+        return y.view(x.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        dx = ctx.norm.backward(dy.reshape(-1, dy.shape[-1]))
-        ctx.norm = None
-        return dx.view(dy.shape), None
+        return ctx.norm.backward(ctx.saved_tensors, dy.reshape(-1, dy.shape[-1])).view(dy.shape), None
 
 
 class GPT:
@@ -266,12 +280,15 @@ class GPT:
         x = F.embedding(tokens, lv["wte"]) + lv["wpe"][:T]
         for i in range(cfg.n_layer):
             if cfg.fused:
-                x = _MlpHalf.apply(_AttentionHalf.apply(x, self, i), self, i)
-                continue
-            h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln1.g"], lv[f"h{i}.ln1.b"])
-            qkv = self._linear(h, f"h{i}.qkv.w", f"h{i}.qkv.b", self.qkv[i])
+                qkv, x = _NormedQkv.apply(x, self, i)
+            else:
+                h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln1.g"], lv[f"h{i}.ln1.b"])
+                qkv = self._linear(h, f"h{i}.qkv.w", f"h{i}.qkv.b", self.qkv[i])
             q, k, v = qkv.view(B, T, 3, cfg.n_head, cfg.d_model // cfg.n_head).permute(2, 0, 3, 1, 4)
             a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+            if cfg.fused:
+                x = _MlpHalf.apply(_ProjResidual.apply(a, x, self, i), self, i)
+                continue
             a = a.transpose(1, 2).reshape(B, T, cfg.d_model)
             x = x + self._linear(a, f"h{i}.proj.w", f"h{i}.proj.b")
             h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln2.g"], lv[f"h{i}.ln2.b"])
