@@ -93,8 +93,10 @@ class _Norm:
         self.g_grad, self.b_grad = Gr[f"{name}.g"], Gr[f"{name}.b"]
         self.bits = model.cfg.act_bits
 
-    def forward(self, x: torch.Tensor):
-        """(y, kept)"""
+    def forward(self, x: torch.Tensor, keep: bool):
+        """(y, kept); nothing is kept where no backward pass can follow."""
+        if not keep:
+            return layer_norm(x, self.g, self.b)[0], ()
         if self.bits == 8:
             y, xhat8, rstd = layer_norm_act8(x, self.g, self.b)
             return y, (self.g, self.b, xhat8.q, xhat8.e, rstd)
@@ -129,7 +131,7 @@ class _NormedQkv(torch.autograd.Function):
     def forward(ctx, x, model, i):
         P, table = model.main.params, model.qkv[i]
         ctx.norm = _Norm(model, f"h{i}.ln1")
-        y, kept = ctx.norm.forward(x.reshape(-1, x.shape[-1]))
+        y, kept = ctx.norm.forward(x.reshape(-1, x.shape[-1]), ctx.needs_input_grad[0])
         if table is not None:
             w, ctx.w_grad = table.params["w"], table.grads["w"]
             qkv = G.ag_linear(y, table, "w", bias=P[f"h{i}.qkv.b"])
@@ -183,11 +185,15 @@ class _MlpHalf(torch.autograd.Function):
         P, Gr = model.main.params, model.main.grads
         x2 = x.reshape(-1, x.shape[-1])
         ctx.norm = _Norm(model, f"h{i}.ln2")
-        y, kept = ctx.norm.forward(x2)
+        keep = ctx.needs_input_grad[0]
+        y, kept = ctx.norm.forward(x2, keep)
         w1, w2 = P[f"h{i}.fc.w"], P[f"h{i}.out.w"]
-        f, h = linear_act(y, w1, P[f"h{i}.fc.b"], act="gelu_tanh", save="act8" if model.cfg.act_bits == 8 else "bf16")
-        ctx.grads = [Gr[f"h{i}.{name}"] for name in ("fc.w", "fc.b", "out.w", "out.b")]
-        ctx.save_for_backward(w1, w2, *((h.q, h.e) if model.cfg.act_bits == 8 else (h, None)), *kept)
+        if not keep:
+            f = linear_act(y, w1, P[f"h{i}.fc.b"], act="gelu_tanh")
+        else:
+            f, h = linear_act(y, w1, P[f"h{i}.fc.b"], act="gelu_tanh", save="act8" if ctx.norm.bits == 8 else "bf16")
+            ctx.grads = [Gr[f"h{i}.{name}"] for name in ("fc.w", "fc.b", "out.w", "out.b")]
+            ctx.save_for_backward(w1, w2, *((h.q, h.e) if ctx.norm.bits == 8 else (h, None)), *kept)
         return linear_act(f, w2, P[f"h{i}.out.b"], residual=x2).view(x.shape)
 
     @staticmethod
@@ -210,7 +216,7 @@ class _FinalNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, model):
         ctx.norm = _Norm(model, "lnf")
-        y, kept = ctx.norm.forward(x.reshape(-1, x.shape[-1]))
+        y, kept = ctx.norm.forward(x.reshape(-1, x.shape[-1]), ctx.needs_input_grad[0])
         ctx.save_for_backward(*kept)
         return y.view(x.shape)
 
@@ -273,6 +279,10 @@ class GPT:
             return _PSLinear.apply(x, ag_table.params["w"], P[bname], ag_table.grads["w"], Gd[bname], ag_table, "w")
         return _PSLinear.apply(x, P[wname], P[bname], Gd[wname], Gd[bname], None, None)
 
+    def _attention(self, qkv: torch.Tensor, B: int, T: int) -> torch.Tensor:
+        q, k, v = qkv.view(B, T, 3, self.cfg.n_head, self.cfg.d_model // self.cfg.n_head).permute(2, 0, 3, 1, 4)
+        return F.scaled_dot_product_attention(q, k, v, is_causal=True)
+
     def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None):
         cfg = self.cfg
         B, T = tokens.shape
@@ -281,14 +291,15 @@ class GPT:
         for i in range(cfg.n_layer):
             if cfg.fused:
                 qkv, x = _NormedQkv.apply(x, self, i)
-            else:
-                h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln1.g"], lv[f"h{i}.ln1.b"])
-                qkv = self._linear(h, f"h{i}.qkv.w", f"h{i}.qkv.b", self.qkv[i])
-            q, k, v = qkv.view(B, T, 3, cfg.n_head, cfg.d_model // cfg.n_head).permute(2, 0, 3, 1, 4)
-            a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-            if cfg.fused:
-                x = _MlpHalf.apply(_ProjResidual.apply(a, x, self, i), self, i)
+                a = self._attention(qkv, B, T)
+                del qkv   # (a forward pass alone holds no more than it needs)
+                x = _ProjResidual.apply(a, x, self, i)
+                del a
+                x = _MlpHalf.apply(x, self, i)
                 continue
+            h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln1.g"], lv[f"h{i}.ln1.b"])
+            qkv = self._linear(h, f"h{i}.qkv.w", f"h{i}.qkv.b", self.qkv[i])
+            a = self._attention(qkv, B, T)
             a = a.transpose(1, 2).reshape(B, T, cfg.d_model)
             x = x + self._linear(a, f"h{i}.proj.w", f"h{i}.proj.b")
             h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln2.g"], lv[f"h{i}.ln2.b"])

@@ -41,3 +41,36 @@ def test_a_layer_keeps_what_its_backward_pass_needs_once(bits):
         rest = 2 * (2 * 2 * D + 8) + 2 * HIDDEN
     per_token = (held(4, bits) - held(2, bits)) / 2 / (BATCH * SEQ)
     assert per_token <= 1.02 * (attention + rest), (per_token, attention + rest)
+
+
+def peak(layers, bits):
+    """Bytes above what was there that a forward pass asks for at most, where no backward pass can follow; and its result."""
+    model = GPT(GPTConfig(n_layer=layers, d_model=D, n_head=HEADS, d_ff=HIDDEN, vocab=512, seq_len=SEQ, fused=True, act_bits=bits), seed=1)
+    t = tokens()
+    with torch.no_grad():
+        model.forward(t)
+        before = requested()
+        torch.cuda.reset_peak_memory_stats()
+        logits, _ = model.forward(t)
+        torch.cuda.synchronize()
+    return torch.cuda.memory_stats()["requested_bytes.all.peak"] - before, logits, model.forward(t)[0].detach()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_a_forward_pass_alone_makes_no_checkpoints(bits):
+    """The most is held where the hidden layer is there beside x, the norm's output and the block's, whatever the model would keep of
+    them; and the values are those of a training pass."""
+    top, logits, training = peak(2, bits)
+    assert torch.equal(logits, training)
+    n = BATCH * SEQ
+    assert top <= 1.02 * n * (2 * HIDDEN + 3 * 2 * D + 8) + (1 << 20), (top / n, 2 * HIDDEN + 3 * 2 * D + 8)
+    assert peak(4, bits)[0] <= 1.001 * top
+
+
+def test_inference_mode_runs_a_fused_model():
+    t = tokens()
+    for bits in (16, 8):
+        model = GPT(GPTConfig(n_layer=2, d_model=D, n_head=HEADS, d_ff=HIDDEN, vocab=512, seq_len=SEQ, fused=True, act_bits=bits), seed=1)
+        want = model.forward(t)[0].detach()
+        with torch.inference_mode():
+            assert torch.equal(model.forward(t)[0], want)
