@@ -557,10 +557,11 @@ int launch_wgrad(const WgParams& p, cudaStream_t s) {
 // kernel: 1000 tokens, 512 x 512: 19.6, 10.1; 8192: 33.9, 20.2; 2048 tokens, 1024 x 1024: 26.5, 14.4; 300, 4096 x 1024: 13.0, 17.6.
 bool wgrad_few(int64_t tokens, int N, int K) {
     const int64_t k_steps = (tokens + BK - 1) / BK, small = (int64_t)((N + BM - 1) / BM) * ((K + BM - 1) / BM);
-    if (small > 4 * kMaxPairs) return false;
+    const int max_pairs = gemm_cta_limit() > 0 ? std::min(kMaxPairs, std::max(1, gemm_cta_limit() / 2)) : kMaxPairs;
+    if (small > 4 * max_pairs) return false;
     const FewPlan plan = few_plan(N, K, tokens, true);
     if (plan.cluster == 0) return false;
-    const TileGrid g = plan_tiles((N + 2 * BM - 1) / (2 * BM), (K + kWgBN - 1) / kWgBN, (int)k_steps, kMaxPairs, 48, 8);
+    const TileGrid g = plan_tiles((N + 2 * BM - 1) / (2 * BM), (K + kWgBN - 1) / kWgBN, (int)k_steps, max_pairs, 48, 8);
     const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles, whole = (tiles - g.shared + g.pairs - 1) / g.pairs;
     const float unpack = 10.f + (float)tokens * (float)K * 2.4e-6f;
     const bool converts = N < kWgUnpackN;

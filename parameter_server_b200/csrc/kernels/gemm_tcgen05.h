@@ -64,11 +64,14 @@ int gemm_bf16_grouped(const GemmOperand* A, const GemmOperand* B, const GemmEpil
                       unsigned* chain_done = nullptr);
 int gemm_chain_scratch_words();
 // Upper bound on the CTAs (= SMs) of the following launches; 0 = all SMs. A GEMM CTA fills its SM, so a smaller grid
-// leaves whole SMs to kernels of another stream that run at the same time (the sparse push beside the dense backward).
+// leaves whole SMs to kernels of another stream that run at the same time (the sparse push beside the dense backward). Holds for
+// these, for linear_fused() and for act8_wgrad(); a pair of CTAs is the least. Not for their memory passes (norms, packing, column
+// sums), which leave an SM to others as they go.
 void gemm_set_cta_limit(int ctas);
 int gemm_cta_limit();
 // CTA pairs (two CTAs of a cluster per 256-row tile) on or off for the following launches. A pair needs two free SMs
-// of one TPC at the same moment; launches that share the GPU with another kernel run better without.
+// of one TPC at the same moment; launches that share the GPU with another kernel run better without. (The GEMMs of this header:
+// linear_fused() and act8_wgrad() have no other form for large products.)
 void gemm_set_pair(int on);
 // Tracing of the following launches (nullptr = off): CTA 0 writes %globaltimer stamps for the first 8 work units it runs
 // into this device buffer of 256 x u64, 32 slots per unit (producer, MMA and epilogue milestones; unit index in slot 7). The tool behind the per-tile timelines in profiles/.

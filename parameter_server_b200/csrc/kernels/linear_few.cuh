@@ -410,7 +410,7 @@ int launch_few(FewParams& p, int cluster, cudaStream_t s) {
     cfg.stream = s;
     cudaLaunchAttribute a[2] = {in_clusters(cluster), start_early()};
     cfg.attrs = a;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = overlap_attrs(2);
     return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
@@ -418,21 +418,24 @@ int launch_few(FewParams& p, int cluster, cudaStream_t s) {
 // Fewer k-steps per CTA against the exchange of the sums: a 64th of a step per token for every doubling, and three steps more where
 // two CTAs are on an SM. There a step of 128 tokens also takes half as long again (64 KB for both), one of fewer tokens less, since
 // two CTAs wait for memory side by side. Measured, us (1, 2, 4, 8 CTAs): 16 x 8192 x 2048: 12.1, 9.7, 8.5; 128 x 2048 x 2048: 13.7, 9.2,
-// 7.4, 8.8; 512 x 2048 x 2048: 13.9, 10.1, 11.3; 16 x 8192 x 512: 5.7, 4.7, 5.6.
+// 7.4, 8.8; 512 x 2048 x 2048: 13.9, 10.1, 11.3; 16 x 8192 x 512: 5.7, 4.7, 5.6. Within gemm_set_cta_limit() there are no more CTAs than
+// that; a product with more tiles is the pairs' (cluster 0).
 struct FewPlan {
     int cluster;
     float steps;
 };
 FewPlan few_plan(int64_t M, int64_t N, int64_t K, bool wgrad = false) {
     const int64_t tiles = (N + BM - 1) / BM * ((M + kFewTokens - 1) / kFewTokens), k_steps = (K + BK - 1) / BK;
-    const int64_t sms = gemm_cta_limit() > 0 ? gemm_cta_limit() : 2 * kMaxPairs;
+    const bool limited = gemm_cta_limit() > 0;
+    const int64_t sms = limited ? gemm_cta_limit() : 2 * kMaxPairs;
     const int columns = few_columns(M);
-    FewPlan best = {0, 0.f};   // wgrad: cluster 0 where the chains never fit TMEM
+    FewPlan best = {0, 0.f};   // (wgrad: cluster 0 where the chains never fit TMEM, too)
     for (int cluster = 1, doublings = 0; cluster <= 8; cluster *= 2, ++doublings) {
         const int64_t ctas = tiles * cluster;
         // (chains past the first take TMEM that a second CTA would need)
-        const int64_t fit = wgrad && k_steps > kFewChain * cluster ? sms : 2 * sms;
+        const int64_t fit = limited || (wgrad && k_steps > kFewChain * cluster) ? sms : 2 * sms;
         const bool crowded = ctas > sms && fit > sms;
+        if (limited && ctas > sms) break;
         if (cluster > 1 && (ctas > fit || cluster > k_steps)) break;
         if (wgrad && (k_steps + cluster - 1) / cluster > (int64_t)kFewChain * 512 / BM) continue;
         // clusters of eight do not all fit the GPCs with an SM for each CTA: they share, with three stages for 128 tokens, or (wgrad with
@@ -447,15 +450,17 @@ FewPlan few_plan(int64_t M, int64_t N, int64_t K, bool wgrad = false) {
     return best;
 }
 
-// Which kernel: up to 128 tokens always this one; above, the one whose longest CTA is done first. A k-step of a pair's tile takes as
+// Which kernel: up to 128 tokens this one wherever it can run; above, the one whose longest CTA is done first. A k-step of a pair's tile takes as
 // long as one here; its launch, its prologue and its last tile's epilogue (half the warps for twice the values) cost 16 more.
 // 512 x 8192 x 2048, in us: 20.5 here, 20.3; 1024 x 4096 x 4096: 31.9, 29.0; 1024 x 2048 x 8192: 31.6, 42.9.
 bool few_tokens(const LinearArgs& a) {
+    const FewPlan plan = few_plan(a.M, a.N, a.K);
+    if (plan.cluster == 0) return false;
     if (a.M <= kFewTokens) return true;
     const int64_t k_steps = (a.K + BK - 1) / BK, pairs = gemm_cta_limit() > 0 ? std::max(1, gemm_cta_limit() / 2) : kMaxPairs;
     const int64_t small = (int64_t)((a.N + BM - 1) / BM) * ((a.M + kFewTokens - 1) / kFewTokens), large = (int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256);
     if (small > 4 * pairs) return false;
-    return few_plan(a.M, a.N, a.K).steps < (float)((large + pairs - 1) / pairs * k_steps) + 16.f;
+    return plan.steps < (float)((large + pairs - 1) / pairs * k_steps) + 16.f;
 }
 
 template <bool DGRAD>

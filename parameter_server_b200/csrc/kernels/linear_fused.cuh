@@ -651,6 +651,9 @@ cudaError_t pairs_of(int threads, int smem, int* pairs) {
     *pairs = std::min(n, kMaxPairs);
     return cudaSuccess;
 }
+// How many of `n` launch attributes hold, the last of which is start_early(): under gemm_set_cta_limit() it does not. A launch that
+// starts beside its predecessor's tail has its CTAs wait on SMs of their own, and those would be the ones that were to stay free.
+inline int overlap_attrs(int n) { return gemm_cta_limit() > 0 ? n - 1 : n; }
 template <typename Kernel, typename Params>
 cudaError_t launch_pairs(Kernel kern, int threads, int smem, int pairs, const Params& p, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
@@ -660,7 +663,7 @@ cudaError_t launch_pairs(Kernel kern, int threads, int smem, int pairs, const Pa
     cfg.stream = s;
     cudaLaunchAttribute a[2] = {in_clusters(2), start_early()};
     cfg.attrs = a;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = overlap_attrs(2);
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 

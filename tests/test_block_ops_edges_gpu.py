@@ -1,10 +1,10 @@
 """Block operators where values, sizes or settings reach an edge: the largest steps of the 8-bit format on every way that the weight
-gradient takes. Against 64 bits, with the bounds of ``test_block_ops_gpu``."""
+gradient takes, a limit on the CTAs of products. Against 64 bits, with the bounds of ``test_block_ops_gpu``."""
 import pytest
 import torch
 
 from parameter_server_b200._lib import C
-from parameter_server_b200.ops import act8
+from parameter_server_b200.ops import act8, linear
 from parameter_server_b200.ops import gemm as G
 
 pytestmark = pytest.mark.gpu
@@ -45,4 +45,63 @@ def test_act8_wgrad_of_the_largest_steps(way, T, N, K):
     assert torch.isnan(got2[:, 32:64]).all()
     got2[:, 32:64] = got[:, 32:64]
     assert torch.equal(got2, got)
+    G.check_gemm_errors()
+
+
+# ---- a limit on the CTAs of products ----------------------------------------------------------------------------------------
+
+def ctas_of(call):
+    """Of the products' kernels that `call` launches (the memory passes have fewer threads): CTAs, and how many there are."""
+    from cuda.bindings import driver
+
+    def ok(result):
+        assert result[0] == driver.CUresult.CUDA_SUCCESS, result[0]
+        return result[1:] if len(result) > 2 else result[-1]
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    raw = driver.CUgraph(graph.raw_cuda_graph())
+    count = ok(driver.cuGraphGetNodes(raw))[-1]
+    nodes = ok(driver.cuGraphGetNodes(raw, count))[0][:count]
+    kernels = [ok(driver.cuGraphKernelNodeGetParams(n)) for n in nodes
+               if ok(driver.cuGraphNodeGetType(n)) == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL]
+    return [k.gridDimX * k.gridDimY * k.gridDimZ for k in kernels if k.blockDimX >= 384]
+
+
+def sum_bound(a, b):
+    """a [M, K], b [K, N] in 64 bits: the tensor core cuts its sum off once per 16 products."""
+    return (a.shape[1] / 16 + 2) * 2.0 ** -23 * (a.abs() @ b.abs())
+
+
+@pytest.mark.parametrize("limit", [2, 17, 32, 100])
+# few tokens, more of them, many; input gradients; weight gradients on clusters, unpacked, and converted
+@pytest.mark.parametrize("kind,M,N,K", [("forward", 1, 300, 200), ("forward", 16, 8192, 512), ("forward", 128, 2048, 2048), ("forward", 512, 2048, 2048),
+                                        ("forward", 1024, 4096, 1024), ("dgrad", 64, 8192, 1024), ("dgrad", 700, 1000, 520), ("wgrad", 4096, 512, 512),
+                                        ("wgrad", 1000, 4096, 1024), ("wgrad", 4096, 1536, 2048)])
+def test_products_keep_to_the_limit_of_ctas(kind, M, N, K, limit):
+    if kind == "wgrad":
+        dy, x8 = rand(M, N), act8.act8_pack(rand(M, K, seed=1))
+        a, b = dy.double().t(), act8.act8_unpack(x8, F32).double()
+        call, slack = (lambda: act8.act8_wgrad(dy, x8)), (34 * 2.0 ** -23 + (M / 512 + 8) * 2.0 ** -24) * (a.abs() @ b.abs())
+    else:
+        x, w = rand(M, K), rand(N, K, seed=1, std=K ** -0.5)
+        a, b = x.double(), w.double().t()
+        call, slack = (lambda: linear.linear_act(x, w)), sum_bound(a, b)
+        if kind == "dgrad":
+            wt = w.t().contiguous()
+            call = lambda: linear.linear_act_dgrad(x, wt, None)  # noqa: E731
+    C.gemm_set_cta_limit(limit)
+    try:
+        got = call()
+        grids = ctas_of(call)
+    finally:
+        C.gemm_set_cta_limit(0)
+    assert len(grids) == 1 and grids[0] <= limit, grids
+    want = a @ b
+    assert ((got.double() - want).abs() <= slack + (2.0 ** -8 if got.dtype == BF else 2.0 ** -23) * want.abs()).all()
+    free = call()   # without a limit: the same sums, perhaps in another order
+    assert ((free.double() - want).abs() <= slack + (2.0 ** -8 if got.dtype == BF else 2.0 ** -23) * want.abs()).all()
     G.check_gemm_errors()
