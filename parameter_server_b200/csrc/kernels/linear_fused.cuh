@@ -142,7 +142,7 @@ __device__ __forceinline__ float act_slope(float h, float* value) {
 __device__ __forceinline__ void load32(const __nv_bfloat16* p, int n, uint4* raw) {
     if (n >= 32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j] = ld_nc_v4(p + 8 * j);
+        for (int j = 0; j < 4; ++j) raw[j] = ld_global_v4(p + 8 * j);
     } else {
         uint32_t w[16];
 #pragma unroll
@@ -464,8 +464,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 if (!live) return;
                 if (kept8) {
                     const int8_t* qp = p.q + (int64_t)row * p.ldq + col;
-                    coming[0] = ld_nc_v4(qp);
-                    if (col + 16 < p.N) coming[1] = ld_nc_v4(qp + 16);
+                    coming[0] = ld_global_v4(qp);
+                    if (col + 16 < p.N) coming[1] = ld_global_v4(qp + 16);
                 } else if (aux_row != nullptr) {
                     load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, coming);
                 }

@@ -105,3 +105,27 @@ def test_products_keep_to_the_limit_of_ctas(kind, M, N, K, limit):
     free = call()   # without a limit: the same sums, perhaps in another order
     assert ((free.double() - want).abs() <= slack + (2.0 ** -8 if got.dtype == BF else 2.0 ** -23) * want.abs()).all()
     G.check_gemm_errors()
+
+
+# ---- a result in the residual's place ---------------------------------------------------------------------------------------
+
+# pairs and clusters; rows that share 32-byte sectors, lines, or neither with their neighbours' tiles
+@pytest.mark.parametrize("M,N,K,start", [(2048, 2048, 512, 0), (2048, 2040, 512, 8), (700, 1000, 512, 8), (16, 2048, 512, 0), (300, 520, 256, 4)])
+def test_a_result_in_the_residuals_place_call_after_call(M, N, K, start):
+    """Each launch reads what the one before wrote, over the same memory, and begins beside its tail: as if it were done one by one."""
+    x, ws = rand(M, K), [rand(N, K, seed=s, std=K ** -0.5) for s in range(1, 4)]
+
+    def chain(wait):
+        room = torch.zeros(M, N + 24, dtype=BF, device="cuda")
+        res = room[:, start:start + N]
+        for k in range(12):
+            linear.linear_act(x, ws[k % 3], act="silu", residual=res, out=res)
+            if wait:
+                torch.cuda.synchronize()
+        assert (room[:, :start] == 0).all() and (room[:, start + N:] == 0).all()
+        return res.clone()
+
+    want = chain(True)
+    for _ in range(3):
+        assert torch.equal(chain(False), want)
+    G.check_gemm_errors()
