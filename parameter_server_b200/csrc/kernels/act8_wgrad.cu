@@ -70,15 +70,6 @@ struct WgParams {
     unsigned long long limit_ns;
 };
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr)
-        : "memory");
-}
 // Two of the bytes of `w` (unsigned, 128 more than the value; chosen by the selectors) as bf16 times the step: byte b in the
 // second byte of 0x4700bb00 is the float 32768 + b, a packed sum takes off 32896 and a packed product scales, both exactly. (One
 // multiply-add with -32896 steps would do, but that is infinite from a step of 2^113 on, and the format's largest is 2^122.)

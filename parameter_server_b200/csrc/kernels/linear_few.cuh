@@ -99,16 +99,6 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, int n, bool wide, const
             if (j < n) p[j] = __float2bfloat16_rn(f[j]);
     }
 }
-__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t* v) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr)
-        : "memory");
-}
-
 // Four features' sums over the S CTAs, in rank order; all loads are on their way before the first is added (one round trip
 // between SMs takes about 0.2 us).
 template <int S>
@@ -303,11 +293,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         const int quarter = warp & 3;
         for (int t0 = (warp >> 2) * 16; t0 < tokens; t0 += kFewThreads / 128 * 16) {
             uint32_t v[16];
-            tmem_ld16_issue(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t0, v);
+            tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)t0, v);
             if constexpr (WGRAD) {
                 for (int c = 1; c * kFewChain < nk; ++c) {
                     uint32_t w[16];
-                    tmem_ld16_issue(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(c * p.columns + t0), w);
+                    tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(c * p.columns + t0), w);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
                 }

@@ -1073,16 +1073,18 @@ int bwd_typed(const T* dy, int64_t lddy, const T* x, int64_t ldx, const Act8View
         const bool vec = aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}) && (!SRC8 || kept_ok(k));
         constexpr bool kLoose = sizeof(T) == 2 && SRC8;   // unaligned rows otherwise: one value at a time
         if (kLoose && !kept_ok(k)) return -2;
-        const bool two = sizeof(T) == 2 && !SRC8 && aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}, 4);
         auto go = [&](auto vec_c, auto loose_c) {
             return launch_bwd<T, decltype(vec_c)::value, SRC8, decltype(loose_c)::value>(dy, lddy, x, ldx, k, w, mean, rstd, join, ldjoin, dx, lddx, part,
                                                                                         rows, (int)d, p, s);
         };
         using No = std::false_type;
-        constexpr int kTwo = sizeof(T) == 2 && !SRC8 ? 2 : 1;
-        rc = vec   ? go(std::integral_constant<int, vec_of<T>()>{}, No{})
-             : two ? go(std::integral_constant<int, kTwo>{}, No{})
-                   : go(std::integral_constant<int, kLoose ? 8 : 1>{}, std::bool_constant<kLoose>{});
+        auto go_unaligned = [&]() -> int {
+            if constexpr (sizeof(T) == 2 && !SRC8) {   // (beside 8-bit rows bf16 ones are loose)
+                if (aligned<T>(d, {{dy, lddy}, {x, ldx}, {dx, lddx}, {join, ldjoin}, {w, 0}}, 4)) return go(std::integral_constant<int, 2>{}, No{});
+            }
+            return go(std::integral_constant<int, kLoose ? 8 : 1>{}, std::bool_constant<kLoose>{});
+        };
+        rc = vec ? go(std::integral_constant<int, vec_of<T>()>{}, No{}) : go_unaligned();
     } else {
         if (rows > 0x7FFFFFFF) return -2;
         layer_norm_bwd_long_kernel<T, SRC8><<<(unsigned)rows, 512, 0, s>>>(dy, lddy, x, ldx, (const int8_t*)k.q, k.ldq, (const uint8_t*)k.e, k.lde,
