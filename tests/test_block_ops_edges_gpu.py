@@ -1,10 +1,10 @@
 """Block operators where values, sizes or settings reach an edge: the largest steps of the 8-bit format on every way that the weight
-gradient takes, a limit on the CTAs of products. Against 64 bits, with the bounds of ``test_block_ops_gpu``."""
+gradient takes, a limit on the CTAs of products, rows anywhere in memory. Against 64 bits, with the bounds of ``test_block_ops_gpu``."""
 import pytest
 import torch
 
 from parameter_server_b200._lib import C
-from parameter_server_b200.ops import act8, linear
+from parameter_server_b200.ops import act8, linear, norm
 from parameter_server_b200.ops import gemm as G
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +129,51 @@ def test_a_result_in_the_residuals_place_call_after_call(M, N, K, start):
     for _ in range(3):
         assert torch.equal(chain(False), want)
     G.check_gemm_errors()
+
+
+# ---- layer norm on rows inside wider ones -----------------------------------------------------------------------------------
+
+def inside(t, start, room):
+    """The same rows at a column `start` of rows `room` wider, among NaN."""
+    rows, d = t.shape
+    wide = torch.full((rows, d + room), float("nan"), dtype=t.dtype, device="cuda")
+    wide[:, start:start + d] = t
+    return wide[:, start:start + d]
+
+
+def within(got, want, slack):
+    one = 2.0 ** -8 if got.dtype == BF else 2.0 ** -23
+    off = (got.double() - want).abs()
+    assert (off <= one * want.abs() + slack + 1e-30).all(), (off / (one * want.abs() + slack + 1e-30)).max()
+
+
+# start 1 of 3 more: rows on every 2-byte boundary; 2 of 4: on 4 bytes; 8 of 8: on 16; and mixed, so that operands differ
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("places", [(1, 3), (2, 4), (8, 8), "mixed"])
+@pytest.mark.parametrize("rows,d", [(5, 2), (700, 34), (3000, 534), (700, 1001), (700, 2050), (3, 4102), (2, 8190), (640, 2048), (2, 8200)])
+def test_layer_norm_of_rows_inside_wider_ones(rows, d, places, dtype):
+    """Forward and backward, from x and from 8-bit rows, with a residual gradient: each value against 64 bits."""
+    at = [(1, 3), (2, 4), (0, 2), (3, 5)] if places == "mixed" else [places] * 4
+    x, dy, join = rand(rows, d, dtype=dtype) * 3 + 1, rand(rows, d, seed=3, dtype=dtype), rand(rows, d, seed=4, dtype=dtype)
+    g, b = rand(d, seed=1, dtype=dtype), rand(d, seed=2, dtype=dtype)
+    xs, dys, js = inside(x, *at[0]), inside(dy, *at[1]), inside(join, *at[2])
+    gs = inside(g.view(1, d), *at[3])[0]
+    y, mean, rstd = norm.layer_norm(xs, gs, b)
+    x64 = x.double()
+    dev = (x64.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    xhat = (x64 - x64.mean(1, keepdim=True)) / dev
+    # x and the mean enter with 2^-24 of the largest |x| over the deviation, the sums' roundings stay below 2^-20 of the values
+    off = 2.0 ** -22 * x64.abs().amax(1, keepdim=True) / dev + 2.0 ** -20 * (1 + xhat.abs())
+    within(y, xhat * g.double() + b.double(), off * (1 + g.double().abs()))
+    y8, x8, rstd8 = norm.layer_norm_act8(xs, gs, b)
+    assert torch.equal(y8, y) and torch.equal(rstd8, rstd)
+    stats = (x64 - mean.double()[:, None]) * rstd.double()[:, None]
+    p = dy.double() * g.double()
+    for hat, result in ((stats, norm.layer_norm_backward(dys, xs, gs, mean, rstd, residual_grad=js)),
+                        (act8.act8_unpack(x8, F32).double(), norm.layer_norm_act8_backward(dys, x8, gs, rstd, residual_grad=js))):
+        dx, dw, db = result
+        want = rstd.double()[:, None] * (p - p.mean(1, keepdim=True) - hat * (p * hat).mean(1, keepdim=True)) + join.double()
+        size = p.abs() + p.abs().mean(1, keepdim=True) + hat.abs() * (p * hat).abs().mean(1, keepdim=True)
+        within(dx, want, 2.0 ** -20 * rstd.double()[:, None] * size + 2.0 ** -24 * want.abs())
+        within(dw, (dy.double() * hat).sum(0), 2.0 ** -20 * (dy.double() * hat).abs().sum(0))
+        within(db, dy.double().sum(0), 2.0 ** -20 * dy.double().abs().sum(0))
