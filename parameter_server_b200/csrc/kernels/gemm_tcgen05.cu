@@ -288,10 +288,10 @@ __device__ void gather_rows(const GemmGather& ag, int K, uint8_t* smem, uint64_t
             if (q > 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             issue_load(qn);
         }
-        if (!mbar_wait(&bars[d], (q / kDepth) & 1u, limit_ns)) {
+        if (!mbar_wait<1>(&bars[d], (q / kDepth) & 1u, limit_ns)) {
             atomicCAS(err_flag, 0u, 6u);
             // the loads still in flight land in this CTA's shared memory: let them finish (bounded) before leaving
-            for (uint32_t w = q + 1; w < total && w <= qn; ++w) mbar_wait(&bars[w % kDepth], (w / kDepth) & 1u, limit_ns);
+            for (uint32_t w = q + 1; w < total && w <= qn; ++w) mbar_wait<1>(&bars[w % kDepth], (w / kDepth) & 1u, limit_ns);
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             return;
         }
@@ -538,7 +538,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ GemmProblemSet ps, unsigned* er
                 for (int kt = 0; kt < num_kt; ++kt, ++it) {
                     const int s = it % L::kStages;
                     const uint32_t ph = (it / L::kStages) & 1u;
-                    if (!mbar_wait(&empty_bar[s], ph ^ 1u, limit_ns)) {
+                    if (!mbar_wait<1>(&empty_bar[s], ph ^ 1u, limit_ns)) {
                         atomicCAS(err_flag, 0u, 1u);
                         ok = false;
                         break;
@@ -604,7 +604,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ GemmProblemSet ps, unsigned* er
                 const int num_kt = decode_unit<BN, PAIR>(ps, unit, ag, cr).num_kt;
                 if (num_kt == 0) continue;
                 const uint32_t buf = tc & 1u, tph = (tc >> 1) & 1u;
-                if (!mbar_wait(&tempty_bar[buf], tph ^ 1u, limit_ns)) {
+                if (!mbar_wait<1>(&tempty_bar[buf], tph ^ 1u, limit_ns)) {
                     atomicCAS(err_flag, 0u, 4u);
                     break;
                 }
@@ -617,7 +617,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ GemmProblemSet ps, unsigned* er
                     const int s = it % L::kStages;
                     const uint32_t ph = (it / L::kStages) & 1u;
                     // consumers wait longer than producers, so that the wait that reports is the one at the root
-                    if (!mbar_wait(&full_bar[s], ph, limit_ns * 2)) {
+                    if (!mbar_wait<1>(&full_bar[s], ph, limit_ns * 2)) {
                         atomicCAS(err_flag, 0u, 2u);
                         ok = false;
                         break;
@@ -719,7 +719,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ GemmProblemSet ps, unsigned* er
                 for (int j = 0; j < 4; ++j) mreg[j] = ld_nc_v4(mrow + j * 8);
                 mhave = true;
             }
-            const bool waited = mbar_wait(&tfull_bar[buf], tph, limit_ns * 4);
+            const bool waited = mbar_wait<1>(&tfull_bar[buf], tph, limit_ns * 4);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (!LEAN && ps.trace != nullptr && cta == 0 && leader && (unit - cta) / n_cta < 8 && ew == 0 && lane == 0)
                 ps.trace[(unit - cta) / n_cta * 32 + 8] = gtimer();
