@@ -1,10 +1,12 @@
-"""A fused decoder under autograd's own tools: a graph that is run twice, hooks on what is saved, changes in place, recomputation."""
+"""A fused decoder under autograd's own tools: a graph that is run twice, hooks on what is saved, changes in place, recomputation; and
+with its QKV weights in tables of their own, as several ranks have them."""
 import pytest
 import torch
 from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
 from torch.utils.checkpoint import checkpoint
 
 from parameter_server_b200.models.gpt import GPT, GPTConfig
+from parameter_server_b200.ops.dense import DenseTable
 
 pytestmark = pytest.mark.gpu
 
@@ -90,4 +92,27 @@ def test_recomputation_gives_the_same(bits):
     loss.backward()
     assert loss.item() == loss0
     close(grads(model), one)
+    model.check()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_qkv_weights_in_tables_of_their_own(bits):
+    """What a model on several ranks does with the tables whose rows it gathers in the product, on one rank, which has all rows."""
+    model = model_of(bits)
+    loss0, one = once(model)
+    d = SIZES["d_model"]
+    for i in range(SIZES["n_layer"]):
+        table = DenseTable({"w": (3 * d, d)}, "adamw", dict(lr=SIZES["lr"]), grad_dtype=torch.float32, device=model.device, scatter_peers=False)
+        table.load({"w": model.main.params[f"h{i}.qkv.w"].detach().float().cpu()})
+        table.zero_grads()
+        model.qkv[i] = table
+    model.zero_grads()
+    _, loss = model.forward(*batch())
+    loss.backward()
+    two = grads(model)
+    for i in range(SIZES["n_layer"]):
+        assert (two[f"h{i}.qkv.w"] == 0).all()
+        two[f"h{i}.qkv.w"] = model.qkv[i].grads["w"].clone()
+    close(two, one)
+    assert abs(loss.item() - loss0) < 2e-3   # the product itself is another kernel's
     model.check()
