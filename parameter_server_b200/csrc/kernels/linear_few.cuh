@@ -440,10 +440,11 @@ FewPlan few_plan(int64_t M, int64_t N, int64_t K, bool wgrad = false) {
     return best;
 }
 
-// Which kernel: up to 128 tokens this one wherever it can run; above, the one whose longest CTA is done first. A k-step of a pair's tile takes as
-// long as one here; its launch, its prologue and its last tile's epilogue (half the warps for twice the values) cost 16 more.
+// Which kernel: up to 128 tokens this one wherever it can run; above, the one whose longest CTA is done first. A k-step of a pair's tile
+// takes as long as one here; its launch, its prologue and its last tile's epilogue (half the warps for twice the values) cost 16 more.
 // 512 x 8192 x 2048, in us: 20.5 here, 20.3; 1024 x 4096 x 4096: 31.9, 29.0; 1024 x 2048 x 8192: 31.6, 42.9.
 bool few_tokens(const LinearArgs& a) {
+    if (gemm_cta_limit() <= 0 && a.M <= kFewTokens) return true;
     const FewPlan plan = few_plan(a.M, a.N, a.K);
     if (plan.cluster == 0) return false;
     if (a.M <= kFewTokens) return true;
