@@ -2,7 +2,8 @@
 // -127..127 steps. With m the largest magnitude of a block,
 //     e    = the smallest exponent (1..249) at which m / 2^(e-127) rounds to at most 127,
 //     q_i  = round-to-nearest-even(x_i / 2^(e-127)),          x_i is rebuilt as q_i * 2^(e-127).
-// The error of a value is at most half a step, a step is between m / 127.5 and m / 63.7. A step is a power of two, so that
+// The error of a value is at most half a step, a step is between m / 127.5 and m / 63.7 (from m = 127.5 * 2^121 = 3.39e38 on, bf16's
+// largest number, q is 64 and its value 2^128, infinity: rounding to nearest beyond the largest number, as everywhere). A step is a power of two, so that
 // scaling never rounds: q * 2^(e-127) has at most 7 significant bits and is exact in bf16, which is what lets the weight
 // gradient feed rebuilt values to the bf16 tensor cores without a second rounding. A block that holds an infinity or NaN is
 // stored as e = 255 with q = 0 (0 * 2^128 = NaN): a training step that has gone wrong shows it in its gradients.

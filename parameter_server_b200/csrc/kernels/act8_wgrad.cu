@@ -12,7 +12,7 @@
 //
 // CTA pairs on 256 x 256 tiles of dw as in linear_fused.cuh, both operands MN-major. Where x is converted, four more warps per
 // CTA turn the pair's half of the checkpoint tile ([64 tokens][128 columns], 8 KB) into the swizzled bf16 tile that the MMA reads:
-// per two values two byte permutes, a packed sum, a packed product and a conversion, 450 of the 750 cycles that a k-step takes; dy, the
+// per two values two byte permutes, a packed sum, a packed product and a conversion (sum and product in one: 450 of the 750 cycles of a k-step); dy, the
 // checkpoint and the bf16 tiles have rings of their own, so that no part waits for another's space.
 // The eight epilogue warps keep the tile's sums in registers: the tensor core adds to its fp32 accumulator with truncation, which
 // loses 1e-9 of the sum per token (2e-5 at 16384, all towards zero), so a chain in TMEM ends after 512 tokens and the chains are
