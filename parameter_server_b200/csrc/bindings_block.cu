@@ -1,15 +1,30 @@
-// Bindings of the decoder-block operators: layer norm, fused linear layers, 8-bit activation checkpoints.
+// Bindings of the decoder-block operators: layer norm, fused linear layers, 8-bit activation checkpoints, dropout, rotary positions.
 #include <pybind11/pybind11.h>
 
+#include <tuple>
+
 #include "kernels/act8_wgrad.h"
+#include "kernels/dropout.h"
 #include "kernels/linear_fused.h"
 #include "kernels/norm.h"
+#include "kernels/rotary.h"
 
 namespace py = pybind11;
 using namespace psb;
 
 namespace {
 Act8View view(uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde) { return Act8View{(void*)q, ldq, (void*)e, lde}; }
+
+DropoutArgs drop_args(uint64_t seed, uintptr_t seed_ptr, uint64_t offset, uint32_t threshold, double scale) {
+    return DropoutArgs{seed, (const void*)seed_ptr, offset, threshold, (float)scale};
+}
+
+// x, its strides between batches, tokens and heads, the result and its own, heads
+using HeadsArgs = std::tuple<uintptr_t, int64_t, int64_t, int64_t, uintptr_t, int64_t, int64_t, int64_t, int>;
+RotaryHeads heads(const HeadsArgs& h) {
+    return RotaryHeads{(const void*)std::get<0>(h), std::get<1>(h), std::get<2>(h), std::get<3>(h), (void*)std::get<4>(h),
+                       std::get<5>(h), std::get<6>(h), std::get<7>(h), std::get<8>(h)};
+}
 }  // namespace
 
 void bind_block(py::module_& m) {
@@ -96,6 +111,32 @@ void bind_block(py::module_& m) {
         return act8_wgrad(x, (void*)s);
     });
     m.def("act8_wgrad_scratch", &act8_wgrad_scratch);
+    m.def("dropout", [](int dtype, uintptr_t x, int64_t ldx, uintptr_t residual, int64_t ldres, uintptr_t out, int64_t ldo, int64_t rows,
+                        int64_t cols, uint64_t seed, uintptr_t seed_ptr, uint64_t offset, uint32_t threshold, double scale, uintptr_t s) {
+        return dropout(dtype, (const void*)x, ldx, (const void*)residual, ldres, (void*)out, ldo, rows, cols,
+                       drop_args(seed, seed_ptr, offset, threshold, scale), (void*)s);
+    });
+    m.def("rotary", [](int dtype, const HeadsArgs& q, const HeadsArgs& k, int64_t batch, int64_t tokens, int dim, int pairs, bool interleaved,
+                       uintptr_t freqs, uintptr_t positions, bool positions32, int64_t pb, int64_t pt, int64_t offset, double scale,
+                       bool backward, uintptr_t s) {
+        RotaryArgs a;
+        a.q = heads(q);
+        a.k = heads(k);
+        a.batch = batch;
+        a.tokens = tokens;
+        a.dim = dim;
+        a.pairs = pairs;
+        a.interleaved = interleaved ? 1 : 0;
+        a.freqs = (const double*)freqs;
+        a.positions = (const void*)positions;
+        a.positions32 = positions32 ? 1 : 0;
+        a.pb = pb;
+        a.pt = pt;
+        a.offset = offset;
+        a.scale = (float)scale;
+        a.backward = backward ? 1 : 0;
+        return rotary(dtype, a, (void*)s);
+    });
     m.def("linear_workspace_bytes", &linear_workspace_bytes);
     m.def("linear_workspace_zeros", &linear_workspace_zeros);
     m.attr("NEEDS_WORKSPACE") = kNeedsWorkspace;

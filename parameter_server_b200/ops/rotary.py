@@ -1,0 +1,111 @@
+"""Rotary positions of queries and keys, forward and backward (``csrc/kernels/rotary.cu``).
+
+Pair ``i`` of a head's values turns by ``position * freqs[i]`` radians. ``rotary_frequencies`` makes the frequencies, also for contexts longer
+than the model was trained on; any others do as well. Angles are formed in 64 bits, values turned in fp32 and rounded once.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from .._lib import C
+from .act8 import _DTYPES, check, launch_stream
+
+_POSITIONS = {torch.int64: False, torch.int32: True}
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
+                       trained_length: Optional[int] = None, fast: float = 32.0, slow: float = 1.0,
+                       device=None) -> Tuple[torch.Tensor, float]:
+    """``(freqs, scale)`` for heads of which ``dim`` values turn: ``dim / 2`` angles per position (fp64, radians), ``base^(-2i/dim)``, and the
+    factor that :func:`rotary` takes with them.
+
+    ``scaling``, for contexts ``factor`` times as long as ``trained_length``: "linear" divides all frequencies by ``factor``; "ntk" raises
+    the base so that the slowest pair is divided by it and the fastest stays; "yarn" (Peng, Quesnelle, Fan, Shippole, 2023) leaves pairs that
+    turn ``fast`` times or more over ``trained_length``, divides those below ``slow`` turns, goes linearly in the number of turns in between, and
+    has ``scale`` = 0.1 ln(factor) + 1."""
+    what = "rotary_frequencies"
+    if dim <= 0 or dim % 2:
+        raise ValueError(f"{what}: dim is even and positive, not {dim}")
+    if not base > 0 or not factor >= 1:
+        raise ValueError(f"{what}: base is positive and factor at least 1, not {base!r} and {factor!r}")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    scale = 1.0
+    if scaling == "ntk" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    freqs = base ** (-i / dim)
+    if scaling == "linear" or (scaling == "ntk" and dim == 2):
+        freqs = freqs / factor
+    elif scaling == "yarn":
+        if trained_length is None or trained_length <= 0 or not fast > slow:
+            raise ValueError(f"{what}: yarn needs trained_length, and fast above slow")
+        kept = ((freqs * trained_length / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        freqs = freqs * kept + freqs / factor * (1 - kept)
+        scale = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "none", "ntk"):
+        raise ValueError(f"{what}: scaling is None, 'linear', 'ntk' or 'yarn', not {scaling!r}")
+    return freqs.to(device if device is not None else torch.device("cuda", torch.cuda.current_device())), scale
+
+
+def _heads(x, out, like, dev, what, name):
+    """(x, result, arguments of the native call) of queries or keys."""
+    if x.dim() not in (3, 4):
+        raise ValueError(f"{what}: {name} is [tokens, heads, dim] or [batch, tokens, heads, dim], not {tuple(x.shape)}")
+    if like is not None and (x.dim() != like.dim() or x.shape[:-2] != like.shape[:-2] or x.shape[-1] != like.shape[-1] or x.dtype != like.dtype
+                             or x.get_device() != dev):
+        raise ValueError(f"{what}: {name} of {tuple(x.shape)} {x.dtype} on {x.device} does not go with q of {tuple(like.shape)} {like.dtype} on {like.device}")
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev or (out.stride(-1) != 1 and out.shape[-1] > 1):
+        raise ValueError(f"{what}: out of {name} must be like it ({tuple(x.shape)} of {x.dtype} on {x.device}), the values of a head side by side")
+    lead = (x.stride(0), out.stride(0)) if x.dim() == 4 else (0, 0)
+    return x, out, (x.data_ptr(), lead[0], x.stride(-3), x.stride(-2), out.data_ptr(), lead[1], out.stride(-3), out.stride(-2), x.shape[-2])
+
+
+def _rotary(q, k, freqs, positions, offset, interleaved, scale, out_q, out_k, backward, what):
+    dt = _DTYPES.get(q.dtype)
+    if dt is None:
+        raise ValueError(f"{what}: bf16 or fp32, not {q.dtype}")
+    s, dev = launch_stream(q), q.get_device()
+    q, out_q, q_args = _heads(q, out_q, None, dev, what, "q")
+    if k is not None:
+        k, out_k, k_args = _heads(k, out_k, q, dev, what, "k")
+    elif out_k is not None:
+        raise ValueError(f"{what}: out_k without k")
+    else:
+        k_args = (0,) * 9
+    batch, tokens, dim = q.shape[0] if q.dim() == 4 else 1, q.shape[-3], q.shape[-1]
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or freqs.get_device() != dev or 2 * freqs.numel() > dim or not freqs.is_contiguous():
+        raise ValueError(f"{what}: freqs must be at most {dim // 2} contiguous fp64 values on {q.device}, got {tuple(freqs.shape)} of {freqs.dtype} on {freqs.device}")
+    pos = (0, False, 0, 0)
+    if positions is not None:
+        narrow = _POSITIONS.get(positions.dtype)
+        if narrow is None or positions.get_device() != dev or tuple(positions.shape) not in ((tokens,), (batch, tokens), (1, tokens)):
+            raise ValueError(f"{what}: positions must be int64 or int32, [{tokens}] or [{batch}, {tokens}], on {q.device}, "
+                             f"got {tuple(positions.shape)} of {positions.dtype} on {positions.device}")
+        pos = (positions.data_ptr(), narrow, positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, positions.stride(-1))
+    check(C.rotary(dt, q_args, k_args, batch, tokens, dim, freqs.numel(), interleaved, freqs.data_ptr(), *pos, offset, scale, backward, s), what)
+    return out_q if k is None else (out_q, out_k)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, positions: Optional[torch.Tensor] = None, *, offset: int = 0,
+           interleaved: bool = False, scale: float = 1.0, out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
+    """``(q, k)`` with the first ``2 * len(freqs)`` values of every head turned, times ``scale``, and the others as they are.
+
+    ``q`` and ``k`` (which may be None; its result is left out then): ``[batch, tokens, heads, dim]`` or ``[tokens, heads, dim]`` with any
+    strides but the last (heads ahead of tokens: ``x.transpose(1, 2)``; heads of a packed QKV product: slices of its view), bf16 or fp32, with heads in any
+    number each. ``freqs``: fp64, one angle per position of each pair. ``positions``: int64 or int32, ``[tokens]`` or ``[batch, tokens]``, any
+    sign; without them a token's place in its row. ``offset`` is added to them. ``interleaved``: a pair is two neighbours, otherwise value
+    ``i`` and value ``i + len(freqs)``. ``out_q`` and ``out_k`` may be ``q`` and ``k`` themselves (the values that do not turn are left alone then), and must
+    not overlap them otherwise. Angles are as exact as a product in 64 bits: 1.5e-6 radians at position 2^31 times one radian."""
+    return _rotary(q, k, freqs, positions, offset, interleaved, scale, out_q, out_k, False, "rotary")
+
+
+def rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], freqs: torch.Tensor, positions: Optional[torch.Tensor] = None, *, offset: int = 0,
+                    interleaved: bool = False, scale: float = 1.0, out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
+    """The gradients that reach ``q`` and ``k`` of :func:`rotary` with the same ``freqs``, ``positions`` and options: turned back, times ``scale``."""
+    return _rotary(dq, dk, freqs, positions, offset, interleaved, scale, out_q, out_k, True, "rotary_backward")
