@@ -15,8 +15,9 @@ using namespace psb;
 namespace {
 Act8View view(uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde) { return Act8View{(void*)q, ldq, (void*)e, lde}; }
 
-DropoutArgs drop_args(uint64_t seed, uintptr_t seed_ptr, uint64_t offset, uint32_t threshold, double scale) {
-    return DropoutArgs{seed, (const void*)seed_ptr, offset, threshold, (float)scale};
+using DropTuple = std::tuple<uint64_t, uintptr_t, uint64_t, uint32_t, double>;   // seed, its place on the device, offset, threshold, scale
+DropoutArgs drop_args(const DropTuple& d) {
+    return DropoutArgs{std::get<0>(d), (const void*)std::get<1>(d), std::get<2>(d), std::get<3>(d), (float)std::get<4>(d)};
 }
 
 // x, its strides between batches, tokens and heads, the result and its own, heads
@@ -55,12 +56,14 @@ void bind_block(py::module_& m) {
     m.def("pad_rows", [](uintptr_t src, int64_t ld, uintptr_t dst, int64_t ldp, int64_t rows, int64_t cols, uintptr_t s) {
         return pad_rows((const void*)src, ld, (void*)dst, ldp, rows, cols, (void*)s);
     });
-    m.def("linear_fused", [](bool dgrad, int act, int M, int N, int K, uintptr_t a, int64_t lda, uintptr_t w, int64_t ldw, uintptr_t bias,
+    m.def("linear_fused", [](bool dgrad, bool gated, int act, int M, int N, int K, uintptr_t a, int64_t lda, uintptr_t w, int64_t ldw, uintptr_t bias,
                              bool bias_f32, uintptr_t residual, int64_t ldres, uintptr_t out, int64_t ldo, uintptr_t out2, int64_t ldo2,
-                             uintptr_t pre, int64_t ldpre, uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde, uintptr_t workspace,
-                             uintptr_t err_flag, double wait_limit_s, uintptr_t s) {
+                             uintptr_t pre, int64_t ldpre, uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde, uintptr_t q_up,
+                             int64_t ldq_up, uintptr_t e_up, int64_t lde_up, const DropTuple& drop, uintptr_t workspace, uintptr_t err_flag,
+                             double wait_limit_s, uintptr_t s) {
         LinearArgs x;
         x.dgrad = dgrad ? 1 : 0;
+        x.gated = gated ? 1 : 0;
         x.act = act;
         x.M = M;
         x.N = N;
@@ -83,6 +86,11 @@ void bind_block(py::module_& m) {
         x.ldq = ldq;
         x.e = (void*)e;
         x.lde = lde;
+        x.q_up = (void*)q_up;
+        x.ldq_up = ldq_up;
+        x.e_up = (void*)e_up;
+        x.lde_up = lde_up;
+        x.drop = drop_args(drop);
         x.workspace = (void*)workspace;
         x.err_flag = (unsigned*)err_flag;
         x.wait_limit_s = wait_limit_s;
@@ -112,9 +120,8 @@ void bind_block(py::module_& m) {
     });
     m.def("act8_wgrad_scratch", &act8_wgrad_scratch);
     m.def("dropout", [](int dtype, uintptr_t x, int64_t ldx, uintptr_t residual, int64_t ldres, uintptr_t out, int64_t ldo, int64_t rows,
-                        int64_t cols, uint64_t seed, uintptr_t seed_ptr, uint64_t offset, uint32_t threshold, double scale, uintptr_t s) {
-        return dropout(dtype, (const void*)x, ldx, (const void*)residual, ldres, (void*)out, ldo, rows, cols,
-                       drop_args(seed, seed_ptr, offset, threshold, scale), (void*)s);
+                        int64_t cols, const DropTuple& drop, uintptr_t s) {
+        return dropout(dtype, (const void*)x, ldx, (const void*)residual, ldres, (void*)out, ldo, rows, cols, drop_args(drop), (void*)s);
     });
     m.def("rotary", [](int dtype, const HeadsArgs& q, const HeadsArgs& k, int64_t batch, int64_t tokens, int dim, int pairs, bool interleaved,
                        uintptr_t freqs, uintptr_t positions, bool positions32, int64_t pb, int64_t pt, int64_t offset, double scale,

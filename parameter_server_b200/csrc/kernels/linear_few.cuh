@@ -55,6 +55,13 @@ struct FewParams {
     uint8_t* e;
     int64_t lde;
     int res_wide, out_wide, out2_wide, pre_wide;   // rows on 8-byte boundaries (wgrad's out: 16)
+    // gated: the second factor's checkpoint, and whether its columns of pre and (dgrad) of out lie on 8-byte boundaries
+    int8_t* q_up;
+    int64_t ldq_up;
+    uint8_t* e_up;
+    int64_t lde_up;
+    int pre_up_wide, out_up_wide;
+    DropoutArgs drop;
     float* dw;            // wgrad: out, with the norm's weight (null: 1) and, with a bias, the sums of dy's rows
     const __nv_bfloat16* gain;
     const float* dy_sum;
@@ -126,9 +133,11 @@ __device__ __forceinline__ void add_parts_apart(uint32_t at, int S, float* v) {
     }
 }
 
-template <int MODE, int ACT>
-__global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid_constant__ FewParams p) {
+template <int MODE, int ACT, int KIND = kLinPlain>
+__global__ void __launch_bounds__(kFewThreads, KIND == kLinDropout ? 2 : 1) linear_few_kernel(const __grid_constant__ FewParams p) {
     constexpr bool DGRAD = MODE == kFewDgrad, WGRAD = MODE == kFewWgrad, W_MN = MODE != kFewFwd;
+    constexpr bool GATED_FWD = KIND == kLinGated && !DGRAD, GATED_DGRAD = KIND == kLinGated && DGRAD;
+    constexpr int kWide = GATED_FWD ? BM / 2 : BM;   // outputs of a tile: of a gated one's features, half are the gate's
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = BM * BK * 2 + p.columns * BK * 2;
@@ -139,7 +148,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     uint32_t* tmem_slot = (uint32_t*)(done_bar + 1);
 
     const int S = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
-    const int tile = (int)blockIdx.x / S, n0 = tile % p.n_tiles * BM, m0 = tile / p.n_tiles * kFewTokens;
+    const int tile = (int)blockIdx.x / S, n0 = tile % p.n_tiles * kWide, m0 = tile / p.n_tiles * kFewTokens;
     const int tokens = min(p.M - m0, kFewTokens);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int k_begin = (int)((int64_t)p.k_steps * rank / S), k_end = (int)((int64_t)p.k_steps * (rank + 1) / S), nk = k_end - k_begin;
@@ -148,7 +157,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         const int k0 = (k_begin + k) * BK;
         uint8_t* sa = smem + s * stage_bytes;
         mbar_expect_tx(&full_bar[s], (uint32_t)stage_bytes);
-        if constexpr (!W_MN) {
+        if constexpr (GATED_FWD) {
+            tma_load_2d(sa, &p.map_w, &full_bar[s], k0, n0);   // [64 features][64 k] of the gate, and of the other factor
+            tma_load_2d(sa + 64 * BK * 2, &p.map_w, &full_bar[s], k0, p.N + n0);
+        } else if constexpr (!W_MN) {
             tma_load_2d(sa, &p.map_w, &full_bar[s], k0, n0);   // [128 features][64 k]
         } else {
             tma_load_2d(sa, &p.map_w, &full_bar[s], n0, k0);   // two blocks of [64 k][64 features]
@@ -236,10 +248,16 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     // what the epilogue needs from memory, on its way meanwhile: a warp has a token, a lane four neighbouring features
     // (wgrad with rows that are not aligned: four features 32 apart, so that the lanes' single values lie side by side)
     const bool apart = WGRAD && p.out_wide == 0;
-    const int n = apart ? n0 + lane : n0 + lane * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
+    // (gated: the lower sixteen lanes have the gate's features, the others those of the second factor at the same places)
+    const bool up = GATED_FWD && lane >= 16;
+    const int n = apart ? n0 + lane : n0 + (GATED_FWD ? lane & 15 : lane) * 4, have = p.N - n;   // features of this lane that exist (4 or more: all)
+    const int bias_at = up ? p.N + n : n;
     const int stride = apart ? 32 : 1;                                 // between them
     const int t_end = min(tokens, (rank + 1) * share), t_first = rank * share + warp;
     float b[4] = {0.f, 0.f, 0.f, 0.f}, gain[4] = {1.f, 1.f, 1.f, 1.f}, aux[4], sum = 0.f;
+    [[maybe_unused]] float aux_up[4];
+    [[maybe_unused]] DropKey key;
+    if constexpr (KIND == kLinDropout) key = drop_key(p.drop);
     if constexpr (WGRAD) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -249,11 +267,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j * stride < have)
-                b[j] = p.bias32 != nullptr ? p.bias32[n + j * stride] : p.bias != nullptr ? __bfloat162float(p.bias[n + j * stride]) : 0.f;
+                b[j] = p.bias32 != nullptr ? p.bias32[bias_at + j * stride] : p.bias != nullptr ? __bfloat162float(p.bias[bias_at + j * stride]) : 0.f;
     }
     auto fetch = [&](int t) {   // residual, or h
 #pragma unroll
         for (int j = 0; j < 4; ++j) aux[j] = 0.f;
+        if constexpr (GATED_DGRAD) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) aux_up[j] = 0.f;
+        }
         if (have <= 0 || t >= t_end) return;
         const int64_t row = m0 + t;
         if constexpr (WGRAD) {
@@ -277,8 +299,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
             aux[1] = s8_of_biased<1>(w) * step;
             aux[2] = s8_of_biased<2>(w) * step;
             aux[3] = s8_of_biased<3>(w) * step;
+            if constexpr (GATED_DGRAD) {
+                const uint32_t wu = *(const uint32_t*)(p.q_up + row * p.ldq_up + n) ^ 0x80808080u;
+                const float step_up = act8_step(p.e_up[row * p.lde_up + n / kAct8Block]);
+                aux_up[0] = s8_of_biased<0>(wu) * step_up;
+                aux_up[1] = s8_of_biased<1>(wu) * step_up;
+                aux_up[2] = s8_of_biased<2>(wu) * step_up;
+                aux_up[3] = s8_of_biased<3>(wu) * step_up;
+            }
         } else if (p.pre != nullptr) {
             load4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, aux);
+            if constexpr (GATED_DGRAD) load4(p.pre + row * p.ldpre + p.N + n, have, p.pre_up_wide != 0, aux_up);
         }
     };
     fetch(t_first);
@@ -340,28 +371,54 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
         } else if constexpr (!DGRAD) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += b[j];   // (0 past the last feature: its weights were read as zeros)
-            if (p.pre != nullptr && have > 0) store4(p.pre + row * p.ldpre + n, have, p.pre_wide != 0, v);
+            if constexpr (GATED_FWD) {   // (behind the gate's last row of w, the tile has the other factor's first)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = j < have ? v[j] : 0.f;
+            }
+            if (p.pre != nullptr && have > 0) store4(p.pre + row * p.ldpre + bias_at, have, (up ? p.pre_up_wide : p.pre_wide) != 0, v);
             if (p.q != nullptr) {   // a block is eight lanes
                 uint32_t m = abs_bits(abs_max(abs_max(v[0], v[1]), abs_max(v[2], v[3])));
 #pragma unroll
                 for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
                 const uint32_t ex = act8_exponent(m);
                 if (have > 0) {
-                    *(uint32_t*)(p.q + row * p.ldq + n) = ex == 255u ? 0u : act8_quantise4(v[0], v[1], v[2], v[3], act8_inverse_step(ex));
-                    if ((lane & 7) == 0) p.e[row * p.lde + n / kAct8Block] = (uint8_t)ex;
+                    int8_t* q = up ? p.q_up + row * p.ldq_up : p.q + row * p.ldq;
+                    uint8_t* e = up ? p.e_up + row * p.lde_up : p.e + row * p.lde;
+                    *(uint32_t*)(q + n) = ex == 255u ? 0u : act8_quantise4(v[0], v[1], v[2], v[3], act8_inverse_step(ex));
+                    if ((lane & 7) == 0) e[n / kAct8Block] = (uint8_t)ex;
                 }
             }
+            if constexpr (GATED_FWD) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = act_of<ACT>(v[j]) + aux[j];
+                for (int j = 0; j < 4; ++j) v[j] = act_of<ACT>(v[j]) * __shfl_xor_sync(0xFFFFFFFFu, v[j], 16);   // (meant in the lower lanes)
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = act_of<ACT>(v[j]);
+                if constexpr (KIND == kLinDropout) drop4(key, p.drop.threshold, p.drop.scale, (uint32_t)row, (uint32_t)n / 4, v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += aux[j];
+            }
             fetch(t + kFewThreads / 32);   // (before the stores: another lane's residual is never what this one writes)
-            if (have > 0) store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
+            if (have > 0 && !up) store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
         } else {
             float a[4];
+            [[maybe_unused]] float du[4];
+            if constexpr (GATED_DGRAD) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= act_slope<ACT>(aux[j], &a[j]);
+                for (int j = 0; j < 4; ++j) {
+                    const float slope = act_slope<ACT>(aux[j], &a[j]);
+                    du[j] = v[j] * a[j];
+                    a[j] *= aux_up[j];
+                    v[j] *= aux_up[j] * slope;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] *= act_slope<ACT>(aux[j], &a[j]);
+            }
             fetch(t + kFewThreads / 32);
             if (have > 0) {
                 store4(p.out + row * p.ldo + n, have, p.out_wide != 0, v);
+                if constexpr (GATED_DGRAD) store4(p.out + row * p.ldo + p.N + n, have, p.out_up_wide != 0, du);
                 if (p.out2 != nullptr) store4(p.out2 + row * p.ldo2 + n, have, p.out2_wide != 0, a);
             }
         }
@@ -370,9 +427,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     cluster_sync_all();   // until here the others may read this CTA's shared memory
 }
 
-template <int MODE, int ACT>
+template <int MODE, int ACT, int KIND = kLinPlain>
 int launch_few(FewParams& p, int cluster, cudaStream_t s) {
-    constexpr auto kern = linear_few_kernel<MODE, ACT>;
+    constexpr auto kern = linear_few_kernel<MODE, ACT, KIND>;
     const int64_t ctas = (int64_t)p.n_tiles * ((p.M + kFewTokens - 1) / kFewTokens) * cluster;
     const int nk = (p.k_steps + cluster - 1) / cluster, chains = MODE == kFewWgrad ? (nk + kFewChain - 1) / kFewChain : 1;
     p.tmem_columns = 128;
@@ -443,19 +500,23 @@ FewPlan few_plan(int64_t M, int64_t N, int64_t K, bool wgrad = false) {
 // Which kernel: up to 128 tokens this one wherever it can run; above, the one whose longest CTA is done first. A k-step of a pair's tile
 // takes as long as one here; its launch, its prologue and its last tile's epilogue (half the warps for twice the values) cost 16 more.
 // 512 x 8192 x 2048, in us: 20.5 here, 20.3; 1024 x 4096 x 4096: 31.9, 29.0; 1024 x 2048 x 8192: 31.6, 42.9.
-bool few_tokens(const LinearArgs& a) {
+bool few_tokens(const LinearArgs& a, int64_t features) {
     if (gemm_cta_limit() <= 0 && a.M <= kFewTokens) return true;
-    const FewPlan plan = few_plan(a.M, a.N, a.K);
+    const FewPlan plan = few_plan(a.M, features, a.K);
     if (plan.cluster == 0) return false;
     if (a.M <= kFewTokens) return true;
     const int64_t k_steps = (a.K + BK - 1) / BK, pairs = gemm_cta_limit() > 0 ? std::max(1, gemm_cta_limit() / 2) : kMaxPairs;
-    const int64_t small = (int64_t)((a.N + BM - 1) / BM) * ((a.M + kFewTokens - 1) / kFewTokens), large = (int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256);
+    const int64_t small = (int64_t)((features + BM - 1) / BM) * ((a.M + kFewTokens - 1) / kFewTokens), large = (int64_t)((features + 255) / 256) * ((a.M + 255) / 256);
     if (small > 4 * pairs) return false;
     return plan.steps < (float)((large + pairs - 1) / pairs * k_steps) + 16.f;
 }
 
-template <bool DGRAD>
+// Rows of products: of a gated layer's, each tile has 64 of the gate and the 64 that go with them
+inline int64_t few_features(const LinearArgs& a) { return a.gated && !a.dgrad ? (a.N + 63) / 64 * (int64_t)BM : a.N; }
+
+template <bool DGRAD, int KIND>
 int linear_few(const LinearArgs& a, cudaStream_t s) {
+    constexpr bool GATED_FWD = KIND == kLinGated && !DGRAD;
     FewParams p;
     p.M = a.M;
     p.N = a.N;
@@ -463,7 +524,7 @@ int linear_few(const LinearArgs& a, cudaStream_t s) {
     p.columns = few_columns(a.M);
     if (!make_map(&p.map_x, a.a, (uint64_t)a.M, (uint64_t)a.K, (uint64_t)a.lda, p.columns)) return -3;
     if (!(DGRAD ? make_map(&p.map_w, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, 64)
-                : make_map(&p.map_w, a.w, (uint64_t)a.N, (uint64_t)a.K, (uint64_t)a.ldw, BM)))
+                : make_map(&p.map_w, a.w, (uint64_t)a.N * (GATED_FWD ? 2 : 1), (uint64_t)a.K, (uint64_t)a.ldw, GATED_FWD ? BM / 2 : BM)))
         return -3;
     p.bias = a.bias_f32 ? nullptr : (const __nv_bfloat16*)a.bias;
     p.bias32 = a.bias_f32 ? (const float*)a.bias : nullptr;
@@ -484,18 +545,35 @@ int linear_few(const LinearArgs& a, cudaStream_t s) {
     p.out_wide = wide(a.out, a.ldo);
     p.out2_wide = wide(a.out2, a.ldo2);
     p.pre_wide = wide(a.pre, a.ldpre);
+    p.drop = a.drop;
+    if constexpr (KIND == kLinGated) {
+        p.q_up = (int8_t*)a.q_up;
+        p.ldq_up = a.ldq_up;
+        p.e_up = (uint8_t*)a.e_up;
+        p.lde_up = a.lde_up;
+        p.pre_up_wide = p.pre != nullptr ? wide(p.pre + a.N, a.ldpre) : 0;
+        p.out_up_wide = wide(p.out + a.N, a.ldo);
+    }
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
-    p.n_tiles = (a.N + BM - 1) / BM;
-    const int cluster = few_plan(a.M, a.N, a.K).cluster;
+    const int64_t features = few_features(a);
+    p.n_tiles = (int)((features + BM - 1) / BM);
+    const int cluster = few_plan(a.M, features, a.K).cluster;
+    constexpr int MODE = DGRAD ? kFewDgrad : kFewFwd;
     switch (a.act) {
-        case kActNone: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActNone>(p, cluster, s);
-        case kActRelu: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActRelu>(p, cluster, s);
-        case kActGelu: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActGelu>(p, cluster, s);
-        case kActGeluTanh: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActGeluTanh>(p, cluster, s);
-        case kActSilu: return launch_few<DGRAD ? kFewDgrad : kFewFwd, kActSilu>(p, cluster, s);
+        case kActNone: return launch_few<MODE, kActNone, KIND>(p, cluster, s);
+        case kActRelu: return launch_few<MODE, kActRelu, KIND>(p, cluster, s);
+        case kActGelu: return launch_few<MODE, kActGelu, KIND>(p, cluster, s);
+        case kActGeluTanh: return launch_few<MODE, kActGeluTanh, KIND>(p, cluster, s);
+        case kActSilu: return launch_few<MODE, kActSilu, KIND>(p, cluster, s);
     }
     return -2;
+}
+
+// The kernel that takes such a product
+template <bool DGRAD, int KIND>
+int linear_by_size(const LinearArgs& a, cudaStream_t s) {
+    return few_tokens(a, few_features(a)) ? linear_few<DGRAD, KIND>(a, s) : linear_typed<DGRAD, KIND>(a, s);
 }
 
 }  // namespace

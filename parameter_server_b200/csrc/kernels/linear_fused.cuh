@@ -3,6 +3,11 @@
 //   forward   h = x w^T + b,   y = act(h) + residual,   h kept for the backward pass in bf16 or in 8 bits
 //   dgrad     dh = (dy w) * act'(h),   and act(h) again, for the weight gradient of the layer that dy belongs to
 //
+// and in the gated form, with w the gate's rows and those of the second factor behind them:
+//
+//   forward   g = x wg^T + bg, u = x wu^T + bu,   y = act(g) * u,   g and u kept
+//   dgrad     da = dy w:   dg = da * u * act'(g) and du = da * act(g) side by side,   and act(g) * u again
+//
 // bf16 operands, fp32 accumulation in TMEM; everything in the epilogue is fp32 and rounded once per output. (The tensor core cuts
 // its sums off instead of rounding them, 1e-9 of the sum per product: 9e-6 at K = 8192, far below the rounding of a bf16 output.)
 // Fusing the neighbours saves their passes over M x N values through HBM; the product itself is bound by the tensor cores and by
@@ -29,6 +34,7 @@
 #include "act8.cuh"
 #include "gemm_tcgen05.h"
 #include "linear_fused.h"
+#include "philox.cuh"
 #include "tcgen05.cuh"
 #include "tile_walk.cuh"
 
@@ -36,6 +42,8 @@ namespace psb {
 
 namespace {
 
+// What the epilogue is of: one product, a gated pair of them, or one with dropout behind its activation
+constexpr int kLinPlain = 0, kLinGated = 1, kLinDropout = 2;
 constexpr int kLinEpilogueWarps = 8;
 constexpr int kLinThreads = 32 * (4 + kLinEpilogueWarps);
 constexpr int kLinRegsIssue = 56, kLinRegsEpilogue = 224;   // 56 + 2 * 224 = 3 * 168, the launch's share
@@ -79,6 +87,15 @@ struct LinParams {
     int aux_width, pre_width, out_width, out2_width;   // rows of residual (forward) / pre / out / out2 start on multiples of 16, 8, 4 or 2
     float* partial;                   // shared tiles: [pair][2 places][cta][warp][BN / 64 pieces][8][32 lanes][4]
     unsigned* arrived;                // [shared tile][cta][warp]
+    // gated: the second factor's columns of pre, of the checkpoint and (dgrad) of out
+    __nv_bfloat16* pre_up;
+    __nv_bfloat16* out_up;
+    int pre_up_width, out_up_width;
+    int8_t* q_up;
+    int64_t ldq_up;
+    uint8_t* e_up;
+    int64_t lde_up;
+    DropoutArgs drop;
     unsigned* err_flag;
     unsigned long long limit_ns;
 };
@@ -159,6 +176,12 @@ __device__ __forceinline__ float bf16_at(const uint4* raw, int j) {   // j is a 
     const uint4 v = raw[j / 8];
     const uint32_t w = (j / 2) % 4 == 0 ? v.x : (j / 2) % 4 == 1 ? v.y : (j / 2) % 4 == 2 ? v.z : v.w;
     return __uint_as_float((j & 1) ? (w & 0xFFFF0000u) : (w << 16));
+}
+// Value j of 32 whole numbers of a checkpoint
+__device__ __forceinline__ float s8_at(const uint4* raw, int j) {   // j is a constant after unrolling
+    const uint4 v = raw[j / 16];
+    const uint32_t w = ((j / 4) % 4 == 0 ? v.x : (j / 4) % 4 == 1 ? v.y : (j / 4) % 4 == 2 ? v.z : v.w) ^ 0x80808080u;
+    return j % 4 == 0 ? s8_of_biased<0>(w) : j % 4 == 1 ? s8_of_biased<1>(w) : j % 4 == 2 ? s8_of_biased<2>(w) : s8_of_biased<3>(w);
 }
 // Where in the warp's 2 KB the bytes [16 j, 16 j + 16) of row r of a [32 rows][64 bytes] piece lie
 __device__ __forceinline__ uint32_t in_piece(uint32_t stage, int r, int byte) {
@@ -281,9 +304,11 @@ __device__ __forceinline__ uint32_t keep_row32(const float* f, int8_t* qp, int n
 }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
-template <bool DGRAD, int ACT, int BN>
+template <bool DGRAD, int ACT, int BN, int KIND>
 __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __grid_constant__ LinParams p) {
     using L = LinSmem<BN>;
+    constexpr bool GATED_FWD = KIND == kLinGated && !DGRAD, GATED_DGRAD = KIND == kLinGated && DGRAD;
+    constexpr int kWide = GATED_FWD ? BN / 2 : BN;   // output columns of a tile: of a gated one's BN products, half are the gate's
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full_bar = (uint64_t*)(smem + L::kTileBytes);
@@ -340,7 +365,8 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 uint32_t it = 0;
                 bool ok = true;
                 while (ok && walk.next(p.grid, t)) {
-                    const int m0 = t.m * 2 * BM + cr * BM, n0 = t.n * BN + cr * (BN / 2);
+                    // (gated: the leader has the gate's rows of w, the other CTA the rows behind them)
+                    const int m0 = t.m * 2 * BM + cr * BM, n0 = t.n * kWide + cr * (GATED_FWD ? p.N : BN / 2);
                     for (int k = 0; k < t.nk; k += L::kSub, ++it) {
                         const int s = it % L::kStages;
                         const int n = min(L::kSub, t.nk - k);
@@ -425,29 +451,32 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLinRegsEpilogue));
         // ---- epilogue ----
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2, etid = ew * 32 + lane;
-        constexpr int kPieces = BN / 64;   // 32-column pieces of a warp
+        constexpr int kPieces = kWide / 64;   // 32-column pieces of a warp
         const uint32_t stage = smem_u32(stage_out) + (uint32_t)ew * 2048;
         TileWalk walk(p.grid, pair);
         Tile t;
         uint32_t tc = 0;
+        [[maybe_unused]] DropKey key;
+        if constexpr (KIND == kLinDropout) key = drop_key(p.drop);
         while (walk.next(p.grid, t)) {
             const uint32_t buf = tc & 1u;
-            const int tile_n = t.n * BN, row0 = t.m * 2 * BM + cr * BM + quarter * 32, row = row0 + lane;
-            const int cbase = half * (BN / 2), colw = tile_n + cbase;   // first column of this warp
+            const int tile_n = t.n * kWide, row0 = t.m * 2 * BM + cr * BM + quarter * 32, row = row0 + lane;
+            const int cbase = half * (kWide / 2), colw = tile_n + cbase;   // first column of this warp
             const bool live = row < p.M;
             const uint32_t bs = smem_u32(bias_smem) + buf * (uint32_t)(BN * 4);
             if constexpr (!DGRAD) {
                 if (etid < BN) {   // (BN = 128: the first four warps)
-                    const int col = tile_n + etid;
+                    const int col = tile_n + etid % kWide, at = GATED_FWD && etid >= kWide ? p.N + col : col;
                     float v = 0.f;
-                    if (col < p.N) v = p.bias32 != nullptr ? p.bias32[col] : p.bias != nullptr ? __bfloat162float(p.bias[col]) : 0.f;
+                    if (col < p.N) v = p.bias32 != nullptr ? p.bias32[at] : p.bias != nullptr ? __bfloat162float(p.bias[at]) : 0.f;
                     asm volatile("st.shared.f32 [%0], %1;" ::"r"(bs + (uint32_t)etid * 4), "f"(v) : "memory");
                 }
             }
             // What a piece needs from memory (residual, or h) is requested before the piece ahead of it is worked on, the first
             // one before the wait for the accumulator.
             uint4 aux[4], coming[4];
-            uint32_t ex = 0;
+            [[maybe_unused]] uint4 aux_up[4], coming_up[4];
+            [[maybe_unused]] uint32_t ex = 0, ex_up = 0;
             const __nv_bfloat16* aux_row = DGRAD ? p.pre : p.res;
             const int64_t aux_ld = DGRAD ? p.ldpre : p.ldres;
             const int aux_width = DGRAD ? p.pre_width : p.aux_width;
@@ -459,23 +488,42 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     get_narrow(stage, lane, aux_row + (int64_t)row0 * aux_ld + col, aux_ld * 2, min(32, p.M - row0), 2 * min(32, p.N - col), aux_width);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) coming[j] = ld_smem_v4(in_piece(stage, lane, j * 16));
-                    return;
-                }
-                if (!live) return;
-                if (kept8) {
+                    if constexpr (!GATED_DGRAD) return;
+                } else if (live && kept8) {
                     const int8_t* qp = p.q + (int64_t)row * p.ldq + col;
                     coming[0] = ld_global_v4(qp);
                     if (col + 16 < p.N) coming[1] = ld_global_v4(qp + 16);
-                } else if (aux_row != nullptr) {
+                } else if (live && aux_row != nullptr) {
                     load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, coming);
+                }
+                if constexpr (GATED_DGRAD) {
+                    if (!kept8 && p.pre_up_width != 16) {
+                        get_narrow(stage, lane, p.pre_up + (int64_t)row0 * aux_ld + col, aux_ld * 2, min(32, p.M - row0), 2 * min(32, p.N - col), p.pre_up_width);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) coming_up[j] = ld_smem_v4(in_piece(stage, lane, j * 16));
+                    } else if (live && kept8) {
+                        const int8_t* qp = p.q_up + (int64_t)row * p.ldq_up + col;
+                        coming_up[0] = ld_global_v4(qp);
+                        if (col + 16 < p.N) coming_up[1] = ld_global_v4(qp + 16);
+                    } else if (live) {
+                        load32(p.pre_up + (int64_t)row * aux_ld + col, p.N - col, coming_up);
+                    }
                 }
             };
 #pragma unroll
             for (int j = 0; j < 4; ++j) coming[j] = make_uint4(0, 0, 0, 0);
+            if constexpr (GATED_DGRAD) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) coming_up[j] = make_uint4(0, 0, 0, 0);
+            }
             if (t.runs == 1) fetch(0);
             if (kept8 && live && colw < p.N) {   // one byte per piece; rows of e are padded to 16
                 if constexpr (kPieces == 4) ex = *(const uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32);
                 else ex = *(const uint16_t*)(p.e + (int64_t)row * p.lde + colw / 32);
+                if constexpr (GATED_DGRAD) {
+                    if constexpr (kPieces == 4) ex_up = *(const uint32_t*)(p.e_up + (int64_t)row * p.lde_up + colw / 32);
+                    else ex_up = *(const uint16_t*)(p.e_up + (int64_t)row * p.lde_up + colw / 32);
+                }
             }
             // One barrier of the epilogue warps per tile: publishes the bias, and makes the decision to give up uniform. One warp
             // asks for the accumulator, the others sleep at this barrier (asking takes issue slots from the MMAs' thread).
@@ -492,24 +540,67 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) mbar_arrive_pair(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
             };
-            // one 32-column piece with its values in f
+            // one 32-column piece with its values in f (gated: the gate's in f, the other factor's in u)
             uint32_t ewrite = 0;
-            auto finish = [&](float* f, int c) {
+            [[maybe_unused]] uint32_t ewrite_up = 0;
+            auto add_bias = [&](float* f, int at) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const uint4 b = ld_smem_v4(bs + (uint32_t)(at + j) * 4);
+                    f[j] += __uint_as_float(b.x); f[j + 1] += __uint_as_float(b.y);
+                    f[j + 2] += __uint_as_float(b.z); f[j + 3] += __uint_as_float(b.w);
+                }
+            };
+            auto finish = [&](float* f, [[maybe_unused]] float* u, int c) {
                 const int col = colw + c * 32;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) aux[j] = coming[j];
-                fetch(c + 1);
-                if constexpr (!DGRAD) {
+                if constexpr (GATED_DGRAD) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const uint4 b = ld_smem_v4(bs + (uint32_t)(cbase + c * 32 + j) * 4);
-                        f[j] += __uint_as_float(b.x); f[j + 1] += __uint_as_float(b.y);
-                        f[j + 2] += __uint_as_float(b.z); f[j + 3] += __uint_as_float(b.w);
+                    for (int j = 0; j < 4; ++j) aux_up[j] = coming_up[j];
+                }
+                fetch(c + 1);
+                if constexpr (GATED_FWD) {
+                    add_bias(f, cbase + c * 32);
+                    add_bias(u, kWide + cbase + c * 32);
+                    if (p.pre != nullptr) {
+                        store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
+                        store_piece(stage, lane, u, p.pre_up, p.ldpre, row0, col, p.M, p.N, p.pre_up_width);
                     }
+                    if (p.q != nullptr) {
+                        if (col + 32 > p.N) {   // behind the gate's last row of w, the tile has the other factor's first
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) f[j] = col + j < p.N ? f[j] : 0.f;
+                        }
+                        ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
+                        ewrite_up |= keep_row32(u, p.q_up + (int64_t)row * p.ldq_up + col, p.N - col, live) << (8 * c);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]) * u[j];
+                } else if constexpr (GATED_DGRAD) {
+                    float a[32], du[32];
+                    const float step = kept8 ? act8_step((ex >> (8 * c)) & 255u) : 0.f, step_up = kept8 ? act8_step((ex_up >> (8 * c)) & 255u) : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float g = kept8 ? s8_at(aux, j) * step : bf16_at(aux, j), up = kept8 ? s8_at(aux_up, j) * step_up : bf16_at(aux_up, j);
+                        float value;
+                        const float slope = act_slope<ACT>(g, &value);
+                        du[j] = f[j] * value;
+                        a[j] = value * up;
+                        f[j] *= up * slope;
+                    }
+                    store_piece(stage, lane, du, p.out_up, p.ldo, row0, col, p.M, p.N, p.out_up_width);
+                    if (p.out2 != nullptr) store_piece(stage, lane, a, p.out2, p.ldo2, row0, col, p.M, p.N, p.out2_width);
+                } else if constexpr (!DGRAD) {
+                    add_bias(f, cbase + c * 32);
                     if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
                     if (p.q != nullptr) ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]);
+                    if constexpr (KIND == kLinDropout) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) drop4(key, p.drop.threshold, p.drop.scale, (uint32_t)row, (uint32_t)(col + j) / 4, f + j);
+                    }
                     if (p.res != nullptr) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) f[j] += bf16_at(aux, j);
@@ -541,7 +632,23 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 continue;
             }
             uint32_t v[32];
-            if (t.runs == 1) {
+            if constexpr (GATED_FWD) {
+                if (t.runs == 1) {
+#pragma unroll 1
+                    for (int c = 0; c < kPieces; ++c) {
+                        if (colw + c * 32 >= p.N) break;   // warp-uniform
+                        float f[32], u[32];
+                        tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
+                        tmem_ld32_issue(taddr + (uint32_t)(kWide + c * 32), (uint32_t*)u);
+                        tmem_wait_ld(v);
+                        tmem_wait_ld((uint32_t*)u);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                        finish(f, u, c);
+                    }
+                    release();
+                }
+            } else if (t.runs == 1) {
                 if (colw < p.N) tmem_ld32_issue(taddr, v);
 #pragma unroll 1
                 for (int c = 0; c < kPieces; ++c) {
@@ -551,20 +658,22 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
 #pragma unroll
                     for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
                     if (c + 1 < kPieces && colw + c * 32 + 32 < p.N) tmem_ld32_issue(taddr + (uint32_t)(c + 1) * 32u, v);
-                    finish(f, c);
+                    finish(f, nullptr, c);
                 }
                 release();
-            } else {
+            }
+            if (t.runs > 1) {
                 // shared tile: this pair's part goes to memory; the last one to arrive adds all parts in run order
-                constexpr int64_t kWarpFloats = kPieces * 1024;
+                constexpr int kParts = BN / 64;   // (gated: the gate's pieces, then the other factor's)
+                constexpr int64_t kWarpFloats = kParts * 1024;
                 auto part_of = [&](int worker, int slot) {
                     return p.partial + ((((int64_t)worker * 2 + slot) * 2 + cr) * kLinEpilogueWarps + ew) * kWarpFloats + lane * 4;
                 };
                 float* mine = part_of(pair, t.slot);
 #pragma unroll 1
-                for (int c = 0; c < kPieces; ++c) {
-                    if (colw + c * 32 >= p.N) break;
-                    tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
+                for (int c = 0; c < kParts; ++c) {
+                    if (colw + c % kPieces * 32 >= p.N) continue;
+                    tmem_ld32_issue(taddr + (uint32_t)(c / kPieces * kWide + c % kPieces * 32), v);
                     tmem_wait_ld(v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -583,19 +692,28 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
 #pragma unroll 1
                     for (int c = 0; c < kPieces; ++c) {
                         if (colw + c * 32 >= p.N) break;
-                        float f[32];
+                        auto joined = [&](float* f, int part) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) f[j] = 0.f;
+                            for (int j = 0; j < 32; ++j) f[j] = 0.f;
 #pragma unroll 1
-                        for (int r = 0; r < t.runs; ++r) {
-                            const float* src = part_of(t.first + r, TileWalk::slot_of(p.grid, t, r)) + c * 1024;
+                            for (int r = 0; r < t.runs; ++r) {
+                                const float* src = part_of(t.first + r, TileWalk::slot_of(p.grid, t, r)) + part * 1024;
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float4 x = __ldcg((const float4*)(src + j * 128));
-                                f[4 * j] += x.x; f[4 * j + 1] += x.y; f[4 * j + 2] += x.z; f[4 * j + 3] += x.w;
+                                for (int j = 0; j < 8; ++j) {
+                                    const float4 x = __ldcg((const float4*)(src + j * 128));
+                                    f[4 * j] += x.x; f[4 * j + 1] += x.y; f[4 * j + 2] += x.z; f[4 * j + 3] += x.w;
+                                }
                             }
+                        };
+                        float f[32];
+                        joined(f, c);
+                        if constexpr (GATED_FWD) {
+                            float u[32];
+                            joined(u, kPieces + c);
+                            finish(f, u, c);
+                        } else {
+                            finish(f, nullptr, c);
                         }
-                        finish(f, c);
                     }
                 } else {
                     ++tc;
@@ -606,6 +724,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 if (p.q != nullptr && live && colw < p.N) {
                     if constexpr (kPieces == 4) *(uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32) = ewrite;
                     else *(uint16_t*)(p.e + (int64_t)row * p.lde + colw / 32) = (uint16_t)ewrite;
+                    if constexpr (GATED_FWD) *(uint16_t*)(p.e_up + (int64_t)row * p.lde_up + colw / 32) = (uint16_t)ewrite_up;
                 }
             }
             ++tc;
@@ -667,29 +786,30 @@ cudaError_t launch_pairs(Kernel kern, int threads, int smem, int pairs, const Pa
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <bool DGRAD, int ACT, int BN>
+template <bool DGRAD, int ACT, int BN, int KIND>
 int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
-    constexpr auto kern = linear_fused_kernel<DGRAD, ACT, BN>;
+    constexpr auto kern = linear_fused_kernel<DGRAD, ACT, BN, KIND>;
+    const int rows_of_w = KIND == kLinGated && !DGRAD ? 2 * p.N : p.N, wide = KIND == kLinGated && !DGRAD ? BN / 2 : BN;
     int pairs = 0;
     cudaError_t e = pairs_of<kern>(kLinThreads, LinSmem<BN>::kTotal, &pairs);
     if (e != cudaSuccess) return (int)e;
     // A weight that L2 holds beside the stream of activations is walked along n (16384 x 2048 x 8192 with a residual, sustained:
     // 429 us, in groups of 8 rows 441); a larger one in blocks (8192^3: 844 us, along n 923).
-    const int group = (int64_t)p.N * k_steps * BK * 2 <= (48ll << 20) ? 1 : 8;
+    const int group = (int64_t)rows_of_w * k_steps * BK * 2 <= (48ll << 20) ? 1 : 8;
     // Joining a cut tile takes 10 to 20 us (its parts are read one after the other, eight 16-byte loads in flight per thread).
-    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + BN - 1) / BN, k_steps, pairs, 64, group);
+    p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + wide - 1) / wide, k_steps, pairs, 64, group);
     if (p.grid.shared > 0 && p.arrived == nullptr) return kNeedsWorkspace;
     return (int)launch_pairs(kern, kLinThreads, LinSmem<BN>::kTotal, p.grid.pairs, p, s);
 }
 
-template <bool DGRAD, int BN>
+template <bool DGRAD, int BN, int KIND>
 int launch_act(int act, LinParams& p, int k_steps, cudaStream_t s) {
     switch (act) {
-        case kActNone: return launch_linear<DGRAD, kActNone, BN>(p, k_steps, s);
-        case kActRelu: return launch_linear<DGRAD, kActRelu, BN>(p, k_steps, s);
-        case kActGelu: return launch_linear<DGRAD, kActGelu, BN>(p, k_steps, s);
-        case kActGeluTanh: return launch_linear<DGRAD, kActGeluTanh, BN>(p, k_steps, s);
-        case kActSilu: return launch_linear<DGRAD, kActSilu, BN>(p, k_steps, s);
+        case kActNone: return launch_linear<DGRAD, kActNone, BN, KIND>(p, k_steps, s);
+        case kActRelu: return launch_linear<DGRAD, kActRelu, BN, KIND>(p, k_steps, s);
+        case kActGelu: return launch_linear<DGRAD, kActGelu, BN, KIND>(p, k_steps, s);
+        case kActGeluTanh: return launch_linear<DGRAD, kActGeluTanh, BN, KIND>(p, k_steps, s);
+        case kActSilu: return launch_linear<DGRAD, kActSilu, BN, KIND>(p, k_steps, s);
     }
     return -2;
 }
@@ -701,16 +821,17 @@ int width_of(const void* p, int64_t ld) {
 }
 bool rows16(const void* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && (ld % 8) == 0; }
 
-template <bool DGRAD>
+template <bool DGRAD, int KIND>
 int linear_typed(const LinearArgs& a, cudaStream_t s) {
+    constexpr bool GATED_FWD = KIND == kLinGated && !DGRAD;
     // tiles 128 wide only where 256 would be more than half padding: they need twice the operand bytes per flop
-    const int BN = a.N > 128 ? 256 : 128;
+    const int BN = a.N > 128 || GATED_FWD ? 256 : 128;
     LinParams p;
     p.M = a.M;
     p.N = a.N;
     p.b_blocked = DGRAD && a.N % 64 == 0 && a.N >= BN ? 1 : 0;
     if (!make_map(&p.map_a, a.a, (uint64_t)a.M, (uint64_t)a.K, (uint64_t)a.lda, BM)) return -3;
-    const bool ok = !DGRAD ? make_map(&p.map_b, a.w, (uint64_t)a.N, (uint64_t)a.K, (uint64_t)a.ldw, BN / 2)
+    const bool ok = !DGRAD ? make_map(&p.map_b, a.w, (uint64_t)a.N * (GATED_FWD ? 2 : 1), (uint64_t)a.K, (uint64_t)a.ldw, BN / 2)
                    : p.b_blocked ? make_map_blocked(&p.map_b, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, BN / 128)
                                  : make_map(&p.map_b, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.ldw, 64);
     if (!ok) return -3;
@@ -732,17 +853,32 @@ int linear_typed(const LinearArgs& a, cudaStream_t s) {
     p.pre_width = width_of(a.pre, a.ldpre);
     p.out_width = width_of(a.out, a.ldo);
     p.out2_width = width_of(a.out2, a.ldo2);
+    p.drop = a.drop;
+    if constexpr (KIND == kLinGated) {
+        p.pre_up = p.pre == nullptr ? nullptr : p.pre + a.N;
+        p.out_up = p.out + a.N;
+        p.q_up = (int8_t*)a.q_up;
+        p.ldq_up = a.ldq_up;
+        p.e_up = (uint8_t*)a.e_up;
+        p.lde_up = a.lde_up;
+        p.pre_up_width = width_of(p.pre_up, a.ldpre);
+        p.out_up_width = width_of(p.out_up, a.ldo);
+    }
     p.arrived = (unsigned*)a.workspace;
     p.partial = a.workspace == nullptr ? nullptr : (float*)((uint8_t*)a.workspace + linear_workspace_zeros());
     p.err_flag = a.err_flag;
     p.limit_ns = (unsigned long long)(a.wait_limit_s * 1e9);
     const int k_steps = (a.K + BK - 1) / BK;
-    return BN == 256 ? launch_act<DGRAD, 256>(a.act, p, k_steps, s) : launch_act<DGRAD, 128>(a.act, p, k_steps, s);
+    if constexpr (GATED_FWD) return launch_act<false, 256, KIND>(a.act, p, k_steps, s);
+    else return BN == 256 ? launch_act<DGRAD, 256, KIND>(a.act, p, k_steps, s) : launch_act<DGRAD, 128, KIND>(a.act, p, k_steps, s);
 }
 
 }  // namespace
 
 int linear_fused_fwd(const LinearArgs& a, cudaStream_t s);
 int linear_fused_dgrad(const LinearArgs& a, cudaStream_t s);
+int linear_gated_fwd(const LinearArgs& a, cudaStream_t s);
+int linear_gated_dgrad(const LinearArgs& a, cudaStream_t s);
+int linear_dropout_fwd(const LinearArgs& a, cudaStream_t s);
 
 }  // namespace psb

@@ -2,6 +2,8 @@
 #pragma once
 #include <cstdint>
 
+#include "dropout.h"
+
 namespace psb {
 
 enum LinearActivation { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
@@ -9,7 +11,12 @@ enum LinearActivation { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh =
 struct LinearArgs {
     // forward:  h = a w^T + bias, out = act(h) + residual; a [M][K], w [N][K]; h kept in `pre` (bf16) or `q` / `e` (8 bits)
     // dgrad:    out = (a w) * act'(h), out2 = act(h);      a [M][K], w [K][N]; h read from `pre` or `q` / `e`
+    // with `drop`:    out = dropout(act(h)) + residual
+    // gated (N counts the outputs): forward  [g | u] = a w^T + bias, out = act(g) * u; w [2N][K], bias [2N]; g and u kept side by side in
+    //                 `pre` [M][2N], or in `q` / `e` and `q_up` / `e_up`;  dgrad  a w = da, out [M][2N] = [da * u * act'(g) | da * act(g)],
+    //                 out2 = act(g) * u; w [K][N]
     int dgrad = 0;
+    int gated = 0;
     int act = 0;
     const void* a = nullptr;
     int64_t lda = 0;
@@ -29,6 +36,11 @@ struct LinearArgs {
     int64_t ldq = 0;
     void* e = nullptr;
     int64_t lde = 0;
+    void* q_up = nullptr;            // gated: the second factor's, like q / e
+    int64_t ldq_up = 0;
+    void* e_up = nullptr;
+    int64_t lde_up = 0;
+    DropoutArgs drop;                // forward; threshold 0: none
     int M = 0, N = 0, K = 0;
     void* workspace = nullptr;       // linear_workspace_bytes() bytes; the first linear_workspace_zeros() are zero before the
                                      // first call and left zero by every call. Null: tried without (see kNeedsWorkspace)

@@ -6,7 +6,7 @@ namespace psb {
 
 int linear_fused_dgrad(const LinearArgs& a, cudaStream_t s) {
     if (a.pre == nullptr && a.q == nullptr && a.act != kActNone) return -2;
-    return few_tokens(a) ? linear_few<true>(a, s) : linear_typed<true>(a, s);
+    return linear_by_size<true, kLinPlain>(a, s);
 }
 
 }  // namespace psb

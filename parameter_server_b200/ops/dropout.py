@@ -63,7 +63,7 @@ def _dropout(x, p, seed, offset, residual, out, what):
     if rows > 0xFFFFFFFF:
         raise ValueError(f"{what}: at most 2^32 - 1 rows")
     if rows and cols:
-        check(C.dropout(dt, x2.data_ptr(), row_stride(x2), rp, ldr, y.data_ptr(), row_stride(y), rows, cols, *drop, s), what)
+        check(C.dropout(dt, x2.data_ptr(), row_stride(x2), rp, ldr, y.data_ptr(), row_stride(y), rows, cols, drop, s), what)
     if out is not None:
         return out
     return y if x.dim() == 2 else y.view(x.shape)

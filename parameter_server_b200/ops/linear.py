@@ -1,7 +1,7 @@
 """Linear layers of a decoder block with their neighbours in the epilogue (``csrc/kernels/linear_fused.cuh``), bf16 operands and
 fp32 sums:
 
-* ``linear_act``: ``act(x w^T + b) + residual``, with the value before the activation kept for the backward pass;
+* ``linear_act``: ``act(x w^T + b) + residual``, with the value before the activation kept for the backward pass, and dropout between;
 * ``linear_act_dgrad``: the gradient that reaches that value, ``(dy w) * act'(h)``, and ``act(h)`` again;
 * ``linear_bias_grad``: the sum of dy's rows in a fixed order.
 
@@ -16,6 +16,7 @@ import torch
 
 from .._lib import C
 from .act8 import _DTYPES, NEEDS_WORKSPACE, Act8, check, launch_stream, operand, result, row_stride, rows2d, vector
+from .dropout import NO_DROPOUT, drop_args
 from .gemm import err_ptr, workspace
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -45,28 +46,30 @@ def _beside(t: torch.Tensor, what: str, device: int):
     return at, ld, t
 
 
-def _run(dev, s, what, head, tail, limit):
-    rc = C.linear_fused(*head, *tail, 0, err_ptr(dev), limit, s)
+def _run(dev, s, what, head, tail, limit, up=_NOT_KEPT, drop=NO_DROPOUT):
+    rc = C.linear_fused(*head, *tail, *up, drop, 0, err_ptr(dev), limit, s)
     if rc == NEEDS_WORKSPACE:   # only where tiles are cut along the contraction
         scratch = workspace(dev, s)
-        rc = C.linear_fused(*head, *tail, scratch.data_ptr(), err_ptr(dev), limit, s)
+        rc = C.linear_fused(*head, *tail, *up, drop, scratch.data_ptr(), err_ptr(dev), limit, s)
     check(rc, what)
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
                residual: Optional[torch.Tensor] = None, save: Optional[str] = None, out: Optional[torch.Tensor] = None,
-               wait_limit_s: float = 2.0):
+               dropout: Optional[tuple] = None, wait_limit_s: float = 2.0):
     """``act(x w^T + bias) + residual`` for ``x`` ``[..., K]``, ``w`` ``[N, K]`` (bf16), ``bias`` ``[N]`` (bf16 or fp32) and
     ``residual`` ``[..., N]`` (bf16). ``act``: "none", "relu", "gelu", "gelu_tanh" or "silu".
 
     ``save`` = "bf16" or "act8" also returns ``h = x w^T + bias`` as :func:`linear_act_dgrad` takes it: ``(y, h)`` with ``h`` a bf16
-    tensor like ``y``, or an :class:`~.act8.Act8`. ``out`` (bf16, may be ``residual`` itself) receives ``y``. Results whose ``N`` is no
+    tensor like ``y``, or an :class:`~.act8.Act8`. ``dropout`` = ``(p, seed, offset)`` drops values behind the activation, ahead of the residual,
+    as :func:`~.dropout.dropout` does with the same three (``dropout_backward`` takes the gradient back). ``out`` (bf16, may be ``residual`` itself) receives ``y``. Results whose ``N`` is no
     multiple of 8 have padded rows (``stride(-2)``), as the next product wants them."""
     what = "linear_act"
     code = _act_code(act, what)
     if save not in (None, "bf16", "act8"):
         raise ValueError(f"{what}: save is None, 'bf16' or 'act8', not {save!r}")
     s, dev = launch_stream(x), x.get_device()
+    drop = NO_DROPOUT if dropout is None else drop_args(*dropout, dev, what)
     x2, xp, ldx, _held = operand(x, "linear_act x", dev)
     w, wp, ldw, _held_w = operand(w, "linear_act w", dev)
     M, K = x2.shape
@@ -92,9 +95,9 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     pre, ldpre = result(x2, M, N) if save == "bf16" else (None, 0)
     kept = Act8.for_rows(y, N) if save == "act8" else None
     if M and N:
-        _run(dev, s, what, (False, code, M, N, K, xp, ldx, wp, ldw, bp, bias is not None and bias.dtype is torch.float32),
+        _run(dev, s, what, (False, False, code, M, N, K, xp, ldx, wp, ldw, bp, bias is not None and bias.dtype is torch.float32),
              (rp, ldr, y.data_ptr(), ldy, 0, 0,
-              0 if pre is None else pre.data_ptr(), ldpre, *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
+              0 if pre is None else pre.data_ptr(), ldpre, *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s, drop=drop)
     if out is not None:
         y = out
     elif x.dim() != 2:
@@ -133,7 +136,7 @@ def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, A
     dh, ld = result(dy2, M, N)
     a = result(dy2, M, N)[0] if recompute else None
     if M and N:
-        _run(dev, s, what, (True, code, M, N, K, dyp, lddy, wp, ldw, 0, False),
+        _run(dev, s, what, (True, False, code, M, N, K, dyp, lddy, wp, ldw, 0, False),
              (0, 0, dh.data_ptr(), ld, 0 if a is None else a.data_ptr(), ld, pre, ldpre,
               *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
     if dy.dim() != 2:

@@ -6,7 +6,7 @@ import philox64
 import pytest
 import torch
 
-from parameter_server_b200.ops import dropout, rotary
+from parameter_server_b200.ops import act8, dropout, gated, linear, rotary
 
 BF = torch.bfloat16
 gpu = pytest.mark.gpu
@@ -25,7 +25,8 @@ def test_the_generator_has_its_published_answers():
 
 def test_host_tensors_are_refused():
     x, f = torch.zeros(2, 3, 8, dtype=BF), torch.ones(4, dtype=torch.float64)
-    for call in (lambda: dropout.dropout(x, 0.1, 1), lambda: dropout.dropout_backward(x, 0.1, 1), lambda: rotary.rotary(x, x, f), lambda: rotary.rotary_backward(x, None, f)):
+    for call in (lambda: dropout.dropout(x, 0.1, 1), lambda: dropout.dropout_backward(x, 0.1, 1), lambda: rotary.rotary(x, x, f), lambda: rotary.rotary_backward(x, None, f),
+                 lambda: gated.gated_linear(x, x), lambda: gated.gated_linear_dgrad(x, x, x)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
 
@@ -96,6 +97,30 @@ def test_types_and_shapes_of_rotary_are_refused():
         lambda: rotary.rotary(q, k, z(16, dtype=torch.float64)[::2]), lambda: rotary.rotary(q, k, f, pos.float()), lambda: rotary.rotary(q, k, f, pos[:2]),
         lambda: rotary.rotary(q, k, f, pos.cpu()), lambda: rotary.rotary(q, k, f, pos.expand(3, 3)), lambda: rotary.rotary(q, k, f, out_q=z(2, 3, 4, 17)),
         lambda: rotary.rotary(q, None, f, out_k=k), lambda: rotary.rotary(q, k, f, out_k=z(2, 3, 16, 2).transpose(2, 3)[:, :, :1]), lambda: rotary.rotary_backward(q, k, f, out_q=q.float()),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_types_and_shapes_of_the_gated_layer_are_refused():
+    z = lambda *s, dtype=BF: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    x, w, w2, h = z(8, 64), z(32, 64), z(64, 16), z(8, 32)
+    x8, wide8 = act8.act8_pack(z(8, 16)), act8.act8_pack(z(8, 32))
+    refused = [
+        lambda: gated.gated_linear(x, z(32, 63)), lambda: gated.gated_linear(x, z(31, 64)), lambda: gated.gated_linear(x.float(), w), lambda: gated.gated_linear(x, w.float()),
+        lambda: gated.gated_linear(x, w, act="tanh"), lambda: gated.gated_linear(x, w, save="int8"), lambda: gated.gated_linear(x, w, z(16)), lambda: gated.gated_linear(x, w, z(32).half()),
+        lambda: gated.gated_linear(x, w, out=z(8, 32)), lambda: gated.gated_linear(x, w, out=z(8, 16, dtype=torch.float32)), lambda: gated.gated_linear(x, w, out=z(16, 8).t()),
+        lambda: gated.gated_linear(z(8, 0), z(32, 0)), lambda: gated.gated_linear(x, w.cpu()),
+        lambda: gated.gated_linear_dgrad(x, z(63, 16), h), lambda: gated.gated_linear_dgrad(x, w2, z(8, 16)), lambda: gated.gated_linear_dgrad(x, w2, h.float()),
+        lambda: gated.gated_linear_dgrad(x, w2, None), lambda: gated.gated_linear_dgrad(x, w2, x8), lambda: gated.gated_linear_dgrad(x, w2, (x8, wide8)),
+        lambda: gated.gated_linear_dgrad(x, w2, (x8,)), lambda: gated.gated_linear_dgrad(x, w2, (h, h)), lambda: gated.gated_linear_dgrad(x, w2, h, act="swish"),
+        lambda: gated.gated_linear_dgrad(z(9, 64), w2, (x8, x8)), lambda: gated.gated_linear_dgrad(z(8, 0), z(0, 16), h),
+        lambda: linear.linear_act(x, w, dropout=(1.0, 1, 0)), lambda: linear.linear_act(x, w, dropout=(0.5, 1 << 64, 0)), lambda: linear.linear_act(x, w, dropout=(0.5, 1, -1)),
+        lambda: linear.linear_act(x, w, dropout=(0.5, torch.zeros(1, dtype=torch.int64), 0)),
     ]
     for i, call in enumerate(refused):
         with pytest.raises(ValueError):
