@@ -17,7 +17,13 @@ Act8View view(uintptr_t q, int64_t ldq, uintptr_t e, int64_t lde) { return Act8V
 
 using DropTuple = std::tuple<uint64_t, uintptr_t, uint64_t, uint32_t, double>;   // seed, its place on the device, offset, threshold, scale
 DropoutArgs drop_args(const DropTuple& d) {
-    return DropoutArgs{std::get<0>(d), (const void*)std::get<1>(d), std::get<2>(d), std::get<3>(d), (float)std::get<4>(d)};
+    DropoutArgs a;
+    a.seed_ptr = (const void*)std::get<1>(d);
+    a.offset = std::get<2>(d);
+    a.threshold = std::get<3>(d);
+    a.scale = (float)std::get<4>(d);
+    if (a.threshold != 0) dropout_keys(std::get<0>(d), a.keys);
+    return a;
 }
 
 // x, its strides between batches, tokens and heads, the result and its own, heads

@@ -5,12 +5,15 @@
 namespace psb {
 
 struct DropoutArgs {
-    uint64_t seed = 0;
-    const void* seed_ptr = nullptr;   // device int64, read when the kernel runs; `seed` is not used then
+    uint32_t keys[20] = {};           // of the generator's rounds, from the seed
+    const void* seed_ptr = nullptr;   // device int64, read when the kernel runs; `keys` are not used then
     uint64_t offset = 0;
     uint32_t threshold = 0;           // values whose word is below are dropped
     float scale = 1.f;                // of the others
 };
+
+// The keys of the rounds, two each, for a seed
+void dropout_keys(uint64_t seed, uint32_t* keys);
 
 // out = x * scale where kept, 0 elsewhere, + residual (optional). out may be x or residual itself.
 // Returns 0, a cudaError_t, or -2 (a shape or dtype that is not supported).

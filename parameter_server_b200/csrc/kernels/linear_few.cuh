@@ -134,7 +134,7 @@ __device__ __forceinline__ void add_parts_apart(uint32_t at, int S, float* v) {
 }
 
 template <int MODE, int ACT, int KIND = kLinPlain>
-__global__ void __launch_bounds__(kFewThreads, KIND == kLinDropout ? 2 : 1) linear_few_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(kFewThreads, KIND >= kLinDropout ? 2 : 1) linear_few_kernel(const __grid_constant__ FewParams p) {
     constexpr bool DGRAD = MODE == kFewDgrad, WGRAD = MODE == kFewWgrad, W_MN = MODE != kFewFwd;
     constexpr bool GATED_FWD = KIND == kLinGated && !DGRAD, GATED_DGRAD = KIND == kLinGated && DGRAD;
     constexpr int kWide = GATED_FWD ? BM / 2 : BM;   // outputs of a tile: of a gated one's features, half are the gate's
@@ -256,8 +256,7 @@ __global__ void __launch_bounds__(kFewThreads, KIND == kLinDropout ? 2 : 1) line
     const int t_end = min(tokens, (rank + 1) * share), t_first = rank * share + warp;
     float b[4] = {0.f, 0.f, 0.f, 0.f}, gain[4] = {1.f, 1.f, 1.f, 1.f}, aux[4], sum = 0.f;
     [[maybe_unused]] float aux_up[4];
-    [[maybe_unused]] DropKey key;
-    if constexpr (KIND == kLinDropout) key = drop_key(p.drop);
+    [[maybe_unused]] const DropKeys<KIND == kLinDropoutSeed> key(p.drop);
     if constexpr (WGRAD) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -394,7 +393,7 @@ __global__ void __launch_bounds__(kFewThreads, KIND == kLinDropout ? 2 : 1) line
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = act_of<ACT>(v[j]);
-                if constexpr (KIND == kLinDropout) drop4(key, p.drop.threshold, p.drop.scale, (uint32_t)row, (uint32_t)n / 4, v);
+                if constexpr (KIND >= kLinDropout) drop4(key, p.drop, (uint32_t)row, (uint32_t)n / 4, v);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] += aux[j];
             }

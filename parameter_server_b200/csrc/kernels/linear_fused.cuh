@@ -42,8 +42,8 @@ namespace psb {
 
 namespace {
 
-// What the epilogue is of: one product, a gated pair of them, or one with dropout behind its activation
-constexpr int kLinPlain = 0, kLinGated = 1, kLinDropout = 2;
+// What the epilogue is of: one product, a gated pair of them, or one with dropout behind its activation (its seed in the call or in memory)
+constexpr int kLinPlain = 0, kLinGated = 1, kLinDropout = 2, kLinDropoutSeed = 3;
 constexpr int kLinEpilogueWarps = 8;
 constexpr int kLinThreads = 32 * (4 + kLinEpilogueWarps);
 constexpr int kLinRegsIssue = 56, kLinRegsEpilogue = 224;   // 56 + 2 * 224 = 3 * 168, the launch's share
@@ -456,8 +456,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
         TileWalk walk(p.grid, pair);
         Tile t;
         uint32_t tc = 0;
-        [[maybe_unused]] DropKey key;
-        if constexpr (KIND == kLinDropout) key = drop_key(p.drop);
+        [[maybe_unused]] const DropKeys<KIND == kLinDropoutSeed> key(p.drop);
         while (walk.next(p.grid, t)) {
             const uint32_t buf = tc & 1u;
             const int tile_n = t.n * kWide, row0 = t.m * 2 * BM + cr * BM + quarter * 32, row = row0 + lane;
@@ -597,9 +596,9 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     if (p.q != nullptr) ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]);
-                    if constexpr (KIND == kLinDropout) {
+                    if constexpr (KIND >= kLinDropout) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) drop4(key, p.drop.threshold, p.drop.scale, (uint32_t)row, (uint32_t)(col + j) / 4, f + j);
+                        for (int j = 0; j < 32; j += 4) drop4(key, p.drop, (uint32_t)row, (uint32_t)(col + j) / 4, f + j);
                     }
                     if (p.res != nullptr) {
 #pragma unroll
@@ -880,5 +879,6 @@ int linear_fused_dgrad(const LinearArgs& a, cudaStream_t s);
 int linear_gated_fwd(const LinearArgs& a, cudaStream_t s);
 int linear_gated_dgrad(const LinearArgs& a, cudaStream_t s);
 int linear_dropout_fwd(const LinearArgs& a, cudaStream_t s);
+int linear_dropout_seed_fwd(const LinearArgs& a, cudaStream_t s);
 
 }  // namespace psb

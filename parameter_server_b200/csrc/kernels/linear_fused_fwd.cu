@@ -19,7 +19,10 @@ int linear_fused(const LinearArgs& a, void* stream) {
         if (a.q != nullptr && (((uintptr_t)a.q_up % 16) || (a.ldq_up % 16) || ((uintptr_t)a.e_up % 16) || (a.lde_up % 16) || a.q_up == nullptr || a.e_up == nullptr)) return -2;
         return a.dgrad ? linear_gated_dgrad(a, (cudaStream_t)stream) : linear_gated_fwd(a, (cudaStream_t)stream);
     }
-    if (a.drop.threshold != 0) return a.dgrad ? -2 : linear_dropout_fwd(a, (cudaStream_t)stream);
+    if (a.drop.threshold != 0) {
+        if (a.dgrad) return -2;
+        return a.drop.seed_ptr == nullptr ? linear_dropout_fwd(a, (cudaStream_t)stream) : linear_dropout_seed_fwd(a, (cudaStream_t)stream);
+    }
     return a.dgrad ? linear_fused_dgrad(a, (cudaStream_t)stream) : linear_fused_fwd(a, (cudaStream_t)stream);
 }
 

@@ -16,35 +16,49 @@ namespace psb {
 
 namespace {
 
-struct DropKey {
-    uint32_t k0, k1, o0, o1;
-};
-__device__ __forceinline__ DropKey drop_key(const DropoutArgs& d) {
-    const uint64_t seed = d.seed_ptr != nullptr ? (uint64_t)*(const volatile int64_t*)d.seed_ptr : d.seed;
-    return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)d.offset, (uint32_t)(d.offset >> 32)};
+__host__ __device__ __forceinline__ void drop_keys(uint64_t seed, uint32_t* keys) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        keys[2 * r] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u;
+        keys[2 * r + 1] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+    }
 }
+// The keys of the rounds: operands from constant memory where the seed came with the call (formed in every thread they were a fifth of the
+// instructions), in registers where it lies in memory.
+template <bool IN_MEMORY>
+struct DropKeys {
+    uint32_t k[20];
+    __device__ __forceinline__ explicit DropKeys(const DropoutArgs& d) { drop_keys((uint64_t)*(const volatile int64_t*)d.seed_ptr, k); }
+    __device__ __forceinline__ uint32_t operator[](int i) const { return k[i]; }
+};
+template <>
+struct DropKeys<false> {
+    const DropoutArgs& d;
+    __device__ __forceinline__ explicit DropKeys(const DropoutArgs& args) : d(args) {}
+    __device__ __forceinline__ uint32_t operator[](int i) const { return d.keys[i]; }
+};
 // The words of columns 4 group .. 4 group + 3 of a row
-__device__ __forceinline__ uint4 drop_words(const DropKey& key, uint32_t row, uint32_t group) {
-    uint32_t c0 = group, c1 = row, c2 = key.o0, c3 = key.o1, k0 = key.k0, k1 = key.k1;
+template <typename Keys>
+__device__ __forceinline__ uint4 drop_words(const Keys& key, uint64_t offset, uint32_t row, uint32_t group) {
+    uint32_t c0 = group, c1 = row, c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ key[2 * r];
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ key[2 * r + 1];
         c3 = (uint32_t)a;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
     }
     return make_uint4(c0, c1, c2, c3);
 }
 // Four neighbours after dropout. What is dropped is 0, whatever it was.
-__device__ __forceinline__ void drop4(const DropKey& key, uint32_t threshold, float scale, uint32_t row, uint32_t group, float* f) {
-    const uint4 w = drop_words(key, row, group);
-    f[0] = w.x >= threshold ? f[0] * scale : 0.f;
-    f[1] = w.y >= threshold ? f[1] * scale : 0.f;
-    f[2] = w.z >= threshold ? f[2] * scale : 0.f;
-    f[3] = w.w >= threshold ? f[3] * scale : 0.f;
+template <typename Keys>
+__device__ __forceinline__ void drop4(const Keys& key, const DropoutArgs& d, uint32_t row, uint32_t group, float* f) {
+    const uint4 w = drop_words(key, d.offset, row, group);
+    f[0] = w.x >= d.threshold ? f[0] * d.scale : 0.f;
+    f[1] = w.y >= d.threshold ? f[1] * d.scale : 0.f;
+    f[2] = w.z >= d.threshold ? f[2] * d.scale : 0.f;
+    f[3] = w.w >= d.threshold ? f[3] * d.scale : 0.f;
 }
 
 }  // namespace
