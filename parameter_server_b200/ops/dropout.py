@@ -23,47 +23,53 @@ def drop_args(p: float, seed: Seed, offset: int, device: int, what: str):
     """``(seed, address of a seed on the device, offset, threshold, scale)`` as the native entry points take them."""
     if not 0.0 <= p < 1.0:
         raise ValueError(f"{what}: p is at least 0 and below 1, not {p!r}")
-    threshold = int(p * 2.0 ** 32 + 0.5)
-    if threshold >> 32:
+    threshold = int(p * 4294967296.0 + 0.5)
+    if threshold == 4294967296:
         raise ValueError(f"{what}: p = {p!r} rounds to 1")
     at = 0
     if isinstance(seed, torch.Tensor):
         if seed.dtype is not torch.int64 or seed.numel() != 1 or seed.get_device() != device:
             raise ValueError(f"{what}: a seed in memory is one int64 on cuda:{device}, got {tuple(seed.shape)} of {seed.dtype} on {seed.device}")
         seed, at = 0, seed.data_ptr()
-    elif not -(1 << 63) <= seed < 1 << 64:
+    elif not -0x8000000000000000 <= seed <= 0xFFFFFFFFFFFFFFFF:
         raise ValueError(f"{what}: the seed has 64 bits, {seed} has more")
-    if not 0 <= offset < 1 << 64:
+    if not 0 <= offset <= 0xFFFFFFFFFFFFFFFF:
         raise ValueError(f"{what}: the offset is a number of 64 bits, not {offset}")
-    return seed & 0xFFFFFFFFFFFFFFFF, at, offset, threshold, 2.0 ** 32 / (2 ** 32 - threshold)
+    return seed & 0xFFFFFFFFFFFFFFFF, at, offset, threshold, 4294967296.0 / (4294967296 - threshold)
+
+
+def _like_x(t, x, what, name):
+    if t.shape != x.shape or t.dtype is not x.dtype or t.get_device() != x.get_device():
+        raise ValueError(f"{what}: {name} must be like x ({tuple(x.shape)} of {x.dtype} on {x.device}), got {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
 def _dropout(x, p, seed, offset, residual, out, what):
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise ValueError(f"{what}: bf16 or fp32, not {x.dtype}")
-    s, dev = launch_stream(x), x.get_device()
-    drop = drop_args(p, seed, offset, dev, what)
+    s = launch_stream(x)
+    drop = drop_args(p, seed, offset, x.get_device(), what)
     x2 = rows2d(x, what)
     rows, cols = x2.shape
     rp = ldr = 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.get_device() != dev:
-            raise ValueError(f"{what}: residual must be like x ({tuple(x.shape)} of {x.dtype} on {x.device})")
+        _like_x(residual, x, what, "residual")
         residual = rows2d(residual, what)
         rp, ldr = residual.data_ptr(), row_stride(residual)
     if out is None:
-        y = torch.empty_like(x2) if x2.is_contiguous() else x2.new_empty((rows, cols))
+        y, ldy = torch.empty_like(x2) if x2.is_contiguous() else x2.new_empty((rows, cols)), cols
     else:
-        if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev:
-            raise ValueError(f"{what}: out must be like x ({tuple(x.shape)} of {x.dtype} on {x.device})")
+        _like_x(out, x, what, "out")
         y = out if out.dim() == 2 else out.view(rows, cols)
         if cols > 1 and y.stride(1) != 1:
             raise ValueError(f"{what}: the values of a row of out must be contiguous")
+        ldy = row_stride(y)
     if rows > 0xFFFFFFFF:
         raise ValueError(f"{what}: at most 2^32 - 1 rows")
     if rows and cols:
-        check(C.dropout(dt, x2.data_ptr(), row_stride(x2), rp, ldr, y.data_ptr(), row_stride(y), rows, cols, drop, s), what)
+        rc = C.dropout(dt, x2.data_ptr(), row_stride(x2), rp, ldr, y.data_ptr(), ldy, rows, cols, drop, s)
+        if rc != 0:
+            check(rc, what)
     if out is not None:
         return out
     return y if x.dim() == 2 else y.view(x.shape)

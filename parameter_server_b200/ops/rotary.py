@@ -14,6 +14,8 @@ from .._lib import C
 from .act8 import _DTYPES, check, launch_stream
 
 _POSITIONS = {torch.int64: False, torch.int32: True}
+_NO_HEADS = (0,) * 9
+_NO_POSITIONS = (0, False, 0, 0)
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
@@ -49,46 +51,67 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str
     return freqs.to(device if device is not None else torch.device("cuda", torch.cuda.current_device())), scale
 
 
-def _heads(x, out, like, dev, what, name):
-    """(x, result, arguments of the native call) of queries or keys."""
-    if x.dim() not in (3, 4):
+def _misfit(x, out, shape, dtype, dev, what, name):
+    """Which argument does not fit (off the path of calls that do)."""
+    if len(x.shape) not in (3, 4):
         raise ValueError(f"{what}: {name} is [tokens, heads, dim] or [batch, tokens, heads, dim], not {tuple(x.shape)}")
-    if like is not None and (x.dim() != like.dim() or x.shape[:-2] != like.shape[:-2] or x.shape[-1] != like.shape[-1] or x.dtype != like.dtype
-                             or x.get_device() != dev):
-        raise ValueError(f"{what}: {name} of {tuple(x.shape)} {x.dtype} on {x.device} does not go with q of {tuple(like.shape)} {like.dtype} on {like.device}")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    if x.shape[:-2] != shape[:-2] or x.shape[-1] != shape[-1] or x.dtype != dtype or x.get_device() != dev:
+        raise ValueError(f"{what}: {name} of {tuple(x.shape)} {x.dtype} on {x.device} does not go with q of {tuple(shape)} {dtype} on cuda:{dev}")
+    raise ValueError(f"{what}: out of {name} must be like it ({tuple(x.shape)} of {dtype} on cuda:{dev}), the values of a head side by side, "
+                     f"got {tuple(out.shape)} of {out.dtype} on {out.device}")
+
+
+def _heads(x, out, shape, dtype, dev, what, name):
+    """(result, arguments of the native call, what to hold) of queries or keys; ``shape``, ``dtype`` and ``dev`` are those of q."""
+    own = x.shape
+    dims, dim = len(own), shape[-1]
+    if dims not in (3, 4) or (own is not shape and (dims != len(shape) or own[0] != shape[0] or own[-3] != shape[-3] or own[-1] != dim
+                                                    or x.dtype is not dtype or x.get_device() != dev)):
+        _misfit(x, out, shape, dtype, dev, what, name)
+    st = x.stride()
+    if st[-1] != 1 and dim > 1:
         x = x.contiguous()
+        st = x.stride()
     if out is None:
         out = torch.empty_like(x)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev or (out.stride(-1) != 1 and out.shape[-1] > 1):
-        raise ValueError(f"{what}: out of {name} must be like it ({tuple(x.shape)} of {x.dtype} on {x.device}), the values of a head side by side")
-    lead = (x.stride(0), out.stride(0)) if x.dim() == 4 else (0, 0)
-    return x, out, (x.data_ptr(), lead[0], x.stride(-3), x.stride(-2), out.data_ptr(), lead[1], out.stride(-3), out.stride(-2), x.shape[-2])
+    elif out.shape != own or out.dtype is not dtype or out.get_device() != dev:
+        _misfit(x, out, shape, dtype, dev, what, name)
+    to = out.stride()
+    if to[-1] != 1 and dim > 1:
+        _misfit(x, out, shape, dtype, dev, what, name)
+    if dims == 3:
+        return out, (x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, to[0], to[1], own[1]), x
+    return out, (x.data_ptr(), st[0], st[1], st[2], out.data_ptr(), to[0], to[1], to[2], own[2]), x
 
 
 def _rotary(q, k, freqs, positions, offset, interleaved, scale, out_q, out_k, backward, what):
-    dt = _DTYPES.get(q.dtype)
+    dtype = q.dtype
+    dt = _DTYPES.get(dtype)
     if dt is None:
-        raise ValueError(f"{what}: bf16 or fp32, not {q.dtype}")
+        raise ValueError(f"{what}: bf16 or fp32, not {dtype}")
     s, dev = launch_stream(q), q.get_device()
-    q, out_q, q_args = _heads(q, out_q, None, dev, what, "q")
+    shape = q.shape
+    out_q, q_args, _held = _heads(q, out_q, shape, dtype, dev, what, "q")
+    k_args = _NO_HEADS
     if k is not None:
-        k, out_k, k_args = _heads(k, out_k, q, dev, what, "k")
+        out_k, k_args, _held_k = _heads(k, out_k, shape, dtype, dev, what, "k")
     elif out_k is not None:
         raise ValueError(f"{what}: out_k without k")
-    else:
-        k_args = (0,) * 9
-    batch, tokens, dim = q.shape[0] if q.dim() == 4 else 1, q.shape[-3], q.shape[-1]
-    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or freqs.get_device() != dev or 2 * freqs.numel() > dim or not freqs.is_contiguous():
+    batch, tokens, dim = shape[0] if len(shape) == 4 else 1, shape[-3], shape[-1]
+    pairs = freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or freqs.get_device() != dev or 2 * pairs > dim or not freqs.is_contiguous():
         raise ValueError(f"{what}: freqs must be at most {dim // 2} contiguous fp64 values on {q.device}, got {tuple(freqs.shape)} of {freqs.dtype} on {freqs.device}")
-    pos = (0, False, 0, 0)
+    pos = _NO_POSITIONS
     if positions is not None:
-        narrow = _POSITIONS.get(positions.dtype)
-        if narrow is None or positions.get_device() != dev or tuple(positions.shape) not in ((tokens,), (batch, tokens), (1, tokens)):
+        narrow, at = _POSITIONS.get(positions.dtype), positions.shape
+        if narrow is None or positions.get_device() != dev or not 1 <= len(at) <= 2 or at[-1] != tokens or (len(at) == 2 and at[0] != batch and at[0] != 1):
             raise ValueError(f"{what}: positions must be int64 or int32, [{tokens}] or [{batch}, {tokens}], on {q.device}, "
-                             f"got {tuple(positions.shape)} of {positions.dtype} on {positions.device}")
-        pos = (positions.data_ptr(), narrow, positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, positions.stride(-1))
-    check(C.rotary(dt, q_args, k_args, batch, tokens, dim, freqs.numel(), interleaved, freqs.data_ptr(), *pos, offset, scale, backward, s), what)
+                             f"got {tuple(at)} of {positions.dtype} on {positions.device}")
+        st = positions.stride()
+        pos = (positions.data_ptr(), narrow, st[0] if len(at) == 2 and at[0] > 1 else 0, st[-1])
+    rc = C.rotary(dt, q_args, k_args, batch, tokens, dim, pairs, interleaved, freqs.data_ptr(), *pos, offset, scale, backward, s)
+    if rc != 0:
+        check(rc, what)
     return out_q if k is None else (out_q, out_k)
 
 
