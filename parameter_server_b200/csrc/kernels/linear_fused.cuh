@@ -49,7 +49,7 @@ constexpr int kLinThreads = 32 * (4 + kLinEpilogueWarps);
 constexpr int kLinRegsIssue = 56, kLinRegsEpilogue = 224;   // 56 + 2 * 224 = 3 * 168, the launch's share
 static_assert(kLinRegsIssue + 2 * kLinRegsEpilogue == 3 * (65536 / kLinThreads / 8 * 8), "setmaxnreg would wait for registers that the launch does not have");
 
-template <int BN>
+template <int BN, bool GATED_DGRAD = false>
 struct LinSmem {
     static constexpr int kABytes = BM * BK * 2;
     static constexpr int kBBytes = BN / 2 * BK * 2;          // a CTA of a pair holds half of the B tile
@@ -60,8 +60,9 @@ struct LinSmem {
     static constexpr int kStages = BN == 256 ? 3 : 4;
     static constexpr int kTileBytes = kStages * kSub * kStageBytes;
     static constexpr int kBarBytes = 256;
-    static constexpr int kBiasBytes = 2 * BN * 4;            // double-buffered with the accumulator
-    static constexpr int kOutBytes = kLinEpilogueWarps * 2048;   // a warp's [32 rows][64 bytes] on the way out
+    static constexpr int kBiasBytes = GATED_DGRAD ? 0 : 2 * BN * 4;   // double-buffered with the accumulator
+    static constexpr int kWarpBytes = GATED_DGRAD ? 4096 : 2048;      // a warp's [32 rows][64 bytes] on the way out; gated dgrad: 32 x 32 sums
+    static constexpr int kOutBytes = kLinEpilogueWarps * kWarpBytes;
     static constexpr int kTotal = kTileBytes + kBarBytes + kBiasBytes + kOutBytes + 1024;   // + alignment slack
 };
 
@@ -183,6 +184,32 @@ __device__ __forceinline__ float s8_at(const uint4* raw, int j) {   // j is a co
     const uint32_t w = ((j / 4) % 4 == 0 ? v.x : (j / 4) % 4 == 1 ? v.y : (j / 4) % 4 == 2 ? v.z : v.w) ^ 0x80808080u;
     return j % 4 == 0 ? s8_of_biased<0>(w) : j % 4 == 1 ? s8_of_biased<1>(w) : j % 4 == 2 ? s8_of_biased<2>(w) : s8_of_biased<3>(w);
 }
+// Eight neighbours of a bf16 row on a 16-byte boundary, of which `n` (one at least) exist
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int n) {
+    if (n >= 8) return ld_global_v4(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        w[j] = (2 * j < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j]) : 0u) | (2 * j + 1 < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j + 1]) : 0u) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, uint4 v) {
+    if (n >= 8) {
+        *(uint4*)p = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < n) ((unsigned short*)p)[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+}
+__device__ __forceinline__ uint4 pack8(const float* f) {
+    uint4 v;
+    __nv_bfloat162* h = (__nv_bfloat162*)&v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+    return v;
+}
 // Where in the warp's 2 KB the bytes [16 j, 16 j + 16) of row r of a [32 rows][64 bytes] piece lie
 __device__ __forceinline__ uint32_t in_piece(uint32_t stage, int r, int byte) {
     return stage + (uint32_t)(r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
@@ -303,11 +330,282 @@ __device__ __forceinline__ uint32_t keep_row32(const float* f, int8_t* qp, int n
     return e;
 }
 
+// ---- gated dgrad: the epilogue ---------------------------------------------------------------------------------------
+// Two neighbours of a sum come in and three go out, twice what the other epilogues move. So the sums change places once, 32 rows and 32 columns at
+// a time through the warp's 4 KB, and a lane then has eight columns of four rows, eight apart, of everything: loads and stores of whole 16-byte
+// blocks, four lanes to a row, none of which goes through shared memory. (16384 tokens, 5504 x 2048, silu: 376 us, with a row to a lane 439; sixteen
+// warps with 16 columns at a time, two lanes to a row, 510.)
+template <int ACT, int BN>
+__device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_t tmem_base, uint64_t* tfull_bar, uint64_t* tempty_bar, uint32_t* tmem_slot,
+                                                     uint32_t stage, int pair, int cr, int ew, int lane) {
+    constexpr int kColumns = BN / 2, kUnits = kColumns / 32;   // of a warp
+    const int quarter = ew & 3, cbase = (ew >> 2) * kColumns;
+    const int qrow = lane >> 2, qcol = (lane & 3) * 8;          // a lane's place in a unit: rows qrow, qrow + 8, ..., eight columns
+    const bool kept8 = p.q != nullptr;
+    const bool wide = (kept8 || (p.pre_width == 16 && p.pre_up_width == 16)) && p.out_width == 16 && p.out_up_width == 16 && p.out2_width == 16;
+    const unsigned long long limit_ns = p.limit_ns;
+    auto first_row = [&](const Tile& t) { return t.m * 2 * BM + cr * BM + quarter * 32; };
+    auto first_column = [&](const Tile& t) { return t.n * BN + cbase; };
+    // whole tiles on 16-byte boundaries: nothing to check, and the neighbours of the next tile's first unit are asked for in this one's last
+    auto whole = [&](const Tile& t) { return wide && t.runs == 1 && first_row(t) + 32 <= p.M && first_column(t) + kColumns <= p.N; };
+    // where four sums of a unit lie: the 16-byte blocks of a row are XOR-swizzled by it, neither side has bank conflicts
+    auto in_unit = [&](int r, int j) { return stage + (uint32_t)(r * 128 + ((j ^ (r & 7)) << 4)); };
+    auto lay_down = [&](const uint32_t* v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st_smem_v4(in_unit(lane, j), make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+    };
+    auto unpack16 = [&](uint4 g, uint4 u, float* vg, float* vu) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            vg[j] = bf16_at(&g, j);
+            vu[j] = bf16_at(&u, j);
+        }
+    };
+    auto unpack8 = [&](uint4 g, uint4 u, uint32_t eg, uint32_t eu, float* vg, float* vu) {
+        const float step = act8_step(eg & 255u), step_up = act8_step(eu & 255u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            vg[j] = s8_at(&g, j) * step;
+            vu[j] = s8_at(&u, j) * step_up;
+        }
+    };
+    // eight columns of row qrow + 8 i: the gradients of g (in vg to begin with) and u (in vu), and act(g) u
+    auto turn = [&](int i, float* vg, float* vu, float* va) {
+        const uint4 lo = ld_smem_v4(in_unit(8 * i + qrow, qcol / 4)), hi = ld_smem_v4(in_unit(8 * i + qrow, qcol / 4 + 1));
+        const uint32_t da[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = __uint_as_float(da[j]);
+            float value;
+            const float slope = act_slope<ACT>(vg[j], &value);
+            va[j] = value * vu[j];
+            vg[j] = d * vu[j] * slope;
+            vu[j] = d * value;
+        }
+    };
+    auto exponents = [&](const uint8_t* e) -> uint32_t {   // a byte for 32 columns; rows of e are padded to 16
+        return kUnits == 4 ? *(const uint32_t*)e : (uint32_t)*(const uint16_t*)e;
+    };
+    uint4 g[4], u[4];
+    uint32_t eg[4], eu[4];
+    // the neighbours of a whole tile's unit `c`, in rows qrow + 8 i
+    auto place = [&](const Tile& t, int c, const char** at, const char** at_up) {
+        const int64_t r = first_row(t) + qrow;
+        const int col = first_column(t) + c * 32 + qcol;
+        *at = kept8 ? (const char*)(p.q + r * p.ldq + col) : (const char*)(p.pre + r * p.ldpre + col);
+        *at_up = kept8 ? (const char*)(p.q_up + r * p.ldq_up + col) : (const char*)(p.pre_up + r * p.ldpre + col);
+    };
+    const int64_t step = kept8 ? 8 * p.ldq : 16 * p.ldpre, step_up = kept8 ? 8 * p.ldq_up : 16 * p.ldpre;   // bytes between rows qrow + 8 i
+    auto load = [&](int i, const char* at, const char* at_up) {
+        if (kept8) {
+            const uint2 a = *(const uint2*)(at + i * step), b = *(const uint2*)(at_up + i * step_up);
+            g[i] = make_uint4(a.x, a.y, 0, 0);
+            u[i] = make_uint4(b.x, b.y, 0, 0);
+        } else {
+            g[i] = ld_global_v4(at + i * step);
+            u[i] = ld_global_v4(at_up + i * step_up);
+        }
+    };
+    auto load_exponents = [&](const Tile& t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = first_row(t) + 8 * i + qrow;
+            const bool there = kept8 && r < p.M && first_column(t) < p.N;
+            eg[i] = there ? exponents(p.e + r * p.lde + first_column(t) / 32) : 0u;
+            eu[i] = there ? exponents(p.e_up + r * p.lde_up + first_column(t) / 32) : 0u;
+        }
+    };
+    TileWalk walk(p.grid, pair);
+    Tile t, coming = {};
+    uint32_t tc = 0;
+    bool loaded = false;
+    for (bool more = walk.next(p.grid, t); more; t = coming, ++tc) {
+        more = walk.next(p.grid, coming);
+        const uint32_t buf = tc & 1u;
+        const int row0 = first_row(t), colw = first_column(t);
+        const bool is_whole = whole(t);
+        if (is_whole && !loaded) {
+            const char *at, *at_up;
+            place(t, 0, &at, &at_up);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load(i, at, at_up);
+        }
+        if (!loaded) load_exponents(t);
+        loaded = false;
+        const bool waited = ew != 0 || mbar_wait(&tfull_bar[buf], (tc >> 1) & 1u, limit_ns * 4);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        if (!meet_all(1, 32 * kLinEpilogueWarps, waited)) {
+            if (!waited && lane == 0) give_up_pair(p.err_flag, 23u, tmem_slot);
+            break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * (uint32_t)BN + (uint32_t)cbase;
+        auto release = [&]() {   // this warp has read the accumulator
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_pair(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
+        };
+        uint32_t v[32];
+        if (is_whole) {
+            const char *at, *at_up;
+            const int64_t place_out = (int64_t)(row0 + qrow) * p.ldo + colw + qcol;
+            char *o = (char*)(p.out + place_out), *o_up = (char*)(p.out_up + place_out);
+            char* o2 = p.out2 == nullptr ? nullptr : (char*)(p.out2 + (int64_t)(row0 + qrow) * p.ldo2 + colw + qcol);
+            const int64_t ostep = 16 * p.ldo, ostep2 = 16 * p.ldo2;
+            loaded = more && whole(coming);
+            tmem_ld32_issue(taddr, v);
+#pragma unroll 1
+            for (int c = 0; c < kUnits; ++c) {
+                const bool last = c + 1 == kUnits, ahead = !last || loaded;
+                if (last) place(coming, 0, &at, &at_up);
+                else place(t, c + 1, &at, &at_up);
+                tmem_wait_ld(v);
+                __syncwarp();   // what was in the warp's memory has been read
+                lay_down(v);
+                if (!last) tmem_ld32_issue(taddr + (uint32_t)(c + 1) * 32u, v);
+                else release();
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float vg[8], vu[8], va[8];
+                    if (kept8) unpack8(g[i], u[i], eg[i] >> (8 * c), eu[i] >> (8 * c), vg, vu);
+                    else unpack16(g[i], u[i], vg, vu);
+                    if (ahead) load(i, at, at_up);
+                    turn(i, vg, vu, va);
+                    *(uint4*)(o + i * ostep) = pack8(vg);
+                    *(uint4*)(o_up + i * ostep) = pack8(vu);
+                    if (o2 != nullptr) *(uint4*)(o2 + i * ostep2) = pack8(va);
+                }
+                o += 64;
+                o_up += 64;
+                if (o2 != nullptr) o2 += 64;
+            }
+            if (loaded) load_exponents(coming);
+            continue;
+        }
+        // a tile with edges, with rows on smaller boundaries, or in parts: one unit with its sums in v, a row to a lane
+        auto finish = [&](int c) {
+            const int col = colw + c * 32, n = p.N - col - qcol;   // columns of this lane that exist
+            auto get = [&](const __nv_bfloat16* pre, int width, const int8_t* q, int64_t ldq, uint4* to) {
+                if (!kept8 && width != 16) {
+                    get_narrow(stage, lane, pre + (int64_t)row0 * p.ldpre + col, p.ldpre * 2, min(32, p.M - row0), 2 * min(32, p.N - col), width);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to[i] = ld_smem_v4(in_piece(stage, 8 * i + qrow, qcol * 2));
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = row0 + 8 * i + qrow;
+                    to[i] = make_uint4(0, 0, 0, 0);
+                    if (r >= p.M || n <= 0) continue;
+                    if (kept8) {
+                        const uint2 b = *(const uint2*)(q + r * ldq + col + qcol);   // (rows are padded to 16 bytes)
+                        to[i] = make_uint4(b.x, b.y, 0, 0);
+                    } else {
+                        to[i] = load8(pre + r * p.ldpre + col + qcol, n);
+                    }
+                }
+            };
+            auto put = [&](const uint4* d, __nv_bfloat16* out, int64_t ldo, int width) {
+                if (width != 16) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st_smem_v4(in_piece(stage, 8 * i + qrow, qcol * 2), d[i]);
+                    __syncwarp();
+                    put_narrow(stage, lane, out + (int64_t)row0 * ldo + col, ldo * 2, min(32, p.M - row0), 2 * min(32, p.N - col), width);
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = row0 + 8 * i + qrow;
+                    if (r < p.M && n > 0) store8(out + r * ldo + col + qcol, n, d[i]);
+                }
+            };
+            get(p.pre, p.pre_width, p.q, p.ldq, g);
+            get(p.pre_up, p.pre_up_width, p.q_up, p.ldq_up, u);
+            __syncwarp();   // what was in the warp's memory has been read
+            lay_down(v);
+            __syncwarp();
+            uint4 a[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float vg[8], vu[8], va[8];
+                if (kept8) unpack8(g[i], u[i], eg[i] >> (8 * c), eu[i] >> (8 * c), vg, vu);
+                else unpack16(g[i], u[i], vg, vu);
+                turn(i, vg, vu, va);
+                g[i] = pack8(vg);
+                u[i] = pack8(vu);
+                a[i] = pack8(va);
+            }
+            put(g, p.out, p.ldo, p.out_width);
+            put(u, p.out_up, p.ldo, p.out_up_width);
+            if (p.out2 != nullptr) put(a, p.out2, p.ldo2, p.out2_width);
+        };
+        if (row0 >= p.M) {   // nothing of this warp's 32 rows exists
+            release();
+            continue;
+        }
+        if (t.runs == 1) {
+#pragma unroll 1
+            for (int c = 0; c < kUnits; ++c) {
+                if (colw + c * 32 >= p.N) break;   // warp-uniform
+                tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
+                tmem_wait_ld(v);
+                finish(c);
+            }
+            release();
+            continue;
+        }
+        // shared tile: see the other epilogue
+        constexpr int64_t kWarpFloats = kUnits * 1024;
+        auto part_of = [&](int worker, int slot) {
+            return p.partial + ((((int64_t)worker * 2 + slot) * 2 + cr) * kLinEpilogueWarps + ew) * kWarpFloats + lane * 4;
+        };
+        float* mine = part_of(pair, t.slot);
+#pragma unroll 1
+        for (int c = 0; c < kUnits; ++c) {
+            if (colw + c * 32 >= p.N) break;
+            tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
+            tmem_wait_ld(v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *(uint4*)(mine + c * 1024 + j * 128) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+        release();
+        __threadfence();
+        __syncwarp();
+        unsigned last = 0;
+        unsigned* count = p.arrived + ((int64_t)t.index * 2 + cr) * kLinEpilogueWarps + ew;
+        if (lane == 0) last = atomicAdd(count, 1u) == (unsigned)(t.runs - 1) ? 1u : 0u;
+        if (__shfl_sync(0xFFFFFFFFu, last, 0) == 0u) continue;
+        __threadfence();
+        if (lane == 0) *count = 0u;   // at rest for the next launch
+#pragma unroll 1
+        for (int c = 0; c < kUnits; ++c) {
+            if (colw + c * 32 >= p.N) break;
+            float f[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = 0.f;
+#pragma unroll 1
+            for (int r = 0; r < t.runs; ++r) {
+                const float* src = part_of(t.first + r, TileWalk::slot_of(p.grid, t, r)) + c * 1024;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float4 x = __ldcg((const float4*)(src + j * 128));
+                    f[4 * j] += x.x; f[4 * j + 1] += x.y; f[4 * j + 2] += x.z; f[4 * j + 3] += x.w;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(f[j]);
+            finish(c);
+        }
+    }
+}
+
 // ---- the kernel ------------------------------------------------------------------------------------------------------
 template <bool DGRAD, int ACT, int BN, int KIND>
 __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __grid_constant__ LinParams p) {
-    using L = LinSmem<BN>;
     constexpr bool GATED_FWD = KIND == kLinGated && !DGRAD, GATED_DGRAD = KIND == kLinGated && DGRAD;
+    using L = LinSmem<BN, GATED_DGRAD>;
     constexpr int kWide = GATED_FWD ? BN / 2 : BN;   // output columns of a tile: of a gated one's BN products, half are the gate's
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -447,6 +745,10 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 }
             }
         }
+    } else if constexpr (GATED_DGRAD) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLinRegsEpilogue));
+        gated_dgrad_epilogue<ACT, BN>(p, tmem_base, tfull_bar, tempty_bar, tmem_slot, smem_u32(stage_out) + (uint32_t)((warp - 4) * L::kWarpBytes), pair, cr,
+                                      warp - 4, lane);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLinRegsEpilogue));
         // ---- epilogue ----
@@ -474,8 +776,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             // What a piece needs from memory (residual, or h) is requested before the piece ahead of it is worked on, the first
             // one before the wait for the accumulator.
             uint4 aux[4], coming[4];
-            [[maybe_unused]] uint4 aux_up[4], coming_up[4];
-            [[maybe_unused]] uint32_t ex = 0, ex_up = 0;
+            uint32_t ex = 0;
             const __nv_bfloat16* aux_row = DGRAD ? p.pre : p.res;
             const int64_t aux_ld = DGRAD ? p.ldpre : p.ldres;
             const int aux_width = DGRAD ? p.pre_width : p.aux_width;
@@ -487,42 +788,23 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     get_narrow(stage, lane, aux_row + (int64_t)row0 * aux_ld + col, aux_ld * 2, min(32, p.M - row0), 2 * min(32, p.N - col), aux_width);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) coming[j] = ld_smem_v4(in_piece(stage, lane, j * 16));
-                    if constexpr (!GATED_DGRAD) return;
-                } else if (live && kept8) {
+                    return;
+                }
+                if (!live) return;
+                if (kept8) {
                     const int8_t* qp = p.q + (int64_t)row * p.ldq + col;
                     coming[0] = ld_global_v4(qp);
                     if (col + 16 < p.N) coming[1] = ld_global_v4(qp + 16);
-                } else if (live && aux_row != nullptr) {
+                } else if (aux_row != nullptr) {
                     load32(aux_row + (int64_t)row * aux_ld + col, p.N - col, coming);
-                }
-                if constexpr (GATED_DGRAD) {
-                    if (!kept8 && p.pre_up_width != 16) {
-                        get_narrow(stage, lane, p.pre_up + (int64_t)row0 * aux_ld + col, aux_ld * 2, min(32, p.M - row0), 2 * min(32, p.N - col), p.pre_up_width);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) coming_up[j] = ld_smem_v4(in_piece(stage, lane, j * 16));
-                    } else if (live && kept8) {
-                        const int8_t* qp = p.q_up + (int64_t)row * p.ldq_up + col;
-                        coming_up[0] = ld_global_v4(qp);
-                        if (col + 16 < p.N) coming_up[1] = ld_global_v4(qp + 16);
-                    } else if (live) {
-                        load32(p.pre_up + (int64_t)row * aux_ld + col, p.N - col, coming_up);
-                    }
                 }
             };
 #pragma unroll
             for (int j = 0; j < 4; ++j) coming[j] = make_uint4(0, 0, 0, 0);
-            if constexpr (GATED_DGRAD) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) coming_up[j] = make_uint4(0, 0, 0, 0);
-            }
             if (t.runs == 1) fetch(0);
             if (kept8 && live && colw < p.N) {   // one byte per piece; rows of e are padded to 16
                 if constexpr (kPieces == 4) ex = *(const uint32_t*)(p.e + (int64_t)row * p.lde + colw / 32);
                 else ex = *(const uint16_t*)(p.e + (int64_t)row * p.lde + colw / 32);
-                if constexpr (GATED_DGRAD) {
-                    if constexpr (kPieces == 4) ex_up = *(const uint32_t*)(p.e_up + (int64_t)row * p.lde_up + colw / 32);
-                    else ex_up = *(const uint16_t*)(p.e_up + (int64_t)row * p.lde_up + colw / 32);
-                }
             }
             // One barrier of the epilogue warps per tile: publishes the bias, and makes the decision to give up uniform. One warp
             // asks for the accumulator, the others sleep at this barrier (asking takes issue slots from the MMAs' thread).
@@ -554,10 +836,6 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 const int col = colw + c * 32;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) aux[j] = coming[j];
-                if constexpr (GATED_DGRAD) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) aux_up[j] = coming_up[j];
-                }
                 fetch(c + 1);
                 if constexpr (GATED_FWD) {
                     add_bias(f, cbase + c * 32);
@@ -576,20 +854,6 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     }
 #pragma unroll
                     for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]) * u[j];
-                } else if constexpr (GATED_DGRAD) {
-                    float a[32], du[32];
-                    const float step = kept8 ? act8_step((ex >> (8 * c)) & 255u) : 0.f, step_up = kept8 ? act8_step((ex_up >> (8 * c)) & 255u) : 0.f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float g = kept8 ? s8_at(aux, j) * step : bf16_at(aux, j), up = kept8 ? s8_at(aux_up, j) * step_up : bf16_at(aux_up, j);
-                        float value;
-                        const float slope = act_slope<ACT>(g, &value);
-                        du[j] = f[j] * value;
-                        a[j] = value * up;
-                        f[j] *= up * slope;
-                    }
-                    store_piece(stage, lane, du, p.out_up, p.ldo, row0, col, p.M, p.N, p.out_up_width);
-                    if (p.out2 != nullptr) store_piece(stage, lane, a, p.out2, p.ldo2, row0, col, p.M, p.N, p.out2_width);
                 } else if constexpr (!DGRAD) {
                     add_bias(f, cbase + c * 32);
                     if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
@@ -790,7 +1054,10 @@ int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
     constexpr auto kern = linear_fused_kernel<DGRAD, ACT, BN, KIND>;
     const int rows_of_w = KIND == kLinGated && !DGRAD ? 2 * p.N : p.N, wide = KIND == kLinGated && !DGRAD ? BN / 2 : BN;
     int pairs = 0;
-    cudaError_t e = pairs_of<kern>(kLinThreads, LinSmem<BN>::kTotal, &pairs);
+    constexpr bool GATED_DGRAD = KIND == kLinGated && DGRAD;
+    constexpr int kSmem = LinSmem<BN, GATED_DGRAD>::kTotal;
+    static_assert(kSmem <= 227 * 1024, "more shared memory than a CTA may have");
+    cudaError_t e = pairs_of<kern>(kLinThreads, kSmem, &pairs);
     if (e != cudaSuccess) return (int)e;
     // A weight that L2 holds beside the stream of activations is walked along n (16384 x 2048 x 8192 with a residual, sustained:
     // 429 us, in groups of 8 rows 441); a larger one in blocks (8192^3: 844 us, along n 923).
@@ -798,7 +1065,7 @@ int launch_linear(LinParams& p, int k_steps, cudaStream_t s) {
     // Joining a cut tile takes 10 to 20 us (its parts are read one after the other, eight 16-byte loads in flight per thread).
     p.grid = plan_tiles((p.M + 2 * BM - 1) / (2 * BM), (p.N + wide - 1) / wide, k_steps, pairs, 64, group);
     if (p.grid.shared > 0 && p.arrived == nullptr) return kNeedsWorkspace;
-    return (int)launch_pairs(kern, kLinThreads, LinSmem<BN>::kTotal, p.grid.pairs, p, s);
+    return (int)launch_pairs(kern, kLinThreads, kSmem, p.grid.pairs, p, s);
 }
 
 template <bool DGRAD, int BN, int KIND>
