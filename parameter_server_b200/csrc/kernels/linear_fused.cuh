@@ -472,9 +472,9 @@ __device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_
                     else unpack16(g[i], u[i], vg, vu);
                     if (ahead) load(i, at, at_up);
                     turn(i, vg, vu, va);
-                    *(uint4*)(o + i * ostep) = pack8(vg);
-                    *(uint4*)(o_up + i * ostep) = pack8(vu);
-                    if (o2 != nullptr) *(uint4*)(o2 + i * ostep2) = pack8(va);
+                    __stcs((uint4*)(o + i * ostep), pack8(vg));
+                    __stcs((uint4*)(o_up + i * ostep), pack8(vu));
+                    if (o2 != nullptr) __stcs((uint4*)(o2 + i * ostep2), pack8(va));
                 }
                 o += 64;
                 o_up += 64;
@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) mbar_arrive_pair(mapa_cluster(smem_u32(&tempty_bar[buf]), 0));
             };
-            // one 32-column piece with its values in f (gated: the gate's in f, the other factor's in u)
+            // one 32-column piece with its values in f (gated: the activated gate in f, the other factor in u)
             uint32_t ewrite = 0;
             [[maybe_unused]] uint32_t ewrite_up = 0;
             auto add_bias = [&](float* f, int at) {
@@ -832,28 +832,32 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                     f[j + 2] += __uint_as_float(b.z); f[j + 3] += __uint_as_float(b.w);
                 }
             };
+            // gated: the gate's piece first, to its activation
+            [[maybe_unused]] auto finish_gate = [&](float* f, int c) {
+                const int col = colw + c * 32;
+                add_bias(f, cbase + c * 32);
+                if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
+                if (p.q != nullptr) {
+                    if (col + 32 > p.N) {   // behind the gate's last row of w, the tile has the other factor's first
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] = col + j < p.N ? f[j] : 0.f;
+                    }
+                    ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]);
+            };
             auto finish = [&](float* f, [[maybe_unused]] float* u, int c) {
                 const int col = colw + c * 32;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) aux[j] = coming[j];
                 fetch(c + 1);
                 if constexpr (GATED_FWD) {
-                    add_bias(f, cbase + c * 32);
                     add_bias(u, kWide + cbase + c * 32);
-                    if (p.pre != nullptr) {
-                        store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
-                        store_piece(stage, lane, u, p.pre_up, p.ldpre, row0, col, p.M, p.N, p.pre_up_width);
-                    }
-                    if (p.q != nullptr) {
-                        if (col + 32 > p.N) {   // behind the gate's last row of w, the tile has the other factor's first
+                    if (p.pre != nullptr) store_piece(stage, lane, u, p.pre_up, p.ldpre, row0, col, p.M, p.N, p.pre_up_width);
+                    if (p.q != nullptr) ewrite_up |= keep_row32(u, p.q_up + (int64_t)row * p.ldq_up + col, p.N - col, live) << (8 * c);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) f[j] = col + j < p.N ? f[j] : 0.f;
-                        }
-                        ewrite |= keep_row32(f, p.q + (int64_t)row * p.ldq + col, p.N - col, live) << (8 * c);
-                        ewrite_up |= keep_row32(u, p.q_up + (int64_t)row * p.ldq_up + col, p.N - col, live) << (8 * c);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) f[j] = act_of<ACT>(f[j]) * u[j];
+                    for (int j = 0; j < 32; ++j) f[j] *= u[j];
                 } else if constexpr (!DGRAD) {
                     add_bias(f, cbase + c * 32);
                     if (p.pre != nullptr) store_piece(stage, lane, f, p.pre, p.ldpre, row0, col, p.M, p.N, p.pre_width);
@@ -897,19 +901,25 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
             uint32_t v[32];
             if constexpr (GATED_FWD) {
                 if (t.runs == 1) {
+                    // the next sums are on their way while these are worked on, and the accumulator is given back with the last
+                    if (colw < p.N) tmem_ld32_issue(taddr, v);
 #pragma unroll 1
                     for (int c = 0; c < kPieces; ++c) {
                         if (colw + c * 32 >= p.N) break;   // warp-uniform
                         float f[32], u[32];
-                        tmem_ld32_issue(taddr + (uint32_t)c * 32u, v);
-                        tmem_ld32_issue(taddr + (uint32_t)(kWide + c * 32), (uint32_t*)u);
                         tmem_wait_ld(v);
-                        tmem_wait_ld((uint32_t*)u);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                        tmem_ld32_issue(taddr + (uint32_t)(kWide + c * 32), v);
+                        finish_gate(f, c);
+                        tmem_wait_ld(v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(v[j]);
+                        if (c + 1 < kPieces && colw + c * 32 + 32 < p.N) tmem_ld32_issue(taddr + (uint32_t)(c + 1) * 32u, v);
+                        else release();
                         finish(f, u, c);
                     }
-                    release();
+                    if (colw >= p.N) release();
                 }
             } else if (t.runs == 1) {
                 if (colw < p.N) tmem_ld32_issue(taddr, v);
@@ -972,6 +982,7 @@ __global__ void __launch_bounds__(kLinThreads, 1) linear_fused_kernel(const __gr
                         joined(f, c);
                         if constexpr (GATED_FWD) {
                             float u[32];
+                            finish_gate(f, c);
                             joined(u, kPieces + c);
                             finish(f, u, c);
                         } else {
