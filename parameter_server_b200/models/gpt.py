@@ -11,6 +11,9 @@ it already multiplies the local rows. Attention itself is model code, not a para
 the block operators of this package: ``ops.norm`` for layer norm, ``ops.linear`` for linear layers with bias, GELU and residual
 in their epilogue. ``act_bits=8`` keeps the norms' rows and the hidden layer before GELU in 8 bits for the backward pass
 (``ops.act8``); what attention itself keeps (q, k, v and its output, which the projection's weight gradient reads too) stays in 16.
+Fused blocks may have a gated hidden layer in place of GELU's (``gated=True``: ``ops.gated``, twice the first layer's weight), rotary positions in
+place of the table of learned ones (``rotary=True``: ``ops.rotary``, on q and k where the QKV product left them), and dropout behind the
+embedding and both halves of a block while training (``dropout=p``: ``ops.dropout``, in the epilogue of the second linear layer of each half).
 
 The reference ships no model code (it is a storage service); this is the dense-table consumer.
 """
@@ -31,8 +34,11 @@ from .._lib import C
 from ..ops import gemm as G
 from ..ops.act8 import Act8, act8_wgrad
 from ..ops.dense import DenseTable
+from ..ops.dropout import drop_args, dropout, dropout_backward
+from ..ops.gated import gated_linear, gated_linear_dgrad
 from ..ops.linear import linear_act, linear_act_dgrad, linear_bias_grad
 from ..ops.norm import layer_norm, layer_norm_act8, layer_norm_act8_backward, layer_norm_backward
+from ..ops.rotary import rotary, rotary_backward, rotary_frequencies
 from ..ops.sparse import _dist_info, _stream
 
 
@@ -48,10 +54,16 @@ class GPTConfig:
     weight_decay: float = 0.1
     fused: bool = False   # blocks on ops.norm / ops.linear instead of torch ops around the GEMM
     act_bits: int = 16    # of what a fused block's norms and hidden layer keep for the backward pass: 16 or 8
+    gated: bool = False   # fused blocks: silu(g) * u in place of gelu(h) in the hidden layer
+    rotary: bool = False  # fused blocks: rotary positions of q and k in place of learned positions
+    rotary_base: float = 10000.0
+    dropout: float = 0.0  # fused blocks: behind the embedding and both halves of a block, in passes that train
 
     def n_params(self) -> int:
         d, f = self.d_model, self.d_ff
-        return self.vocab * d + self.seq_len * d + self.n_layer * (3 * d * d + d * d + 2 * d * f + 9 * d + f) + 2 * d
+        hidden = 2 * f if self.gated else f
+        return (self.vocab * d + (0 if self.rotary else self.seq_len * d)
+                + self.n_layer * (3 * d * d + d * d + d * hidden + d * f + 9 * d + hidden) + 2 * d)
 
 
 class _PSLinear(torch.autograd.Function):
@@ -152,64 +164,125 @@ class _NormedQkv(torch.autograd.Function):
         return dx2.view(dx.shape), None, None
 
 
-class _ProjResidual(torch.autograd.Function):
-    """x + proj(a) of a fused block, for attention's output ``a`` ``[B, heads, T, d / heads]``. Attention's own graph keeps ``a`` too (laid
-    out by rows: a matrix of rows is a view of it)."""
+class _NormedHeads(torch.autograd.Function):
+    """(q, k, v, x) of a fused block with rotary positions: :class:`_NormedQkv`, with q and k turned where the product left them, as heads
+    ``[B, heads, T, d / heads]``. Their gradients meet in one matrix again on the way back."""
 
     @staticmethod
-    def forward(ctx, a, x, model, i):
+    def _heads(qkv, model, B, T):
+        H = model.cfg.n_head
+        return qkv.view(B, T, 3, H, model.cfg.d_model // H).unbind(2)
+
+    @staticmethod
+    def forward(ctx, x, model, i):
+        qkv, _ = _NormedQkv.forward(ctx, x, model, i)
+        ctx.model = model
+        q, k, v = _NormedHeads._heads(qkv, model, *x.shape[:2])
+        rotary(q, k, model.freqs, out_q=q, out_k=k)
+        return q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), x
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv, dx):
+        B, T, d = dx.shape
+        dqkv = dq.new_empty((B * T, 3 * d))
+        q, k, v = _NormedHeads._heads(dqkv, ctx.model, B, T)
+        rotary_backward(dq.transpose(1, 2), dk.transpose(1, 2), ctx.model.freqs, out_q=q, out_k=k)
+        v.copy_(dv.transpose(1, 2))
+        return _NormedQkv.backward(ctx, dqkv, dx)
+
+
+class _Dropout(torch.autograd.Function):
+    """Dropout with ``drop`` = (p, seed, offset); what it dropped is formed again on the way back."""
+
+    @staticmethod
+    def forward(ctx, x, drop):
+        ctx.drop = drop
+        return dropout(x, *drop)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return dropout_backward(dy, *ctx.drop), None
+
+
+class _ProjResidual(torch.autograd.Function):
+    """x + dropout(proj(a)) of a fused block, for attention's output ``a`` ``[B, heads, T, d / heads]``. Attention's own graph keeps ``a`` too
+    (laid out by rows: a matrix of rows is a view of it)."""
+
+    @staticmethod
+    def forward(ctx, a, x, model, i, drop):
         P, Gr = model.main.params, model.main.grads
         w = P[f"h{i}.proj.w"]
         ctx.w_grad, ctx.b_grad = Gr[f"h{i}.proj.w"], Gr[f"h{i}.proj.b"]
         ctx.save_for_backward(w, a)
+        ctx.drop = drop
         d = x.shape[-1]
-        return linear_act(a.transpose(1, 2).reshape(-1, d), w, P[f"h{i}.proj.b"], residual=x.reshape(-1, d)).view(x.shape)
+        return linear_act(a.transpose(1, 2).reshape(-1, d), w, P[f"h{i}.proj.b"], residual=x.reshape(-1, d), dropout=drop).view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         w, a = ctx.saved_tensors
         B, heads, T, hd = a.shape
-        dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
-        G.gemm(dy2, a.transpose(1, 2).reshape(-1, heads * hd), a_mn=True, b_mn=True, out=ctx.w_grad, accumulate=True)
-        linear_bias_grad(dy2, out=ctx.b_grad, accumulate=True)
-        da = linear_act_dgrad(dy2, w, None)
-        return da.view(B, T, heads, hd).transpose(1, 2), dy, None, None
+        dz = _before_dropout(dy.reshape(-1, dy.shape[-1]).contiguous(), ctx.drop)
+        G.gemm(dz, a.transpose(1, 2).reshape(-1, heads * hd), a_mn=True, b_mn=True, out=ctx.w_grad, accumulate=True)
+        linear_bias_grad(dz, out=ctx.b_grad, accumulate=True)
+        da = linear_act_dgrad(dz, w, None)
+        return da.view(B, T, heads, hd).transpose(1, 2), dy, None, None, None
+
+
+def _before_dropout(dy, drop):
+    return dy if drop is None else dropout_backward(dy, *drop)
 
 
 class _MlpHalf(torch.autograd.Function):
-    """x + out(gelu(fc(norm(x)))) of a fused block. The hidden layer is kept before GELU only, and formed again behind it."""
+    """x + dropout(out(gelu(fc(norm(x))))) of a fused block, or of one whose hidden layer is gated, silu(g) * u with [g | u] = fc(norm(x)). The
+    hidden layer is kept before its activation only, and formed again behind it."""
 
     @staticmethod
-    def forward(ctx, x, model, i):
+    def forward(ctx, x, model, i, drop):
         P, Gr = model.main.params, model.main.grads
         x2 = x.reshape(-1, x.shape[-1])
         ctx.norm = _Norm(model, f"h{i}.ln2")
         keep = ctx.needs_input_grad[0]
         y, kept = ctx.norm.forward(x2, keep)
         w1, w2 = P[f"h{i}.fc.w"], P[f"h{i}.out.w"]
+        hidden, act = (gated_linear, "silu") if model.cfg.gated else (linear_act, "gelu_tanh")
         if not keep:
-            f = linear_act(y, w1, P[f"h{i}.fc.b"], act="gelu_tanh")
+            f = hidden(y, w1, P[f"h{i}.fc.b"], act=act)
         else:
-            f, h = linear_act(y, w1, P[f"h{i}.fc.b"], act="gelu_tanh", save="act8" if ctx.norm.bits == 8 else "bf16")
+            f, h = hidden(y, w1, P[f"h{i}.fc.b"], act=act, save="act8" if ctx.norm.bits == 8 else "bf16")
+            ctx.gated, ctx.drop = model.cfg.gated, drop
             ctx.grads = [Gr[f"h{i}.{name}"] for name in ("fc.w", "fc.b", "out.w", "out.b")]
-            ctx.save_for_backward(w1, w2, *((h.q, h.e) if ctx.norm.bits == 8 else (h, None)), *kept)
-        return linear_act(f, w2, P[f"h{i}.out.b"], residual=x2).view(x.shape)
+            # (in 8 bits: whole numbers and exponents of the hidden layer, or of both factors of a gated one)
+            saved = (h,) if ctx.norm.bits != 8 else (h[0].q, h[0].e, h[1].q, h[1].e) if ctx.gated else (h.q, h.e)
+            ctx.n_hidden = len(saved)
+            ctx.save_for_backward(w1, w2, *saved, *kept)
+        return linear_act(f, w2, P[f"h{i}.out.b"], residual=x2, dropout=drop).view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w1, w2, h, e, *kept = ctx.saved_tensors
+        w1, w2, *rest = ctx.saved_tensors
+        h, kept = rest[:ctx.n_hidden], rest[ctx.n_hidden:]
+        del rest
         w1_grad, b1_grad, w2_grad, b2_grad = ctx.grads
         dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
-        dh, f = linear_act_dgrad(dy2, w2, h if e is None else Act8(h, e, w1.shape[0]), act="gelu_tanh", recompute=True)
-        del h, e
-        G.gemm(dy2, f, a_mn=True, b_mn=True, out=w2_grad, accumulate=True)
+        dz = _before_dropout(dy2, ctx.drop)
+        if ctx.gated:
+            F2 = w2.shape[1]
+            dh, f = gated_linear_dgrad(dz, w2, h[0] if len(h) == 1 else (Act8(h[0], h[1], F2), Act8(h[2], h[3], F2)), act="silu", recompute=True)
+        else:
+            dh, f = linear_act_dgrad(dz, w2, h[0] if len(h) == 1 else Act8(h[0], h[1], w1.shape[0]), act="gelu_tanh", recompute=True)
+        del h
+        G.gemm(dz, f, a_mn=True, b_mn=True, out=w2_grad, accumulate=True)
         del f
-        linear_bias_grad(dy2, out=b2_grad, accumulate=True)
+        linear_bias_grad(dz, out=b2_grad, accumulate=True)
+        del dz
         ctx.norm.wgrad(kept, dh, w1_grad, b1_grad)
         dx = ctx.norm.backward(kept, linear_act_dgrad(dh, w1, None), residual_grad=dy2)
-        return dx.view(dy.shape), None, None
+        return dx.view(dy.shape), None, None, None
 
 
 class _FinalNorm(torch.autograd.Function):
@@ -230,6 +303,11 @@ class GPT:
     def __init__(self, cfg: GPTConfig, *, device=None, group=None, seed: int = 0, fuse_qkv_gather: bool = True):
         if cfg.act_bits not in (8, 16) or (cfg.act_bits == 8 and not cfg.fused):
             raise ValueError("GPTConfig: act_bits is 16, or 8 with fused=True")
+        if (cfg.gated or cfg.rotary or cfg.dropout) and not cfg.fused:
+            raise ValueError("GPTConfig: gated, rotary and dropout need fused=True")
+        if cfg.rotary and cfg.d_model // cfg.n_head % 2:
+            raise ValueError(f"GPTConfig: rotary needs heads of an even number of values, not {cfg.d_model // cfg.n_head}")
+        drop_args(cfg.dropout, 0, 0, -1, "GPTConfig: dropout")
         self.cfg = cfg
         self.group = group
         self.world, self.rank = _dist_info(group)
@@ -237,10 +315,16 @@ class GPT:
         d, f, L = cfg.d_model, cfg.d_ff, cfg.n_layer
         opt = dict(lr=cfg.lr, weight_decay=cfg.weight_decay, beta2=0.95)
         shapes: Dict[str, tuple] = {"wte": (cfg.vocab, d), "wpe": (cfg.seq_len, d), "lnf.g": (d,), "lnf.b": (d,)}
+        if cfg.rotary:
+            del shapes["wpe"]
+            self.freqs = rotary_frequencies(d // cfg.n_head, cfg.rotary_base, device=self.device)[0]
+        # every rank drops values of its own; `drop_passes` counts the forward passes that did, so that each of them draws anew
+        self.drop_seed, self.drop_passes = (seed << 16) + self.rank & 0xFFFFFFFFFFFFFFFF, 0
+        h = 2 * f if cfg.gated else f   # outputs of the hidden layer's product
         for i in range(L):
             shapes.update({f"h{i}.ln1.g": (d,), f"h{i}.ln1.b": (d,), f"h{i}.qkv.b": (3 * d,), f"h{i}.proj.w": (d, d),
-                           f"h{i}.proj.b": (d,), f"h{i}.ln2.g": (d,), f"h{i}.ln2.b": (d,), f"h{i}.fc.w": (f, d),
-                           f"h{i}.fc.b": (f,), f"h{i}.out.w": (d, f), f"h{i}.out.b": (d,)})
+                           f"h{i}.proj.b": (d,), f"h{i}.ln2.g": (d,), f"h{i}.ln2.b": (d,), f"h{i}.fc.w": (h, d),
+                           f"h{i}.fc.b": (h,), f"h{i}.out.w": (d, f), f"h{i}.out.b": (d,)})
         # the QKV weights can be gathered lazily by their consumer: one table per layer, rows sharded by rank
         self.lazy_qkv = fuse_qkv_gather and self.world > 1 and (3 * d) % (256 * self.world) == 0
         if not self.lazy_qkv:
@@ -287,15 +371,27 @@ class GPT:
         cfg = self.cfg
         B, T = tokens.shape
         lv = self._leaves
-        x = F.embedding(tokens, lv["wte"]) + lv["wpe"][:T]
+        x = F.embedding(tokens, lv["wte"])
+        if not cfg.rotary:
+            x = x + lv["wpe"][:T]
+        drops = [None] * (2 * cfg.n_layer + 1)
+        if cfg.dropout and targets is not None and torch.is_grad_enabled():
+            drops = [(cfg.dropout, self.drop_seed, (self.drop_passes << 16) + site) for site in range(2 * cfg.n_layer + 1)]
+            self.drop_passes += 1
+            x = _Dropout.apply(x, drops[-1])
         for i in range(cfg.n_layer):
             if cfg.fused:
-                qkv, x = _NormedQkv.apply(x, self, i)
-                a = self._attention(qkv, B, T)
-                del qkv   # (a forward pass alone holds no more than it needs)
-                x = _ProjResidual.apply(a, x, self, i)
+                if cfg.rotary:
+                    q, k, v, x = _NormedHeads.apply(x, self, i)
+                    a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+                    del q, k, v
+                else:
+                    qkv, x = _NormedQkv.apply(x, self, i)
+                    a = self._attention(qkv, B, T)
+                    del qkv   # (a forward pass alone holds no more than it needs)
+                x = _ProjResidual.apply(a, x, self, i, drops[2 * i])
                 del a
-                x = _MlpHalf.apply(x, self, i)
+                x = _MlpHalf.apply(x, self, i, drops[2 * i + 1])
                 continue
             h = F.layer_norm(x, (cfg.d_model,), lv[f"h{i}.ln1.g"], lv[f"h{i}.ln1.b"])
             qkv = self._linear(h, f"h{i}.qkv.w", f"h{i}.qkv.b", self.qkv[i])
@@ -362,7 +458,7 @@ def _bench(args) -> None:
     torch.cuda.set_device(local)
     if world > 1:
         dist.init_process_group("nccl", device_id=torch.device("cuda", local))
-    cfg = GPTConfig(n_layer=args.layers, fused=args.fused, act_bits=args.act_bits)
+    cfg = GPTConfig(n_layer=args.layers, d_ff=args.d_ff, fused=args.fused, act_bits=args.act_bits, gated=args.gated, rotary=args.rotary, dropout=args.dropout)
     model = GPT(cfg, fuse_qkv_gather=not args.no_fuse)
     B = args.seqs_per_gpu
     gen = torch.Generator().manual_seed(local)
@@ -395,6 +491,7 @@ def _bench(args) -> None:
                           "model_tflops_per_gpu": flops / (ms / 1e3) / 1e12 / world, "layers": cfg.n_layer,
                           "params": cfg.n_params(), "global_batch_seqs": B * world, "seq_len": cfg.seq_len,
                           "qkv_gather_fused": model.lazy_qkv, "blocks_fused": cfg.fused, "act_bits": cfg.act_bits,
+                          "d_ff": cfg.d_ff, "gated": cfg.gated, "rotary": cfg.rotary, "dropout": cfg.dropout,
                           "peak_gb": torch.cuda.max_memory_allocated() / 1e9, "loss": float(loss.item())}))
     if world > 1:
         dist.destroy_process_group()
@@ -409,5 +506,9 @@ if __name__ == "__main__":
     ap.add_argument("--warmup", type=int, default=2)
     ap.add_argument("--no-fuse", action="store_true", help="all-gather the QKV weights in the dense push instead of in the GEMM")
     ap.add_argument("--fused", action="store_true", help="blocks on ops.norm / ops.linear")
+    ap.add_argument("--d-ff", type=int, default=8192, help="hidden values of a block's MLP")
+    ap.add_argument("--gated", action="store_true", help="fused blocks: silu(g) * u in place of gelu(h)")
+    ap.add_argument("--rotary", action="store_true", help="fused blocks: rotary positions in place of learned ones")
+    ap.add_argument("--dropout", type=float, default=0.0, help="fused blocks: share of values dropped behind the embedding and both halves of a block")
     ap.add_argument("--act-bits", type=int, default=16, choices=(16, 8), help="of what a fused block's norms and hidden layer keep for the backward pass")
     _bench(ap.parse_args())
