@@ -13,6 +13,7 @@
 #include "dropout.h"
 #include "launch.cuh"
 #include "philox.cuh"
+#include "unaligned.cuh"
 
 namespace psb {
 
@@ -36,48 +37,11 @@ struct DropParams {
     DropoutArgs drop;
 };
 
-// 16 bytes of 32, from byte `past` (a multiple of W) on
-template <int W>
-__device__ __forceinline__ uint4 from_byte(uint32_t* w, uint32_t past) {
-    if (past & 8u) {
-#pragma unroll
-        for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
-    }
-    if constexpr (W <= 4) {
-        if (past & 4u) {
-#pragma unroll
-            for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
-        }
-    }
-    if constexpr (W == 2) {
-        const uint32_t shift = (past & 2u) * 8u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], shift);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// 16 bytes of a row, of which `n` exist, by aligned blocks of 16, which never reach past an allocation; what lies in them beside the row is not
-// used. Where rows start on smaller boundaries, out of two (the second only where the row has bytes in it).
+// 16 bytes of a row, of which `n` exist
 template <int W>
 __device__ __forceinline__ uint4 load_unit(const char* p, int n) {
     if constexpr (W == 16) return *(const uint4*)p;
-    const uint32_t past = (uint32_t)(uintptr_t)p & 15u;
-    const char* block = p - past;
-    const uint4 a = *(const uint4*)block;
-    uint4 b = make_uint4(0, 0, 0, 0);
-    if (past + n > 16) b = *(const uint4*)(block + 16);
-    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    return from_byte<W>(w, past);
-}
-// The values in bytes [from, to) of 32, one by one
-template <typename T>
-__device__ __forceinline__ void store_some(char* p, const uint32_t* w, int from, int to) {
-#pragma unroll
-    for (int b = 0; b < 32; b += (int)sizeof(T)) {
-        if (b < from || b >= to) continue;
-        if constexpr (sizeof(T) == 4) *(uint32_t*)(p + b) = w[b / 4];
-        else *(unsigned short*)(p + b) = (unsigned short)(w[b / 4] >> (8 * (b % 4)));
-    }
+    else return load_across<W>(p, n);
 }
 // A warp's units, side by side in their rows. Rows on boundaries of 8 and 4 bytes take that many at a time (4099 x 1001 in fp32: 8.2 us, as below
 // 10.1). Where they start on 2, a lane writes the aligned block that begins inside its unit, with the first bytes of the next lane's, and what no

@@ -37,6 +37,7 @@
 #include "philox.cuh"
 #include "tcgen05.cuh"
 #include "tile_walk.cuh"
+#include "unaligned.cuh"
 
 namespace psb {
 
@@ -210,6 +211,40 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
     for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
     return v;
 }
+// Four rows' pieces of 64 bytes, four lanes to a row with eight neighbours each (`d`), in rows that start on no 16-byte boundary: a lane writes the
+// aligned block that ends among its values, with the last ones of the lane before it, the first lane of a row with those of the piece before
+// (`carry`). Only a row's ends go value by value. `at` + i * step: where the lane's values of row i go; `rows`: how many of the four exist;
+// `n`: how many of a lane's values exist (any number). All lanes of the warp come here.
+__device__ __forceinline__ void put_joined(const uint4* d, uint4* carry, char* at, int64_t step, int rows, int n, int lane, bool first, bool last) {
+    const bool opens = (lane & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w[8] = {0, 0, 0, 0, d[i].x, d[i].y, d[i].z, d[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __shfl_up_sync(0xFFFFFFFFu, w[4 + j], 1);
+        if (opens) {
+            w[0] = carry[i].x; w[1] = carry[i].y; w[2] = carry[i].z; w[3] = carry[i].w;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) (&carry[i].x)[j] = __shfl_sync(0xFFFFFFFFu, w[4 + j], lane | 3);
+        char* p = at + i * step;
+        const int past = (int)((uintptr_t)p & 15u), own = 2 * min(max(n, 0), 8);   // bytes behind a boundary; bytes that exist
+        if (i >= rows || n <= -8) continue;
+        // of the 32 bytes from p - 16 on: the block [16 - past, 32 - past), and what of it exists
+        const int from = (opens && first) ? 16 : 16 - past, to = 16 + min(own, 16 - past);
+        if (to - from == 16) {
+            uint32_t t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = w[j];
+            *(uint4*)(p - past) = past == 0 ? d[i] : from_byte<2>(t, (uint32_t)(16 - past));
+        } else if (n > 0) {
+            store_some<unsigned short>(p - 16, w, from, to);
+        } else {   // nothing of its own: the end of the lane's before it
+            store_some<unsigned short>(p - 16, w, 16 - past, 16 + 2 * n);
+        }
+        if (last && (lane & 3) == 3 && own > 16 - past) store_some<unsigned short>(p - 16, w, 32 - past, 16 + own);
+    }
+}
 // Where in the warp's 2 KB the bytes [16 j, 16 j + 16) of row r of a [32 rows][64 bytes] piece lie
 __device__ __forceinline__ uint32_t in_piece(uint32_t stage, int r, int byte) {
     return stage + (uint32_t)(r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
@@ -342,7 +377,7 @@ __device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_
     const int quarter = ew & 3, cbase = (ew >> 2) * kColumns;
     const int qrow = lane >> 2, qcol = (lane & 3) * 8;          // a lane's place in a unit: rows qrow, qrow + 8, ..., eight columns
     const bool kept8 = p.q != nullptr;
-    const bool wide = (kept8 || (p.pre_width == 16 && p.pre_up_width == 16)) && p.out_width == 16 && p.out_up_width == 16 && p.out2_width == 16;
+    const bool wide = (kept8 || (p.pre_width == 16 && p.pre_up_width == 16)) && p.out_up_width == 16;   // (out and out2 always are)
     const unsigned long long limit_ns = p.limit_ns;
     auto first_row = [&](const Tile& t) { return t.m * 2 * BM + cr * BM + quarter * 32; };
     auto first_column = [&](const Tile& t) { return t.n * BN + cbase; };
@@ -484,15 +519,10 @@ __device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_
             continue;
         }
         // a tile with edges, with rows on smaller boundaries, or in parts: one unit with its sums in v, a row to a lane
+        uint4 carry[4];
         auto finish = [&](int c) {
             const int col = colw + c * 32, n = p.N - col - qcol;   // columns of this lane that exist
-            auto get = [&](const __nv_bfloat16* pre, int width, const int8_t* q, int64_t ldq, uint4* to) {
-                if (!kept8 && width != 16) {
-                    get_narrow(stage, lane, pre + (int64_t)row0 * p.ldpre + col, p.ldpre * 2, min(32, p.M - row0), 2 * min(32, p.N - col), width);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) to[i] = ld_smem_v4(in_piece(stage, 8 * i + qrow, qcol * 2));
-                    return;
-                }
+            auto get = [&](const __nv_bfloat16* pre, const int8_t* q, int64_t ldq, uint4* to) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int64_t r = row0 + 8 * i + qrow;
@@ -502,27 +532,19 @@ __device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_
                         const uint2 b = *(const uint2*)(q + r * ldq + col + qcol);   // (rows are padded to 16 bytes)
                         to[i] = make_uint4(b.x, b.y, 0, 0);
                     } else {
-                        to[i] = load8(pre + r * p.ldpre + col + qcol, n);
+                        to[i] = load_across<2>((const char*)(pre + r * p.ldpre + col + qcol), 2 * min(n, 8));
                     }
                 }
             };
-            auto put = [&](const uint4* d, __nv_bfloat16* out, int64_t ldo, int width) {
-                if (width != 16) {
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) st_smem_v4(in_piece(stage, 8 * i + qrow, qcol * 2), d[i]);
-                    __syncwarp();
-                    put_narrow(stage, lane, out + (int64_t)row0 * ldo + col, ldo * 2, min(32, p.M - row0), 2 * min(32, p.N - col), width);
-                    return;
-                }
+            auto put = [&](const uint4* d, __nv_bfloat16* out, int64_t ldo) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int64_t r = row0 + 8 * i + qrow;
                     if (r < p.M && n > 0) store8(out + r * ldo + col + qcol, n, d[i]);
                 }
             };
-            get(p.pre, p.pre_width, p.q, p.ldq, g);
-            get(p.pre_up, p.pre_up_width, p.q_up, p.ldq_up, u);
+            get(p.pre, p.q, p.ldq, g);
+            get(p.pre_up, p.q_up, p.ldq_up, u);
             __syncwarp();   // what was in the warp's memory has been read
             lay_down(v);
             __syncwarp();
@@ -537,9 +559,15 @@ __device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_
                 u[i] = pack8(vu);
                 a[i] = pack8(va);
             }
-            put(g, p.out, p.ldo, p.out_width);
-            put(u, p.out_up, p.ldo, p.out_up_width);
-            if (p.out2 != nullptr) put(a, p.out2, p.ldo2, p.out2_width);
+            put(g, p.out, p.ldo);
+            if (p.out2 != nullptr) put(a, p.out2, p.ldo2);
+            if (p.out_up_width == 16) {
+                put(u, p.out_up, p.ldo);
+            } else {
+                const int r = row0 + qrow;
+                put_joined(u, carry, (char*)(p.out_up + (int64_t)r * p.ldo + col + qcol), 16 * p.ldo, r >= p.M ? 0 : min(4, (p.M - r + 7) / 8), n, lane, c == 0,
+                           c + 1 == kUnits || col + 32 >= p.N);
+            }
         };
         if (row0 >= p.M) {   // nothing of this warp's 32 rows exists
             release();

@@ -14,7 +14,7 @@ struct LinearArgs {
     // with `drop`:    out = dropout(act(h)) + residual
     // gated (N counts the outputs): forward  [g | u] = a w^T + bias, out = act(g) * u; w [2N][K], bias [2N]; g and u kept side by side in
     //                 `pre` [M][2N], or in `q` / `e` and `q_up` / `e_up`;  dgrad  a w = da, out [M][2N] = [da * u * act'(g) | da * act(g)],
-    //                 out2 = act(g) * u; w [K][N]
+    //                 out2 = act(g) * u, both with rows on 16-byte boundaries; w [K][N]
     int dgrad = 0;
     int gated = 0;
     int act = 0;

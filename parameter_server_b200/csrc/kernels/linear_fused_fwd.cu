@@ -16,6 +16,7 @@ int linear_fused(const LinearArgs& a, void* stream) {
     if (a.q != nullptr && (((uintptr_t)a.q % 16) || (a.ldq % 16) || ((uintptr_t)a.e % 16) || (a.lde % 16))) return -2;
     if (a.gated) {
         if (a.residual != nullptr || a.drop.threshold != 0) return -2;
+        if (a.dgrad && (!rows16(a.out, a.ldo) || (a.out2 != nullptr && !rows16(a.out2, a.ldo2)))) return -2;
         if (a.q != nullptr && (((uintptr_t)a.q_up % 16) || (a.ldq_up % 16) || ((uintptr_t)a.e_up % 16) || (a.lde_up % 16) || a.q_up == nullptr || a.e_up == nullptr)) return -2;
         return a.dgrad ? linear_gated_dgrad(a, (cudaStream_t)stream) : linear_gated_fwd(a, (cudaStream_t)stream);
     }

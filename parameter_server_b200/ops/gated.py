@@ -15,8 +15,8 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from .act8 import Act8, launch_stream, operand, result, row_stride, vector
-from .linear import _BIAS_TYPES, _NOT_KEPT, _act_code, _beside, _like, _run
+from .act8 import Act8, launch_stream, operand, result, row_stride, rows2d, vector
+from .linear import _BIAS_TYPES, _NOT_KEPT, _act_code, _like, _run
 
 Kept = Union[torch.Tensor, Tuple[Act8, Act8]]
 
@@ -87,7 +87,8 @@ def gated_linear_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Kept, *, act: Optio
     pre, ldpre, _held_h, kept = 0, 0, None, (_NOT_KEPT, _NOT_KEPT)
     if isinstance(h, torch.Tensor):
         _like(h, dy.shape[:-1] + (2 * F,), dev, "gated_linear_dgrad: h")
-        pre, ldpre, _held_h = _beside(h, what, dev)
+        _held_h = rows2d(h, what)
+        pre, ldpre = _held_h.data_ptr(), row_stride(_held_h)
     elif isinstance(h, (tuple, list)) and len(h) == 2 and all(isinstance(k, Act8) for k in h):
         for k in h:
             if k.rows != M or k.cols != F or k.device_index != dev:
