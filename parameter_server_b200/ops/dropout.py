@@ -8,6 +8,7 @@ are counted over the leading dimensions together. Calls of one step differ in th
 """
 from __future__ import annotations
 
+from operator import index
 from typing import Optional, Union
 
 import torch
@@ -31,8 +32,11 @@ def drop_args(p: float, seed: Seed, offset: int, device: int, what: str):
         if seed.dtype is not torch.int64 or seed.numel() != 1 or seed.get_device() != device:
             raise ValueError(f"{what}: a seed in memory is one int64 on cuda:{device}, got {tuple(seed.shape)} of {seed.dtype} on {seed.device}")
         seed, at = 0, seed.data_ptr()
-    elif not -0x8000000000000000 <= seed <= 0xFFFFFFFFFFFFFFFF:
-        raise ValueError(f"{what}: the seed has 64 bits, {seed} has more")
+    else:
+        seed = index(seed)
+        if not -0x8000000000000000 <= seed <= 0xFFFFFFFFFFFFFFFF:
+            raise ValueError(f"{what}: the seed has 64 bits, {seed} has more")
+    offset = index(offset)
     if not 0 <= offset <= 0xFFFFFFFFFFFFFFFF:
         raise ValueError(f"{what}: the offset is a number of 64 bits, not {offset}")
     return seed & 0xFFFFFFFFFFFFFFFF, at, offset, threshold, 4294967296.0 / (4294967296 - threshold)
@@ -57,13 +61,15 @@ def _dropout(x, p, seed, offset, residual, out, what):
         residual = rows2d(residual, what)
         rp, ldr = residual.data_ptr(), row_stride(residual)
     if out is None:
-        y, ldy = torch.empty_like(x2) if x2.is_contiguous() else x2.new_empty((rows, cols)), cols
+        y, ldy = torch.empty_like(x2) if x2.is_contiguous() else torch.empty_strided((rows, cols), (cols, 1), dtype=x2.dtype, device=x2.device), cols
     else:
         _like_x(out, x, what, "out")
         y = out if out.dim() == 2 else out.view(rows, cols)
         if cols > 1 and y.stride(1) != 1:
             raise ValueError(f"{what}: the values of a row of out must be contiguous")
         ldy = row_stride(y)
+        if rows > 1 and ldy < cols:
+            raise ValueError(f"{what}: rows of out lie on one another")
     if rows > 0xFFFFFFFF:
         raise ValueError(f"{what}: at most 2^32 - 1 rows")
     if rows and cols:

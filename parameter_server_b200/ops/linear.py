@@ -46,12 +46,14 @@ def _beside(t: torch.Tensor, what: str, device: int):
     return at, ld, t
 
 
-def _run(dev, s, what, head, tail, limit, up=_NOT_KEPT, drop=NO_DROPOUT):
-    rc = C.linear_fused(*head, *tail, *up, drop, 0, err_ptr(dev), limit, s)
+def _run(dev, s, what, args, limit):
+    err = err_ptr(dev)
+    rc = C.linear_fused(*args, 0, err, limit, s)
     if rc == NEEDS_WORKSPACE:   # only where tiles are cut along the contraction
         scratch = workspace(dev, s)
-        rc = C.linear_fused(*head, *tail, *up, drop, scratch.data_ptr(), err_ptr(dev), limit, s)
-    check(rc, what)
+        rc = C.linear_fused(*args, scratch.data_ptr(), err, limit, s)
+    if rc != 0:
+        check(rc, what)
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
@@ -69,7 +71,11 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     if save not in (None, "bf16", "act8"):
         raise ValueError(f"{what}: save is None, 'bf16' or 'act8', not {save!r}")
     s, dev = launch_stream(x), x.get_device()
-    drop = NO_DROPOUT if dropout is None else drop_args(*dropout, dev, what)
+    drop = NO_DROPOUT
+    if dropout is not None:
+        if not isinstance(dropout, (tuple, list)) or len(dropout) != 3:
+            raise ValueError(f"{what}: dropout is (p, seed, offset), not {dropout!r}")
+        drop = drop_args(*dropout, dev, what)
     x2, xp, ldx, _held = operand(x, "linear_act x", dev)
     w, wp, ldw, _held_w = operand(w, "linear_act w", dev)
     M, K = x2.shape
@@ -95,9 +101,9 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     pre, ldpre = result(x2, M, N) if save == "bf16" else (None, 0)
     kept = Act8.for_rows(y, N) if save == "act8" else None
     if M and N:
-        _run(dev, s, what, (False, False, code, M, N, K, xp, ldx, wp, ldw, bp, bias is not None and bias.dtype is torch.float32),
-             (rp, ldr, y.data_ptr(), ldy, 0, 0,
-              0 if pre is None else pre.data_ptr(), ldpre, *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s, drop=drop)
+        _run(dev, s, what, (False, False, code, M, N, K, xp, ldx, wp, ldw, bp, bias is not None and bias.dtype is torch.float32,
+                            rp, ldr, y.data_ptr(), ldy, 0, 0, 0 if pre is None else pre.data_ptr(), ldpre,
+                            *(_NOT_KEPT if kept is None else kept._args), 0, 0, 0, 0, drop), wait_limit_s)
     if out is not None:
         y = out
     elif x.dim() != 2:
@@ -136,9 +142,8 @@ def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, h: Union[torch.Tensor, A
     dh, ld = result(dy2, M, N)
     a = result(dy2, M, N)[0] if recompute else None
     if M and N:
-        _run(dev, s, what, (True, False, code, M, N, K, dyp, lddy, wp, ldw, 0, False),
-             (0, 0, dh.data_ptr(), ld, 0 if a is None else a.data_ptr(), ld, pre, ldpre,
-              *(_NOT_KEPT if kept is None else kept._args)), wait_limit_s)
+        _run(dev, s, what, (True, False, code, M, N, K, dyp, lddy, wp, ldw, 0, False, 0, 0, dh.data_ptr(), ld, 0 if a is None else a.data_ptr(), ld,
+                            pre, ldpre, *(_NOT_KEPT if kept is None else kept._args), 0, 0, 0, 0, NO_DROPOUT), wait_limit_s)
     if dy.dim() != 2:
         shape = dy.shape[:-1] + (N,)
         dh = dh.view(shape)

@@ -57,8 +57,8 @@ def _misfit(x, out, shape, dtype, dev, what, name):
         raise ValueError(f"{what}: {name} is [tokens, heads, dim] or [batch, tokens, heads, dim], not {tuple(x.shape)}")
     if x.shape[:-2] != shape[:-2] or x.shape[-1] != shape[-1] or x.dtype != dtype or x.get_device() != dev:
         raise ValueError(f"{what}: {name} of {tuple(x.shape)} {x.dtype} on {x.device} does not go with q of {tuple(shape)} {dtype} on cuda:{dev}")
-    raise ValueError(f"{what}: out of {name} must be like it ({tuple(x.shape)} of {dtype} on cuda:{dev}), the values of a head side by side, "
-                     f"got {tuple(out.shape)} of {out.dtype} on {out.device}")
+    raise ValueError(f"{what}: out of {name} must be like it ({tuple(x.shape)} of {dtype} on cuda:{dev}), the values of a head side by side and no two "
+                     f"at one place, got {tuple(out.shape)} of {out.dtype} on {out.device} with strides {out.stride()}")
 
 
 def _heads(x, out, shape, dtype, dev, what, name):
@@ -77,7 +77,7 @@ def _heads(x, out, shape, dtype, dev, what, name):
     elif out.shape != own or out.dtype is not dtype or out.get_device() != dev:
         _misfit(x, out, shape, dtype, dev, what, name)
     to = out.stride()
-    if to[-1] != 1 and dim > 1:
+    if (to[-1] != 1 and dim > 1) or (0 in to and any(n > 1 and d == 0 for n, d in zip(own, to))):
         _misfit(x, out, shape, dtype, dev, what, name)
     if dims == 3:
         return out, (x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, to[0], to[1], own[1]), x
@@ -124,7 +124,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
     number each. ``freqs``: fp64, one angle per position of each pair. ``positions``: int64 or int32, ``[tokens]`` or ``[batch, tokens]``, any
     sign; without them a token's place in its row. ``offset`` is added to them. ``interleaved``: a pair is two neighbours, otherwise value
     ``i`` and value ``i + len(freqs)``. ``out_q`` and ``out_k`` may be ``q`` and ``k`` themselves (the values that do not turn are left alone then), and must
-    not overlap them otherwise. Angles are as exact as a product in 64 bits: 1.5e-6 radians at position 2^31 times one radian."""
+    not overlap them otherwise. Angles are as exact as a product in 64 bits (1.5e-6 radians at position 2^31 times one radian), up to 2^51 radians."""
     return _rotary(q, k, freqs, positions, offset, interleaved, scale, out_q, out_k, False, "rotary")
 
 

@@ -1,5 +1,7 @@
 """Calls that the gated block's operators refuse before anything is launched, and what they compute on the host."""
 import math
+import re
+from pathlib import Path
 
 import numpy as np
 import philox64
@@ -29,6 +31,21 @@ def test_host_tensors_are_refused():
                  lambda: gated.gated_linear(x, x), lambda: gated.gated_linear_dgrad(x, x, x)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_launches_that_overlap_their_predecessor_read_coherently():
+    """A non-coherent load is defined only for memory that nothing writes while the kernel runs; these may begin before their predecessor
+    has ended, or put their result in their input's place."""
+    for name in ("dropout.cu", "rotary.cu", "philox.cuh", "unaligned.cuh", "linear_fused.cuh", "linear_few.cuh"):
+        text = (Path(dropout.__file__).parent.parent / "csrc" / "kernels" / name).read_text()
+        assert not re.search(r"ld_nc|ld\.global\.nc|__ldg\(|__restrict__", text), name
+
+
+def test_seeds_are_whole_numbers():
+    assert dropout.drop_args(0.5, np.int64(-5), np.int32(3), 0, "dropout")[:3] == ((1 << 64) - 5, 0, 3)
+    for seed, offset in ((0.5, 0), (1, 0.5), ("1", 0)):
+        with pytest.raises(TypeError):
+            dropout.drop_args(0.5, seed, offset, 0, "dropout")
 
 
 @pytest.mark.parametrize("p", [-0.1, 1.0, 1.5, math.nan, 1 - 2.0 ** -40])
@@ -76,7 +93,7 @@ def test_types_and_shapes_of_dropout_are_refused():
         lambda: dropout.dropout(x.half(), 0.1, 1), lambda: dropout.dropout(x, 0.1, 1, residual=z(8, 63)), lambda: dropout.dropout(x, 0.1, 1, residual=x.float()),
         lambda: dropout.dropout(x, 0.1, 1, residual=x.cpu()), lambda: dropout.dropout(x, 0.1, 1, out=z(9, 64)), lambda: dropout.dropout(x, 0.1, 1, out=x.float()),
         lambda: dropout.dropout(x, 0.1, 1, out=z(64, 8).t()), lambda: dropout.dropout(x, 1.0, 1), lambda: dropout.dropout(x, 0.1, z(1, dtype=torch.int32)),
-        lambda: dropout.dropout(x, 0.1, torch.zeros(1, dtype=torch.int64)), lambda: dropout.dropout(z(()), 0.1, 1), lambda: dropout.dropout_backward(x, -0.5, 1),
+        lambda: dropout.dropout(x, 0.1, torch.zeros(1, dtype=torch.int64)), lambda: dropout.dropout(x, 0.1, 1, out=z(1, 64).expand(8, 64)), lambda: dropout.dropout(z(()), 0.1, 1), lambda: dropout.dropout_backward(x, -0.5, 1),
     ]
     for i, call in enumerate(refused):
         with pytest.raises(ValueError):
@@ -96,7 +113,7 @@ def test_types_and_shapes_of_rotary_are_refused():
         lambda: rotary.rotary(q, k.cpu(), f), lambda: rotary.rotary(q, k, f.float()), lambda: rotary.rotary(q, k, f.cpu()), lambda: rotary.rotary(q, k, z(9, dtype=torch.float64)),
         lambda: rotary.rotary(q, k, z(16, dtype=torch.float64)[::2]), lambda: rotary.rotary(q, k, f, pos.float()), lambda: rotary.rotary(q, k, f, pos[:2]),
         lambda: rotary.rotary(q, k, f, pos.cpu()), lambda: rotary.rotary(q, k, f, pos.expand(3, 3)), lambda: rotary.rotary(q, k, f, out_q=z(2, 3, 4, 17)),
-        lambda: rotary.rotary(q, None, f, out_k=k), lambda: rotary.rotary(q, k, f, out_k=z(2, 3, 16, 2).transpose(2, 3)[:, :, :1]), lambda: rotary.rotary_backward(q, k, f, out_q=q.float()),
+        lambda: rotary.rotary(q, None, f, out_k=k), lambda: rotary.rotary(q, k, f, out_q=z(2, 3, 1, 16).expand(2, 3, 4, 16)), lambda: rotary.rotary(q, k, f, pos.view(1, 1, 3)), lambda: rotary.rotary(q, k, f, out_k=z(2, 3, 16, 2).transpose(2, 3)[:, :, :1]), lambda: rotary.rotary_backward(q, k, f, out_q=q.float()),
     ]
     for i, call in enumerate(refused):
         with pytest.raises(ValueError):
@@ -113,14 +130,14 @@ def test_types_and_shapes_of_the_gated_layer_are_refused():
     refused = [
         lambda: gated.gated_linear(x, z(32, 63)), lambda: gated.gated_linear(x, z(31, 64)), lambda: gated.gated_linear(x.float(), w), lambda: gated.gated_linear(x, w.float()),
         lambda: gated.gated_linear(x, w, act="tanh"), lambda: gated.gated_linear(x, w, save="int8"), lambda: gated.gated_linear(x, w, z(16)), lambda: gated.gated_linear(x, w, z(32).half()),
-        lambda: gated.gated_linear(x, w, out=z(8, 32)), lambda: gated.gated_linear(x, w, out=z(8, 16, dtype=torch.float32)), lambda: gated.gated_linear(x, w, out=z(16, 8).t()),
+        lambda: gated.gated_linear(x, w, out=z(8, 32)), lambda: gated.gated_linear(x, w, out=z(8, 16, dtype=torch.float32)), lambda: gated.gated_linear(x, w, out=z(16, 8).t()), lambda: gated.gated_linear(x, w, out=z(1, 16).expand(8, 16)),
         lambda: gated.gated_linear(z(8, 0), z(32, 0)), lambda: gated.gated_linear(x, w.cpu()),
         lambda: gated.gated_linear_dgrad(x, z(63, 16), h), lambda: gated.gated_linear_dgrad(x, w2, z(8, 16)), lambda: gated.gated_linear_dgrad(x, w2, h.float()),
         lambda: gated.gated_linear_dgrad(x, w2, None), lambda: gated.gated_linear_dgrad(x, w2, x8), lambda: gated.gated_linear_dgrad(x, w2, (x8, wide8)),
         lambda: gated.gated_linear_dgrad(x, w2, (x8,)), lambda: gated.gated_linear_dgrad(x, w2, (h, h)), lambda: gated.gated_linear_dgrad(x, w2, h, act="swish"),
         lambda: gated.gated_linear_dgrad(z(9, 64), w2, (x8, x8)), lambda: gated.gated_linear_dgrad(z(8, 0), z(0, 16), h),
         lambda: linear.linear_act(x, w, dropout=(1.0, 1, 0)), lambda: linear.linear_act(x, w, dropout=(0.5, 1 << 64, 0)), lambda: linear.linear_act(x, w, dropout=(0.5, 1, -1)),
-        lambda: linear.linear_act(x, w, dropout=(0.5, torch.zeros(1, dtype=torch.int64), 0)),
+        lambda: linear.linear_act(x, w, dropout=(0.5, torch.zeros(1, dtype=torch.int64), 0)), lambda: linear.linear_act(x, w, dropout=0.5), lambda: linear.linear_act(x, w, dropout=(0.5, 1)),
     ]
     for i, call in enumerate(refused):
         with pytest.raises(ValueError):

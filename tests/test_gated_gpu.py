@@ -174,6 +174,7 @@ def test_strides_dims_and_nothing():
     y0, h0 = gated.gated_linear(rand(0, K), w, save="bf16")
     assert y0.shape == (0, N) and gated.gated_linear_dgrad(rand(0, 24), w2, h0).shape == (0, 2 * N)
     assert gated.gated_linear(rand(3, K), rand(0, K)).shape == (3, 0)
+    assert torch.equal(gated.gated_linear(wide[:, :K], w.view(2, N, K)), gated.gated_linear(wide[:, :K], w))   # both weights in one tensor
     G.check_gemm_errors()
 
 
