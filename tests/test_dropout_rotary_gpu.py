@@ -222,6 +222,30 @@ def test_positions(dtype):
     check_rotary(q, k, freqs, offset=-100)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot", [(8, 2), (8, 6), (40, 38), (64, 2), (96, 50), (192, 130), (256, 254), (1024, 1022), (2048, 6), (4096, 10)])
+@pytest.mark.parametrize("batch,tokens,hq,hk", [(1, 1, 1, 0), (2, 130, 5, 2), (1, 700, 40, 8)])
+def test_parts_of_heads_on_whole_blocks(batch, tokens, hq, hk, dim, rot, interleaved, dtype):
+    """Heads of whole 16-byte blocks whose halves, or whose turning part, end inside one; also in place."""
+    freqs = rotary.rotary_frequencies(rot)[0]
+    qkv = rand(batch, tokens, hq + hk + 1, dim, dtype=dtype)
+    q, k = qkv[:, :, :hq], qkv[:, :, hq:hq + hk] if hk else None
+    check_rotary(q, k, freqs, interleaved=interleaved, offset=3, scale=1.5)
+    want = rotary.rotary(q, k, freqs, interleaved=interleaved)
+    last = qkv[:, :, -1].clone()
+    rotary.rotary(q, k, freqs, interleaved=interleaved, out_q=q, out_k=k)
+    assert torch.equal(q, want[0] if hk else want) and (not hk or torch.equal(k, want[1])) and torch.equal(qkv[:, :, -1], last)
+
+
+def test_values_that_do_not_turn_keep_their_bits():
+    x = torch.zeros(1, 3, 2, 16, dtype=BF, device="cuda")
+    x.view(torch.int16)[..., 6:] = torch.tensor([0x7FC1, -1, 0x7F80, -0x80, 0x0001, -0x8000, 0x7FFF, 5, 6, 7], dtype=torch.int16, device="cuda")
+    for interleaved in (False, True):
+        y = rotary.rotary(x, None, rotary.rotary_frequencies(6)[0], interleaved=interleaved)
+        assert torch.equal(y.view(torch.int16)[..., 6:], x.view(torch.int16)[..., 6:])
+
+
 def test_scaled_frequencies():
     q, k = rand(1, 50, 4, 128), rand(1, 50, 4, 128, seed=1)
     for scaling in ("linear", "ntk", "yarn"):
