@@ -62,11 +62,14 @@ def operand(t: torch.Tensor, what: str, device: int):
     address is the copy's then, which the caller holds until its launch."""
     if t.dtype is not torch.bfloat16 or t.get_device() != device:
         raise ValueError(f"{what}: expected bf16 on cuda:{device}, got {t.dtype} on {t.device}")
-    t = rows2d(t, what)
+    strides = t.stride()
+    if len(strides) != 2 or strides[1] != 1:
+        t = rows2d(t, what)
+        strides = t.stride()
     rows, cols = t.shape
     at = t.data_ptr()
     if at % 16 == 0:
-        ld = t.stride(0)
+        ld = strides[0]
         if rows <= 1:
             return t, at, -(-cols // 8) * 8, None   # one row has no stride to speak of, but a tensor map wants a multiple of 16 bytes
         if ld % 8 == 0 and ld > 0:
@@ -74,7 +77,7 @@ def operand(t: torch.Tensor, what: str, device: int):
     ld = -(-cols // 8) * 8
     padded = t.new_empty((rows, ld))
     to = padded.data_ptr()
-    check(C.pad_rows(at, t.stride(0), to, ld, rows, cols, _raw_stream(device)), what)
+    check(C.pad_rows(at, strides[0], to, ld, rows, cols, _raw_stream(device)), what)
     return t, to, ld, padded
 
 
@@ -110,12 +113,12 @@ class Act8:
             raise ValueError("Act8: q and e are on different devices")
         if cols < 0 or q.shape[1] < cols or e.shape[1] * BLOCK < cols:
             raise ValueError(f"Act8: {cols} columns do not fit q of {q.shape[1]} and e of {e.shape[1]} columns")
-        if q.numel() and (q.stride(1) != 1 or e.stride(1) != 1 or row_stride(q) % 16 or row_stride(e) % 16
-                          or q.data_ptr() % 16 or e.data_ptr() % 16):
+        args = q.data_ptr(), row_stride(q), e.data_ptr(), row_stride(e)
+        if q.numel() and (q.stride(1) != 1 or e.stride(1) != 1 or (args[0] | args[1] | args[2] | args[3]) % 16):
             raise ValueError("Act8: rows of q and e start on 16-byte boundaries")
         self._q, self._e, self._both, self.rows, self.cols = q, e, None, q.shape[0], cols
         self.device_index = q.get_device()
-        self._args = (q.data_ptr(), row_stride(q), e.data_ptr(), row_stride(e))
+        self._args = args
 
     @classmethod
     def empty(cls, rows: int, cols: int, device) -> "Act8":

@@ -53,13 +53,21 @@ def _dropout(x, p, seed, offset, residual, out, what):
         raise ValueError(f"{what}: bf16 or fp32, not {x.dtype}")
     s = launch_stream(x)
     drop = drop_args(p, seed, offset, x.get_device(), what)
-    x2 = rows2d(x, what)
+    x2, shape = x, x.shape
+    strides = x.stride()
+    if len(strides) != 2 or strides[1] != 1:
+        x2 = rows2d(x, what)
+        strides = x2.stride()
     rows, cols = x2.shape
-    rp = ldr = 0
+    ldx, rp, ldr = strides[0] if rows > 1 else cols, 0, 0
     if residual is not None:
-        _like_x(residual, x, what, "residual")
-        residual = rows2d(residual, what)
-        rp, ldr = residual.data_ptr(), row_stride(residual)
+        if residual.shape != shape or residual.dtype is not x.dtype or residual.get_device() != x.get_device():
+            _like_x(residual, x, what, "residual")
+        rs = residual.stride()
+        if len(rs) != 2 or rs[1] != 1:
+            residual = rows2d(residual, what)
+            rs = residual.stride()
+        rp, ldr = residual.data_ptr(), rs[0] if rows > 1 else cols
     if out is None:
         y, ldy = torch.empty_like(x2) if x2.is_contiguous() else torch.empty_strided((rows, cols), (cols, 1), dtype=x2.dtype, device=x2.device), cols
     else:
@@ -73,12 +81,12 @@ def _dropout(x, p, seed, offset, residual, out, what):
     if rows > 0xFFFFFFFF:
         raise ValueError(f"{what}: at most 2^32 - 1 rows")
     if rows and cols:
-        rc = C.dropout(dt, x2.data_ptr(), row_stride(x2), rp, ldr, y.data_ptr(), ldy, rows, cols, drop, s)
+        rc = C.dropout(dt, x2.data_ptr(), ldx, rp, ldr, y.data_ptr(), ldy, rows, cols, drop, s)
         if rc != 0:
             check(rc, what)
     if out is not None:
         return out
-    return y if x.dim() == 2 else y.view(x.shape)
+    return y if len(shape) == 2 else y.view(shape)
 
 
 def dropout(x: torch.Tensor, p: float, seed: Seed, offset: int = 0, *, residual: Optional[torch.Tensor] = None,

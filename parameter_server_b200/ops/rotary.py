@@ -15,7 +15,6 @@ from .act8 import _DTYPES, check, launch_stream
 
 _POSITIONS = {torch.int64: False, torch.int32: True}
 _NO_HEADS = (0,) * 9
-_NO_POSITIONS = (0, False, 0, 0)
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
@@ -61,55 +60,59 @@ def _misfit(x, out, shape, dtype, dev, what, name):
                      f"at one place, got {tuple(out.shape)} of {out.dtype} on {out.device} with strides {out.stride()}")
 
 
-def _heads(x, out, shape, dtype, dev, what, name):
-    """(result, arguments of the native call, what to hold) of queries or keys; ``shape``, ``dtype`` and ``dev`` are those of q."""
-    own = x.shape
-    dims, dim = len(own), shape[-1]
-    if dims not in (3, 4) or (own is not shape and (dims != len(shape) or own[0] != shape[0] or own[-3] != shape[-3] or own[-1] != dim
-                                                    or x.dtype is not dtype or x.get_device() != dev)):
-        _misfit(x, out, shape, dtype, dev, what, name)
+def _heads(x, own, out, shape, dtype, dev, what, name):
+    """(result, arguments of the native call, what to hold) of queries or keys ``x`` of shape ``own``; ``shape``, ``dtype`` and ``dev`` are q's."""
     st = x.stride()
-    if st[-1] != 1 and dim > 1:
+    if st[-1] != 1 and own[-1] > 1:
         x = x.contiguous()
         st = x.stride()
     if out is None:
         out = torch.empty_like(x)
-    elif out.shape != own or out.dtype is not dtype or out.get_device() != dev:
-        _misfit(x, out, shape, dtype, dev, what, name)
-    to = out.stride()
-    if (to[-1] != 1 and dim > 1) or (0 in to and any(n > 1 and d == 0 for n, d in zip(own, to))):
-        _misfit(x, out, shape, dtype, dev, what, name)
-    if dims == 3:
-        return out, (x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, to[0], to[1], own[1]), x
-    return out, (x.data_ptr(), st[0], st[1], st[2], out.data_ptr(), to[0], to[1], to[2], own[2]), x
+        to = out.stride()
+    else:
+        to = out.stride()
+        if out.shape != own or out.dtype is not dtype or out.get_device() != dev or (to[-1] != 1 and own[-1] > 1) or (
+                0 in to and any(n > 1 and d == 0 for n, d in zip(own, to))):
+            _misfit(x, out, shape, dtype, dev, what, name)
+    if len(own) == 4:
+        return out, (x.data_ptr(), st[0], st[1], st[2], out.data_ptr(), to[0], to[1], to[2], own[2]), x
+    return out, (x.data_ptr(), 0, st[0], st[1], out.data_ptr(), 0, to[0], to[1], own[1]), x
 
 
 def _rotary(q, k, freqs, positions, offset, interleaved, scale, out_q, out_k, backward, what):
-    dtype = q.dtype
+    dtype, shape, s, dev = q.dtype, q.shape, launch_stream(q), q.get_device()
     dt = _DTYPES.get(dtype)
     if dt is None:
         raise ValueError(f"{what}: bf16 or fp32, not {dtype}")
-    s, dev = launch_stream(q), q.get_device()
-    shape = q.shape
-    out_q, q_args, _held = _heads(q, out_q, shape, dtype, dev, what, "q")
+    if len(shape) == 4:
+        batch, tokens, _, dim = shape
+    elif len(shape) == 3:
+        (tokens, _, dim), batch = shape, 1
+    else:
+        _misfit(q, out_q, shape, dtype, dev, what, "q")
+    out_q, q_args, _held = _heads(q, shape, out_q, shape, dtype, dev, what, "q")
     k_args = _NO_HEADS
     if k is not None:
-        out_k, k_args, _held_k = _heads(k, out_k, shape, dtype, dev, what, "k")
+        own = k.shape
+        if len(own) != len(shape) or own[-1] != dim or own[-3] != tokens or (own[0] != batch and len(own) == 4) or k.dtype is not dtype or k.get_device() != dev:
+            _misfit(k, out_k, shape, dtype, dev, what, "k")
+        out_k, k_args, _held_k = _heads(k, own, out_k, shape, dtype, dev, what, "k")
     elif out_k is not None:
         raise ValueError(f"{what}: out_k without k")
-    batch, tokens, dim = shape[0] if len(shape) == 4 else 1, shape[-3], shape[-1]
     pairs = freqs.numel()
     if freqs.dtype is not torch.float64 or freqs.dim() != 1 or freqs.get_device() != dev or 2 * pairs > dim or not freqs.is_contiguous():
         raise ValueError(f"{what}: freqs must be at most {dim // 2} contiguous fp64 values on {q.device}, got {tuple(freqs.shape)} of {freqs.dtype} on {freqs.device}")
-    pos = _NO_POSITIONS
+    at, narrow, pb, pt = 0, False, 0, 0
     if positions is not None:
-        narrow, at = _POSITIONS.get(positions.dtype), positions.shape
-        if narrow is None or positions.get_device() != dev or not 1 <= len(at) <= 2 or at[-1] != tokens or (len(at) == 2 and at[0] != batch and at[0] != 1):
+        narrow, places, st = _POSITIONS.get(positions.dtype), positions.shape, positions.stride()
+        dims = len(places)
+        if narrow is None or positions.get_device() != dev or not 1 <= dims <= 2 or places[-1] != tokens or (dims == 2 and places[0] != batch and places[0] != 1):
             raise ValueError(f"{what}: positions must be int64 or int32, [{tokens}] or [{batch}, {tokens}], on {q.device}, "
-                             f"got {tuple(at)} of {positions.dtype} on {positions.device}")
-        st = positions.stride()
-        pos = (positions.data_ptr(), narrow, st[0] if len(at) == 2 and at[0] > 1 else 0, st[-1])
-    rc = C.rotary(dt, q_args, k_args, batch, tokens, dim, pairs, interleaved, freqs.data_ptr(), *pos, offset, scale, backward, s)
+                             f"got {tuple(places)} of {positions.dtype} on {positions.device}")
+        at, pt = positions.data_ptr(), st[-1]
+        if dims == 2 and places[0] > 1:
+            pb = st[0]
+    rc = C.rotary(dt, q_args, k_args, batch, tokens, dim, pairs, interleaved, freqs.data_ptr(), at, narrow, pb, pt, offset, scale, backward, s)
     if rc != 0:
         check(rc, what)
     return out_q if k is None else (out_q, out_k)
