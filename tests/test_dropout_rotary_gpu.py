@@ -63,6 +63,18 @@ def test_dropout_is_its_mask(rows, cols, residual, dtype):
     near(dropout.dropout_backward(x, 0.3, 0x123456789ABCDEF0, 5), dropped(x, 0.3, 0x123456789ABCDEF0, 5)[0], 2.0 ** -23 * x.double().abs() * 2)
 
 
+@pytest.mark.parametrize("rows,cols", [(2500, 2048), (2500, 2056), (5001, 1001), (4001, 1302), (3001, 1636), (700001, 8), (620001, 9), (1300001, 5), (5000001, 1), (1, 5000003)])
+def test_dropout_of_many_values(rows, cols):
+    """32 bytes of a thread at a time, on every boundary, with every end of a row."""
+    x, r = rand(rows, cols), rand(rows, cols, seed=1)
+    check_dropout(x, 0.3, 77, 6, r)
+    wide = torch.full((rows, cols + 3), 7.0, dtype=BF, device="cuda")
+    got, mask = check_dropout(x, 0.3, 77, 6, out=wide[:, 1:cols + 1])
+    assert (got[~mask] == 0).all() and (wide[:, 0] == 7).all() and (wide[:, cols + 1:] == 7).all()
+    want = got.clone()
+    assert torch.equal(dropout.dropout(x, 0.3, 77, 6, out=x), want)   # in place
+
+
 @pytest.mark.parametrize("p", [0.0, 2.0 ** -32, 1e-3, 0.5, 0.9, 1 - 2.0 ** -20])
 def test_every_share(p):
     x = rand(64, 257) + 4
