@@ -23,6 +23,7 @@ import argparse
 import json
 import math
 import os
+import weakref
 from dataclasses import dataclass
 from typing import Dict, List, Optional
 
@@ -192,18 +193,29 @@ class _NormedHeads(torch.autograd.Function):
         return _NormedQkv.backward(ctx, dqkv, dx)
 
 
+class _DropPass:
+    """A forward pass that drops values. ``number`` is another one for every pass, and for a pass that is computed again the one it had.
+    ``alone``: no other pass whose graph lives began with torch's generator in the same state."""
+
+    __slots__ = ("number", "alone", "__weakref__")
+
+    def __init__(self, number: int):
+        self.number, self.alone = number, True
+
+
 class _Dropout(torch.autograd.Function):
-    """Dropout with ``drop`` = (p, seed, offset); what it dropped is formed again on the way back."""
+    """Dropout with ``drop`` = (p, seed, offset); what it dropped is formed again on the way back. ``of``, the :class:`_DropPass` that it begins,
+    lives as long as the pass's graph."""
 
     @staticmethod
-    def forward(ctx, x, drop):
-        ctx.drop = drop
+    def forward(ctx, x, drop, of):
+        ctx.drop, ctx.of = drop, of
         return dropout(x, *drop)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return dropout_backward(dy, *ctx.drop), None
+        return dropout_backward(dy, *ctx.drop), None, None
 
 
 class _ProjResidual(torch.autograd.Function):
@@ -320,6 +332,7 @@ class GPT:
             self.freqs = rotary_frequencies(d // cfg.n_head, cfg.rotary_base, device=self.device)[0]
         # every rank drops values of its own; `drop_passes` counts the forward passes that did, so that each of them draws anew
         self.drop_seed, self.drop_passes = (seed << 16) + self.rank & 0xFFFFFFFFFFFFFFFF, 0
+        self._drop_known = weakref.WeakValueDictionary()   # by what they drew of torch's generator: the passes whose graphs live
         h = 2 * f if cfg.gated else f   # outputs of the hidden layer's product
         for i in range(L):
             shapes.update({f"h{i}.ln1.g": (d,), f"h{i}.ln1.b": (d,), f"h{i}.qkv.b": (3 * d,), f"h{i}.proj.w": (d, d),
@@ -367,6 +380,23 @@ class GPT:
         q, k, v = qkv.view(B, T, 3, self.cfg.n_head, self.cfg.d_model // self.cfg.n_head).permute(2, 0, 3, 1, 4)
         return F.scaled_dot_product_attention(q, k, v, is_causal=True)
 
+    def _drop_pass(self) -> _DropPass:
+        """A new pass that drops values, or the one that is being computed again: recomputation (``torch.utils.checkpoint``) runs ``forward``
+        once more inside the backward pass, and puts torch's generators back to where they were, so that the number which every pass draws of
+        the CPU's tells which one it is."""
+        drawn = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
+        known = self._drop_known.get(drawn)
+        if torch._C._current_graph_task_id() == -1:   # not inside a backward pass
+            one = self._drop_known[drawn] = _DropPass(self.drop_passes)
+            self.drop_passes += 1
+            if known is not None:
+                one.alone = known.alone = False
+            return one
+        if known is None or not known.alone:
+            raise RuntimeError("GPT: a pass with dropout that is recomputed inside a backward pass finds its masks only where torch.utils.checkpoint has "
+                               "use_reentrant=False and preserve_rng_state=True, and torch's generators were not seeded alike ahead of several passes")
+        return known
+
     def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None):
         cfg = self.cfg
         B, T = tokens.shape
@@ -376,9 +406,9 @@ class GPT:
             x = x + lv["wpe"][:T]
         drops = [None] * (2 * cfg.n_layer + 1)
         if cfg.dropout and targets is not None and torch.is_grad_enabled():
-            drops = [(cfg.dropout, self.drop_seed, (self.drop_passes << 16) + site) for site in range(2 * cfg.n_layer + 1)]
-            self.drop_passes += 1
-            x = _Dropout.apply(x, drops[-1])
+            of = self._drop_pass()
+            drops = [(cfg.dropout, self.drop_seed, (of.number << 16) + site) for site in range(2 * cfg.n_layer + 1)]
+            x = _Dropout.apply(x, drops[-1], of)
         for i in range(cfg.n_layer):
             if cfg.fused:
                 if cfg.rotary:
