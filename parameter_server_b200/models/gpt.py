@@ -467,18 +467,38 @@ class GPT:
         G.check_gemm_errors()
 
     def save_checkpoint(self, uri: str) -> None:
-        """Collective, between steps: every dense table (values, optimizer slots, step count) under ``<uri>/table_<i>``."""
+        """Collective, between steps: every dense table (values, optimizer slots, step count) under ``<uri>/table_<i>``, and what the next
+        pass draws its dropout masks from in ``<uri>/dropout.json``."""
         from ..parallel import checkpoint
-        torch.cuda.synchronize(self.device)
+        self._settle()
+        if self.rank == 0:   # (ahead of the tables, whose end all ranks wait for)
+            folder = uri.split("?", 1)[0]
+            if checkpoint._is_remote(folder):
+                raise ValueError("GPT.save_checkpoint writes to a local directory")
+            os.makedirs(folder, exist_ok=True)
+            tmp = os.path.join(folder, ".dropout.json.tmp")
+            with open(tmp, "w") as f:
+                json.dump({"seed": self.drop_seed, "passes": self.drop_passes}, f)
+            os.replace(tmp, os.path.join(folder, "dropout.json"))
         for i, t in enumerate(self.tables):
             checkpoint.dump_dense(t, f"{uri.rstrip('/')}/table_{i}")
 
     def load_checkpoint(self, uri: str) -> None:
-        """Collective, between steps; the checkpoint may come from a job with another number of ranks."""
+        """Collective, between steps; the checkpoint may come from a job with another number of ranks. Dropout goes on with the masks that the
+        job which wrote it would draw next (``drop_seed`` and ``drop_passes`` stay as they are where the checkpoint does not hold them)."""
         from ..parallel import checkpoint
-        torch.cuda.synchronize(self.device)
+        self._settle()
         for i, t in enumerate(self.tables):
             checkpoint.load_dense(t, f"{uri.rstrip('/')}/table_{i}")
+        at = os.path.join(uri.split("?", 1)[0], "dropout.json")
+        if os.path.exists(at):
+            with open(at) as f:
+                kept = json.load(f)
+            self.drop_seed, self.drop_passes = int(kept["seed"]) + self.rank & 0xFFFFFFFFFFFFFFFF, int(kept["passes"])   # (rank 0 wrote it)
+
+    def _settle(self) -> None:
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
 
 
 def _bench(args) -> None:
