@@ -194,13 +194,13 @@ class _NormedHeads(torch.autograd.Function):
 
 
 class _DropPass:
-    """A forward pass that drops values. ``number`` is another one for every pass, and for a pass that is computed again the one it had.
-    ``alone``: no other pass whose graph lives began with torch's generator in the same state."""
+    """A forward pass that drops values. ``number`` is another one for every pass, and for a pass that is computed again the one it had, as
+    ``seed`` is. ``alone``: no other pass whose graph lives began with torch's generator in the same state."""
 
-    __slots__ = ("number", "alone", "__weakref__")
+    __slots__ = ("number", "seed", "alone", "__weakref__")
 
-    def __init__(self, number: int):
-        self.number, self.alone = number, True
+    def __init__(self, number: int, seed):
+        self.number, self.seed, self.alone = number, seed, True
 
 
 class _Dropout(torch.autograd.Function):
@@ -333,6 +333,7 @@ class GPT:
         # every rank drops values of its own; `drop_passes` counts the forward passes that did, so that each of them draws anew
         self.drop_seed, self.drop_passes = (seed << 16) + self.rank & 0xFFFFFFFFFFFFFFFF, 0
         self._drop_known = weakref.WeakValueDictionary()   # by what they drew of torch's generator: the passes whose graphs live
+        self._replays = torch.zeros((), dtype=torch.int64, device=self.device) if cfg.dropout and self.device.type == "cuda" else None
         h = 2 * f if cfg.gated else f   # outputs of the hidden layer's product
         for i in range(L):
             shapes.update({f"h{i}.ln1.g": (d,), f"h{i}.ln1.b": (d,), f"h{i}.qkv.b": (3 * d,), f"h{i}.proj.w": (d, d),
@@ -380,6 +381,13 @@ class GPT:
         q, k, v = qkv.view(B, T, 3, self.cfg.n_head, self.cfg.d_model // self.cfg.n_head).permute(2, 0, 3, 1, 4)
         return F.scaled_dot_product_attention(q, k, v, is_causal=True)
 
+    def _pass_seed(self):
+        """The seed of a pass. While a graph is captured it is one in memory, another at every replay (``2^40`` on, past those of other ranks),
+        which the pass's backward pass reads, too."""
+        if self._replays is None or not torch.cuda.is_current_stream_capturing():
+            return self.drop_seed
+        return self._replays.add_(1 << 40) + (self.drop_seed - (self.drop_seed >> 63 << 64))   # (as a number with a sign)
+
     def _drop_pass(self) -> _DropPass:
         """A new pass that drops values, or the one that is being computed again: recomputation (``torch.utils.checkpoint``) runs ``forward``
         once more inside the backward pass, and puts torch's generators back to where they were, so that the number which every pass draws of
@@ -387,7 +395,7 @@ class GPT:
         drawn = int(torch.empty((), dtype=torch.int64, device="cpu").random_())
         known = self._drop_known.get(drawn)
         if torch._C._current_graph_task_id() == -1:   # not inside a backward pass
-            one = self._drop_known[drawn] = _DropPass(self.drop_passes)
+            one = self._drop_known[drawn] = _DropPass(self.drop_passes, self._pass_seed())
             self.drop_passes += 1
             if known is not None:
                 one.alone = known.alone = False
@@ -407,7 +415,7 @@ class GPT:
         drops = [None] * (2 * cfg.n_layer + 1)
         if cfg.dropout and targets is not None and torch.is_grad_enabled():
             of = self._drop_pass()
-            drops = [(cfg.dropout, self.drop_seed, (of.number << 16) + site) for site in range(2 * cfg.n_layer + 1)]
+            drops = [(cfg.dropout, of.seed, (of.number << 16) + site) for site in range(2 * cfg.n_layer + 1)]
             x = _Dropout.apply(x, drops[-1], of)
         for i in range(cfg.n_layer):
             if cfg.fused:
