@@ -405,7 +405,9 @@ class GPT:
                                "use_reentrant=False and preserve_rng_state=True, and torch's generators were not seeded alike ahead of several passes")
         return known
 
-    def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None):
+    def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None, *, drop: Optional[bool] = None):
+        """``(logits, loss)``; without ``targets`` the loss is None. ``drop``: whether the pass has the dropout of the model's configuration; if
+        it is not said, a pass with targets and gradients has it."""
         cfg = self.cfg
         B, T = tokens.shape
         lv = self._leaves
@@ -413,7 +415,9 @@ class GPT:
         if not cfg.rotary:
             x = x + lv["wpe"][:T]
         drops = [None] * (2 * cfg.n_layer + 1)
-        if cfg.dropout and targets is not None and torch.is_grad_enabled():
+        if drop is None:
+            drop = targets is not None and torch.is_grad_enabled()
+        if cfg.dropout and drop:
             of = self._drop_pass()
             drops = [(cfg.dropout, of.seed, (of.number << 16) + site) for site in range(2 * cfg.n_layer + 1)]
             x = _Dropout.apply(x, drops[-1], of)
