@@ -69,6 +69,9 @@ def _heads(x, own, out, shape, dtype, dev, what, name):
     if out is None:
         out = torch.empty_like(x)
         to = out.stride()
+        if to[-1] != 1 and own[-1] > 1:   # (heads that share memory: a stride of 1 that is not the last)
+            out = torch.empty(own, dtype=dtype, device=x.device)
+            to = out.stride()
     else:
         to = out.stride()
         if out.shape != own or out.dtype is not dtype or out.get_device() != dev or (to[-1] != 1 and own[-1] > 1) or (
@@ -127,7 +130,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor, posi
     number each. ``freqs``: fp64, one angle per position of each pair. ``positions``: int64 or int32, ``[tokens]`` or ``[batch, tokens]``, any
     sign; without them a token's place in its row. ``offset`` is added to them. ``interleaved``: a pair is two neighbours, otherwise value
     ``i`` and value ``i + len(freqs)``. ``out_q`` and ``out_k`` may be ``q`` and ``k`` themselves (the values that do not turn are left alone then), and must
-    not overlap them otherwise. Angles are as exact as a product in 64 bits (1.5e-6 radians at position 2^31 times one radian), up to 2^51 radians."""
+    not overlap them otherwise, nor have heads that share memory. Angles are as exact as a product in 64 bits (1.5e-6 radians at position 2^31 times one radian), up to 2^51 radians."""
     return _rotary(q, k, freqs, positions, offset, interleaved, scale, out_q, out_k, False, "rotary")
 
 
