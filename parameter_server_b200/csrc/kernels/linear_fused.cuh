@@ -186,15 +186,7 @@ __device__ __forceinline__ float s8_at(const uint4* raw, int j) {   // j is a co
     const uint32_t w = ((j / 4) % 4 == 0 ? v.x : (j / 4) % 4 == 1 ? v.y : (j / 4) % 4 == 2 ? v.z : v.w) ^ 0x80808080u;
     return j % 4 == 0 ? s8_of_biased<0>(w) : j % 4 == 1 ? s8_of_biased<1>(w) : j % 4 == 2 ? s8_of_biased<2>(w) : s8_of_biased<3>(w);
 }
-// Eight neighbours of a bf16 row on a 16-byte boundary, of which `n` (one at least) exist
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int n) {
-    if (n >= 8) return ld_global_v4(p);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        w[j] = (2 * j < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j]) : 0u) | (2 * j + 1 < n ? (uint32_t)__bfloat16_as_ushort(p[2 * j + 1]) : 0u) << 16;
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
+// Eight neighbours into a bf16 row on a 16-byte boundary, of which `n` (one at least) have a place there
 __device__ __forceinline__ void store8(__nv_bfloat16* p, int n, uint4 v) {
     if (n >= 8) {
         *(uint4*)p = v;
