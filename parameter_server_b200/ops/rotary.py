@@ -25,8 +25,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Optional[str
 
     ``scaling``, for contexts ``factor`` times as long as ``trained_length``: "linear" divides all frequencies by ``factor``; "ntk" raises
     the base so that the slowest pair is divided by it and the fastest stays; "yarn" (Peng, Quesnelle, Fan, Shippole, 2023) leaves pairs that
-    turn ``fast`` times or more over ``trained_length``, divides those below ``slow`` turns, goes linearly in the number of turns in between, and
-    has ``scale`` = 0.1 ln(factor) + 1."""
+    turn ``fast`` times or more over ``trained_length``, divides those below ``slow`` turns, goes linearly in the number of turns in between, as
+    that paper has it, and has ``scale`` = 0.1 ln(factor) + 1. (A model that was trained with a ramp that is linear in the number of the pair has other
+    frequencies in between: :func:`rotary` takes any.)"""
     what = "rotary_frequencies"
     if dim <= 0 or dim % 2:
         raise ValueError(f"{what}: dim is even and positive, not {dim}")
