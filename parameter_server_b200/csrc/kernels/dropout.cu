@@ -2,9 +2,10 @@
 // the same without a residual.
 //
 // 6 bytes a value in bf16 (4 backward) beside ten rounds of the generator for four of them: twenty wide products and as many three-way XORs, which
-// take the integer pipes about as long as the bytes take HBM. A thread has units of 16 bytes, whose columns are whole blocks of four random words; in
+// take about as long as the bytes take HBM: the half of the FMA pipe that has the wide products is busy 72 % of the time (76 % backward), the ALU,
+// which has the XORs, 58 %, HBM 61 % (34 %). A thread has units of 16 bytes, whose columns are whole blocks of four random words; in
 // bf16, where there are many, of 32: their four blocks share what hangs on the row alone, and are four chains side by side. 16384 x 2048: bf16 31 us
-// (6.5 TB/s, as a plain copy; 16 bytes at a time 36), backward 28 (33; the integer pipes); fp32 59 (6.8). A second unit on its way while one is worked
+// (6.5 TB/s, as a plain copy; 16 bytes at a time 36), backward 28 (33: the wide products); fp32 59 (6.8). A second unit on its way while one is worked
 // on, or four, took registers and with them warps: 38 to 46 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

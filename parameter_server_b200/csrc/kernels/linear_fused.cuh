@@ -364,7 +364,9 @@ __device__ __forceinline__ uint32_t keep_row32(const float* f, int8_t* qp, int n
 // blocks, four lanes to a row, none of which goes through shared memory (16384 tokens, 5504 x 2048, silu: 439 us with a row to a lane, 376 so; sixteen
 // warps with 16 columns at a time, two lanes to a row, 510). Whole tiles need no checks, and ask for the neighbours of the next unit, also of the
 // next tile's first, while one is worked on: 350. The accumulator is given back with the last read; what is written leaves L2 first: 345.
-// Bound by an SM's port to L2, which the MMAs' operands share: without these loads 300, without these stores 300, with neither 240.
+// Without these loads 300, without these stores 300, with neither 240, which is 20 waves of MMAs: 64 x 22 tiles, the last column's half padding, on 74
+// pairs, where the values fill 18.6. What the rest waits for is not known: nothing is full (4096 tokens, from bf16 / from 8 bits: the tensor pipe busy 64 %
+// of the time, L1 64 and 65 %, L2 42 and 40 %, HBM 34 and 25 %, issue slots 28 and 41 %).
 template <int ACT, int BN>
 __device__ __forceinline__ void gated_dgrad_epilogue(const LinParams& p, uint32_t tmem_base, uint64_t* tfull_bar, uint64_t* tempty_bar, uint32_t* tmem_slot,
                                                      uint32_t stage, int pair, int cr, int ew, int lane) {
