@@ -490,7 +490,7 @@ class GPT:
             os.makedirs(folder, exist_ok=True)
             tmp = os.path.join(folder, ".dropout.json.tmp")
             with open(tmp, "w") as f:
-                json.dump({"seed": self.drop_seed, "passes": self.drop_passes}, f)
+                json.dump({"seed": int(self.drop_seed), "passes": int(self.drop_passes)}, f)
             os.replace(tmp, os.path.join(folder, "dropout.json"))
         for i, t in enumerate(self.tables):
             checkpoint.dump_dense(t, f"{uri.rstrip('/')}/table_{i}")

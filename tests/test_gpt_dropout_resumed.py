@@ -2,6 +2,7 @@
 import os
 import socket
 
+import numpy as np
 import pytest
 import torch
 import torch.distributed as dist
@@ -52,6 +53,14 @@ def test_seeds_of_any_size(tmp_path, seed):
     other = GPT(GPTConfig(**CPU, dropout=0.1), device="cpu")
     other.load_checkpoint(str(tmp_path))
     assert other.drop_seed == model.drop_seed == (seed << 16) & 0xFFFFFFFFFFFFFFFF
+
+
+def test_a_count_of_another_whole_number_type(tmp_path):
+    model, other = (GPT(GPTConfig(**CPU, dropout=0.1), device="cpu") for _ in range(2))
+    model.drop_passes, model.drop_seed = np.int64(41), torch.tensor(5)
+    model.save_checkpoint(str(tmp_path))
+    other.load_checkpoint(str(tmp_path))
+    assert (other.drop_seed, other.drop_passes) == (5, 41)
 
 
 def _rank(rank, world, port, uri):
